@@ -40,6 +40,7 @@ extern "C" {
 #define DSPARK_DEVICE_WAIT_TIMEOUT 1u
 #define DSPARK_DEVICE_BAD_SCHEDULE 2u
 #define DSPARK_DEVICE_BAD_ARGUMENT 4u
+#define DSPARK_DEVICE_EMPTY_MASK 8u
 
 int dspark_abi_version(void);
 const char* dspark_status_string(int status);
@@ -427,6 +428,98 @@ int dspark_train_plan(int num_seqs, const int32_t* ctx_len, const int32_t* num_b
                       int block_size, int grid_limit, int32_t* plan, long long plan_capacity, long long* plan_words);
 int dspark_train_attn(const void* q, const void* k, const void* v, int total_q, long long total_k,
                       const int32_t* plan, int grid, float scale, void* out, cudaStream_t stream);
+
+/*
+ * Attention of a batch whose requests share long prefixes. A group is a run of
+ * consecutive requests with one shared prefix; the keys of request i are, in this
+ * order, its group's prefix rows (source prefix), its own cached rows (source own) and
+ * its new rows (source new, optional), each source [rows, 8, 128] read in place.
+ * `causal` is the bottom-right mask over those keys: row x of a request with q rows
+ * and n keys sees keys j <= n - q + x (own + new rows must then number at least q).
+ * A prefix row is read once per 128 query rows of its group instead of once per
+ * request. No reference counterpart: the reference gathers every request's keys
+ * (persistent_target_kv.py:441-460).
+ *
+ * dspark_prefix_plan runs on the host only (all pointers HOST memory): group_size,
+ * prefix_start / prefix_len [num_groups]; q_len, own_start / own_len and, with a new
+ * source, new_start / new_len [num_requests] (both NULL without one). Lengths may be
+ * zero. It cuts the work into pieces for at most grid_limit persistent CTAs. With
+ * plan == NULL it returns the plan size in int32 words in *plan_words. The plan is
+ * copied to the device once and serves every call with these lengths (all layers of
+ * a round); its first DSPARK_PREFIX_HEAD_WORDS words also stay on the host as
+ * plan_head. DSPARK_ERR_UNSUPPORTED when a row index or a plan offset reaches 2^30.
+ *
+ * dspark_prefix_attn: q and out [total_q, 16, 128]; source s holds `rows` rows of
+ * which the plan's rows start at row `off` (a layer's first row). A source that the
+ * plan does not read may be NULL. bf16 (16-byte aligned pointers; workspace of
+ * dspark_prefix_workspace_bytes(plan_head) bytes, 16-byte aligned, never needing a
+ * clear, one per call in flight) or fp32. A device plan that is not the one plan_head
+ * belongs to sets DSPARK_DEVICE_BAD_ARGUMENT and computes nothing. out may be q.
+ */
+#define DSPARK_PREFIX_HEAD_WORDS 32
+int dspark_prefix_plan(int num_groups, const int32_t* group_size, const int32_t* prefix_start,
+                       const int32_t* prefix_len, int num_requests, const int32_t* q_len, const int32_t* own_start,
+                       const int32_t* own_len, const int32_t* new_start, const int32_t* new_len, int causal,
+                       int grid_limit, int32_t* plan, long long plan_capacity, long long* plan_words);
+size_t dspark_prefix_workspace_bytes(const int32_t* plan_head);
+int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const void* prefix_v,
+                       long long prefix_rows, long long prefix_off, const void* own_k, const void* own_v,
+                       long long own_rows, long long own_off, const void* new_k, const void* new_v,
+                       long long new_rows, long long new_off, const int32_t* plan_head, const int32_t* plan,
+                       float scale, int dtype, void* out, void* workspace, size_t workspace_bytes,
+                       cudaStream_t stream);
+
+/*
+ * Logits controls of a verify round or a decode step: penalties for repeated tokens,
+ * biases and grammar masks, in float32. Request i owns logits rows [cu_q[i], cu_q[i+1])
+ * (cu_q NULL: row i) and the table row slots[i]. Row j of its chunk x_0 .. x_j
+ * (tokens[cu_q[i]..]; x_0, the newest emitted token, is counted already; tokens NULL:
+ * no proposals), for token v:
+ *   c = counts[slot][v] + #{1 <= k <= j : x_k = v},  seen = prompt bit v or c > 0
+ *   z = logit;  z = z > 0 ? z / repetition : z * repetition    where seen
+ *   z = (z - frequency * c) - presence                         where c > 0
+ *   z = z + (the request's biases of v, added in list order)
+ *   z = mask_value                      where bit v of mask row mask_index[row] is 0
+ * each step one rounded float32 operation. Tables: counts [num_slots] rows of ld_counts
+ * int16 (ld_counts even; counts saturate at 32767), prompt_bits [num_slots] rows of
+ * ld_bits 32-bit words (bit v & 31 of word v >> 5), penalties [num_slots, 3] float32
+ * (repetition > 0, frequency, presence), bias_ids / bias_values [num_slots, max_bias]
+ * with bias_len [num_slots] entries in use (max_bias 0: none); masks [num_masks] rows of
+ * ld_mask words with mask_index [rows], -1 for a row without a mask (both NULL: none).
+ * logits bf16 or float32, row stride ld. A slot, offset, token or mask index out of
+ * range is skipped and sets DSPARK_DEVICE_BAD_ARGUMENT; logits rows outside every
+ * request are neither read nor written. Device memory throughout. No reference
+ * counterpart (the reference samples the raw logits, tensor_sampling.py:38-51).
+ *
+ * dspark_control_logits writes z to out (row stride ld_out; out_dtype the logits' type
+ * or float32). out may be logits itself (same stride and type), else they must not
+ * overlap. dspark_control_argmax writes each row's index of the largest allowed z to
+ * pred (ties: the lowest; NaN is largest); a row whose mask allows nothing gets -1 and
+ * sets DSPARK_DEVICE_EMPTY_MASK. scratch: dspark_control_argmax_scratch_bytes(rows,
+ * vocab) bytes, 8-byte aligned, never needing a clear, one per call in flight.
+ *
+ * dspark_control_tokens adds tokens[cu[i] .. cu[i+1]), cut to n[i] where n is not NULL,
+ * to table row slots[i]: to the counts, or (counts NULL) to the prompt bits; with
+ * dspark_greedy_accept's emitted, cu_q and n_commit it commits a round's tokens.
+ */
+int dspark_control_logits(const void* logits, long long ld, int dtype, int rows, int vocab, const int32_t* cu_q,
+                          const long long* tokens, const int32_t* slots, int num_requests, const int16_t* counts,
+                          long long ld_counts, const uint32_t* prompt_bits, long long ld_bits, const float* penalties,
+                          int num_slots, const int32_t* bias_ids, const float* bias_values, const int32_t* bias_len,
+                          int max_bias, const uint32_t* masks, long long ld_mask, int num_masks,
+                          const int32_t* mask_index, float mask_value, void* out, long long ld_out, int out_dtype,
+                          cudaStream_t stream);
+size_t dspark_control_argmax_scratch_bytes(int rows, int vocab);
+int dspark_control_argmax(const void* logits, long long ld, int dtype, int rows, int vocab, const int32_t* cu_q,
+                          const long long* tokens, const int32_t* slots, int num_requests, const int16_t* counts,
+                          long long ld_counts, const uint32_t* prompt_bits, long long ld_bits, const float* penalties,
+                          int num_slots, const int32_t* bias_ids, const float* bias_values, const int32_t* bias_len,
+                          int max_bias, const uint32_t* masks, long long ld_mask, int num_masks,
+                          const int32_t* mask_index, int32_t* pred, void* scratch, size_t scratch_bytes,
+                          cudaStream_t stream);
+int dspark_control_tokens(const long long* tokens, int num_tokens, const int32_t* cu, const int32_t* n,
+                          const int32_t* slots, int num_requests, int vocab, int num_slots, int16_t* counts,
+                          long long ld_counts, uint32_t* prompt_bits, long long ld_bits, cudaStream_t stream);
 
 /*
  * Allocation-free variant of dspark_varlen_attn (bf16 only). No counterpart in

@@ -7,6 +7,10 @@ Drop-in replacements for the two attention hot paths of qwen3-dspark:
   ``B200CapacityKernel``, and ``B200PersistentTargetKV`` with the fused
   QK-norm + RoPE + KV-append verify layer and one-launch commit/rollback.
 
+Beside them: attention of requests that share long prefixes (``B200SharedPrefixKernel``
+with ``SharedPrefixLayout``) and penalties, biases and grammar masks on the logits
+(``TokenControls``, ``control_logits``, ``control_argmax``).
+
 The kernels live in ``lib/libdspark_b200.so`` (C ABI, include/dspark_b200.h),
 built from ``csrc/`` by ``build.py``. Importing this package does not touch
 the GPU; constructing a kernel object loads the library and fails loudly if it
@@ -15,11 +19,12 @@ is missing or the device is not an sm_100 GPU.
 from . import _lib
 from .build import LIB_PATH, build
 from .kernels import (add_rms_norm, BACKEND, CAPACITY_BACKEND, DRAFT_BACKEND, SCALE, TRAIN_BACKEND, B200CapacityKernel,
-                      B200DraftKernel, B200TrainingLayoutKernel, B200VarlenKernel, draft_append, float64_law, greedy_accept, markov_greedy, qk_norm_rope, rms_norm, silu_mul,
+                      B200DraftKernel, B200SharedPrefixKernel, B200TrainingLayoutKernel, B200VarlenKernel, draft_append, float64_law, greedy_accept, markov_greedy, qk_norm_rope, rms_norm, silu_mul,
                       sample_rows, stochastic_accept, stochastic_propose,
                       runtime_identity, segment_attention)
 from .kv_store import B200PersistentTargetKV, Slot, Transaction, rope_inv_freq
-from .layout import PackedLayout, PersistentAttentionLayout, TrainingLayout
+from .controls import TokenControls, control_argmax, control_logits
+from .layout import PackedLayout, PersistentAttentionLayout, SharedPrefixLayout, TrainingLayout
 
 
 def __getattr__(name):
@@ -45,4 +50,5 @@ __all__ = ['add_rms_norm', 'BACKEND', 'CAPACITY_BACKEND', 'DRAFT_BACKEND', 'SCAL
            'PackedLayout', 'PersistentAttentionLayout', 'TrainingLayout', 'Slot', 'Transaction', 'B200PackedDraft',
            'DSparkDraftModel', 'DraftSpec', 'B200Qwen3Target', 'speculative_greedy', 'speculative_greedy_pipelined', 'speculative_sample', 'accept_greedy', 'build',
            'draft_append', 'float64_law', 'greedy_accept', 'markov_greedy', 'qk_norm_rope', 'rms_norm', 'silu_mul', 'sample_rows', 'stochastic_accept', 'stochastic_propose', 'launch_count', 'load_library', 'read_device_status', 'rope_inv_freq', 'runtime_identity',
-           'segment_attention']
+           'segment_attention', 'B200SharedPrefixKernel', 'SharedPrefixLayout', 'TokenControls', 'control_argmax',
+           'control_logits']

@@ -12,10 +12,14 @@ from .build import LIB_PATH
 
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F32 = 0, 1
-DEVICE_WAIT_TIMEOUT, DEVICE_BAD_SCHEDULE, DEVICE_BAD_ARGUMENT = 1, 2, 4
+DEVICE_WAIT_TIMEOUT, DEVICE_BAD_SCHEDULE, DEVICE_BAD_ARGUMENT, DEVICE_EMPTY_MASK = 1, 2, 4, 8
 VERIFY_PATHS = {'auto': -1, 'fused': 0, 'prep': 1}
 
 _vp, _i, _ll, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
+
+# logits, tables, biases and masks of the logits controls
+_CONTROL_ARGS = [_vp, _ll, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _ll, _vp, _ll, _vp, _i, _vp, _vp, _vp, _i, _vp, _ll, _i,
+                 _vp]
 
 # name -> (restype, argtypes); mirrors include/dspark_b200.h
 SIGNATURES = {
@@ -54,6 +58,15 @@ SIGNATURES = {
     'dspark_stochastic_scratch_bytes': (_sz, [_i]),
     'dspark_stochastic_accept': (_i, [_vp, _ll, _i, _i, ctypes.c_double, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _i,
                                       _vp, _vp, _vp, _vp, _sz, _vp]),
+    'dspark_prefix_plan': (_i, [_i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _ll,
+                                ctypes.POINTER(_ll)]),
+    'dspark_prefix_workspace_bytes': (_sz, [_vp]),
+    'dspark_prefix_attn': (_i, [_vp, _i, _vp, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _vp, _f, _i,
+                                _vp, _vp, _sz, _vp]),
+    'dspark_control_logits': (_i, _CONTROL_ARGS + [_f, _vp, _ll, _i, _vp]),
+    'dspark_control_argmax_scratch_bytes': (_sz, [_i, _i]),
+    'dspark_control_argmax': (_i, _CONTROL_ARGS + [_vp, _vp, _sz, _vp]),
+    'dspark_control_tokens': (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _ll, _vp, _ll, _vp]),
     'dspark_draft_append': (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _vp, _vp, _ll, _ll,
                                  _vp]),
 }
@@ -103,7 +116,8 @@ def read_device_status(clear=True):
 
 
 STATUS_NAMES = {DEVICE_WAIT_TIMEOUT: 'a bounded wait ran out', DEVICE_BAD_SCHEDULE: 'tile schedules disagreed',
-                DEVICE_BAD_ARGUMENT: 'a kernel refused an out-of-range index'}
+                DEVICE_BAD_ARGUMENT: 'a kernel refused an out-of-range index',
+                DEVICE_EMPTY_MASK: "a row's mask allowed no token"}
 
 
 def describe_status(status):
@@ -146,3 +160,27 @@ def train_plan(context_lengths, num_blocks, anchors, block_size, grid_limit):
     check(lib.dspark_train_plan(n, ctx, nb, anc, block_size, grid_limit, plan, words.value, ctypes.byref(words)),
           'dspark_train_plan')
     return list(plan)
+
+
+PREFIX_HEAD_WORDS = 32
+
+
+def prefix_plan(groups, requests, causal, grid_limit):
+    """Host-built work plan of the shared-prefix attention; no GPU needed. ``groups``: int32
+    CPU tensors (sizes, prefix starts, prefix lengths); ``requests``: (query lengths, own
+    starts, own lengths, new starts or None, new lengths or None). Returns an int32 CPU
+    tensor."""
+    import torch
+    lib = load_library()
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    words = ctypes.c_longlong(0)
+    # a guess that fits most plans saves building the plan twice
+    buf = torch.empty(1 << 15, dtype=torch.int32)
+    for _ in range(2):
+        args = (groups[0].numel(), *map(ptr, groups), requests[0].numel(), *map(ptr, requests), int(causal), grid_limit)
+        status = lib.dspark_prefix_plan(*args, buf.data_ptr(), buf.numel(), ctypes.byref(words))
+        if status == OK or words.value <= buf.numel():
+            break
+        buf = torch.empty(words.value, dtype=torch.int32)
+    check(status, 'dspark_prefix_plan')
+    return buf[:words.value].clone()

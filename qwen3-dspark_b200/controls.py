@@ -1,0 +1,221 @@
+"""Logits controls: penalties for repeated tokens, biases and grammar masks.
+
+``TokenControls`` keeps, per request slot, the tables the kernels read (how often each
+token was emitted, which tokens the prompt holds, the penalties and the biases) on the
+GPU. ``control_logits`` applies them to the logits of a verify round or decode step,
+``control_argmax`` returns each row's controlled maximum without writing the logits, and
+``TokenControls.commit`` adds a round's emitted tokens, from device tensors, so a decode
+loop never reads them back. The rows of a verified chunk see the chunk's own proposals:
+row j counts proposals 1 .. j on top of the table.
+
+The arithmetic (float32, one rounding per step; ``dspark_control_logits``):
+seen tokens (in the prompt, or emitted) are divided (positive) or multiplied by
+``repetition``; emitted ones lose ``frequency * count + presence``; biases are added in
+list order; tokens the row's mask forbids become ``mask_value``.
+"""
+import math
+
+import torch
+
+from . import _lib
+from .kernels import _DTYPES, _stream
+from .kv_store import _upload
+
+
+class TokenControls:
+    """Control tables of ``slots`` requests over a vocabulary of ``vocab`` tokens.
+
+    ``counts`` int16 [slots, vocab rounded up to 8] (saturating at 32767), ``prompt_bits``
+    int32 [slots, words] (bit ``v & 31`` of word ``v >> 5``), ``penalties`` float32
+    [slots, 3], ``bias_ids`` / ``bias_values`` [slots, max_bias] and ``bias_len`` [slots].
+    All work is on the current stream of the tables' device.
+    """
+
+    def __init__(self, slots, vocab, *, device='cuda', max_bias=0):
+        if any(type(x) is not int for x in (slots, vocab, max_bias)) or slots < 1 or vocab < 1 or max_bias < 0:
+            raise ValueError('Positive slots and vocab and a nonnegative max_bias required')
+        self.device = torch.device(device)
+        if self.device.type != 'cuda':
+            raise RuntimeError('Logits controls require a CUDA device; no CPU fallback')
+        if self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
+        self.slots, self.vocab, self.max_bias = slots, vocab, max_bias
+        self.words = (vocab + 31) // 32
+        dev = dict(device=self.device)
+        self.counts = torch.zeros((slots, (vocab + 7) // 8 * 8), dtype=torch.int16, **dev)
+        self.prompt_bits = torch.zeros((slots, self.words), dtype=torch.int32, **dev)
+        self.penalties = torch.zeros((slots, 3), dtype=torch.float32, **dev)
+        self.penalties[:, 0] = 1.0
+        self.bias_ids = torch.zeros((slots, max_bias), dtype=torch.int32, **dev)
+        self.bias_values = torch.zeros((slots, max_bias), dtype=torch.float32, **dev)
+        self.bias_len = torch.zeros(slots, dtype=torch.int32, **dev)
+        self._slots = {}
+        self._free = list(range(slots))
+
+    # -- request lifecycle -----------------------------------------------------------
+    def _ids(self, tokens, what):
+        if tokens is None:
+            return torch.empty(0, dtype=torch.long, device=self.device)
+        if not isinstance(tokens, torch.Tensor):
+            tokens = torch.tensor(list(tokens), dtype=torch.long)
+        if tokens.ndim != 1 or tokens.dtype not in (torch.long, torch.int32):
+            raise ValueError(f'{what} must be one-dimensional integer token ids')
+        if not tokens.is_cuda and tokens.numel() and not 0 <= int(tokens.min()) <= int(tokens.max()) < self.vocab:
+            raise ValueError(f'{what} holds a token outside the vocabulary')
+        return tokens.to(self.device, torch.long).contiguous()
+
+    def add_request(self, request, *, prompt=None, output=None, repetition=1.0, frequency=0.0, presence=0.0,
+                    bias=None):
+        """Take a free slot for ``request``. ``prompt`` / ``output``: its prompt tokens and the
+        tokens emitted so far (ids on the host, or integer tensors; on-device ids outside the
+        vocabulary are skipped and flagged in the device status). ``bias``: {token: value},
+        or (ids, values) whose duplicates add in order. Returns the slot."""
+        if not isinstance(request, str) or not request or request in self._slots:
+            raise ValueError('Require a fresh nonempty request name')
+        if not self._free:
+            raise ValueError('Control slots exhausted')
+        repetition, frequency, presence = float(repetition), float(frequency), float(presence)
+        if not (math.isfinite(repetition) and repetition > 0 and math.isfinite(frequency) and math.isfinite(presence)):
+            raise ValueError('repetition must be finite and positive, frequency and presence finite')
+        prompt, output = self._ids(prompt, 'prompt'), self._ids(output, 'output')
+        ids = values = None
+        if bias is not None:
+            ids, values = (list(bias.keys()), list(bias.values())) if isinstance(bias, dict) else bias
+            ids = self._ids(ids, 'bias')
+            values = torch.as_tensor(values, dtype=torch.float32).to(self.device)
+            if values.shape != ids.shape or ids.numel() > self.max_bias:
+                raise ValueError(f'bias: one value per token and at most max_bias = {self.max_bias} entries required')
+        slot = self._free.pop(0)
+        self._slots[request] = slot
+        self.counts[slot].zero_()
+        self.prompt_bits[slot].zero_()
+        self.penalties[slot].copy_(_row([repetition, frequency, presence], self.device))
+        self.bias_len[slot:slot + 1].fill_(0 if ids is None else ids.numel())
+        if ids is not None:
+            self.bias_ids[slot, :ids.numel()].copy_(ids)
+            self.bias_values[slot, :ids.numel()].copy_(values)
+        index = _upload([slot], self.device)
+        for tokens, to_counts in ((prompt, False), (output, True)):
+            if tokens.numel():
+                self._add(tokens, _upload([0, tokens.numel()], self.device), None, index, to_counts)
+        return slot
+
+    def remove_request(self, request):
+        if request not in self._slots:
+            raise KeyError(request)
+        self._free.append(self._slots.pop(request))
+        self._free.sort()
+
+    def slot_index(self, requests):
+        """int32 device tensor of the requests' slots, for the kernels' ``slots`` argument."""
+        for r in requests:
+            if r not in self._slots:
+                raise KeyError(r)
+        return _upload([self._slots[r] for r in requests], self.device)
+
+    def _add(self, tokens, cu, n, slots, to_counts):
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.load_library().dspark_control_tokens(
+                tokens.data_ptr(), tokens.numel(), cu.data_ptr(), None if n is None else n.data_ptr(),
+                slots.data_ptr(), slots.numel(), self.vocab, self.slots,
+                self.counts.data_ptr() if to_counts else None, self.counts.stride(0),
+                None if to_counts else self.prompt_bits.data_ptr(), self.prompt_bits.stride(0),
+                _stream(self.device)), 'dspark_control_tokens')
+
+    def commit(self, slots, emitted, cu_query, n_commit=None):
+        """Count a round's emitted tokens: request i's are ``emitted[cu_query[i] ..]``, the first
+        ``n_commit[i]`` of them (all without ``n_commit``); ``greedy_accept``'s outputs as they
+        are. Device tensors, no host read: capturable."""
+        r = slots.numel()
+        if (slots.dtype != torch.int32 or slots.shape != (r,) or emitted.dtype != torch.long or emitted.ndim != 1
+                or not emitted.is_contiguous() or cu_query.dtype != torch.int32 or cu_query.shape != (r + 1,)
+                or (n_commit is not None and (n_commit.dtype != torch.int32 or n_commit.shape != (r,)))
+                or any(t.device != self.device or not t.is_contiguous()
+                       for t in (slots, emitted, cu_query) + (() if n_commit is None else (n_commit,)))):
+            raise ValueError('commit: contiguous int32 [R] slots, int64 [N] emitted, int32 [R + 1] cu_query and int32 '
+                             '[R] n_commit on the tables\' device required')
+        self._add(emitted, cu_query, n_commit, slots, True)
+
+
+def _row(values, device):
+    return torch.tensor(values, dtype=torch.float32).pin_memory().to(device, non_blocking=True)
+
+
+def _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index):
+    device = controls.device
+    if (not isinstance(logits, torch.Tensor) or logits.ndim != 2 or logits.dtype not in _DTYPES
+            or logits.device != device or logits.shape[1] != controls.vocab or logits.stride(1) != 1
+            or (logits.shape[0] > 1 and logits.stride(0) < controls.vocab) or logits.requires_grad):
+        raise ValueError('logits must be no-autograd bf16/fp32 [N, vocab] rows with unit column stride on the tables\' '
+                         'device')
+    n, r = logits.shape[0], slots.numel()
+    if slots.dtype != torch.int32 or slots.ndim != 1 or slots.device != device or not slots.is_contiguous() or r < 1:
+        raise ValueError('slots must be contiguous int32 [R] on the tables\' device')
+    if cu_query is None:
+        if n != r or tokens is not None:
+            raise ValueError('Without cu_query there is one row per request, and no proposals')
+    elif (cu_query.dtype != torch.int32 or cu_query.shape != (r + 1,) or cu_query.device != device
+          or not cu_query.is_contiguous()):
+        raise ValueError('cu_query must be contiguous int32 [R + 1] on the tables\' device')
+    if tokens is not None and (tokens.dtype != torch.long or tokens.shape != (n,) or tokens.device != device
+                               or not tokens.is_contiguous()):
+        raise ValueError('tokens must be contiguous int64 [N] on the tables\' device')
+    if (masks is None) != (mask_index is None):
+        raise ValueError('masks and mask_index go together')
+    if masks is not None and (masks.dtype != torch.int32 or masks.ndim != 2 or masks.shape[1] < controls.words
+                              or masks.shape[0] < 1 or masks.stride(1) != 1 or masks.stride(0) < controls.words
+                              or masks.device != device or mask_index.dtype != torch.int32
+                              or mask_index.shape != (n,) or mask_index.device != device
+                              or not mask_index.is_contiguous()):
+        raise ValueError('masks must be int32 [M, ceil(vocab / 32)] and mask_index int32 [N] on the tables\' device')
+    c = controls
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    return [logits.data_ptr(), max(logits.stride(0), c.vocab), _DTYPES[logits.dtype], n, c.vocab, ptr(cu_query),
+            ptr(tokens), slots.data_ptr(), r, c.counts.data_ptr(), c.counts.stride(0), c.prompt_bits.data_ptr(),
+            c.prompt_bits.stride(0), c.penalties.data_ptr(), c.slots, c.bias_ids.data_ptr() if c.max_bias else None,
+            c.bias_values.data_ptr() if c.max_bias else None, c.bias_len.data_ptr(), c.max_bias, ptr(masks),
+            0 if masks is None else masks.stride(0), 0 if masks is None else masks.shape[0], ptr(mask_index)]
+
+
+def control_logits(logits, controls, slots, *, cu_query=None, tokens=None, masks=None, mask_index=None,
+                   mask_value=float('-inf'), out=None, out_dtype=None):
+    """Controlled logits of a verify round or decode step (``dspark_control_logits``).
+
+    ``logits`` [N, vocab] bf16/fp32 (rows may be strided); ``slots`` int32 [R] from
+    ``controls.slot_index``; ``cu_query`` int32 [R + 1] the requests' rows (without it: one row
+    per request); ``tokens`` int64 [N] the verified chunks (anchor, then proposals), as in
+    ``greedy_accept``. ``masks`` int32 [M, ceil(vocab / 32)] grammar masks (bit set: allowed)
+    and ``mask_index`` int32 [N] the row of each logits row, -1 for none. Returns [N, vocab] in
+    ``out_dtype`` (the logits' dtype or float32); ``out=logits`` changes them in place.
+    ``mask_value`` replaces forbidden logits: a finite one (``torch.finfo(dtype).min``) keeps
+    the rows acceptable to ``stochastic_accept``, which refuses infinities."""
+    args = _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=out_dtype or logits.dtype, device=logits.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError('out has another dtype than out_dtype')
+    if (out.shape != logits.shape or out.device != logits.device or out.stride(1) != 1
+            or (len(out) > 1 and out.stride(0) < controls.vocab)
+            or out.dtype not in (logits.dtype, torch.float32)):
+        raise ValueError('out must be [N, vocab] rows of the logits\' dtype or float32 on their device')
+    with torch.cuda.device(logits.device):
+        _lib.check(_lib.load_library().dspark_control_logits(
+            *args, float(mask_value), out.data_ptr(), max(out.stride(0), controls.vocab), _DTYPES[out.dtype],
+            _stream(logits.device)), 'dspark_control_logits')
+    return out
+
+
+def control_argmax(logits, controls, slots, *, cu_query=None, tokens=None, masks=None, mask_index=None):
+    """Index of each row's largest controlled logit, int32 [N] (``dspark_control_argmax``): the
+    arguments of ``control_logits``, nothing written but the indices. Ties give the lowest
+    index, NaN is largest, and a row whose mask allows nothing gives -1 and sets the
+    device status bit ``DEVICE_EMPTY_MASK``."""
+    args = _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index)
+    lib = _lib.load_library()
+    with torch.cuda.device(logits.device):
+        pred = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
+        nbytes = int(lib.dspark_control_argmax_scratch_bytes(*logits.shape))
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+        _lib.check(lib.dspark_control_argmax(*args, pred.data_ptr(), scratch.data_ptr(), nbytes,
+                                             _stream(logits.device)), 'dspark_control_argmax')
+    return pred

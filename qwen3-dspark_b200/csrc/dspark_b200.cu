@@ -18,8 +18,10 @@
 #include "accept.cuh"
 #include "append.cuh"
 #include "attention.cuh"
+#include "controls.cuh"
 #include "markov.cuh"
 #include "norm.cuh"
+#include "prefix.cuh"
 #include "sampling.cuh"
 #include "train.cuh"
 #include "verify.cuh"
@@ -314,6 +316,62 @@ int encode_rows_map(CUtensorMap* m, const void* base, long long rows, int heads,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? DSPARK_OK : DSPARK_ERR_CUDA;
+}
+
+}  // namespace
+
+namespace {
+
+bool control_params(controls::Params& p, const void* logits, long long ld, int dtype, int rows, int vocab,
+                    const int32_t* cu_q, const long long* tokens, const int32_t* slots, int num_requests,
+                    const int16_t* counts, long long ld_counts, const uint32_t* prompt_bits, long long ld_bits,
+                    const float* penalties, int num_slots, const int32_t* bias_ids, const float* bias_values,
+                    const int32_t* bias_len, int max_bias, const uint32_t* masks, long long ld_mask, int num_masks,
+                    const int32_t* mask_index) {
+  const int words = (vocab + 31) / 32;
+  const size_t align = dtype == DSPARK_DTYPE_F32 ? 4 : 2;
+  if ((dtype != DSPARK_DTYPE_BF16 && dtype != DSPARK_DTYPE_F32) || !logits || !aligned(logits, align) || vocab < 1 ||
+      vocab > (1 << 30) || ld < vocab || rows < 1 || !slots || num_requests < 1 || (!cu_q && num_requests > rows) ||
+      !counts || !aligned(counts, 4) || ld_counts < vocab || ld_counts % 2 != 0 || !prompt_bits || ld_bits < words ||
+      !penalties || num_slots < 1 || max_bias < 0 || (max_bias > 0 && (!bias_ids || !bias_values || !bias_len)) ||
+      (masks != nullptr) != (mask_index != nullptr) || (masks && (ld_mask < words || num_masks < 1)))
+    return false;
+  p.logits = logits;
+  p.ld = ld;
+  p.rows = rows;
+  p.vocab = vocab;
+  p.cu_q = cu_q;
+  p.tokens = tokens;
+  p.slots = slots;
+  p.num_requests = num_requests;
+  p.counts = counts;
+  p.ld_counts = ld_counts;
+  p.prompt_bits = prompt_bits;
+  p.ld_bits = ld_bits;
+  p.penalties = penalties;
+  p.num_slots = num_slots;
+  p.bias_ids = max_bias > 0 ? bias_ids : nullptr;
+  p.bias_values = bias_values;
+  p.bias_len = bias_len;
+  p.max_bias = max_bias;
+  p.masks = masks;
+  p.ld_mask = ld_mask;
+  p.num_masks = num_masks;
+  p.mask_index = mask_index;
+  p.chunks = (vocab + controls::kChunk - 1) / controls::kChunk;
+  return static_cast<long long>(p.chunks) * num_requests < (1ll << 31);
+}
+
+bool rows_aligned(const void* base, long long ld, int size) { return aligned(base, 16) && ld * size % 16 == 0; }
+
+template <typename TIn, typename TOut, bool kArgmax>
+int launch_control(const controls::Params& p, bool vec, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(p.chunks) * static_cast<unsigned>(p.num_requests);
+  if (vec)
+    controls::control_kernel<TIn, TOut, kArgmax, true><<<grid, controls::kThreads, 0, stream>>>(p);
+  else
+    controls::control_kernel<TIn, TOut, kArgmax, false><<<grid, controls::kThreads, 0, stream>>>(p);
+  return launch_status();
 }
 
 }  // namespace
@@ -1044,6 +1102,160 @@ int dspark_train_attn(const void* q, const void* k, const void* v, int total_q, 
   train::train_attn_kernel<<<grid, train::kThreads, train::kSmemBytes, stream>>>(
       qm, km, vm, plan, static_cast<__nv_bfloat16*>(out), total_q, static_cast<int>(total_k),
       scale * 1.4426950408889634f);
+  return launch_status();
+}
+
+int dspark_prefix_plan(int num_groups, const int32_t* group_size, const int32_t* prefix_start,
+                       const int32_t* prefix_len, int num_requests, const int32_t* q_len, const int32_t* own_start,
+                       const int32_t* own_len, const int32_t* new_start, const int32_t* new_len, int causal,
+                       int grid_limit, int32_t* plan, long long plan_capacity, long long* plan_words) {
+  if (num_groups < 1 || num_requests < 1 || !group_size || !prefix_start || !prefix_len || !q_len || !own_start ||
+      !own_len || (new_start == nullptr) != (new_len == nullptr) || (causal != 0 && causal != 1) || grid_limit < 1 ||
+      grid_limit > 65535 || !plan_words)
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  try {
+    std::vector<int32_t> words;
+    const prefix::PlanInput in{num_groups, group_size, prefix_start, prefix_len, num_requests, q_len, own_start,
+                               own_len, new_start, new_len, causal == 1, grid_limit};
+    const int st = prefix::build_plan(in, words);
+    if (st == prefix::kPlanInvalid) return DSPARK_ERR_INVALID_ARGUMENT;
+    if (st != prefix::kPlanOk) return DSPARK_ERR_UNSUPPORTED;
+    *plan_words = static_cast<long long>(words.size());
+    if (plan_capacity < *plan_words) return plan == nullptr ? DSPARK_OK : DSPARK_ERR_INVALID_ARGUMENT;
+    if (plan != nullptr) std::copy(words.begin(), words.end(), plan);
+    return DSPARK_OK;
+  } catch (const std::bad_alloc&) {
+    return DSPARK_ERR_UNSUPPORTED;
+  }
+}
+
+size_t dspark_prefix_workspace_bytes(const int32_t* plan_head) {
+  if (plan_head == nullptr || plan_head[prefix::kHMagic] != prefix::kPlanMagic) return 0;
+  return prefix::workspace_bytes(plan_head[prefix::kHSlots]);
+}
+
+int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const void* prefix_v,
+                       long long prefix_rows, long long prefix_off, const void* own_k, const void* own_v,
+                       long long own_rows, long long own_off, const void* new_k, const void* new_v,
+                       long long new_rows, long long new_off, const int32_t* plan_head, const int32_t* plan,
+                       float scale, int dtype, void* out, void* workspace, size_t workspace_bytes,
+                       cudaStream_t stream) {
+  using namespace prefix;
+  if (!plan_head || !plan || !aligned(plan, 16) || plan_head[kHMagic] != kPlanMagic || total_q < 0 ||
+      total_q != plan_head[kHTotalQ] || !(scale > 0.f) || (dtype != DSPARK_DTYPE_BF16 && dtype != DSPARK_DTYPE_F32))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  if (total_q == 0) return DSPARK_OK;
+  const size_t align = dtype == DSPARK_DTYPE_F32 ? 4 : 16;
+  if (!q || !out || !aligned(q, align) || !aligned(out, align)) return DSPARK_ERR_INVALID_ARGUMENT;
+  Params p{};
+  p.q = q;
+  p.out = out;
+  p.plan = plan;
+  p.check = plan_head[kHCheck];
+  p.total_q = total_q;
+  p.grid = plan_head[kHGrid];
+  p.slots = plan_head[kHSlots];
+  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.src[0] = Source{prefix_k, prefix_v, prefix_off, prefix_rows};
+  p.src[1] = Source{own_k, own_v, own_off, own_rows};
+  p.src[2] = Source{new_k, new_v, new_off, new_rows};
+  for (int s = 0; s < 3; ++s) {
+    const long long need = plan_head[kHPrefixRows + s];
+    const Source& x = p.src[s];
+    if (need == 0) continue;                     // the plan reads nothing from this source
+    if (!x.k || !x.v || !aligned(x.k, align) || !aligned(x.v, align) || x.off < 0 || x.rows >= (1ll << 31) ||
+        x.off > x.rows - need)
+      return DSPARK_ERR_INVALID_ARGUMENT;
+  }
+  DeviceInfo dev;
+  const int st = current_device_info(&dev);
+  if (st != DSPARK_OK) return st;
+  const int max_q = plan_head[kHMaxQ];
+  const dim3 grid(plan_head[kHRequests], (max_q + kQBlock - 1) / kQBlock, kKVHeads);
+  if (grid.y > 65535) return DSPARK_ERR_UNSUPPORTED;
+  if (dtype == DSPARK_DTYPE_F32)
+    prefix_simple_kernel<float><<<grid, kSimpleThreads, 0, stream>>>(p);
+  else
+    prefix_simple_kernel<__nv_bfloat16><<<grid, kSimpleThreads, 0, stream>>>(p);
+  return launch_status();
+}
+
+int dspark_control_logits(const void* logits, long long ld, int dtype, int rows, int vocab, const int32_t* cu_q,
+                          const long long* tokens, const int32_t* slots, int num_requests, const int16_t* counts,
+                          long long ld_counts, const uint32_t* prompt_bits, long long ld_bits, const float* penalties,
+                          int num_slots, const int32_t* bias_ids, const float* bias_values, const int32_t* bias_len,
+                          int max_bias, const uint32_t* masks, long long ld_mask, int num_masks,
+                          const int32_t* mask_index, float mask_value, void* out, long long ld_out, int out_dtype,
+                          cudaStream_t stream) {
+  if (rows == 0) return DSPARK_OK;
+  controls::Params p{};
+  if (!control_params(p, logits, ld, dtype, rows, vocab, cu_q, tokens, slots, num_requests, counts, ld_counts,
+                      prompt_bits, ld_bits, penalties, num_slots, bias_ids, bias_values, bias_len, max_bias, masks,
+                      ld_mask, num_masks, mask_index) ||
+      !out || ld_out < vocab || (out_dtype != dtype && out_dtype != DSPARK_DTYPE_F32) ||
+      !aligned(out, out_dtype == DSPARK_DTYPE_F32 ? 4 : 2))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  const int in_size = dtype == DSPARK_DTYPE_F32 ? 4 : 2, out_size = out_dtype == DSPARK_DTYPE_F32 ? 4 : 2;
+  // the output is the input itself (same rows, same type) or shares no byte with it
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(logits), b0 = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t a1 = a0 + (static_cast<uintptr_t>(rows - 1) * ld + vocab) * in_size;
+  const uintptr_t b1 = b0 + (static_cast<uintptr_t>(rows - 1) * ld_out + vocab) * out_size;
+  p.in_place = a0 == b0 && ld == ld_out && dtype == out_dtype;
+  if (!p.in_place && a0 < b1 && b0 < a1) return DSPARK_ERR_INVALID_ARGUMENT;
+  p.mask_value = mask_value;
+  p.out = out;
+  p.ld_out = ld_out;
+  const bool vec = rows_aligned(logits, ld, in_size) && rows_aligned(out, ld_out, out_size) &&
+                   rows_aligned(counts, ld_counts, 2);
+  if (dtype == DSPARK_DTYPE_F32) return launch_control<float, float, false>(p, vec, stream);
+  if (out_dtype == DSPARK_DTYPE_F32) return launch_control<__nv_bfloat16, float, false>(p, vec, stream);
+  return launch_control<__nv_bfloat16, __nv_bfloat16, false>(p, vec, stream);
+}
+
+size_t dspark_control_argmax_scratch_bytes(int rows, int vocab) {
+  if (rows < 0 || vocab < 1) return 0;
+  return static_cast<size_t>(rows) * ((static_cast<size_t>(vocab) + controls::kChunk - 1) / controls::kChunk) *
+         sizeof(unsigned long long);
+}
+
+int dspark_control_argmax(const void* logits, long long ld, int dtype, int rows, int vocab, const int32_t* cu_q,
+                          const long long* tokens, const int32_t* slots, int num_requests, const int16_t* counts,
+                          long long ld_counts, const uint32_t* prompt_bits, long long ld_bits, const float* penalties,
+                          int num_slots, const int32_t* bias_ids, const float* bias_values, const int32_t* bias_len,
+                          int max_bias, const uint32_t* masks, long long ld_mask, int num_masks,
+                          const int32_t* mask_index, int32_t* pred, void* scratch, size_t scratch_bytes,
+                          cudaStream_t stream) {
+  if (rows == 0) return DSPARK_OK;
+  controls::Params p{};
+  if (!control_params(p, logits, ld, dtype, rows, vocab, cu_q, tokens, slots, num_requests, counts, ld_counts,
+                      prompt_bits, ld_bits, penalties, num_slots, bias_ids, bias_values, bias_len, max_bias, masks,
+                      ld_mask, num_masks, mask_index) ||
+      !pred || !aligned(pred, 4) || !scratch || !aligned(scratch, 8) ||
+      scratch_bytes < dspark_control_argmax_scratch_bytes(rows, vocab))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  p.part = static_cast<unsigned long long*>(scratch);
+  p.pred = pred;
+  const bool vec = rows_aligned(logits, ld, dtype == DSPARK_DTYPE_F32 ? 4 : 2) && rows_aligned(counts, ld_counts, 2);
+  const int st = dtype == DSPARK_DTYPE_F32 ? launch_control<float, float, true>(p, vec, stream)
+                                           : launch_control<__nv_bfloat16, __nv_bfloat16, true>(p, vec, stream);
+  if (st != DSPARK_OK) return st;
+  controls::control_argmax_finish_kernel<<<num_requests, 128, 0, stream>>>(p);
+  return launch_status();
+}
+
+int dspark_control_tokens(const long long* tokens, int num_tokens, const int32_t* cu, const int32_t* n,
+                          const int32_t* slots, int num_requests, int vocab, int num_slots, int16_t* counts,
+                          long long ld_counts, uint32_t* prompt_bits, long long ld_bits, cudaStream_t stream) {
+  if (num_tokens < 0 || num_requests < 0 || vocab < 1 || num_slots < 1 || (counts == nullptr) == (prompt_bits == nullptr) ||
+      (counts && (!aligned(counts, 4) || ld_counts < vocab || ld_counts % 2 != 0)) ||
+      (prompt_bits && ld_bits < (vocab + 31) / 32))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  if (num_tokens == 0 || num_requests == 0) return DSPARK_OK;
+  if (!tokens || !cu || !slots) return DSPARK_ERR_INVALID_ARGUMENT;
+  const controls::TokenParams tp{tokens, cu, n, slots, num_tokens, num_slots, vocab, counts, ld_counts, prompt_bits,
+                                 ld_bits};
+  controls::control_tokens_kernel<<<num_requests, 256, 0, stream>>>(tp);
   return launch_status();
 }
 

@@ -14,6 +14,7 @@ enum : unsigned {
   kStatusWaitTimeout = 1u << 0,   // an mbarrier wait ran past its time limit
   kStatusBadSchedule = 1u << 1,   // producer/consumer tile walks disagreed
   kStatusBadArgument = 1u << 2,   // a device-side bounds check rejected an index
+  kStatusEmptyMask = 1u << 3,     // a row whose grammar mask allows no token
 };
 __device__ unsigned int g_device_status;
 

@@ -15,6 +15,8 @@ no fallback, retry or split tuning.
 * ``B200TrainingLayoutKernel`` - the training-layout draft attention of
   ``DraftAttention.forward`` + ``block_mask`` (model.py:12-19,47-61) for packed
   sequences, on the tcgen05 tensor cores
+* ``B200SharedPrefixKernel`` - attention of requests that share long prefixes, each
+  prefix row read once per 128 query rows of its group instead of once per request
 
 bf16 runs on the tensor-core kernel; float32 inputs (the reference's exact CPU
 configurations) run on the library's float32 CUDA-core kernel.
@@ -31,6 +33,7 @@ BACKEND = 'b200_sm100a_varlen_causal_v1'
 DRAFT_BACKEND = 'b200_sm100a_noncausal_v1'
 CAPACITY_BACKEND = 'b200_sm100a_capacity_causal_v1'
 TRAIN_BACKEND = 'b200_sm100a_train_layout_tcgen05_v1'
+PREFIX_BACKEND = 'b200_sm100a_shared_prefix_tcgen05_v1'
 HQ, HKV, HEAD_DIM = 16, 8, 128
 SCALE = HEAD_DIM ** -0.5
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
@@ -205,6 +208,74 @@ class B200TrainingLayoutKernel:
         out = torch.empty_like(query)
         self._operator(query.data_ptr(), key.data_ptr(), value.data_ptr(), query.shape[0], key.shape[0],
                        layout.plan.data_ptr(), layout.grid, float(scale), out.data_ptr(), _stream(self.device))
+        return out
+
+
+class B200SharedPrefixKernel:
+    """Attention of requests that share long prefixes (``dspark_prefix_attn``).
+
+    ``kernel(query, key, value, layout, *, scale, prefix_key, prefix_value, new_key=None,
+    new_value=None)`` with a ``SharedPrefixLayout``: ``query`` [sum q, 16, 128];
+    ``prefix_key``/``prefix_value`` the groups' shared rows, ``key``/``value`` the requests'
+    own cached rows and ``new_key``/``new_value`` their new rows, each [rows, 8, 128] and
+    read in place (they may be the same tensor). ``prefix_off``/``own_off``/``new_off`` are
+    the source rows at which the layout's row 0 lies, so one layout serves every layer
+    of a store. Contiguous tensors of one dtype on the kernel's GPU: bf16 (tensor cores)
+    or float32 (CUDA cores). A row without a visible key gives zeros. ``out`` (default: a
+    new tensor) may be ``query`` itself.
+
+    bf16 partial rows live in a workspace that each call allocates on its own stream, so
+    calls on different streams and in different captured graphs share nothing.
+    """
+    backend_name = PREFIX_BACKEND
+    native_varlen_calls_per_layer = 1
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+        if self.device.type == 'cuda' and self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
+        self.runtime = runtime_identity(self.device)
+        self._operator = _NativeEntry('dspark_prefix_attn')
+
+    def __call__(self, query, key, value, layout, *, scale, prefix_key, prefix_value, new_key=None, new_value=None,
+                 prefix_off=0, own_off=0, new_off=0, out=None):
+        device, dtype = self.device, query.dtype
+        if (new_key is None) != (new_value is None):
+            raise ValueError('B200 shared prefix requires new_key and new_value together')
+        sources = [(prefix_key, prefix_value), (key, value)] + ([(new_key, new_value)] if new_key is not None else [])
+        for t in (query, *(x for pair in sources for x in pair)) + ((out,) if out is not None else ()):
+            if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or dtype not in _DTYPES
+                    or t.requires_grad or t.ndim != 3 or not t.is_contiguous()):
+                raise ValueError('B200 shared prefix requires no-autograd contiguous BF16 (or FP32) THD tensors on '
+                                 'its GPU')
+        if query.shape[1:] != (HQ, HEAD_DIM) or (out is not None and out.shape != query.shape):
+            raise ValueError('B200 shared prefix supports Hq16/Hkv8/D128 Qwen tensors only')
+        if any(k.shape[1:] != (HKV, HEAD_DIM) or v.shape != k.shape for k, v in sources):
+            raise ValueError('B200 shared prefix supports Hq16/Hkv8/D128 Qwen tensors only')
+        if not isinstance(scale, (float, int)) or not math.isfinite(scale) or scale != SCALE:
+            raise ValueError('B200 shared prefix requires the 1/sqrt(128) scale')
+        if not hasattr(layout, 'workspace_bytes') or len(query) != layout.query_tokens or layout.plan.device != device:
+            raise ValueError('Query rows must match the shared-prefix layout on this device')
+        offs = (prefix_off, own_off, new_off)
+        need = (layout.prefix_rows, layout.own_rows, layout.new_rows)
+        rows = [len(k) for k, _ in sources] + [0] * (3 - len(sources))
+        if any(type(o) is not int or o < 0 or (n > 0 and o + n > r) for o, n, r in zip(offs, need, rows)):
+            raise ValueError('A key source holds fewer rows than the layout reads at its offset')
+        if out is None:
+            out = torch.empty_like(query)
+        if layout.query_tokens == 0:
+            return out
+        args = []
+        for (k, v), off in zip(sources, offs):
+            args += [k.data_ptr(), v.data_ptr(), len(k), off]
+        if len(sources) < 3:
+            args += [None, None, 0, 0]
+        nbytes = layout.workspace_bytes if dtype == torch.bfloat16 else 0
+        with torch.cuda.device(device):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+            self._operator(query.data_ptr(), len(query), *args, layout.head.data_ptr(), layout.plan.data_ptr(),
+                           float(scale), _DTYPES[dtype], out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
+                           _stream(device))
         return out
 
 

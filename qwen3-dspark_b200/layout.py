@@ -189,6 +189,90 @@ class TrainingLayout:
         return sum(self.key_lengths)
 
 
+@dataclass(frozen=True)
+class SharedPrefixLayout:
+    """Packed layout of requests that share long prefixes.
+
+    Group g is a run of ``group_sizes[g]`` consecutive requests whose keys begin with the
+    same ``prefix_lengths[g]`` rows (from row ``prefix_starts[g]`` of the prefix source).
+    Behind them request i has ``own_lengths[i]`` cached rows (from ``own_starts[i]`` of the
+    own source) and, with ``new_lengths``, that many new rows (from ``new_starts[i]`` of
+    the new source). Starts default to back-to-back packing. With ``causal`` (bottom
+    right) row r of a request with q query rows and n keys sees keys ``j <= n - q + r``,
+    and its own + new rows must number at least q. Lengths may be zero.
+
+    ``plan`` is the kernel's work plan (``dspark_prefix_plan``), built once on the host and
+    kept on the device: build the layout once per round and use it for every layer.
+    ``head`` holds the plan's first words on the host.
+    """
+    prefix_lengths: tuple
+    group_sizes: tuple
+    query_lengths: tuple
+    own_lengths: tuple
+    new_lengths: tuple
+    causal: bool
+    plan: torch.Tensor
+    head: torch.Tensor
+    query_tokens: int
+    prefix_rows: int       # rows of each source that the plan reaches
+    own_rows: int
+    new_rows: int
+    workspace_bytes: int
+
+    @classmethod
+    def from_lengths(cls, prefix_lengths, group_sizes, query_lengths, own_lengths, new_lengths=None, *,
+                     prefix_starts=None, own_starts=None, new_starts=None, causal=True, device='cuda',
+                     grid_limit=None):
+        from . import _lib
+
+        def ints(values, n, what):
+            out = [int(x) for x in values]
+            if len(out) != n or any(not 0 <= x < 2 ** 30 for x in out):
+                raise ValueError(f'{what}: {n} nonnegative integers below 2^30 required')
+            return out
+
+        def starts(values, lengths, what):
+            if values is not None:
+                return ints(values, len(lengths), what)
+            out = [0]
+            for x in lengths[:-1]:
+                out.append(out[-1] + x)
+            return ints(out, len(lengths), what)
+
+        groups, requests = len(group_sizes), len(query_lengths)
+        if groups < 1 or requests < 1:
+            raise ValueError('At least one group and one request required')
+        sizes = ints(group_sizes, groups, 'group_sizes')
+        if min(sizes) < 1 or sum(sizes) != requests:
+            raise ValueError('group_sizes must be positive and sum to the number of requests')
+        plen = ints(prefix_lengths, groups, 'prefix_lengths')
+        qlen = ints(query_lengths, requests, 'query_lengths')
+        own = ints(own_lengths, requests, 'own_lengths')
+        if new_lengths is None and new_starts is not None:
+            raise ValueError('new_starts needs new_lengths')
+        new = [0] * requests if new_lengths is None else ints(new_lengths, requests, 'new_lengths')
+        if type(causal) is not bool:
+            raise ValueError('causal must be a bool')
+        if causal and any(a + b < q for a, b, q in zip(own, new, qlen)):
+            raise ValueError('A causal request needs at least its query rows among its own and new rows')
+        device = torch.device(device)
+        if grid_limit is None:
+            grid_limit = torch.cuda.get_device_properties(device).multi_processor_count
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+        plan = _lib.prefix_plan(
+            (i32(sizes), i32(starts(prefix_starts, plen, 'prefix_starts')), i32(plen)),
+            (i32(qlen), i32(starts(own_starts, own, 'own_starts')), i32(own),
+             None if new_lengths is None else i32(starts(new_starts, new, 'new_starts')),
+             None if new_lengths is None else i32(new)), causal, int(grid_limit))
+        head = plan[:_lib.PREFIX_HEAD_WORDS].clone()
+        rows = head[12:15].tolist()
+        nbytes = int(_lib.load_library().dspark_prefix_workspace_bytes(head.data_ptr()))
+        if device.type == 'cuda':
+            plan = plan.pin_memory().to(device, non_blocking=True)
+        return cls(tuple(plen), tuple(sizes), tuple(qlen), tuple(own), tuple(new), causal, plan, head, sum(qlen),
+                   *rows, nbytes)
+
+
 def cumulative(lengths, device):
     ends = [0]
     for n in lengths:
