@@ -71,7 +71,8 @@ int device_info(int dev, DeviceInfo* out) {
       return DSPARK_ERR_CUDA;
     if (d.cc_major != 10) return DSPARK_ERR_UNSUPPORTED;   // built for sm_100a only
     if (static_cast<size_t>(d.max_smem_optin) < kAttnSmemBytes ||
-        static_cast<size_t>(d.max_smem_optin) < train::kSmemBytes)
+        static_cast<size_t>(d.max_smem_optin) < train::kSmemBytes ||
+        static_cast<size_t>(d.max_smem_optin) < prefix::kSmemBytes)
       return DSPARK_ERR_UNSUPPORTED;
     int cur = -1;
     cudaGetDevice(&cur);
@@ -82,6 +83,8 @@ int device_info(int dev, DeviceInfo* out) {
                              static_cast<int>(kAttnSmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(attn_bf16_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(kAttnSmemBytes)) != cudaSuccess ||
+        cudaFuncSetAttribute(prefix::prefix_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(prefix::kSmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(train::train_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(train::kSmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(markov::markov_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1171,13 +1174,47 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   DeviceInfo dev;
   const int st = current_device_info(&dev);
   if (st != DSPARK_OK) return st;
-  const int max_q = plan_head[kHMaxQ];
-  const dim3 grid(plan_head[kHRequests], (max_q + kQBlock - 1) / kQBlock, kKVHeads);
-  if (grid.y > 65535) return DSPARK_ERR_UNSUPPORTED;
-  if (dtype == DSPARK_DTYPE_F32)
+  if (dtype == DSPARK_DTYPE_F32) {
+    const int max_q = plan_head[kHMaxQ];
+    const dim3 grid(plan_head[kHRequests], (max_q + kQBlock - 1) / kQBlock, kKVHeads);
+    if (grid.y > 65535) return DSPARK_ERR_UNSUPPORTED;
     prefix_simple_kernel<float><<<grid, kSimpleThreads, 0, stream>>>(p);
-  else
-    prefix_simple_kernel<__nv_bfloat16><<<grid, kSimpleThreads, 0, stream>>>(p);
+    return launch_status();
+  }
+  if (p.slots > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < prefix::workspace_bytes(p.slots)))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  Maps maps;
+  int rc = encode_rows_map(&maps.q, q, total_q, kQHeads, 2, kHalfTile);
+  if (rc != DSPARK_OK) return rc;
+  for (int s = 0; s < 3; ++s) {
+    const Source& x = p.src[s];
+    if (plan_head[kHPrefixRows + s] == 0) {      // never read
+      maps.kv[2 * s] = maps.kv[2 * s + 1] = maps.q;
+      continue;
+    }
+    if ((rc = encode_rows_map(&maps.kv[2 * s], x.k, x.rows, kKVHeads, 1, kBoxRows)) != DSPARK_OK) return rc;
+    if ((rc = encode_rows_map(&maps.kv[2 * s + 1], x.v, x.rows, kKVHeads, 1, kBoxRows)) != DSPARK_OK) return rc;
+  }
+  float* part = static_cast<float*>(workspace);
+  prefix_attn_kernel<<<p.grid, kAttThreads, prefix::kSmemBytes, stream>>>(maps, p, part);
+  rc = launch_status();
+  if (rc != DSPARK_OK || p.slots == 0) return rc;
+  // the merge as a programmatic dependent: its CTAs are resident when the attention ends
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(total_q) * kQHeads + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const float* cpart = part;
+  if (cudaLaunchKernelEx(&cfg, prefix_merge_kernel, p, cpart) != cudaSuccess) {
+    cudaGetLastError();
+    cfg.numAttrs = 0;
+    if (cudaLaunchKernelEx(&cfg, prefix_merge_kernel, p, cpart) != cudaSuccess) return DSPARK_ERR_CUDA;
+  }
   return launch_status();
 }
 
