@@ -26,12 +26,14 @@ struct Params {
   const void* q;     // [total_q, 16, 128]
   void* out;
   const int* plan;
-  int check, total_q, grid, slots;
+  int check, total_q, grid, slots, items_at;
   Source src[3];     // prefix, own, new
   float scale, scale_log2;
 };
 
-// Partial rows of one MMA tile: [128][128] fp32 (normalised), then 128 log2-sum-exp2.
+// Partial rows of one MMA tile: 128 x 128 fp32 (normalised) as [d / 4][row][4], so that
+// the 32 rows of a warp store 512 contiguous bytes (row by row, each store instruction
+// touched 32 lines: 7,000 cycles a tile), then 128 log2-sum-exp2.
 constexpr size_t kSlotFloats = 128 * kHeadDim;
 inline size_t workspace_bytes(int slots) { return static_cast<size_t>(slots) * (kSlotFloats + 128) * sizeof(float); }
 
@@ -184,7 +186,7 @@ constexpr uint32_t kSmemBar = kSmemRing + kStagesN * 32768;
 enum Bar {
   kBQFull = 0, kBQEmpty, kBFull, kBEmpty = kBFull + kStagesN, kBFixed = kBEmpty + kStagesN,
   kBSFull = kBFixed + kStagesN, kBPFull = kBSFull + 2, kBODone = kBPFull + 2, kBOFree = kBODone + 2,
-  kBDrain = kBOFree + 2, kNumBars
+  kBTurn = kBOFree + 2, kBDrain = kBTurn + 2, kNumBars
 };
 constexpr uint32_t kSmemSlot = kSmemBar + kNumBars * 8;
 constexpr uint32_t kSmemAbort = kSmemSlot + 4;
@@ -202,7 +204,7 @@ struct ItemView {
 };
 
 __device__ __forceinline__ bool load_item(const Params& p, int idx, ItemView& x) {
-  const int4* w = reinterpret_cast<const int4*>(p.plan + p.plan[kHItemsAt] + static_cast<size_t>(idx) * kItemWords);
+  const int4* w = reinterpret_cast<const int4*>(p.plan + p.items_at + static_cast<size_t>(idx) * kItemWords);
   const int4 a = __ldg(w), b = __ldg(w + 1);
   x.q0 = a.x;
   x.nq = a.y;
@@ -276,6 +278,9 @@ __device__ __forceinline__ void producer_role(const Params& p, const Maps& maps,
   auto bar = [&](int i) { return bars + 8u * i; };
   Ring ring;
   int it = 0, armed_q = 0;
+  prefetch_tmap(&maps.q);
+#pragma unroll
+  for (int i = 0; i < 6; ++i) prefetch_tmap(&maps.kv[i]);
   uint32_t last_full[kStagesN] = {};      // phase + 1 of the last load into each stage
   bool ok = true;
   for (int idx = first; idx < last && ok; ++idx) {
@@ -319,93 +324,139 @@ __device__ __forceinline__ void producer_role(const Params& p, const Maps& maps,
     if (last_full[s]) train::wait_or_abort(bar(kBFull + s), last_full[s] - 1, &never);
 }
 
+// The whole warp runs the issue loop, so that descriptors stay in uniform registers; one
+// elected lane issues each MMA and commit. (A role run by one lane of a divergent warp
+// took 105-115 cycles per MMA of 64.)
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+
 __device__ __forceinline__ void issue_role(const Params& p, int tile, int first, int last, uint32_t sbase,
                                            uint32_t bars, uint32_t tmem, volatile int* abort_flag) {
   auto bar = [&](int i) { return bars + 8u * i; };
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  const uint32_t leader = elected();
   Ring ring;
   int it = 0, mine = 0;                   // items with blocks; of them, items with this tile
   uint32_t p_phase = 0, fixed_phase = 0;  // fixed_phase: one parity bit per stage
+  uint32_t turns = 0;                     // turns taken
   const uint32_t s_col = tmem + kTmemS + tile * 128, o_col = tmem + kTmemO + tile * 128;
-  const uint32_t qbase = sbase + kSmemQ + tile * 32768;
+  const uint64_t q_desc = train::smem_desc(sbase + kSmemQ + tile * 32768, 16, 1024);
+  const uint64_t k_desc = train::smem_desc(sbase + kSmemRing, 16, 1024);
+  const uint64_t v_desc = train::smem_desc(sbase + kSmemRing, 16384, 1024);
   bool ok = true;
   for (int idx = first; idx < last && ok; ++idx) {
     ItemView x;
     if (!load_item(p, idx, x) || x.blocks == 0) continue;
+    if (!(ok = wait(kBQFull, it & 1))) break;
+    BlockWalk w;
     if (tile == 1 && x.nq <= kHalfTile) {
       // no rows in this tile: release the stages as they fill (every phase is waited for, so
-      // no barrier runs two phases ahead of this thread)
-      ok = train::wait_or_abort(bar(kBQFull), it & 1, abort_flag);
-      BlockWalk w;
+      // no barrier runs two phases ahead of this warp)
       for (int b = 0; b < x.blocks && ok; ++b, w.next(x)) {
         for (int v = 0; v < 2 && ok; ++v) {
-          ok = train::wait_or_abort(bar(kBFull + ring.stage), ring.phase, abort_flag);
-          if (!ok) break;
+          if (!(ok = wait(kBFull + ring.stage, ring.phase))) break;
           if (v == 1 && (w.keys(x) & 15)) fixed_phase ^= 1u << ring.stage;
-          mbar_arrive(bar(kBEmpty + ring.stage));
+          if (leader) mbar_arrive(bar(kBEmpty + ring.stage));
           ring.next();
         }
       }
-      if (ok) mbar_arrive(bar(kBQEmpty));
+      if (ok && leader) mbar_arrive(bar(kBQEmpty));
       ++it;
       continue;
     }
-    if (!(ok = train::wait_or_abort(bar(kBQFull), it & 1, abort_flag))) break;
-    BlockWalk w;
-    auto qk = [&](int keys, bool final) {
-      if (!(ok = train::wait_or_abort(bar(kBFull + ring.stage), ring.phase, abort_flag))) return;
-      train::tc_fence_after();
-      const uint32_t kbase = sbase + kSmemRing + ring.stage * 32768;
+    // The issuers of a two-tile item take turns, A before B: a turn is PV(b) and QK(b + 1)
+    // of one tile, so the tiles stay half a block apart and each one's softmax runs under
+    // the other's products. Issuing freely, both tiles' MMAs interleave on the pipe, both
+    // softmaxes start together and the pipe idles under them (5,800 cycles a block).
+    const bool paired = x.nq > kHalfTile;
+    auto take_turn = [&]() {
+      if (!paired) return true;
+      const bool got = wait(kBTurn + tile, (turns & 1) ^ (tile == 0 ? 1u : 0u));
+      ++turns;
+      return got;
+    };
+    auto pass_turn = [&]() {
+      if (paired && leader) mbar_arrive(bar(kBTurn + (tile ^ 1)));
+    };
+    auto issue_qk = [&](int stage, int keys) {
+      const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (32768 >> 4));
       const uint32_t idesc = instr_desc_n(0, static_cast<uint32_t>((keys + 15) & ~15));
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-        train::umma_bf16(s_col, train::smem_desc(qbase + off, 16, 1024), train::smem_desc(kbase + off, 16, 1024),
-                         idesc, kk > 0);
+        const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+        train::umma_bf16(s_col, q_desc + off, kd + off, idesc, kk > 0);
       }
+    };
+    // S(0)
+    if (!(ok = wait(kBFull + ring.stage, ring.phase)) || !(ok = take_turn())) break;
+    train::tc_fence_after();
+    if (leader) {
+      issue_qk(ring.stage, w.keys(x));
       train::umma_commit(bar(kBSFull + tile));
       train::umma_commit(bar(kBEmpty + ring.stage));
-      if (final) train::umma_commit(bar(kBQEmpty));
-      ring.next();
-    };
-    qk(w.keys(x), x.blocks == 1);
+      if (x.blocks == 1) train::umma_commit(bar(kBQEmpty));
+    }
+    __syncwarp();
+    pass_turn();
+    ring.next();
     for (int b = 0; b < x.blocks && ok; ++b) {
-      const int keys = w.keys(x);
-      if (!(ok = train::wait_or_abort(bar(kBPFull + tile), p_phase, abort_flag))) break;
-      p_phase ^= 1;
-      if (b == 0 && !(ok = train::wait_or_abort(bar(kBOFree + tile), (mine & 1) ^ 1, abort_flag))) break;
-      if (!(ok = train::wait_or_abort(bar(kBFull + ring.stage), ring.phase, abort_flag))) break;
+      const int keys = w.keys(x), vs = ring.stage;
+      const bool more = b + 1 < x.blocks;
+      // every wait comes before the first MMA, every commit behind the last: PV(b) and
+      // QK(b + 1) run back to back on the pipe
+      if (b == 0 && !(ok = wait(kBOFree + tile, (mine & 1) ^ 1))) break;
+      if (!(ok = wait(kBFull + vs, ring.phase))) break;
       if (keys & 15) {
-        if (!(ok = train::wait_or_abort(bar(kBFixed + ring.stage), (fixed_phase >> ring.stage) & 1, abort_flag))) break;
-        fixed_phase ^= 1u << ring.stage;
+        if (!(ok = wait(kBFixed + vs, (fixed_phase >> vs) & 1))) break;
+        fixed_phase ^= 1u << vs;
       }
+      ring.next();
+      if (more) {
+        w.next(x);
+        if (!(ok = wait(kBFull + ring.stage, ring.phase))) break;
+      }
+      if (!(ok = take_turn())) break;
+      if (!(ok = wait(kBPFull + tile, p_phase))) break;
+      p_phase ^= 1;
       train::tc_fence_after();
-      const uint32_t vbase = sbase + kSmemRing + ring.stage * 32768;
-      const int steps = (keys + 15) >> 4;
-      if (steps == 8) {
+      if (leader) {
+        const uint64_t vd = v_desc + static_cast<uint32_t>(vs * (32768 >> 4));
+        const int steps = (keys + 15) >> 4;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          train::umma_bf16_ts(o_col, s_col + kk * 8, train::smem_desc(vbase + kk * 2048, 16384, 1024),
-                              instr_desc_n(1, 128), (b > 0 || kk > 0) ? 1u : 0u);
-      } else {
-        for (int kk = 0; kk < steps; ++kk)
-          train::umma_bf16_ts(o_col, s_col + kk * 8, train::smem_desc(vbase + kk * 2048, 16384, 1024),
-                              instr_desc_n(1, 128), (b > 0 || kk > 0) ? 1u : 0u);
+          if (kk < steps)
+            train::umma_bf16_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), instr_desc_n(1, 128),
+                                (b > 0 || kk > 0) ? 1u : 0u);
+        if (more) {
+          issue_qk(ring.stage, w.keys(x));
+          train::umma_commit(bar(kBSFull + tile));
+          train::umma_commit(bar(kBEmpty + ring.stage));
+          if (b + 2 == x.blocks) train::umma_commit(bar(kBQEmpty));
+        } else {
+          train::umma_commit(bar(kBODone + tile));
+        }
+        train::umma_commit(bar(kBEmpty + vs));
       }
-      train::umma_commit(bar(kBEmpty + ring.stage));
-      ring.next();
-      if (b + 1 == x.blocks) {
-        train::umma_commit(bar(kBODone + tile));
-      } else {
-        w.next(x);
-        qk(w.keys(x), b + 2 == x.blocks);
-      }
+      __syncwarp();
+      if (more) ring.next();
+      pass_turn();
     }
     ++it;
     ++mine;
   }
   if (!ok) *abort_flag = 1;
   // Every MMA issued above completes before TMEM is released.
-  train::umma_commit(bar(kBDrain));
+  if (leader) train::umma_commit(bar(kBDrain));
+  __syncwarp();
   volatile int never = 0;
   train::wait_or_abort(bar(kBDrain), 0, &never);
 }
@@ -522,48 +573,64 @@ __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, 
 __device__ __forceinline__ void softmax_role(const Params& p, float* part, int first, int last, uint32_t bars,
                                              uint32_t tmem, volatile int* abort_flag) {
   auto bar = [&](int i) { return bars + 8u * i; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = warp >> 2, quarter = warp & 3;
-  const int m = quarter * 32 + lane;                        // row of the tile == TMEM lane
+  const int tile = threadIdx.x >> 7;
+  const int m = threadIdx.x & 127;                          // row of the tile == TMEM lane
   const int lt = tile * kHalfTile + (m >> 1);               // query row of the item
-  const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+  const uint32_t lanes = static_cast<uint32_t>(m & ~31) << 16;
   const uint32_t s_addr = tmem + lanes + kTmemS + tile * 128, o_addr = tmem + lanes + kTmemO + tile * 128;
   uint32_t s_phase = 0, o_phase = 0;
   bool ok = true;
+#pragma unroll 1
   for (int idx = first; idx < last && ok; ++idx) {
-    ItemView x;
-    if (!load_item(p, idx, x)) {
-      if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
-      continue;
-    }
-    if (tile == 1 && x.nq <= kHalfTile) continue;
-    const bool row_ok = lt < x.nq;
-    const bool warp_ok = tile * kHalfTile + quarter * 16 < x.nq;
-    RowState st{-1e30f, 0.f};
-    if (x.blocks > 0) {
-      BlockWalk w;
-      for (int b = 0; b < x.blocks; ++b, w.next(x)) {
-        ok = train::wait_or_abort(bar(kBSFull + tile), s_phase, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        s_phase ^= 1;
-        if (warp_ok) {
-          train::tc_fence_after();
-          const int keys = w.keys(x);
-          const int see = row_ok ? min(keys, x.visible + lt - w.pos(x)) : 0;
-          if (keys > 64)
-            softmax_block<128>(s_addr, o_addr, see, p.scale_log2, b == 0, st);
-          else if (keys > 32)
-            softmax_block<64>(s_addr, o_addr, see, p.scale_log2, b == 0, st);
-          else
-            softmax_block<32>(s_addr, o_addr, see, p.scale_log2, b == 0, st);
-          train::tc_fence_before();
-        }
-        mbar_arrive(bar(kBPFull + tile));
+    int nq, blocks, len0, len1, len2, see0;                 // what the block loop keeps of the item
+    {
+      ItemView x;
+      if (!load_item(p, idx, x)) {
+        if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
+        continue;
       }
-      if (!ok) break;
+      nq = x.nq;
+      blocks = x.blocks;
+      len0 = x.len[0];
+      len1 = x.len[1];
+      len2 = x.len[2];
+      // the item's keys are consecutive chain positions from pos[0]
+      see0 = lt < nq ? x.visible + lt - x.pos[0] : 0;
+    }
+    if (tile == 1 && nq <= kHalfTile) continue;
+    const bool warp_ok = tile * kHalfTile + ((m & ~31) >> 1) < nq;
+    RowState st{-1e30f, 0.f};
+#pragma unroll 1
+    for (int b = 0; b < blocks; ++b) {
+      ok = train::wait_or_abort(bar(kBSFull + tile), s_phase, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      s_phase ^= 1;
+      const int keys = min(kBlock, len0);
+      if (warp_ok) {
+        train::tc_fence_after();
+        if (keys > 32)
+          softmax_block<128>(s_addr, o_addr, min(keys, see0), p.scale_log2, b == 0, st);
+        else
+          softmax_block<32>(s_addr, o_addr, min(keys, see0), p.scale_log2, b == 0, st);
+        train::tc_fence_before();
+      }
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(bar(kBPFull + tile));
+      see0 -= keys;
+      len0 -= keys;
+      if (len0 == 0) {
+        len0 = len1;
+        len1 = len2;
+        len2 = 0;
+      }
+    }
+    if (!ok) break;
+    ItemView x;
+    load_item(p, idx, x);                                   // again: its registers were the scores'
+    if (blocks > 0) {
       ok = train::wait_or_abort(bar(kBODone + tile), o_phase, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -573,15 +640,15 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
       train::tc_fence_after();
     }
     if (warp_ok) {
+      const bool row_ok = lt < nq;
       const float inv = st.l > 0.f ? 1.f / st.l : 0.f;
+      float* prow = part + static_cast<size_t>(max(x.slot, 0) + tile) * (kSlotFloats + 128);
       __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) +
                             (static_cast<size_t>(x.q0 + (row_ok ? lt : 0)) * kQHeads + 2 * x.head + (m & 1)) * kHeadDim;
-      const size_t slot = static_cast<size_t>(max(x.slot, 0) + tile);
-      float* prow = part + slot * (kSlotFloats + 128) + static_cast<size_t>(m) * kHeadDim;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         float o[32];
-        if (x.blocks > 0) {
+        if (blocks > 0) {
           train::tmem_ld32(o_addr + 32 * c, o);
         } else {
 #pragma unroll
@@ -602,16 +669,16 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
         } else if (row_ok) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            __stcg(reinterpret_cast<float4*>(prow + 32 * c + 4 * j),
+            __stcg(reinterpret_cast<float4*>(prow + (8 * c + j) * 512 + 4 * m),
                    make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
         }
       }
-      if (row_ok && x.slot >= 0)
-        __stcg(part + slot * (kSlotFloats + 128) + kSlotFloats + m, st.l > 0.f ? st.m + log2f(st.l) : -INFINITY);
+      if (row_ok && x.slot >= 0) __stcg(prow + kSlotFloats + m, st.l > 0.f ? st.m + log2f(st.l) : -INFINITY);
     }
-    if (x.blocks > 0) {
+    if (blocks > 0) {
       train::tc_fence_before();
-      mbar_arrive(bar(kBOFree + tile));
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(bar(kBOFree + tile));
     }
   }
   if (!ok) *abort_flag = 1;
@@ -624,7 +691,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   const uint32_t sbase = smem_u32(smem), bars = sbase + kSmemBar;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemAbort);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;");
   int first = 0, last = 0;
   if (plan_ok(p) && p.plan[kHGrid] == static_cast<int>(gridDim.x)) {
     const int* offs = p.plan + p.plan[kHCtaAt] + blockIdx.x;
@@ -639,7 +705,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       uint32_t count = 1;
       if (i == kBQEmpty || i == kBDrain) count = 2;                     // both issuers
       if (i >= kBEmpty && i < kBEmpty + kStagesN) count = 3;            // both issuers and warp 11
-      if ((i >= kBPFull && i < kBPFull + 2) || (i >= kBOFree && i < kBOFree + 2)) count = 128;
+      if ((i >= kBPFull && i < kBPFull + 2) || (i >= kBOFree && i < kBOFree + 2)) count = 4;   // softmax warps
       mbar_init(bars + 8u * i, count);
     }
     *abort_flag = 0;
@@ -650,11 +716,18 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   __syncthreads();
   train::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kSmemSlot);
+  // 384 threads are launched with 168 registers each (64,512). A softmax thread holds a row
+  // of 128 scores: its warpgroups grow to 208 each out of what the third one gives back
+  // (2 x 128 x 208 + 128 x 72 = 62,464); without this the row spills to local memory.
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  }
   if (warp < 8) {
     softmax_role(p, part, first, last, bars, tmem, abort_flag);
   } else if (warp < 10) {
-    if (lane == 0) issue_role(p, warp - 8, first, last, sbase, bars, tmem, abort_flag);
-    __syncwarp();
+    issue_role(p, warp - 8, first, last, sbase, bars, tmem, abort_flag);
   } else if (warp == 10) {
     if (lane == 0) producer_role(p, maps, first, last, sbase, bars, abort_flag);
     __syncwarp();
@@ -667,60 +740,76 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   if (warp == 8) train::tmem_dealloc(tmem, 512);
 }
 
-// Combines the partial rows: one warp per (query row, head), lane l owns d = 4 l ..
+// Combines the partial rows: one warp per (query row, KV head), both of its query heads
+// (adjacent rows of a slot, so a lane reads whole 32-byte sectors); lane l owns d = 4 l ..
 //   out = sum_c 2^(L_c - M) o_c / sum_c 2^(L_c - M),  M = max_c L_c
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const float* part) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!plan_ok(p)) return;
   const int lane = threadIdx.x & 31;
   const long long u = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (u >= static_cast<long long>(p.total_q) * kQHeads) return;
-  const int t = static_cast<int>(u / kQHeads), h = static_cast<int>(u % kQHeads);
+  if (u >= static_cast<long long>(p.total_q) * kHeads) return;
+  const int t = static_cast<int>(u / kHeads), h = static_cast<int>(u % kHeads);
   const int run = p.plan[p.plan[kHTokenRunAt] + t];
   if (run < 0 || run >= p.plan[kHRuns]) return;
   const int* w = p.plan + p.plan[kHRunsAt] + static_cast<size_t>(run) * kRunWords;
-  const int tiles = w[kRunTiles];
-  const int n0 = w[kRunTile0 + 1], total = n0 + (tiles > 1 ? w[kRunTile0 + kRunTileWords + 1] : 0);
-  // slot and row of contribution c
-  auto where = [&](int c) -> size_t {
-    const int* k = w + kRunTile0 + (c < n0 ? 0 : kRunTileWords);
-    const int piece = c < n0 ? c : c - n0, lt = t - k[3];
-    const int slot = min(max(k[0] + (piece * kHeads + (h >> 1)) * k[2] + (lt >> 6), 0), p.slots - 1);
-    return static_cast<size_t>(slot) * (kSlotFloats + 128);
+  const int4 k0 = *reinterpret_cast<const int4*>(w + kRunTile0);
+  const int4 k1 = *reinterpret_cast<const int4*>(w + kRunTile0 + kRunTileWords);
+  const int n0 = k0.y, total = n0 + (w[kRunTiles] > 1 ? k1.y : 0);
+  const int lt0 = t - k0.w, lt1 = t - k1.w;
+  // floats before contribution c's slot, and its first row (head 0)
+  auto base = [&](int c) -> const float* {
+    const bool first = c < n0;
+    const int slot = first ? k0.x + (c * kHeads + h) * k0.z + (lt0 >> 6)
+                           : k1.x + ((c - n0) * kHeads + h) * k1.z + (lt1 >> 6);
+    return part + static_cast<size_t>(min(max(slot, 0), p.slots - 1)) * (kSlotFloats + 128);
   };
-  const int* k0 = w + kRunTile0;
-  const int* k1 = w + kRunTile0 + kRunTileWords;
-  auto row_of = [&](int c) { return 2 * ((t - (c < n0 ? k0[3] : k1[3])) & 63) + (h & 1); };
-  float top = -INFINITY;
-  for (int c = lane; c < total; c += 32) top = fmaxf(top, __ldcg(part + where(c) + kSlotFloats + row_of(c)));
+  auto row_of = [&](int c) { return 2 * ((c < n0 ? lt0 : lt1) & 63); };
+  float2 top = make_float2(-INFINITY, -INFINITY);
+  for (int c = lane; c < total; c += 32) {
+    const float2 v = __ldcg(reinterpret_cast<const float2*>(base(c) + kSlotFloats + row_of(c)));
+    top.x = fmaxf(top.x, v.x);
+    top.y = fmaxf(top.y, v.y);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float den = 0.f;
-  if (top > -INFINITY) {
-    for (int c0 = 0; c0 < total; c0 += 32) {
-      const int c = c0 + lane;
-      const float mine = c < total ? ex2(__ldcg(part + where(c) + kSlotFloats + row_of(c)) - top) : 0.f;
-      const int n = min(32, total - c0);
+  for (int o = 16; o > 0; o >>= 1) {
+    top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
+    top.y = fmaxf(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
+  }
+  // a row whose contributions all see nothing: weights 0
+  const float mx = top.x > -INFINITY ? top.x : 0.f, my = top.y > -INFINITY ? top.y : 0.f;
+  float a[8] = {}, den0 = 0.f, den1 = 0.f;
+  for (int c0 = 0; c0 < total; c0 += 32) {
+    const int c = c0 + lane;
+    float2 f = make_float2(0.f, 0.f);
+    if (c < total) {
+      f = __ldcg(reinterpret_cast<const float2*>(base(c) + kSlotFloats + row_of(c)));
+      f.x = ex2(f.x - mx);
+      f.y = ex2(f.y - my);
+    }
+    const int n = min(32, total - c0);
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float f = __shfl_sync(0xffffffffu, mine, i);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(
-            part + where(c0 + i) + static_cast<size_t>(row_of(c0 + i)) * kHeadDim + 4 * lane));
-        den += f;
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
-      }
+    for (int i = 0; i < n; ++i) {
+      const float f0 = __shfl_sync(0xffffffffu, f.x, i), f1 = __shfl_sync(0xffffffffu, f.y, i);
+      const float4* src =
+          reinterpret_cast<const float4*>(base(c0 + i) + static_cast<size_t>(lane) * 512 + 4 * row_of(c0 + i));
+      const float4 v0 = __ldcg(src), v1 = __ldcg(src + 1);
+      den0 += f0;
+      den1 += f1;
+      a[0] = fmaf(f0, v0.x, a[0]);
+      a[1] = fmaf(f0, v0.y, a[1]);
+      a[2] = fmaf(f0, v0.z, a[2]);
+      a[3] = fmaf(f0, v0.w, a[3]);
+      a[4] = fmaf(f1, v1.x, a[4]);
+      a[5] = fmaf(f1, v1.y, a[5]);
+      a[6] = fmaf(f1, v1.z, a[6]);
+      a[7] = fmaf(f1, v1.w, a[7]);
     }
   }
-  const float inv = den > 0.f ? 1.f / den : 0.f;
-  uint2 res;
-  res.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-  res.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) +
-                            (static_cast<size_t>(t) * kQHeads + h) * kHeadDim + 4 * lane) = res;
+  const float i0 = den0 > 0.f ? 1.f / den0 : 0.f, i1 = den1 > 0.f ? 1.f / den1 : 0.f;
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (static_cast<size_t>(t) * kQHeads + 2 * h) * kHeadDim + 4 * lane;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a[0] * i0, a[1] * i0), pack_bf16x2(a[2] * i0, a[3] * i0));
+  *reinterpret_cast<uint2*>(dst + kHeadDim) =
+      make_uint2(pack_bf16x2(a[4] * i1, a[5] * i1), pack_bf16x2(a[6] * i1, a[7] * i1));
 }
 
 }  // namespace prefix
