@@ -305,6 +305,20 @@ int varlen_common(const void* q, const void* k, const void* v, const int32_t* cu
   return run_attention(p, src, dtype, max_q, workspace, workspace_bytes, stream);
 }
 
+// K/V [rows, 8, 128] bf16 as dims (64 d, row, half, head): one box of 128 rows x both halves
+// of a head lands in shared memory as two 16 KB halves of 128-byte rows, 128-byte swizzle.
+int encode_block_map(CUtensorMap* m, const void* base, long long rows) {
+  if (!aligned(base, 16) || rows < 1 || rows >= (1ll << 31)) return DSPARK_ERR_INVALID_ARGUMENT;
+  cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(rows), 2, static_cast<cuuint64_t>(kKVHeads)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(kKVHeads * kHeadDim * 2), 128, static_cast<cuuint64_t>(kHeadDim * 2)};
+  cuuint32_t box[4] = {64, 128, 2, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DSPARK_OK : DSPARK_ERR_CUDA;
+}
+
 // Packed q or K/V [rows, heads, 128] bf16 as dims (d, head, row): one box of
 // (64 d, box_heads, box_rows) lands in shared memory as [row][head][64 d] rows of
 // 128 bytes in the 128-byte swizzle, the K-major operand layout of tcgen05.mma.
@@ -1159,6 +1173,9 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   p.grid = plan_head[kHGrid];
   p.slots = plan_head[kHSlots];
   p.items_at = plan_head[kHItemsAt];
+  p.runs = plan_head[kHRuns];
+  p.runs_at = plan_head[kHRunsAt];
+  p.token_run_at = plan_head[kHTokenRunAt];
   p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.src[0] = Source{prefix_k, prefix_v, prefix_off, prefix_rows};
@@ -1185,16 +1202,19 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   if (p.slots > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < prefix::workspace_bytes(p.slots)))
     return DSPARK_ERR_INVALID_ARGUMENT;
   Maps maps;
-  int rc = encode_rows_map(&maps.q, q, total_q, kQHeads, 2, kHalfTile);
+  int rc = encode_rows_map(&maps.q, q, total_q, kQHeads, 2, kHalfTile / 2);
   if (rc != DSPARK_OK) return rc;
   for (int s = 0; s < 3; ++s) {
     const Source& x = p.src[s];
     if (plan_head[kHPrefixRows + s] == 0) {      // never read
-      maps.kv[2 * s] = maps.kv[2 * s + 1] = maps.q;
+      maps.block[2 * s] = maps.block[2 * s + 1] = maps.box[2 * s] = maps.box[2 * s + 1] = maps.q;
       continue;
     }
-    if ((rc = encode_rows_map(&maps.kv[2 * s], x.k, x.rows, kKVHeads, 1, kBoxRows)) != DSPARK_OK) return rc;
-    if ((rc = encode_rows_map(&maps.kv[2 * s + 1], x.v, x.rows, kKVHeads, 1, kBoxRows)) != DSPARK_OK) return rc;
+    for (int v = 0; v < 2; ++v) {
+      const void* base = v ? x.v : x.k;
+      if ((rc = encode_rows_map(&maps.box[2 * s + v], base, x.rows, kKVHeads, 1, kBoxRows)) != DSPARK_OK) return rc;
+      if ((rc = encode_block_map(&maps.block[2 * s + v], base, x.rows)) != DSPARK_OK) return rc;
+    }
   }
   float* part = static_cast<float*>(workspace);
   prefix_attn_kernel<<<p.grid, kAttThreads, prefix::kSmemBytes, stream>>>(maps, p, part);
@@ -1204,8 +1224,11 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   // the attention's third warpgroup gives back before its softmax warps draw them, and
   // with the trigger behind that point small batches measured slower (R = 8 rows behind
   // 32768 keys: 102 us against 60).
-  prefix_merge_kernel<<<static_cast<unsigned>((static_cast<long long>(total_q) * kHeads + 7) / 8), 256, 0, stream>>>(p,
-                                                                                                              part);
+  const long long pairs = static_cast<long long>(total_q) * kHeads;
+  if (plan_head[kHMaxParts] > kMergeWideParts && pairs <= kMergeWidePairs)
+    prefix_merge_kernel<8><<<static_cast<unsigned>(pairs), 256, 0, stream>>>(p, part);
+  else
+    prefix_merge_kernel<1><<<static_cast<unsigned>((pairs + 7) / 8), 256, 0, stream>>>(p, part);
   return launch_status();
 }
 

@@ -26,7 +26,7 @@ struct Params {
   const void* q;     // [total_q, 16, 128]
   void* out;
   const int* plan;
-  int check, total_q, grid, slots, items_at;
+  int check, total_q, grid, slots, items_at, runs, runs_at, token_run_at;
   Source src[3];     // prefix, own, new
   float scale, scale_log2;
 };
@@ -195,11 +195,13 @@ constexpr uint32_t kTmemS = 0, kTmemO = 256;              // tile x: S at 128 x,
 constexpr int kBoxRows = 32;
 
 struct Maps {
-  CUtensorMap q, kv[6];                                   // kv[2 s], kv[2 s + 1]: K and V of source s
+  CUtensorMap q;                                          // boxes of 32 query rows x 2 heads x 64 d
+  CUtensorMap block[6], box[6];                           // [2 s], [2 s + 1]: K and V of source s
 };
 
 struct ItemView {
   int q0, nq, head, slot, visible, nsegs, blocks;
+  bool dual;
   int src[kMaxSegs], row[kMaxSegs], len[kMaxSegs], pos[kMaxSegs];
 };
 
@@ -212,9 +214,12 @@ __device__ __forceinline__ bool load_item(const Params& p, int idx, ItemView& x)
   x.slot = a.w;
   x.visible = b.x;
   x.nsegs = b.y;
+  x.dual = b.z != 0;
   x.blocks = 0;
   bool ok = x.nq >= 1 && x.nq <= kTileRows && x.q0 >= 0 && x.q0 <= p.total_q - x.nq && x.head >= 0 &&
-            x.head < kHeads && x.nsegs >= 0 && x.nsegs <= kMaxSegs && x.slot < p.slots - (x.nq > kHalfTile ? 1 : 0);
+            x.head < kHeads && x.nsegs >= 0 && x.nsegs <= kMaxSegs &&
+            x.slot < p.slots - (x.nq > kHalfTile || x.dual ? 1 : 0) &&
+            (!x.dual || (x.nq <= kHalfTile && x.slot >= 0));
 #pragma unroll
   for (int s = 0; s < kMaxSegs; ++s) {
     const int4 g = __ldg(w + 2 + s);
@@ -229,7 +234,7 @@ __device__ __forceinline__ bool load_item(const Params& p, int idx, ItemView& x)
       x.blocks += (g.z + kBlock - 1) / kBlock;
     }
   }
-  return ok;
+  return ok && (!x.dual || x.blocks >= 2);
 }
 
 // Walks an item's key blocks.
@@ -273,60 +278,7 @@ struct Ring {
   }
 };
 
-__device__ __forceinline__ void producer_role(const Params& p, const Maps& maps, int first, int last, uint32_t sbase,
-                                              uint32_t bars, volatile int* abort_flag) {
-  auto bar = [&](int i) { return bars + 8u * i; };
-  Ring ring;
-  int it = 0, armed_q = 0;
-  prefetch_tmap(&maps.q);
-#pragma unroll
-  for (int i = 0; i < 6; ++i) prefetch_tmap(&maps.kv[i]);
-  uint32_t last_full[kStagesN] = {};      // phase + 1 of the last load into each stage
-  bool ok = true;
-  for (int idx = first; idx < last && ok; ++idx) {
-    ItemView x;
-    if (!load_item(p, idx, x) || x.blocks == 0) continue;
-    if (!(ok = train::wait_or_abort(bar(kBQEmpty), (it & 1) ^ 1, abort_flag))) break;
-    const int tiles = x.nq > kHalfTile ? 2 : 1;
-    mbar_arrive_expect_tx(bar(kBQFull), 32768u * tiles);
-    for (int t = 0; t < tiles; ++t) {
-      tma_load_3d(sbase + kSmemQ + t * 32768, &maps.q, 0, 2 * x.head, x.q0 + t * kHalfTile, bar(kBQFull));
-      tma_load_3d(sbase + kSmemQ + t * 32768 + 16384, &maps.q, 64, 2 * x.head, x.q0 + t * kHalfTile, bar(kBQFull));
-    }
-    ++armed_q;
-    BlockWalk w;
-    for (int b = 0; b < x.blocks && ok; ++b, w.next(x)) {
-      const int boxes = (w.keys(x) + kBoxRows - 1) / kBoxRows, src = w.src(x);
-      const int row = static_cast<int>(p.src[src].off) + w.row(x);
-      for (int v = 0; v < 2; ++v) {
-        if (!(ok = train::wait_or_abort(bar(kBEmpty + ring.stage), ring.phase ^ 1, abort_flag))) break;
-        const uint32_t full = bar(kBFull + ring.stage), dst = sbase + kSmemRing + ring.stage * 32768;
-        mbar_arrive_expect_tx(full, static_cast<uint32_t>(boxes) * kBoxRows * 256u);
-        const CUtensorMap* m = &maps.kv[2 * src + v];
-        for (int i = 0; i < boxes; ++i) {
-          tma_load_3d(dst + i * kBoxRows * 128, m, 0, x.head, row + i * kBoxRows, full);
-          tma_load_3d(dst + 16384 + i * kBoxRows * 128, m, 64, x.head, row + i * kBoxRows, full);
-        }
-#pragma unroll
-        for (int s = 0; s < kStagesN; ++s)
-          if (s == ring.stage) last_full[s] = ring.phase + 1;
-        ring.next();
-      }
-    }
-    ++it;
-  }
-  if (!ok) *abort_flag = 1;
-  // Copies in flight land before the CTA can exit (a no-op when all were consumed).
-  volatile int never = 0;
-  if (armed_q) train::wait_or_abort(bar(kBQFull), (armed_q - 1) & 1, &never);
-#pragma unroll
-  for (int s = 0; s < kStagesN; ++s)
-    if (last_full[s]) train::wait_or_abort(bar(kBFull + s), last_full[s] - 1, &never);
-}
-
-// The whole warp runs the issue loop, so that descriptors stay in uniform registers; one
-// elected lane issues each MMA and commit. (A role run by one lane of a divergent warp
-// took 105-115 cycles per MMA of 64.)
+// One lane of a converged warp.
 __device__ __forceinline__ uint32_t elected() {
   uint32_t e;
   asm volatile(
@@ -337,6 +289,88 @@ __device__ __forceinline__ uint32_t elected() {
   return e;
 }
 
+// First row of tile B in a dual item: up to 64 rows move to the other two warps' lanes, so
+// that the tiles' softmax warps with rows lie on different SM quarters.
+__device__ __forceinline__ int dual_shift(int nq) { return nq <= 32 ? 64 : 0; }
+
+// A whole block of 128 keys is one copy: the map's dimensions (64 d, row, half, head) put
+// the 16 KB halves of 128-byte rows one behind the other. A short block takes boxes of 32
+// rows per half. (Boxes throughout, issued by one lane of a divergent warp, cost 1,050
+// cycles a stage and bounded every memory-bound case.)
+__device__ __forceinline__ void producer_role(const Params& p, const Maps& maps, int first, int last, uint32_t sbase,
+                                              uint32_t bars, volatile int* abort_flag) {
+  auto bar = [&](int i) { return bars + 8u * i; };
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  const uint32_t leader = elected();
+  Ring ring;
+  int it = 0, uses = 0;
+  if (leader) prefetch_tmap(&maps.q);
+  bool ok = true;
+  for (int idx = first; idx < last && ok; ++idx) {
+    ItemView x;
+    if (!load_item(p, idx, x) || x.blocks == 0) continue;
+    if (!(ok = wait(kBQEmpty, (it & 1) ^ 1))) break;
+    if (leader) {
+      // 32 query rows (64 MMA rows, 8 KB per half) a box
+      const int boxes = (x.nq + 31) >> 5;
+      mbar_arrive_expect_tx(bar(kBQFull), 16384u * boxes * (x.dual ? 2 : 1));
+      for (int t = 0; t < boxes; ++t) {
+        const uint32_t dst = sbase + kSmemQ + (t >> 1) * 32768 + (t & 1) * 8192;
+        tma_load_3d(dst, &maps.q, 0, 2 * x.head, x.q0 + 32 * t, bar(kBQFull));
+        tma_load_3d(dst + 16384, &maps.q, 64, 2 * x.head, x.q0 + 32 * t, bar(kBQFull));
+        if (x.dual) {
+          // tile B holds the same rows, from row dual_shift on
+          const uint32_t d2 = sbase + kSmemQ + 32768 + ((t ^ (dual_shift(x.nq) >> 6)) & 1) * 8192;
+          tma_load_3d(d2, &maps.q, 0, 2 * x.head, x.q0 + 32 * t, bar(kBQFull));
+          tma_load_3d(d2 + 16384, &maps.q, 64, 2 * x.head, x.q0 + 32 * t, bar(kBQFull));
+        }
+      }
+    }
+    __syncwarp();
+    BlockWalk w;
+    for (int b = 0; b < x.blocks && ok; ++b, w.next(x)) {
+      const int keys = w.keys(x), src = w.src(x);
+      const int row = static_cast<int>(p.src[src].off) + w.row(x);
+      for (int v = 0; v < 2; ++v) {
+        if (!(ok = wait(kBEmpty + ring.stage, ring.phase ^ 1))) break;
+        const uint32_t full = bar(kBFull + ring.stage), dst = sbase + kSmemRing + ring.stage * 32768;
+        if (leader) {
+          if (keys == kBlock) {
+            mbar_arrive_expect_tx(full, 32768u);
+            tma_load_4d(dst, &maps.block[2 * src + v], 0, row, 0, x.head, full);
+          } else {
+            const int boxes = (keys + kBoxRows - 1) / kBoxRows;
+            mbar_arrive_expect_tx(full, static_cast<uint32_t>(boxes) * kBoxRows * 256u);
+            for (int i = 0; i < boxes; ++i) {
+              tma_load_3d(dst + i * kBoxRows * 128, &maps.box[2 * src + v], 0, x.head, row + i * kBoxRows, full);
+              tma_load_3d(dst + 16384 + i * kBoxRows * 128, &maps.box[2 * src + v], 64, x.head, row + i * kBoxRows,
+                          full);
+            }
+          }
+        }
+        __syncwarp();
+        ++uses;
+        ring.next();
+      }
+    }
+    ++it;
+  }
+  if (!ok) *abort_flag = 1;
+  // Copies in flight land before the CTA can exit (a no-op when all were consumed): the
+  // last load of each stage that was used.
+  volatile int never = 0;
+  if (it) train::wait_or_abort(bar(kBQFull), (it - 1) & 1, &never);
+  for (int s = 0; s < kStagesN && s < uses; ++s) {
+    const int last_use = uses - 1 - (uses - 1 - s) % kStagesN;
+    train::wait_or_abort(bar(kBFull + s), (last_use / kStagesN) & 1, &never);
+  }
+}
+
+// The whole warp runs the issue loop, so that descriptors stay in uniform registers; one
+// elected lane issues each MMA and commit. (A role run by one lane of a divergent warp
+// took 105-115 cycles per MMA of 64.)
 __device__ __forceinline__ void issue_role(const Params& p, int tile, int first, int last, uint32_t sbase,
                                            uint32_t bars, uint32_t tmem, volatile int* abort_flag) {
   auto bar = [&](int i) { return bars + 8u * i; };
@@ -349,7 +383,6 @@ __device__ __forceinline__ void issue_role(const Params& p, int tile, int first,
   uint32_t p_phase = 0, fixed_phase = 0;  // fixed_phase: one parity bit per stage
   uint32_t turns = 0;                     // turns taken
   const uint32_t s_col = tmem + kTmemS + tile * 128, o_col = tmem + kTmemO + tile * 128;
-  const uint64_t q_desc = train::smem_desc(sbase + kSmemQ + tile * 32768, 16, 1024);
   const uint64_t k_desc = train::smem_desc(sbase + kSmemRing, 16, 1024);
   const uint64_t v_desc = train::smem_desc(sbase + kSmemRing, 16384, 1024);
   bool ok = true;
@@ -358,21 +391,27 @@ __device__ __forceinline__ void issue_role(const Params& p, int tile, int first,
     if (!load_item(p, idx, x) || x.blocks == 0) continue;
     if (!(ok = wait(kBQFull, it & 1))) break;
     BlockWalk w;
-    if (tile == 1 && x.nq <= kHalfTile) {
-      // no rows in this tile: release the stages as they fill (every phase is waited for, so
-      // no barrier runs two phases ahead of this warp)
-      for (int b = 0; b < x.blocks && ok; ++b, w.next(x)) {
-        for (int v = 0; v < 2 && ok; ++v) {
-          if (!(ok = wait(kBFull + ring.stage, ring.phase))) break;
-          if (v == 1 && (w.keys(x) & 15)) fixed_phase ^= 1u << ring.stage;
-          if (leader) mbar_arrive(bar(kBEmpty + ring.stage));
-          ring.next();
-        }
+    // releases the stages of a block that this tile does not use, as they fill (every phase
+    // is waited for, so no barrier runs two phases ahead of this warp)
+    auto skip_block = [&]() {
+      for (int v = 0; v < 2 && ok; ++v) {
+        if (!(ok = wait(kBFull + ring.stage, ring.phase))) return;
+        if (v == 1 && (w.keys(x) & 15)) fixed_phase ^= 1u << ring.stage;
+        if (leader) mbar_arrive(bar(kBEmpty + ring.stage));
+        ring.next();
       }
+      w.next(x);
+    };
+    if (tile == 1 && x.nq <= kHalfTile && !x.dual) {
+      for (int b = 0; b < x.blocks && ok; ++b) skip_block();
       if (ok && leader) mbar_arrive(bar(kBQEmpty));
       ++it;
       continue;
     }
+    const int step = x.dual ? 2 : 1, b0 = x.dual ? tile : 0;
+    const uint64_t q_desc = train::smem_desc(sbase + kSmemQ + tile * 32768, 16, 1024);
+    if (b0 > 0) skip_block();
+    if (!ok) break;
     // The issuers of a two-tile item take turns, A before B: a turn is PV(b) and QK(b + 1)
     // of one tile, so the tiles stay half a block apart and each one's softmax runs under
     // the other's products. Issuing freely, both tiles' MMAs interleave on the pipe, both
@@ -396,46 +435,74 @@ __device__ __forceinline__ void issue_role(const Params& p, int tile, int first,
         train::umma_bf16(s_col, q_desc + off, kd + off, idesc, kk > 0);
       }
     };
-    // S(0)
+    // S of the first block
     if (!(ok = wait(kBFull + ring.stage, ring.phase)) || !(ok = take_turn())) break;
     train::tc_fence_after();
     if (leader) {
       issue_qk(ring.stage, w.keys(x));
       train::umma_commit(bar(kBSFull + tile));
       train::umma_commit(bar(kBEmpty + ring.stage));
-      if (x.blocks == 1) train::umma_commit(bar(kBQEmpty));
+      if (b0 + step >= x.blocks) train::umma_commit(bar(kBQEmpty));
     }
     __syncwarp();
     pass_turn();
     ring.next();
-    for (int b = 0; b < x.blocks && ok; ++b) {
+    for (int b = b0; b < x.blocks && ok; b += step) {
       const int keys = w.keys(x), vs = ring.stage;
-      const bool more = b + 1 < x.blocks;
-      // every wait comes before the first MMA, every commit behind the last: PV(b) and
-      // QK(b + 1) run back to back on the pipe
-      if (b == 0 && !(ok = wait(kBOFree + tile, (mine & 1) ^ 1))) break;
+      const bool more = b + step < x.blocks;
+      if (b == b0 && !(ok = wait(kBOFree + tile, (mine & 1) ^ 1))) break;
       if (!(ok = wait(kBFull + vs, ring.phase))) break;
       if (keys & 15) {
         if (!(ok = wait(kBFixed + vs, (fixed_phase >> vs) & 1))) break;
         fixed_phase ^= 1u << vs;
       }
       ring.next();
-      if (more) {
-        w.next(x);
-        if (!(ok = wait(kBFull + ring.stage, ring.phase))) break;
-      }
-      if (!(ok = take_turn())) break;
-      if (!(ok = wait(kBPFull + tile, p_phase))) break;
-      p_phase ^= 1;
-      train::tc_fence_after();
-      if (leader) {
+      w.next(x);
+      auto issue_pv = [&]() {
         const uint64_t vd = v_desc + static_cast<uint32_t>(vs * (32768 >> 4));
         const int steps = (keys + 15) >> 4;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           if (kk < steps)
             train::umma_bf16_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), instr_desc_n(1, 128),
-                                (b > 0 || kk > 0) ? 1u : 0u);
+                                (b > b0 || kk > 0) ? 1u : 0u);
+      };
+      if (x.dual) {
+        // Two chains over one ring: PV(b) releases its stage as soon as P is there; waiting
+        // for K(b + 2) first would leave every load in the ring behind the next one.
+        if (!(ok = wait(kBPFull + tile, p_phase))) break;
+        p_phase ^= 1;
+        train::tc_fence_after();
+        if (leader) {
+          issue_pv();
+          train::umma_commit(bar(kBEmpty + vs));
+          if (!more) train::umma_commit(bar(kBODone + tile));
+        }
+        __syncwarp();
+        if (b + 1 < x.blocks) skip_block();
+        if (!ok) break;
+        if (more) {
+          if (!(ok = wait(kBFull + ring.stage, ring.phase))) break;
+          if (leader) {
+            issue_qk(ring.stage, w.keys(x));
+            train::umma_commit(bar(kBSFull + tile));
+            train::umma_commit(bar(kBEmpty + ring.stage));
+            if (b + 2 * step >= x.blocks) train::umma_commit(bar(kBQEmpty));
+          }
+          __syncwarp();
+          ring.next();
+        }
+        continue;
+      }
+      // every wait comes before the first MMA, every commit behind the last: PV(b) and
+      // QK(b + 1) run back to back on the pipe
+      if (more && !(ok = wait(kBFull + ring.stage, ring.phase))) break;
+      if (!(ok = take_turn())) break;
+      if (!(ok = wait(kBPFull + tile, p_phase))) break;
+      p_phase ^= 1;
+      train::tc_fence_after();
+      if (leader) {
+        issue_pv();
         if (more) {
           issue_qk(ring.stage, w.keys(x));
           train::umma_commit(bar(kBSFull + tile));
@@ -509,6 +576,25 @@ __device__ __forceinline__ float max_n(const float (&s)[N]) {
   return fmaxf(train::max3f(a[0], a[1], a[2]), a[3]);
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 struct RowState {
   float m, l;                             // running maximum (log2 units), sum of 2^(s - m)
 };
@@ -537,37 +623,33 @@ __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, 
     st.m = m_new;
   }
   if (!first && __any_sync(0xffffffffu, raise)) {
-    // the block's S was committed behind the previous PV: O is complete
+    // the block's S was committed behind the previous PV: O is complete (16 columns at a
+    // time: the row's scores are live in registers)
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+      uint32_t o[16];
+      tmem_ld16(o_addr + 16 * c, o);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float o[32];
-      train::tmem_ld32(o_addr + 32 * c, o);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] *= alpha;
-      train::tmem_st32(o_addr + 32 * c, o);
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+      tmem_st16(o_addr + 16 * c, o);
     }
+    tmem_st_wait();
   }
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float sum[2] = {0.f, 0.f};
 #pragma unroll
-  for (int c = 0; c < kCols / 64 + (kCols < 64); ++c) {
-    constexpr int kW = kCols < 64 ? kCols / 2 : 32;
-    uint32_t pk[32];
+  for (int c = 0; c < kCols / 32; ++c) {
+    uint32_t pk[16];
 #pragma unroll
-    for (int i = 0; i < kW; ++i) {
-      const float a = ex2(fmaf(s[64 * c + 2 * i], scale_log2, -st.m));
-      const float b = ex2(fmaf(s[64 * c + 2 * i + 1], scale_log2, -st.m));
-      sum[i & 3] += a + b;
+    for (int i = 0; i < 16; ++i) {
+      const float a = ex2(fmaf(s[32 * c + 2 * i], scale_log2, -st.m));
+      const float b = ex2(fmaf(s[32 * c + 2 * i + 1], scale_log2, -st.m));
+      sum[i & 1] += a + b;
       pk[i] = pack_bf16x2(a, b);
     }
-    if constexpr (kW == 32) {
-      train::tmem_st32(s_addr + 32 * c, *reinterpret_cast<const float(*)[32]>(pk));
-    } else {
-#pragma unroll
-      for (int i = kW; i < 32; ++i) pk[i] = 0u;
-      train::tmem_st32(s_addr + 32 * c, *reinterpret_cast<const float(*)[32]>(pk));
-    }
+    tmem_st16(s_addr + 16 * c, pk);
   }
-  st.l = st.l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  tmem_st_wait();
+  st.l = st.l * alpha + (sum[0] + sum[1]);
 }
 
 __device__ __forceinline__ void softmax_role(const Params& p, float* part, int first, int last, uint32_t bars,
@@ -575,61 +657,62 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
   auto bar = [&](int i) { return bars + 8u * i; };
   const int tile = threadIdx.x >> 7;
   const int m = threadIdx.x & 127;                          // row of the tile == TMEM lane
-  const int lt = tile * kHalfTile + (m >> 1);               // query row of the item
   const uint32_t lanes = static_cast<uint32_t>(m & ~31) << 16;
   const uint32_t s_addr = tmem + lanes + kTmemS + tile * 128, o_addr = tmem + lanes + kTmemO + tile * 128;
   uint32_t s_phase = 0, o_phase = 0;
   bool ok = true;
+  ItemView nx;                                              // the next item, loaded a step ahead
+  bool nx_ok = first < last && load_item(p, first, nx);
 #pragma unroll 1
-  for (int idx = first; idx < last && ok; ++idx) {
-    int nq, blocks, len0, len1, len2, see0;                 // what the block loop keeps of the item
-    {
-      ItemView x;
-      if (!load_item(p, idx, x)) {
-        if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
-        continue;
-      }
-      nq = x.nq;
-      blocks = x.blocks;
-      len0 = x.len[0];
-      len1 = x.len[1];
-      len2 = x.len[2];
-      // the item's keys are consecutive chain positions from pos[0]
-      see0 = lt < nq ? x.visible + lt - x.pos[0] : 0;
-    }
-    if (tile == 1 && nq <= kHalfTile) continue;
-    const bool warp_ok = tile * kHalfTile + ((m & ~31) >> 1) < nq;
+  for (int idx = first; idx < last; ++idx) {
+    // what the block loop keeps of the item; its keys are consecutive chain positions
+    const bool valid = nx_ok, dual = nx.dual;
+    const int nq = nx.nq, blocks = nx.blocks;
+    const int rm = dual && tile == 1 ? (m + dual_shift(nq)) & 127 : m;     // row of the MMA tile's rows
+    const int lt = (dual ? 0 : tile * kHalfTile) + (rm >> 1);  // query row of the item
+    const bool active = valid && (tile == 0 || dual || nq > kHalfTile);
+    const bool row_ok = lt < nq, warp_ok = lt - ((rm & 31) >> 1) < nq;
+    int len0 = nx.len[0], len1 = nx.len[1], len2 = nx.len[2];
+    int see0 = row_ok ? nx.visible + lt - nx.pos[0] : 0;
+    if (!valid && threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
     RowState st{-1e30f, 0.f};
+    if (active) {
+      const int b0 = dual ? tile : 0;
 #pragma unroll 1
-    for (int b = 0; b < blocks; ++b) {
-      ok = train::wait_or_abort(bar(kBSFull + tile), s_phase, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
+      for (int b = 0; b < blocks; ++b) {
+        const int keys = min(kBlock, len0);
+        if (!dual || (b & 1) == tile) {
+          ok = train::wait_or_abort(bar(kBSFull + tile), s_phase, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          s_phase ^= 1;
+          if (warp_ok) {
+            train::tc_fence_after();
+            if (keys > 32)
+              softmax_block<128>(s_addr, o_addr, min(keys, see0), p.scale_log2, b == b0, st);
+            else
+              softmax_block<32>(s_addr, o_addr, min(keys, see0), p.scale_log2, b == b0, st);
+            train::tc_fence_before();
+          }
+          __syncwarp();
+          if ((threadIdx.x & 31) == 0) mbar_arrive(bar(kBPFull + tile));
+        }
+        see0 -= keys;
+        len0 -= keys;
+        if (len0 == 0) {
+          len0 = len1;
+          len1 = len2;
+          len2 = 0;
+        }
       }
-      s_phase ^= 1;
-      const int keys = min(kBlock, len0);
-      if (warp_ok) {
-        train::tc_fence_after();
-        if (keys > 32)
-          softmax_block<128>(s_addr, o_addr, min(keys, see0), p.scale_log2, b == 0, st);
-        else
-          softmax_block<32>(s_addr, o_addr, min(keys, see0), p.scale_log2, b == 0, st);
-        train::tc_fence_before();
-      }
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(bar(kBPFull + tile));
-      see0 -= keys;
-      len0 -= keys;
-      if (len0 == 0) {
-        len0 = len1;
-        len1 = len2;
-        len2 = 0;
-      }
+      if (!ok) break;
     }
-    if (!ok) break;
-    ItemView x;
-    load_item(p, idx, x);                                   // again: its registers were the scores'
+    const int4 where = __ldg(reinterpret_cast<const int4*>(p.plan + p.items_at + static_cast<size_t>(idx) * kItemWords));
+    const int q0 = where.x, head = where.z, slot = where.w;    // (their registers were the scores')
+    nx_ok = idx + 1 < last && load_item(p, idx + 1, nx);
+    if (!active) continue;
     if (blocks > 0) {
       ok = train::wait_or_abort(bar(kBODone + tile), o_phase, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
@@ -639,41 +722,38 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
       o_phase ^= 1;
       train::tc_fence_after();
     }
+    const float inv = st.l > 0.f ? 1.f / st.l : (st.l != st.l ? st.l : 0.f);   // (a NaN sum stays NaN)
+    float* prow = part + static_cast<size_t>(max(slot, 0) + tile) * (kSlotFloats + 128);
+    __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) +
+                          (static_cast<size_t>(q0 + (row_ok ? lt : 0)) * kQHeads + 2 * head + (rm & 1)) * kHeadDim;
     if (warp_ok) {
-      const bool row_ok = lt < nq;
-      const float inv = st.l > 0.f ? 1.f / st.l : 0.f;
-      float* prow = part + static_cast<size_t>(max(x.slot, 0) + tile) * (kSlotFloats + 128);
-      __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) +
-                            (static_cast<size_t>(x.q0 + (row_ok ? lt : 0)) * kQHeads + 2 * x.head + (m & 1)) * kHeadDim;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float o[32];
-        if (blocks > 0) {
-          train::tmem_ld32(o_addr + 32 * c, o);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = st.l > 0.f ? o[i] * inv : 0.f;
-        if (row_ok && x.slot < 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 v;
-            v.x = pack_bf16x2(o[8 * j], o[8 * j + 1]);
-            v.y = pack_bf16x2(o[8 * j + 2], o[8 * j + 3]);
-            v.z = pack_bf16x2(o[8 * j + 4], o[8 * j + 5]);
-            v.w = pack_bf16x2(o[8 * j + 6], o[8 * j + 7]);
-            *reinterpret_cast<uint4*>(orow + 32 * c + 8 * j) = v;
-          }
-        } else if (row_ok) {
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r0[32], r1[32];
+        train::tmem_ld32_async(o_addr + 64 * c, r0);
+        train::tmem_ld32_async(o_addr + 64 * c + 32, r1);
+        train::tmem_ld_wait();
+        train::tmem_ld_landed(r0);
+        train::tmem_ld_landed(r1);
+        // (without a visible key O was never written, or holds products of zeros)
+        auto o = [&](int i) {
+          return inv != 0.f ? __uint_as_float(i < 32 ? r0[i & 31] : r1[i & 31]) * inv : 0.f;
+        };
+        if (row_ok && slot < 0) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            __stcg(reinterpret_cast<float4*>(prow + (8 * c + j) * 512 + 4 * m),
-                   make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
+            *reinterpret_cast<uint4*>(orow + 64 * c + 8 * j) =
+                make_uint4(pack_bf16x2(o(8 * j), o(8 * j + 1)), pack_bf16x2(o(8 * j + 2), o(8 * j + 3)),
+                           pack_bf16x2(o(8 * j + 4), o(8 * j + 5)), pack_bf16x2(o(8 * j + 6), o(8 * j + 7)));
+        } else if (row_ok) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            __stcg(reinterpret_cast<float4*>(prow + (16 * c + j) * 512 + 4 * rm),
+                   make_float4(o(4 * j), o(4 * j + 1), o(4 * j + 2), o(4 * j + 3)));
         }
       }
-      if (row_ok && x.slot >= 0) __stcg(prow + kSlotFloats + m, st.l > 0.f ? st.m + log2f(st.l) : -INFINITY);
+      if (row_ok && slot >= 0)
+        __stcg(prow + kSlotFloats + rm, st.l > 0.f ? st.m + log2f(st.l) : (st.l != st.l ? st.l : -INFINITY));
     }
     if (blocks > 0) {
       train::tc_fence_before();
@@ -690,7 +770,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem), bars = sbase + kSmemBar;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemAbort);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   int first = 0, last = 0;
   if (plan_ok(p) && p.plan[kHGrid] == static_cast<int>(gridDim.x)) {
     const int* offs = p.plan + p.plan[kHCtaAt] + blockIdx.x;
@@ -729,8 +809,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   } else if (warp < 10) {
     issue_role(p, warp - 8, first, last, sbase, bars, tmem, abort_flag);
   } else if (warp == 10) {
-    if (lane == 0) producer_role(p, maps, first, last, sbase, bars, abort_flag);
-    __syncwarp();
+    producer_role(p, maps, first, last, sbase, bars, abort_flag);
   } else {
     fix_role(p, first, last, smem, bars, abort_flag);
   }
@@ -740,33 +819,47 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   if (warp == 8) train::tmem_dealloc(tmem, 512);
 }
 
-// Combines the partial rows: one warp per (query row, KV head), both of its query heads
-// (adjacent rows of a slot, so a lane reads whole 32-byte sectors); lane l owns d = 4 l ..
+// Combines the partial rows of a query row's head pair (adjacent rows of a slot, so a lane
+// reads whole 32-byte sectors); lane l owns d = 4 l ..
 //   out = sum_c 2^(L_c - M) o_c / sum_c 2^(L_c - M),  M = max_c L_c
+// kWarps = 1: a warp per (query row, KV head), 8 to a CTA. kWarps = 8: a CTA per pair, its
+// warps taking every eighth contribution, for the many pieces of a long prefix behind few
+// rows (18 pieces of 32768 keys behind 8 rows: one warp each walked them in 16 us); with
+// many rows the warps are there anyway (1024 rows of 8 parts: 14 us slower in CTAs).
+constexpr int kMergeWideParts = 6, kMergeWidePairs = 2048;
+
+template <int kWarps>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const float* part) {
+  __shared__ float s_acc[kWarps > 1 ? 8 : 1][8][33];
+  __shared__ float2 s_den[8];
   if (!plan_ok(p)) return;
-  const int lane = threadIdx.x & 31;
-  const long long u = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long u = kWarps > 1 ? static_cast<long long>(blockIdx.x) : static_cast<long long>(blockIdx.x) * 8 + warp;
   if (u >= static_cast<long long>(p.total_q) * kHeads) return;
   const int t = static_cast<int>(u / kHeads), h = static_cast<int>(u % kHeads);
-  const int run = p.plan[p.plan[kHTokenRunAt] + t];
-  if (run < 0 || run >= p.plan[kHRuns]) return;
-  const int* w = p.plan + p.plan[kHRunsAt] + static_cast<size_t>(run) * kRunWords;
+  const int run = p.plan[p.token_run_at + t];
+  if (run < 0 || run >= p.runs) return;
+  const int* w = p.plan + p.runs_at + static_cast<size_t>(run) * kRunWords;
   const int4 k0 = *reinterpret_cast<const int4*>(w + kRunTile0);
   const int4 k1 = *reinterpret_cast<const int4*>(w + kRunTile0 + kRunTileWords);
-  const int n0 = k0.y, total = n0 + (w[kRunTiles] > 1 ? k1.y : 0);
+  // (a dual tile's pieces are two contributions each, in consecutive slots)
+  const bool d0 = k0.z == kDualSlots, d1 = k1.z == kDualSlots;
+  const int n0 = k0.y << d0, total = n0 + (w[kRunTiles] > 1 ? k1.y << d1 : 0);
   const int lt0 = t - k0.w, lt1 = t - k1.w;
-  // floats before contribution c's slot, and its first row (head 0)
   auto base = [&](int c) -> const float* {
     const bool first = c < n0;
-    const int slot = first ? k0.x + (c * kHeads + h) * k0.z + (lt0 >> 6)
-                           : k1.x + ((c - n0) * kHeads + h) * k1.z + (lt1 >> 6);
+    const bool dual = first ? d0 : d1;
+    const int4 k = first ? k0 : k1;
+    const int i = first ? c : c - n0, lt = first ? lt0 : lt1;
+    const int slot = dual ? k.x + ((i >> 1) * kHeads + h) * 2 + (i & 1) : k.x + (i * kHeads + h) * k.z + (lt >> 6);
     return part + static_cast<size_t>(min(max(slot, 0), p.slots - 1)) * (kSlotFloats + 128);
   };
   auto row_of = [&](int c) { return 2 * ((c < n0 ? lt0 : lt1) & 63); };
+  auto lse = [&](int c) { return __ldcg(reinterpret_cast<const float2*>(base(c) + kSlotFloats + row_of(c))); };
   float2 top = make_float2(-INFINITY, -INFINITY);
   for (int c = lane; c < total; c += 32) {
-    const float2 v = __ldcg(reinterpret_cast<const float2*>(base(c) + kSlotFloats + row_of(c)));
+    const float2 v = lse(c);
+    // fmaxf drops a NaN: it comes back through the weights below
     top.x = fmaxf(top.x, v.x);
     top.y = fmaxf(top.y, v.y);
   }
@@ -778,34 +871,39 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const
   // a row whose contributions all see nothing: weights 0
   const float mx = top.x > -INFINITY ? top.x : 0.f, my = top.y > -INFINITY ? top.y : 0.f;
   float a[8] = {}, den0 = 0.f, den1 = 0.f;
-  for (int c0 = 0; c0 < total; c0 += 32) {
-    const int c = c0 + lane;
-    float2 f = make_float2(0.f, 0.f);
-    if (c < total) {
-      f = __ldcg(reinterpret_cast<const float2*>(base(c) + kSlotFloats + row_of(c)));
-      f.x = ex2(f.x - mx);
-      f.y = ex2(f.y - my);
-    }
-    const int n = min(32, total - c0);
+  const int c_first = kWarps > 1 ? warp : 0;
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float f0 = __shfl_sync(0xffffffffu, f.x, i), f1 = __shfl_sync(0xffffffffu, f.y, i);
-      const float4* src =
-          reinterpret_cast<const float4*>(base(c0 + i) + static_cast<size_t>(lane) * 512 + 4 * row_of(c0 + i));
-      const float4 v0 = __ldcg(src), v1 = __ldcg(src + 1);
-      den0 += f0;
-      den1 += f1;
-      a[0] = fmaf(f0, v0.x, a[0]);
-      a[1] = fmaf(f0, v0.y, a[1]);
-      a[2] = fmaf(f0, v0.z, a[2]);
-      a[3] = fmaf(f0, v0.w, a[3]);
-      a[4] = fmaf(f1, v1.x, a[4]);
-      a[5] = fmaf(f1, v1.y, a[5]);
-      a[6] = fmaf(f1, v1.z, a[6]);
-      a[7] = fmaf(f1, v1.w, a[7]);
+  for (int c = c_first; c < total; c += kWarps) {
+    const float2 f = lse(c);
+    const float4* src = reinterpret_cast<const float4*>(base(c) + static_cast<size_t>(lane) * 512 + 4 * row_of(c));
+    const float4 v0 = __ldcg(src), v1 = __ldcg(src + 1);
+    const float f0 = ex2(f.x - mx), f1 = ex2(f.y - my);
+    den0 += f0;
+    den1 += f1;
+    a[0] = fmaf(f0, v0.x, a[0]);
+    a[1] = fmaf(f0, v0.y, a[1]);
+    a[2] = fmaf(f0, v0.z, a[2]);
+    a[3] = fmaf(f0, v0.w, a[3]);
+    a[4] = fmaf(f1, v1.x, a[4]);
+    a[5] = fmaf(f1, v1.y, a[5]);
+    a[6] = fmaf(f1, v1.z, a[6]);
+    a[7] = fmaf(f1, v1.w, a[7]);
+  }
+  if (kWarps > 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_acc[warp][i][lane] = a[i];
+    if (lane == 0) s_den[warp] = make_float2(den0, den1);
+    __syncthreads();
+    if (warp != 0) return;
+    for (int o = 1; o < 8; ++o) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] += s_acc[o][i][lane];
+      den0 += s_den[o].x;
+      den1 += s_den[o].y;
     }
   }
-  const float i0 = den0 > 0.f ? 1.f / den0 : 0.f, i1 = den1 > 0.f ? 1.f / den1 : 0.f;
+  auto inverse = [](float d) { return d > 0.f ? 1.f / d : (d != d ? d : 0.f); };
+  const float i0 = inverse(den0), i1 = inverse(den1);
   __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (static_cast<size_t>(t) * kQHeads + 2 * h) * kHeadDim + 4 * lane;
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a[0] * i0, a[1] * i0), pack_bf16x2(a[2] * i0, a[3] * i0));
   *reinterpret_cast<uint2*>(dst + kHeadDim) =

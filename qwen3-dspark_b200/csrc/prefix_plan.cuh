@@ -42,22 +42,28 @@ constexpr int kAllVisible = 1 << 30;
 
 enum Head {
   kHMagic = 0, kHRequests, kHTotalQ, kHGrid, kHItems, kHCtaAt, kHItemsAt, kHRequestsAt, kHSlots, kHRuns, kHRunsAt,
-  kHTokenRunAt, kHPrefixRows, kHOwnRows, kHNewRows, kHCausal, kHMaxQ, kHWords, kHCheck
+  kHTokenRunAt, kHPrefixRows, kHOwnRows, kHNewRows, kHCausal, kHMaxQ, kHWords, kHCheck, kHMaxParts
 };
 // Request record: first query row, query rows, then (first row, rows) of prefix, own, new.
 enum RequestField { kRQ0 = 0, kRNq, kRPrefixRow, kRPrefixLen, kROwnRow, kROwnLen, kRNewRow, kRNewLen };
 // Item record: a tile, a KV head and a piece of the tile's key chain. Query row t of
 // the item sees the keys whose chain position is below kIVisible + t.
 enum ItemField {
-  kIQ0 = 0, kINq, kIHead, kISlot /* -1: write the output */, kIVisible, kISegs, kISeg0 = 8,
+  kIQ0 = 0, kINq, kIHead, kISlot /* -1: write the output */, kIVisible, kISegs,
+  kIDual /* one MMA tile's rows, even key blocks on tile A and odd ones on tile B */, kISeg0 = 8,
   kISegWords = 4 /* source (0 prefix, 1 own, 2 new), first row, keys, chain position of the first key */
 };
 // Run record: query rows [kRunQ0, + kRunNq) merge the same tiles' partials.
-enum RunField { kRunQ0 = 0, kRunNq, kRunTiles, kRunTile0 = 4, kRunTileWords = 4 /* slot, pieces, MMA tiles, q0 */ };
+enum RunField {
+  kRunQ0 = 0, kRunNq, kRunTiles, kRunTile0 = 4,
+  kRunTileWords = 4 /* slot, pieces, slots per (piece, head): 1, 2 or kDualSlots, q0 */
+};
+constexpr int kDualSlots = 3;              // two slots, both holding (part of) every row
 
 // Costs the schedule balances, in units of one two-tile key block.
 constexpr double kCostPair = 1.0;
-constexpr double kCostSingle = 0.7;
+constexpr double kCostSingle = 0.9;
+constexpr double kCostDual = 0.6;
 constexpr double kCostItem = 1.6;
 constexpr double kCostPartial = 0.5;       // writing one MMA tile's partial rows (and reading them back)
 constexpr int kChainRows = 96;             // mean query rows from which a group's requests get chain tiles
@@ -74,7 +80,17 @@ struct PlanTile {
   bool complete;      // holds every key of its rows
   int blocks;
   int pieces, slot;
+  bool dual;
+  int slots() const { return dual || nq > kHalfTile ? 2 : 1; }
 };
+
+// Whether a one-tile piece runs its blocks on both MMA tiles: a single tile's chain
+// (product, softmax, product) is bound by its latency, two of them overlap. A complete
+// tile pays with a merge, which is worth it from kDualBlocks blocks.
+constexpr int kDualBlocks = 8;
+inline bool dual_piece(int nq, bool complete, int blocks, int pieces) {
+  return nq <= kHalfTile && blocks / pieces >= 2 && (!complete || pieces > 1 || blocks >= kDualBlocks);
+}
 
 inline int blocks_of(const Seg& s) { return (s.len + kBlock - 1) / kBlock; }
 
@@ -106,9 +122,10 @@ inline void add_tiles(std::vector<PlanTile>& tiles, int q0, int nq, const Seg* s
   }
 }
 
-inline double piece_cost(const PlanTile& t, int blocks, bool direct) {
+inline double piece_cost(const PlanTile& t, int blocks, bool direct, bool dual) {
   const bool pair = t.nq > kHalfTile;
-  return kCostItem + blocks * (pair ? kCostPair : kCostSingle) + (direct ? 0.0 : kCostPartial * (pair ? 2 : 1));
+  return kCostItem + blocks * (pair ? kCostPair : (dual ? kCostDual : kCostSingle)) +
+         (direct ? 0.0 : kCostPartial * (pair ? 2 : 1));
 }
 
 // Largest-first assignment of the pieces' costs to `grid` CTAs; returns the makespan.
@@ -210,12 +227,12 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   // Cut the chains: try several piece lengths and keep the shortest schedule. Pieces
   // are the same for the 8 KV heads, so a slot index is computed from (piece, head).
   double total = 0.0;
-  for (const PlanTile& t : tiles) total += kHeads * piece_cost(t, t.blocks, t.complete);
+  for (const PlanTile& t : tiles) total += kHeads * piece_cost(t, t.blocks, t.complete, dual_piece(t.nq, t.complete, t.blocks, 1));
   auto cut = [&](double target, std::vector<int>& pieces) {
     pieces.resize(tiles.size());
     for (size_t i = 0; i < tiles.size(); ++i) {
       const PlanTile& t = tiles[i];
-      const double per = t.nq > kHalfTile ? kCostPair : kCostSingle;
+      const double per = t.nq > kHalfTile ? kCostPair : kCostDual;
       const double room = std::max(per, target - kCostItem);
       pieces[i] = static_cast<int>(std::max(1.0, std::min<double>(t.blocks, std::ceil(t.blocks * per / room))));
     }
@@ -227,7 +244,8 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
         for (int p = 0; p < pieces[i]; ++p) {
           const int b0 = static_cast<int>(static_cast<long long>(tiles[i].blocks) * p / pieces[i]);
           const int b1 = static_cast<int>(static_cast<long long>(tiles[i].blocks) * (p + 1) / pieces[i]);
-          cost.push_back(piece_cost(tiles[i], b1 - b0, tiles[i].complete && pieces[i] == 1));
+          const bool dual = dual_piece(tiles[i].nq, tiles[i].complete, tiles[i].blocks, pieces[i]);
+          cost.push_back(piece_cost(tiles[i], b1 - b0, tiles[i].complete && pieces[i] == 1 && !dual, dual));
         }
   };
   std::vector<int> pieces, best;
@@ -249,9 +267,10 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
     PlanTile& t = tiles[i];
     t.pieces = best[i];
     t.slot = -1;
-    if (!(t.complete && t.pieces == 1)) {
+    t.dual = dual_piece(t.nq, t.complete, t.blocks, t.pieces);
+    if (!(t.complete && t.pieces == 1 && !t.dual)) {
       t.slot = static_cast<int>(slots);
-      slots += static_cast<long long>(t.pieces) * kHeads * (t.nq > kHalfTile ? 2 : 1);
+      slots += static_cast<long long>(t.pieces) * kHeads * t.slots();
       if (slots > kLimit) return kPlanTooLarge;
     }
   }
@@ -272,7 +291,8 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
         it[kIQ0] = t.q0;
         it[kINq] = t.nq;
         it[kIHead] = h;
-        it[kISlot] = t.slot < 0 ? -1 : t.slot + (p * kHeads + h) * (t.nq > kHalfTile ? 2 : 1);
+        it[kISlot] = t.slot < 0 ? -1 : t.slot + (p * kHeads + h) * t.slots();
+        it[kIDual] = t.dual ? 1 : 0;
         it[kIVisible] = t.visible;
         int at = 0, pos = 0, n = 0;
         for (int s = 0; s < t.nsegs; ++s) {
@@ -295,6 +315,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
 
   // Merge runs: maximal row ranges whose rows merge the same tiles.
   std::vector<int32_t> runs, token_run;
+  int max_parts = 0;                             // partial rows that one output row merges
   if (slots > 0) {
     token_run.assign(q0, -1);
     auto add_run = [&](int a, int b, const PlanTile* x, const PlanTile* y) {
@@ -304,15 +325,17 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
       int32_t* w = runs.data() + static_cast<size_t>(id) * kRunWords;
       w[kRunQ0] = a;
       w[kRunNq] = b - a;
-      int n = 0;
+      int n = 0, parts = 0;
       for (const PlanTile* t : {x, y})
         if (t) {
           int32_t* k = w + kRunTile0 + kRunTileWords * n++;
           k[0] = t->slot;
           k[1] = t->pieces;
-          k[2] = t->nq > kHalfTile ? 2 : 1;
+          k[2] = t->dual ? kDualSlots : t->slots();
           k[3] = t->q0;
+          parts += t->pieces * (t->dual ? 2 : 1);
         }
+      max_parts = std::max(max_parts, parts);
       w[kRunTiles] = n;
       std::fill(token_run.begin() + a, token_run.begin() + b, id);
     };
@@ -364,6 +387,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   plan[kHNewRows] = static_cast<int32_t>(new_rows);
   plan[kHCausal] = in.causal ? 1 : 0;
   plan[kHMaxQ] = max_q;
+  plan[kHMaxParts] = max_parts;
   plan[kHWords] = static_cast<int32_t>(words);
   int next = 0;
   for (int c = 0; c < grid; ++c) {

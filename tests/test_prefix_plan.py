@@ -28,15 +28,30 @@ def interpret(plan, x, case):
     offs = plan[cta_at:cta_at + grid + 1]
     assert offs[0] == 0 and offs[-1] == n_items and (np.diff(offs) >= 0).all()
     for it in plan[items_at:items_at + n_items * ITEM].reshape(n_items, ITEM):
-        q0, nq, head, slot, visible, nseg = (int(v) for v in it[:6])
+        q0, nq, head, slot, visible, nseg, dual = (int(v) for v in it[:7])
         assert 1 <= nq <= 128 and 0 <= head < 8 and 0 <= nseg <= 3
-        keys, values, pos = [], [], []
+        keys, values, pos, block, len_b = [], [], [], [], 0
         for s in range(nseg):
             which, row, n, at = (int(v) for v in it[8 + 4 * s:12 + 4 * s])
             assert n >= 1
             keys.append(src[which][0][row:row + n, head])
             values.append(src[which][1][row:row + n, head])
             pos.append(torch.arange(at, at + n))
+            block += [len_b + i // BLOCK for i in range(n)]
+            len_b += -(-n // BLOCK)
+        if dual:                       # even blocks to the first slot, odd ones to the second
+            assert nq <= 64 and slot >= 0 and len_b >= 2
+            k, v, p, b = torch.cat(keys), torch.cat(values), torch.cat(pos), torch.tensor(block)
+            for half in range(2):
+                for t in range(nq):
+                    for g in range(2):
+                        see = (p < visible + t) & (b % 2 == half)
+                        s = (k[see] @ q[q0 + t, 2 * head + g]) * SCALE
+                        key = (slot + half, 2 * t + g)
+                        assert key not in part and key[0] < slots
+                        part[key] = ((torch.logsumexp(s, 0), torch.softmax(s, 0) @ v[see]) if see.any()
+                                     else (torch.tensor(-np.inf), torch.zeros(D, dtype=torch.float64)))
+            continue
         for t in range(nq):
             for g in range(2):
                 h = 2 * head + g
@@ -69,6 +84,9 @@ def interpret(plan, x, case):
                     slot, pieces, mma, q0 = (int(v) for v in run[4 + 4 * c:8 + 4 * c])
                     lt = t - q0
                     for p in range(pieces):
+                        if mma == 3:
+                            parts += [part[(slot + (p * 8 + h // 2) * 2 + i, 2 * lt + (h & 1))] for i in range(2)]
+                            continue
                         parts.append(part[(slot + (p * 8 + h // 2) * mma + (lt >> 6), 2 * (lt & 63) + (h & 1))])
                 lse = torch.stack([torch.as_tensor(a, dtype=torch.float64) for a, _ in parts])
                 top = torch.logsumexp(lse, 0)
