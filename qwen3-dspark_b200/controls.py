@@ -18,7 +18,7 @@ import math
 import torch
 
 from . import _lib
-from .kernels import _DTYPES, _stream
+from .kernels import _DTYPES, _on_device, _stream
 from .kv_store import _upload
 
 
@@ -49,6 +49,11 @@ class TokenControls:
         self.bias_ids = torch.zeros((slots, max_bias), dtype=torch.int32, **dev)
         self.bias_values = torch.zeros((slots, max_bias), dtype=torch.float32, **dev)
         self.bias_len = torch.zeros(slots, dtype=torch.int32, **dev)
+        # the tables stay where they are: the kernels' arguments that name them
+        self._table_args = (self.counts.data_ptr(), self.counts.stride(0), self.prompt_bits.data_ptr(),
+                            self.prompt_bits.stride(0), self.penalties.data_ptr(), slots,
+                            self.bias_ids.data_ptr() if max_bias else None,
+                            self.bias_values.data_ptr() if max_bias else None, self.bias_len.data_ptr(), max_bias)
         self._slots = {}
         self._free = list(range(slots))
 
@@ -114,7 +119,7 @@ class TokenControls:
         return _upload([self._slots[r] for r in requests], self.device)
 
     def _add(self, tokens, cu, n, slots, to_counts):
-        with torch.cuda.device(self.device):
+        with _on_device(self.device):
             _lib.check(_lib.load_library().dspark_control_tokens(
                 tokens.data_ptr(), tokens.numel(), cu.data_ptr(), None if n is None else n.data_ptr(),
                 slots.data_ptr(), slots.numel(), self.vocab, self.slots,
@@ -142,39 +147,46 @@ def _row(values, device):
 
 
 def _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index):
-    device = controls.device
+    device, vocab = controls.device, controls.vocab
     if (not isinstance(logits, torch.Tensor) or logits.ndim != 2 or logits.dtype not in _DTYPES
-            or logits.device != device or logits.shape[1] != controls.vocab or logits.stride(1) != 1
-            or (logits.shape[0] > 1 and logits.stride(0) < controls.vocab) or logits.requires_grad):
-        raise ValueError('logits must be no-autograd bf16/fp32 [N, vocab] rows with unit column stride on the tables\' '
-                         'device')
-    n, r = logits.shape[0], slots.numel()
+            or logits.device != device or logits.requires_grad):
+        raise ValueError("logits must be no-autograd bf16/fp32 [N, vocab] rows on the tables' device")
+    (n, columns), (ld, step) = logits.shape, logits.stride()
+    if columns != vocab or step != 1 or (n > 1 and ld < vocab):
+        raise ValueError('logits must have vocab columns with unit stride and rows that do not overlap')
+    r = slots.numel()
     if slots.dtype != torch.int32 or slots.ndim != 1 or slots.device != device or not slots.is_contiguous() or r < 1:
-        raise ValueError('slots must be contiguous int32 [R] on the tables\' device')
+        raise ValueError("slots must be contiguous int32 [R] on the tables' device")
+    cu = token = mask = index = None
+    ld_mask = num_masks = 0
     if cu_query is None:
         if n != r or tokens is not None:
             raise ValueError('Without cu_query there is one row per request, and no proposals')
-    elif (cu_query.dtype != torch.int32 or cu_query.shape != (r + 1,) or cu_query.device != device
-          or not cu_query.is_contiguous()):
-        raise ValueError('cu_query must be contiguous int32 [R + 1] on the tables\' device')
-    if tokens is not None and (tokens.dtype != torch.long or tokens.shape != (n,) or tokens.device != device
-                               or not tokens.is_contiguous()):
-        raise ValueError('tokens must be contiguous int64 [N] on the tables\' device')
+    else:
+        if (cu_query.dtype != torch.int32 or cu_query.ndim != 1 or len(cu_query) != r + 1
+                or cu_query.device != device or not cu_query.is_contiguous()):
+            raise ValueError("cu_query must be contiguous int32 [R + 1] on the tables' device")
+        cu = cu_query.data_ptr()
+    if tokens is not None:
+        if (tokens.dtype != torch.long or tokens.ndim != 1 or len(tokens) != n or tokens.device != device
+                or not tokens.is_contiguous()):
+            raise ValueError("tokens must be contiguous int64 [N] on the tables' device")
+        token = tokens.data_ptr()
     if (masks is None) != (mask_index is None):
         raise ValueError('masks and mask_index go together')
-    if masks is not None and (masks.dtype != torch.int32 or masks.ndim != 2 or masks.shape[1] < controls.words
-                              or masks.shape[0] < 1 or masks.stride(1) != 1 or masks.stride(0) < controls.words
-                              or masks.device != device or mask_index.dtype != torch.int32
-                              or mask_index.shape != (n,) or mask_index.device != device
-                              or not mask_index.is_contiguous()):
-        raise ValueError('masks must be int32 [M, ceil(vocab / 32)] and mask_index int32 [N] on the tables\' device')
-    c = controls
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    return [logits.data_ptr(), max(logits.stride(0), c.vocab), _DTYPES[logits.dtype], n, c.vocab, ptr(cu_query),
-            ptr(tokens), slots.data_ptr(), r, c.counts.data_ptr(), c.counts.stride(0), c.prompt_bits.data_ptr(),
-            c.prompt_bits.stride(0), c.penalties.data_ptr(), c.slots, c.bias_ids.data_ptr() if c.max_bias else None,
-            c.bias_values.data_ptr() if c.max_bias else None, c.bias_len.data_ptr(), c.max_bias, ptr(masks),
-            0 if masks is None else masks.stride(0), 0 if masks is None else masks.shape[0], ptr(mask_index)]
+    if masks is not None:
+        words = controls.words
+        if (masks.dtype != torch.int32 or masks.ndim != 2 or masks.device != device
+                or mask_index.dtype != torch.int32 or mask_index.ndim != 1 or len(mask_index) != n
+                or mask_index.device != device or not mask_index.is_contiguous()):
+            raise ValueError("masks must be int32 [M, ceil(vocab / 32)] and mask_index int32 [N] on the tables' device")
+        (num_masks, wide), (ld_mask, step) = masks.shape, masks.stride()
+        if num_masks < 1 or wide < words or step != 1 or (num_masks > 1 and ld_mask < words):
+            raise ValueError('masks must have ceil(vocab / 32) words a row with unit stride')
+        ld_mask = max(ld_mask, words)
+        mask, index = masks.data_ptr(), mask_index.data_ptr()
+    return (logits.data_ptr(), max(ld, vocab), _DTYPES[logits.dtype], n, vocab, cu, token, slots.data_ptr(), r,
+            *controls._table_args, mask, ld_mask, num_masks, index)
 
 
 def control_logits(logits, controls, slots, *, cu_query=None, tokens=None, masks=None, mask_index=None,
@@ -196,9 +208,9 @@ def control_logits(logits, controls, slots, *, cu_query=None, tokens=None, masks
         raise ValueError('out has another dtype than out_dtype')
     if (out.shape != logits.shape or out.device != logits.device or out.stride(1) != 1
             or (len(out) > 1 and out.stride(0) < controls.vocab)
-            or out.dtype not in (logits.dtype, torch.float32)):
+            or (out.dtype != logits.dtype and out.dtype != torch.float32)):
         raise ValueError('out must be [N, vocab] rows of the logits\' dtype or float32 on their device')
-    with torch.cuda.device(logits.device):
+    with _on_device(logits.device):
         _lib.check(_lib.load_library().dspark_control_logits(
             *args, float(mask_value), out.data_ptr(), max(out.stride(0), controls.vocab), _DTYPES[out.dtype],
             _stream(logits.device)), 'dspark_control_logits')
@@ -212,7 +224,7 @@ def control_argmax(logits, controls, slots, *, cu_query=None, tokens=None, masks
     device status bit ``DEVICE_EMPTY_MASK``."""
     args = _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index)
     lib = _lib.load_library()
-    with torch.cuda.device(logits.device):
+    with _on_device(logits.device):
         pred = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
         nbytes = int(lib.dspark_control_argmax_scratch_bytes(*logits.shape))
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)

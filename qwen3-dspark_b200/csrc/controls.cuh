@@ -9,10 +9,14 @@
 // the same steps in torch float32. A forbidden entry is selected, never added to, so
 // infinities and NaN there do not spread.
 //
-// A request's tables (counts 2 bytes, prompt bits 1/8 byte per token) are read once per
-// vocabulary chunk and serve all rows of its chunk: one CTA owns (request, 2048 tokens),
-// keeps the chunk's counts and biases in registers and walks the rows, adding each row's
-// proposal to the count of the thread that owns it.
+// One CTA owns (request, 4096 tokens) and serves all rows of the request's chunk, so the
+// request's tables (counts 2 bytes, prompt bits 1/8 byte per token) are read once. Few tokens
+// are seen or biased: they go into a list in shared memory first. Then the rows stream
+// through untouched - bf16 stays packed, masks are applied to pairs, maxima are packed - and
+// a second pass over the list computes the penalised values and stores them over, or
+// compares them. The streaming pass is bound by DRAM; with the penalties inside it (per
+// token, or in loops over set bits) the instructions bound it: 896 rows x 151936 tokens
+// took 252 and 165 us.
 #pragma once
 #include "accept.cuh"
 
@@ -20,9 +24,11 @@ namespace dspark {
 namespace controls {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 8;                        // tokens per thread
+constexpr int kPer = 16;                       // tokens per thread: two runs of 8
 constexpr int kChunk = kThreads * kPer;
-constexpr int kRowBatch = 16;                  // argmax rows reduced per barrier
+constexpr int kRun = kThreads * 8;             // tokens between a thread's two runs
+constexpr int kListCap = 512;                  // biases of a chunk staged in shared memory
+constexpr int kRowBatch = 16;                  // rows whose indices are staged at a time
 constexpr int kMaxCount = 32767;               // counts saturate here
 
 struct Params {
@@ -64,36 +70,102 @@ __device__ __forceinline__ bool request_rows(const Params& p, int r, int& q0, in
   return q0 >= 0 && nq >= 0 && q1 <= p.rows;
 }
 
-// Order-preserving key of a candidate: NaN above numbers, -0 equal to +0, then the
-// lowest index. 0 is no candidate.
-__device__ __forceinline__ unsigned long long arg_key(float z, int v) {
-  uint32_t u = __float_as_uint(z + 0.f);
-  u = z != z ? 0xffffffffu : ((u & 0x80000000u) ? ~u : u | 0x80000000u);
-  return (static_cast<unsigned long long>(u) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
+// Order-preserving key of a number: NaN above all, -0 equal to +0; never 0.
+__device__ __forceinline__ uint32_t order_key(float z) {
+  const uint32_t u = __float_as_uint(z + 0.f);
+  return z != z ? 0xffffffffu : ((u & 0x80000000u) ? ~u : u | 0x80000000u);
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 __device__ __forceinline__ unsigned long long max_u64(unsigned long long a, unsigned long long b) {
   return a > b ? a : b;
 }
 
-template <typename T>
-__device__ __forceinline__ void put(T* dst, float z);
-template <>
-__device__ __forceinline__ void put<float>(float* dst, float z) { *dst = z; }
-template <>
-__device__ __forceinline__ void put<__nv_bfloat16>(__nv_bfloat16* dst, float z) { *dst = __float2bfloat16_rn(z); }
+// a / b rounded to nearest, from r = 1 / b rounded to nearest: q = a r is within an ulp, its
+// residual a - q b is exact in one fma, and q + (a - q b) r rounds to the quotient
+// (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990) as long as nothing over- or underflows; __fdiv_rn otherwise. A
+// penalised warp is bound by its instructions, and this takes four.
+constexpr float kDivLow = 1e-20f, kDivHigh = 1e20f;
+__device__ __forceinline__ float divide(float a, float b, float r, bool b_safe) {
+  if (b_safe && a > kDivLow && a < kDivHigh) {
+    const float q = __fmul_rn(a, r);
+    return __fmaf_rn(__fmaf_rn(-q, b, a), r, q);
+  }
+  return __fdiv_rn(a, b);
+}
 
-// kVec: rows of every table start on 16-byte boundaries and a thread owns 8 consecutive
-// tokens (16-byte accesses); otherwise its tokens lie 256 apart, so that the element
-// accesses of a warp stay contiguous whatever the row's alignment.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 32 bytes in one access (sm_100), 32-byte aligned.
+__device__ __forceinline__ void load_f32x8(const float* p, float (&z)[8]) {
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(z[0]), "=f"(z[1]), "=f"(z[2]), "=f"(z[3]), "=f"(z[4]), "=f"(z[5]), "=f"(z[6]), "=f"(z[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store_f32x8(float* p, const float (&z)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(z[0]), "f"(z[1]), "f"(z[2]),
+               "f"(z[3]), "f"(z[4]), "f"(z[5]), "f"(z[6]), "f"(z[7])
+               : "memory");
+}
+
+// Masks of packed pairs from a bit per token: `spread_bits` puts the bits of tokens 2 k and
+// 2 k + 1 at 2 k and 2 k + 16; shifted to the top bits of bytes 0 and 2, prmt replicates them
+// over the halves.
+__device__ __forceinline__ uint32_t spread_bits(uint32_t allow) { return (allow & 0x5555u) | ((allow & 0xaaaau) << 15); }
+__device__ __forceinline__ uint32_t pair_mask(uint32_t spread, int k) {
+  const uint32_t t = 2 * k <= 7 ? spread << (7 - 2 * k) : spread >> (2 * k - 7);
+  uint32_t m;
+  asm("prmt.b32 %0, %1, 0, 0xAA88;" : "=r"(m) : "r"(t));
+  return m;
+}
+
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// 0xffff in each half whose values are equal.
+__device__ __forceinline__ uint32_t equal_bf16x2(uint32_t a, uint32_t b) {
+  return __heq2_mask(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+}
+
+__device__ __forceinline__ float bf16_half(uint32_t w, int high) {
+  return __uint_as_float(high ? w & 0xffff0000u : w << 16);
+}
+
+// List entry: token - base (12 bits), count (15 bits), in the prompt, has a bias.
+constexpr uint32_t kEntryPrompt = 1u << 27, kEntryBias = 1u << 28;
+
+// kVec: every row starts on a boundary of the vector accesses and a thread owns two runs of
+// 8 consecutive tokens; otherwise its tokens lie 256 apart, so that the element accesses of
+// a warp stay contiguous whatever the row's alignment.
 template <typename TIn, typename TOut, bool kArgmax, bool kVec>
-__global__ void __launch_bounds__(kThreads) control_kernel(const Params p) {
-  __shared__ int s_id[kThreads];
-  __shared__ float s_val[kThreads];
-  __shared__ int s_warp[kThreads / 32];
-  __shared__ unsigned long long s_best[kRowBatch][kThreads / 32];
+__global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
+  __shared__ uint32_t s_list[kChunk];
+  __shared__ float s_bias[kChunk];
+  __shared__ int s_id[kListCap];
+  __shared__ float s_val[kListCap];
+  __shared__ int s_count[kThreads / 32];
+  __shared__ unsigned long long s_best[kRowBatch][kThreads / 32], s_list_best[kRowBatch];
+  __shared__ uint32_t s_top[kRowBatch];
+  __shared__ int s_mask[kRowBatch], s_token[kRowBatch];
+  __shared__ int s_n, s_proposals;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
+  // chunks in order, so that the first ones (low token ids are the frequent ones: long lists)
+  // do not start last
+  const int r = blockIdx.x % p.num_requests, chunk = blockIdx.x / p.num_requests;
   const int base = chunk * kChunk;
   int q0, nq;
   const int slot = p.slots[r];
@@ -101,161 +173,414 @@ __global__ void __launch_bounds__(kThreads) control_kernel(const Params p) {
     if (tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
     return;
   }
-  auto index = [&](int e) { return kVec ? base + tid * kPer + e : base + e * kThreads + tid; };
-
-  int c[kPer];
-  uint32_t prompt = 0;
-  {
-    const short* cr = p.counts + static_cast<long long>(slot) * p.ld_counts;
-    const uint32_t* br = p.prompt_bits + static_cast<long long>(slot) * p.ld_bits;
-    if (kVec && index(kPer - 1) < p.vocab) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(cr + index(0)));
-      const short* s = reinterpret_cast<const short*>(&raw);
+  // token of bit e, less base
+  auto rel = [&](int e) { return kVec ? (e >> 3) * kRun + tid * 8 + (e & 7) : e * kThreads + tid; };
+  auto index = [&](int e) { return base + rel(e); };
+  auto owner = [&](int x) { return kVec ? (x % kRun) >> 3 : x % kThreads; };
+  auto bit_of = [&](int x) { return kVec ? (x / kRun) * 8 + (x & 7) : x / kThreads; };
+  const bool whole0 = kVec && index(7) < p.vocab, whole1 = kVec && index(15) < p.vocab;
+  auto whole = [&](int o) { return o == 0 ? whole0 : whole1; };
+  uint32_t inside = 0xffffu;                     // tokens of the vocabulary
+  if (!(whole0 && whole1)) {
+    inside = 0;
+#pragma unroll 1
+    for (int e = 0; e < kPer; ++e) inside |= static_cast<uint32_t>(index(e) < p.vocab) << e;
+  }
+  // The request's tables, on their way while the rows' indices and the biases are staged.
+  const short* cr = p.counts + static_cast<long long>(slot) * p.ld_counts;
+  const uint32_t* br = p.prompt_bits + static_cast<long long>(slot) * p.ld_bits;
+  uint32_t cw[8], prompt = 0, used = 0;          // counts in pairs; bit e: in the prompt, emitted
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) c[e] = s[e];
-      prompt = (br[index(0) >> 5] >> (index(0) & 31)) & 0xffu;
+  for (int o = 0; o < 2; ++o) {
+    if (whole(o)) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(cr + index(8 * o)));
+      cw[4 * o] = raw.x;
+      cw[4 * o + 1] = raw.y;
+      cw[4 * o + 2] = raw.z;
+      cw[4 * o + 3] = raw.w;
+      prompt |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint8_t*>(br) + (index(8 * o) >> 3))) << (8 * o);
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int v = index(e);
-        c[e] = v < p.vocab ? cr[v] : 0;
-        if (v < p.vocab) prompt |= ((br[v >> 5] >> (v & 31)) & 1u) << e;
+      for (int e = 8 * o; e < 8 * o + 8; e += 2) {
+        uint32_t lo = 0, hi = 0;
+        if (index(e) < p.vocab) {
+          lo = static_cast<uint16_t>(cr[index(e)]);
+          prompt |= ((br[index(e) >> 5] >> (index(e) & 31)) & 1u) << e;
+        }
+        if (index(e + 1) < p.vocab) {
+          hi = static_cast<uint16_t>(cr[index(e + 1)]);
+          prompt |= ((br[index(e + 1) >> 5] >> (index(e + 1) & 31)) & 1u) << (e + 1);
+        }
+        cw[e >> 1] = lo | (hi << 16);
       }
     }
   }
   const float rep = p.penalties[3 * slot], freq = p.penalties[3 * slot + 1], pres = p.penalties[3 * slot + 2];
-
-  // biases of the chunk, added in list order whatever the number of entries per token
-  float bias[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) bias[e] = 0.f;
-  const int nb = p.bias_ids ? min(max(p.bias_len[slot], 0), p.max_bias) : 0;
-  for (int b0 = 0; b0 < nb; b0 += kThreads) {
-    const int b = b0 + tid;
-    const int id = b < nb ? p.bias_ids[static_cast<long long>(slot) * p.max_bias + b] : -1;
-    const bool in = id >= base && id < base + kChunk;
-    const unsigned ballot = __ballot_sync(0xffffffffu, in);
-    if (lane == 0) s_warp[warp] = __popc(ballot);
-    __syncthreads();
-    int at = __popc(ballot & ((1u << lane) - 1)), n = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) at += s_warp[w];
-      n += s_warp[w];
-    }
-    if (in) {
-      s_id[at] = id;
-      s_val[at] = p.bias_values[static_cast<long long>(slot) * p.max_bias + b];
-    }
-    __syncthreads();
-    for (int k = 0; k < n; ++k) {
-      const int x = s_id[k] - base;
-      const int owner = kVec ? x / kPer : x % kThreads, el = kVec ? x % kPer : x / kThreads;
-      if (owner == tid) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          if (e == el) bias[e] = __fadd_rn(bias[e], s_val[k]);
-      }
-    }
-    __syncthreads();
-  }
-
+  const float inv_rep = __frcp_rn(rep);
+  const bool rep_safe = rep > 1e-10f && rep < 1e10f;
   const TIn* lg = static_cast<const TIn*>(p.logits);
-  for (int j = 0; j < nq; ++j) {
-    const int row = q0 + j;
-    if (j > 0 && p.tokens) {
-      const long long x = p.tokens[row];
-      if (x >= base && x < base + kChunk && x < p.vocab) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          if (index(e) == static_cast<int>(x)) c[e] = min(c[e] + 1, kMaxCount);
-      } else if ((x < 0 || x >= p.vocab) && chunk == 0 && tid == 0) {
-        atomicOr(&g_device_status, kStatusBadArgument);
-      }
+  constexpr bool kPacked = kVec && sizeof(TIn) == 2;
+
+  uint32_t changed = 0;                          // bit e: token e is in the list
+
+  for (int j0 = 0; j0 < nq; j0 += kRowBatch) {
+    // the batch's mask rows (-1: none) and proposals (-1: none in this chunk)
+    const int batch = min(kRowBatch, nq - j0);
+    __syncthreads();
+    if (tid == 0) {
+      s_proposals = 0;
+      if (j0 == 0) s_n = 0;
     }
-    uint32_t allow = 0xffu;
-    if (p.masks) {
-      const int mi = p.mask_index[row];
-      if (mi >= p.num_masks) {
-        if (chunk == 0 && tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
-      } else if (mi >= 0) {
-        const uint32_t* mr = p.masks + static_cast<long long>(mi) * p.ld_mask;
-        if (kVec) {
-          allow = index(0) < p.vocab ? (__ldg(mr + (index(0) >> 5)) >> (index(0) & 31)) & 0xffu : 0u;
-        } else {
-          allow = 0;
+    if (tid < batch) {
+      const int row = q0 + j0 + tid;
+      int mi = p.masks ? p.mask_index[row] : -1, x = -1;
+      if (mi >= p.num_masks) mi = -2;
+      if (j0 + tid > 0 && p.tokens) {
+        const long long t = p.tokens[row];
+        if (t < 0 || t >= p.vocab)
+          x = -2;
+        else if (t >= base && t < base + kChunk)
+          x = static_cast<int>(t) - base;
+      }
+      if (chunk == 0 && (mi == -2 || x == -2)) atomicOr(&g_device_status, kStatusBadArgument);
+      s_mask[tid] = mi;
+      s_token[tid] = x;
+      s_top[tid] = 0;
+      s_list_best[tid] = 0;
+    }
+    __syncthreads();
+    const bool masked = p.masks != nullptr;
+    auto allowed = [&](int j) -> uint32_t {
+      if (j >= batch) return 0u;
+      const int mi = masked ? s_mask[j] : -1;
+      if (mi < 0) return inside;
+      const uint32_t* mr = p.masks + static_cast<long long>(mi) * p.ld_mask;
+      uint32_t m = 0;
+      if (kVec) {
+        // the byte of tokens index(8 o) .. + 7 (little endian words)
+        const uint8_t* mb = reinterpret_cast<const uint8_t*>(mr) + (base >> 3) + tid;
+        if (whole0 || index(0) < p.vocab) m = __ldg(mb);
+        if (whole1 || index(8) < p.vocab) m |= static_cast<uint32_t>(__ldg(mb + kRun / 8)) << 8;
+      } else {
 #pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            const int v = index(e);
-            if (v < p.vocab) allow |= ((__ldg(mr + (v >> 5)) >> (v & 31)) & 1u) << e;
+        for (int e = 0; e < kPer; ++e) {
+          const int v = index(e);
+          if (v < p.vocab) m |= ((__ldg(mr + (v >> 5)) >> (v & 31)) & 1u) << e;
+        }
+      }
+      return m & inside;
+    };
+    // whether the streaming pass needs run o's logits
+    auto wanted = [&](int o, uint32_t allow) {
+      const uint32_t a = (allow >> (8 * o)) & 0xffu, all = (inside >> (8 * o)) & 0xffu;
+      return a != 0 && (kArgmax || !(p.in_place && a == all));
+    };
+    // packed: word 4 o + k holds tokens 8 o + 2 k and + 1; otherwise one token a word
+    constexpr int kWords = kPacked ? 8 : 16;
+    auto fetch = [&](int j, uint32_t allow, uint32_t (&w)[kWords], bool all = false) {
+      if (j >= batch) return;
+      const TIn* lr = lg + static_cast<long long>(q0 + j0 + j) * p.ld;
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        if (!all && !wanted(o, allow)) continue;
+        if constexpr (kPacked) {
+          if (whole(o)) {
+            const uint4 v = *reinterpret_cast<const uint4*>(lr + index(8 * o));
+            w[4 * o] = v.x;
+            w[4 * o + 1] = v.y;
+            w[4 * o + 2] = v.z;
+            w[4 * o + 3] = v.w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t lo = 0, hi = 0;
+              if (index(8 * o + 2 * k) < p.vocab) lo = __bfloat16_as_ushort(lr[index(8 * o + 2 * k)]);
+              if (index(8 * o + 2 * k + 1) < p.vocab) hi = __bfloat16_as_ushort(lr[index(8 * o + 2 * k + 1)]);
+              w[4 * o + k] = lo | (hi << 16);
+            }
+          }
+        } else {
+          if (kVec && whole(o)) {
+            float z[8];
+            load_f32x8(reinterpret_cast<const float*>(lr) + index(8 * o), z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[8 * o + e] = __float_as_uint(z[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              w[8 * o + e] = index(8 * o + e) < p.vocab ? __float_as_uint(to_f32(lr[index(8 * o + e)])) : 0u;
           }
         }
       }
-    }
-    const TIn* lr = lg + static_cast<long long>(row) * p.ld;
-    float z[kPer];
-    const bool whole = kVec && index(kPer - 1) < p.vocab;
-    if (allow == 0) {
-      // nothing of this thread's tokens is allowed: their logits are not read
-    } else if (whole) {
-      if (sizeof(TIn) == 2) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(lr + index(0)));
-        const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(&raw);
+    };
+    // Pipelined by rows: while row j is decided, row j + 1's logits and row j + 2's mask words
+    // are in flight. (Row 0 is read whole, before its mask is there.)
+    uint32_t next[kWords];
+    fetch(0, inside, next, !p.in_place || p.masks);
+    uint32_t allow = allowed(0), allow1 = allowed(1);
+    if (j0 == 0) {
+      // The chunk's biases, compacted in list order (so that a token's entries add in that order);
+      // more than kListCap of them are read from the list itself.
+      int listed = 0;
+      const int nb = p.bias_ids ? min(max(p.bias_len[slot], 0), p.max_bias) : 0;
+      const int* list_id = p.bias_ids + static_cast<long long>(slot) * p.max_bias;
+      const float* list_val = p.bias_values + static_cast<long long>(slot) * p.max_bias;
+      for (int b0 = 0; b0 < nb; b0 += kThreads) {
+        const int b = b0 + tid;
+        const int id = b < nb ? list_id[b] : -1;
+        const bool in = id >= base && id < base + kChunk && id < p.vocab;
+        const unsigned ballot = __ballot_sync(0xffffffffu, in);
+        __syncthreads();
+        if (lane == 0) s_count[warp] = __popc(ballot);
+        __syncthreads();
+        int at = listed + __popc(ballot & ((1u << lane) - 1));
+        for (int w = 0; w < kThreads / 32; ++w) {
+          if (w < warp) at += s_count[w];
+          listed += s_count[w];
+        }
+        if (in && at < kListCap) {
+          s_id[at] = id;
+          s_val[at] = list_val[b];
+        }
+      }
+      const bool in_smem = listed <= kListCap;
+      const int list_n = in_smem ? listed : nb;
+      __syncthreads();
+      uint32_t biased = 0;
+      if (listed > 0) {
+        for (int k = 0; k < list_n; ++k) {
+          const int x = (in_smem ? s_id[k] : list_id[k]) - base;
+          if (x >= 0 && x < kChunk && owner(x) == tid) biased |= 1u << bit_of(x);
+        }
+        biased &= inside;
+      }
+      // Tokens that were seen or have a bias, into the list (in any order).
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) z[e] = __bfloat162float(x[e]);
+      for (int k = 0; k < 8; ++k) {
+        used |= static_cast<uint32_t>(static_cast<short>(cw[k] & 0xffffu) > 0) << (2 * k);
+        used |= static_cast<uint32_t>(static_cast<int>(cw[k]) >> 16 > 0) << (2 * k + 1);
+      }
+      changed = prompt | used | biased;
+      int at = __popc(changed);                      // the warp's entries lie behind one another
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += v;
+      }
+      int first = 0;
+      if (lane == 31 && at > 0) first = atomicAdd(&s_n, at);
+      at += __shfl_sync(0xffffffffu, first, 31) - __popc(changed);
+#pragma unroll 1
+      for (uint32_t m = changed; m != 0; m &= m - 1, ++at) {
+        const int e = __ffs(m) - 1;
+        uint32_t count = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) count = k == (e >> 1) ? cw[k] : count;
+        count = ((used >> e) & 1u) ? (count >> (16 * (e & 1))) & 0x7fffu : 0u;
+        s_list[at] = static_cast<uint32_t>(rel(e)) | (count << 12) | (((prompt >> e) & 1u) ? kEntryPrompt : 0u) |
+                     (((biased >> e) & 1u) ? kEntryBias : 0u);
+        if ((biased >> e) & 1u) {
+          float sum = 0.f;
+          for (int k = 0; k < list_n; ++k)
+            if ((in_smem ? s_id[k] : list_id[k]) == index(e)) sum = __fadd_rn(sum, in_smem ? s_val[k] : list_val[k]);
+          s_bias[at] = sum;
+        }
+      }
+    }
+    // proposals join the list (count 0 until their row)
+    for (int j = 0; j < batch; ++j) {
+      const int x = s_token[j];
+      if (x < 0 || owner(x) != tid) continue;
+      s_proposals = 1;
+      if (!((changed >> bit_of(x)) & 1u)) {
+        changed |= 1u << bit_of(x);
+        const int at = atomicAdd(&s_n, 1);
+        s_list[at] = static_cast<uint32_t>(x);
+      }
+    }
+    const uint32_t plain = inside & ~changed;    // tokens the streaming pass decides by itself
+#pragma unroll 1
+    for (int j = 0; j < batch; ++j) {
+      uint32_t w[kWords];
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[k] = next[k];
+      fetch(j + 1, allow1, next);
+      const uint32_t allow2 = allowed(j + 2);
+      if constexpr (kArgmax) {
+        const uint32_t keep = allow & plain;
+        if (!__any_sync(0xffffffffu, keep != 0)) {
+          if (lane == 0) s_best[j][warp] = 0;
+        } else {
+          float top;
+          if constexpr (kPacked) {
+            if (keep != 0xffffu) {
+              const uint32_t spread = spread_bits(keep);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint32_t m = pair_mask(spread, k);
+                w[k] = (w[k] & m) | (0xff80ff80u & ~m);
+              }
+            }
+            uint32_t t = max_nan_bf16x2(w[0], w[1]);
+#pragma unroll
+            for (int k = 2; k < 8; ++k) t = max_nan_bf16x2(t, w[k]);
+            top = max_nan(bf16_half(t, 0), bf16_half(t, 1));
+          } else {
+            top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+              w[e] = ((keep >> e) & 1u) ? w[e] : 0xff800000u;
+              top = max_nan(top, __uint_as_float(w[e]));
+            }
+          }
+          const uint32_t key = keep ? order_key(top) : 0u;
+          const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+          // a warp below the row's maximum so far has nothing to add (a stale read is lower)
+          const uint32_t so_far = *reinterpret_cast<volatile uint32_t*>(&s_top[j]);
+          unsigned long long mine = 0;
+          if (__any_sync(0xffffffffu, best >= so_far)) {
+            uint32_t at = 0xffffffffu;
+            if (key == best && keep) {
+              if (top == -INFINITY) {              // left-out tokens look the same: the first kept one
+                at = static_cast<uint32_t>(index(__ffs(keep) - 1));
+              } else if (kPacked && top == top) {
+                // bit k of each half: the pair's low or high token has the maximum
+                const uint32_t t2 = pack_bf16x2(top, top);
+                uint32_t hit = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) hit |= equal_bf16x2(w[k % kWords], t2) & (0x00010001u << k);
+                const uint32_t lo = hit & 0xffffu, hi = hit >> 16;
+                at = static_cast<uint32_t>(index(min(lo ? 2 * (__ffs(lo) - 1) : kPer, hi ? 2 * (__ffs(hi) - 1) + 1 : kPer)));
+              } else {
+#pragma unroll
+                for (int e = kPer - 1; e >= 0; --e) {
+                  const float y = kPacked ? bf16_half(w[(e >> 1) % kWords], e & 1) : __uint_as_float(w[e % kWords]);
+                  if (y == top || (top != top && y != y)) at = static_cast<uint32_t>(index(e));
+                }
+              }
+            }
+            at = __reduce_min_sync(0xffffffffu, at);
+            mine = (static_cast<unsigned long long>(best) << 32) | (0xffffffffu - at);
+            if (lane == 0) atomicMax(&s_top[j], best);
+          }
+          if (lane == 0) s_best[j][warp] = mine;
+        }
       } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(lr + index(0)));
-        const uint4 b = __ldg(reinterpret_cast<const uint4*>(lr + index(0)) + 1);
-        const float* x = reinterpret_cast<const float*>(&a);
-        const float* y = reinterpret_cast<const float*>(&b);
+        TOut* orow = static_cast<TOut*>(p.out) + static_cast<long long>(q0 + j0 + j) * p.ld_out;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          z[e] = x[e];
-          z[e + 4] = y[e];
+        for (int o = 0; o < 2; ++o) {
+          const uint32_t a = (allow >> (8 * o)) & 0xffu, all = (inside >> (8 * o)) & 0xffu;
+          if (all == 0 || (p.in_place && a == all)) continue;      // in place, nothing forbidden: as it is
+          if constexpr (kPacked && sizeof(TOut) == 2) {
+            const uint32_t hidden = pack_bf16x2(p.mask_value, p.mask_value);
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t m = a == 0xffu ? 0xffffffffu : pair_mask(spread_bits(a), k);
+              v[k] = (w[(4 * o + k) % kWords] & m) | (hidden & ~m);
+            }
+            if (whole(o)) {
+              *reinterpret_cast<uint4*>(orow + index(8 * o)) = make_uint4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (index(8 * o + e) < p.vocab)
+                  orow[index(8 * o + e)] = __ushort_as_bfloat16(static_cast<unsigned short>(v[e >> 1] >> (16 * (e & 1))));
+            }
+          } else {
+            float z[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float y = kPacked ? bf16_half(w[(4 * o + (e >> 1)) % kWords], e & 1)
+                                      : __uint_as_float(w[(8 * o + e) % kWords]);
+              z[e] = ((a >> e) & 1u) ? y : p.mask_value;
+            }
+            if (sizeof(TOut) == 4 && whole(o)) {
+              store_f32x8(reinterpret_cast<float*>(orow) + index(8 * o), z);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (index(8 * o + e) < p.vocab) {
+                  if constexpr (sizeof(TOut) == 4)
+                    orow[index(8 * o + e)] = z[e];
+                  else
+                    orow[index(8 * o + e)] = __float2bfloat16_rn(z[e]);
+                }
+            }
+          }
         }
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) z[e] = index(e) < p.vocab ? to_f32(lr[index(e)]) : 0.f;
+      allow = allow1;
+      allow1 = allow2;
     }
-    unsigned long long best = 0;
+    __syncthreads();                             // the list is complete, the streamed stores are done
+    const int n = s_n;
+    const bool proposals = s_proposals != 0;
+    // units of 32 entries of one row, spread over the warps
+    const int units = ((n + 31) >> 5) * batch;
+    constexpr int kAhead = 4;                    // units whose loads are in flight together
+    for (int u0 = warp; u0 < units; u0 += kAhead * (kThreads / 32)) {
+      uint32_t entry[kAhead];
+      float value[kAhead], shift[kAhead];
+      bool ok[kAhead];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      float y = z[e];
-      if (((prompt >> e) & 1u) || c[e] > 0) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-      if (c[e] > 0) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(c[e]))), pres);
-      if (nb > 0) y = __fadd_rn(y, bias[e]);
-      const bool ok = (allow >> e) & 1u;
-      z[e] = ok ? y : p.mask_value;
-      if (kArgmax && ok && index(e) < p.vocab) best = max_u64(best, arg_key(y, index(e)));
-    }
-    if (kArgmax) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, o));
-      if (lane == 0) s_best[j % kRowBatch][warp] = best;
-      if (j % kRowBatch == kRowBatch - 1 || j + 1 == nq) {
-        const int j0 = j - j % kRowBatch;
-        __syncthreads();
-        if (tid <= j - j0) {
-          unsigned long long m = 0;
-          for (int w = 0; w < kThreads / 32; ++w) m = max_u64(m, s_best[tid][w]);
-          p.part[static_cast<long long>(q0 + j0 + tid) * p.chunks + chunk] = m;
-        }
-        __syncthreads();
+      for (int h = 0; h < kAhead; ++h) {
+        const int u = u0 + h * (kThreads / 32), j = u % batch, i = (u / batch) * 32 + lane;
+        ok[h] = u < units && i < n;
+        entry[h] = ok[h] ? s_list[i] : 0u;
+        shift[h] = ok[h] && (entry[h] & kEntryBias) ? s_bias[i] : 0.f;
+        const int v = base + static_cast<int>(entry[h] & 0xfffu), mi = s_mask[j];
+        uint32_t word = 0xffffffffu;
+        if (ok[h] && mi >= 0) word = __ldg(p.masks + static_cast<long long>(mi) * p.ld_mask + (v >> 5));
+        value[h] = ok[h] ? to_f32(lg[static_cast<long long>(q0 + j0 + j) * p.ld + v]) : 0.f;
+        ok[h] = ok[h] && ((word >> (v & 31)) & 1u);
       }
-      continue;
+#pragma unroll
+      for (int h = 0; h < kAhead; ++h) {
+        const int u = u0 + h * (kThreads / 32), j = u % batch;
+        if (u >= units) break;
+        const int x = static_cast<int>(entry[h] & 0xfffu), v = base + x;
+        int count = static_cast<int>((entry[h] >> 12) & 0x7fffu);
+        if (proposals) {
+          for (int k = 0; k <= j; ++k) count += s_token[k] == x;
+          count = min(count, kMaxCount);
+        }
+        float y = value[h];
+        if (count > 0 || (entry[h] & kEntryPrompt)) y = y > 0.f ? divide(y, rep, inv_rep, rep_safe) : __fmul_rn(y, rep);
+        if (count > 0) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(count))), pres);
+        if (entry[h] & kEntryBias) y = __fadd_rn(y, shift[h]);
+        if constexpr (kArgmax) {
+          const uint32_t key = ok[h] ? order_key(y) : 0u;
+          const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+          if (best != 0) {
+            const uint32_t at =
+                __reduce_min_sync(0xffffffffu, ok[h] && key == best ? static_cast<uint32_t>(v) : 0xffffffffu);
+            if (lane == 0)
+              atomicMax(&s_list_best[j], (static_cast<unsigned long long>(best) << 32) | (0xffffffffu - at));
+          }
+        } else if (ok[h]) {
+          TOut* orow = static_cast<TOut*>(p.out) + static_cast<long long>(q0 + j0 + j) * p.ld_out;
+          if constexpr (sizeof(TOut) == 4)
+            orow[v] = y;
+          else
+            orow[v] = __float2bfloat16_rn(y);
+        }
+      }
     }
-    TOut* orow = static_cast<TOut*>(p.out) + static_cast<long long>(row) * p.ld_out;
-    if (whole) {
-      uint4 w[sizeof(TOut) / 2];
-      TOut* t = reinterpret_cast<TOut*>(w);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) put(t + e, z[e]);
-#pragma unroll
-      for (int k = 0; k < static_cast<int>(sizeof(TOut) / 2); ++k) reinterpret_cast<uint4*>(orow + index(0))[k] = w[k];
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (index(e) < p.vocab) put(orow + index(e), z[e]);
+    __syncthreads();
+    if (kArgmax && tid < batch) {
+      unsigned long long m = s_list_best[tid];
+      for (int w = 0; w < kThreads / 32; ++w) m = max_u64(m, s_best[tid][w]);
+      p.part[static_cast<long long>(q0 + j0 + tid) * p.chunks + chunk] = m;
+    }
+    if (j0 + kRowBatch < nq && proposals) {
+      // the next batch counts this one's proposals
+      for (int i = tid; i < n; i += kThreads) {
+        const uint32_t entry = s_list[i];
+        int count = static_cast<int>((entry >> 12) & 0x7fffu);
+        for (int k = 0; k < batch; ++k) count += s_token[k] == static_cast<int>(entry & 0xfffu);
+        s_list[i] = (entry & ~(0x7fffu << 12)) | (static_cast<uint32_t>(min(count, kMaxCount)) << 12);
+      }
     }
   }
 }

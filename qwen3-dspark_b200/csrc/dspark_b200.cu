@@ -379,7 +379,10 @@ bool control_params(controls::Params& p, const void* logits, long long ld, int d
   return static_cast<long long>(p.chunks) * num_requests < (1ll << 31);
 }
 
-bool rows_aligned(const void* base, long long ld, int size) { return aligned(base, 16) && ld * size % 16 == 0; }
+// Rows on the boundaries of the vector accesses: 8 elements, 16 (bf16, int16) or 32 bytes.
+bool rows_aligned(const void* base, long long ld, int size) {
+  return aligned(base, 8 * static_cast<size_t>(size)) && ld % 8 == 0;
+}
 
 template <typename TIn, typename TOut, bool kArgmax>
 int launch_control(const controls::Params& p, bool vec, cudaStream_t stream) {

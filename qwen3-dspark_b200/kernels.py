@@ -21,6 +21,7 @@ no fallback, retry or split tuning.
 bf16 runs on the tensor-core kernel; float32 inputs (the reference's exact CPU
 configurations) run on the library's float32 CUDA-core kernel.
 """
+import contextlib
 import math
 
 import numpy as np
@@ -52,6 +53,15 @@ def runtime_identity(device):
 
 def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on_device(device):
+    """Context with ``device`` current (the library launches on the current device); free of
+    device calls where it is current already."""
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 class _NativeEntry:
@@ -242,40 +252,43 @@ class B200SharedPrefixKernel:
         device, dtype = self.device, query.dtype
         if (new_key is None) != (new_value is None):
             raise ValueError('B200 shared prefix requires new_key and new_value together')
-        sources = [(prefix_key, prefix_value), (key, value)] + ([(new_key, new_value)] if new_key is not None else [])
-        for t in (query, *(x for pair in sources for x in pair)) + ((out,) if out is not None else ()):
+        rows = []
+        for t, heads in ((query, HQ), (prefix_key, HKV), (prefix_value, HKV), (key, HKV), (value, HKV), (new_key, HKV),
+                         (new_value, HKV), (out, HQ)):
+            if t is None:
+                rows.append(0)
+                continue
             if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or dtype not in _DTYPES
                     or t.requires_grad or t.ndim != 3 or not t.is_contiguous()):
                 raise ValueError('B200 shared prefix requires no-autograd contiguous BF16 (or FP32) THD tensors on '
                                  'its GPU')
-        if query.shape[1:] != (HQ, HEAD_DIM) or (out is not None and out.shape != query.shape):
-            raise ValueError('B200 shared prefix supports Hq16/Hkv8/D128 Qwen tensors only')
-        if any(k.shape[1:] != (HKV, HEAD_DIM) or v.shape != k.shape for k, v in sources):
-            raise ValueError('B200 shared prefix supports Hq16/Hkv8/D128 Qwen tensors only')
+            n, h, d = t.shape
+            if h != heads or d != HEAD_DIM:
+                raise ValueError('B200 shared prefix supports Hq16/Hkv8/D128 Qwen tensors only')
+            rows.append(n)
+        total, p_rows, pv_rows, a_rows, av_rows, b_rows, bv_rows, out_rows = rows
+        if p_rows != pv_rows or a_rows != av_rows or b_rows != bv_rows or (out is not None and out_rows != total):
+            raise ValueError('Keys and values (and query and out) must have the same rows')
         if not isinstance(scale, (float, int)) or not math.isfinite(scale) or scale != SCALE:
             raise ValueError('B200 shared prefix requires the 1/sqrt(128) scale')
-        if not hasattr(layout, 'workspace_bytes') or len(query) != layout.query_tokens or layout.plan.device != device:
+        if not hasattr(layout, 'workspace_bytes') or total != layout.query_tokens or layout.plan.device != device:
             raise ValueError('Query rows must match the shared-prefix layout on this device')
-        offs = (prefix_off, own_off, new_off)
-        need = (layout.prefix_rows, layout.own_rows, layout.new_rows)
-        rows = [len(k) for k, _ in sources] + [0] * (3 - len(sources))
-        if any(type(o) is not int or o < 0 or (n > 0 and o + n > r) for o, n, r in zip(offs, need, rows)):
-            raise ValueError('A key source holds fewer rows than the layout reads at its offset')
-        if out is None:
-            out = torch.empty_like(query)
-        if layout.query_tokens == 0:
-            return out
-        args = []
-        for (k, v), off in zip(sources, offs):
-            args += [k.data_ptr(), v.data_ptr(), len(k), off]
-        if len(sources) < 3:
-            args += [None, None, 0, 0]
-        nbytes = layout.workspace_bytes if dtype == torch.bfloat16 else 0
-        with torch.cuda.device(device):
+        for off, need, held in ((prefix_off, layout.prefix_rows, p_rows), (own_off, layout.own_rows, a_rows),
+                                (new_off, layout.new_rows, b_rows)):
+            if type(off) is not int or off < 0 or (need > 0 and off + need > held):
+                raise ValueError('A key source holds fewer rows than the layout reads at its offset')
+        with _on_device(device):
+            if out is None:
+                out = torch.empty_like(query)
+            if total == 0:
+                return out
+            nbytes = layout.workspace_bytes if dtype == torch.bfloat16 else 0
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-            self._operator(query.data_ptr(), len(query), *args, layout.head.data_ptr(), layout.plan.data_ptr(),
-                           float(scale), _DTYPES[dtype], out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
-                           _stream(device))
+            new = (new_key.data_ptr(), new_value.data_ptr()) if new_key is not None else (None, None)
+            self._operator(query.data_ptr(), total, prefix_key.data_ptr(), prefix_value.data_ptr(), p_rows, prefix_off,
+                           key.data_ptr(), value.data_ptr(), a_rows, own_off, *new, b_rows, new_off,
+                           layout.head.data_ptr(), layout.plan.data_ptr(), float(scale), _DTYPES[dtype],
+                           out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, _stream(device))
         return out
 
 
