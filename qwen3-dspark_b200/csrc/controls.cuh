@@ -223,9 +223,10 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
 
   uint32_t changed = 0;                          // bit e: token e is in the list
 
-  for (int j0 = 0; j0 < nq; j0 += kRowBatch) {
+  int j0 = 0, batch = 0;
+  auto stage = [&]() {
     // the batch's mask rows (-1: none) and proposals (-1: none in this chunk)
-    const int batch = min(kRowBatch, nq - j0);
+    batch = min(kRowBatch, nq - j0);
     __syncthreads();
     if (tid == 0) {
       s_proposals = 0;
@@ -249,144 +250,151 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
       s_list_best[tid] = 0;
     }
     __syncthreads();
-    const bool masked = p.masks != nullptr;
-    auto allowed = [&](int j) -> uint32_t {
-      if (j >= batch) return 0u;
-      const int mi = masked ? s_mask[j] : -1;
-      if (mi < 0) return inside;
-      const uint32_t* mr = p.masks + static_cast<long long>(mi) * p.ld_mask;
-      uint32_t m = 0;
-      if (kVec) {
-        // the byte of tokens index(8 o) .. + 7 (little endian words)
-        const uint8_t* mb = reinterpret_cast<const uint8_t*>(mr) + (base >> 3) + tid;
-        if (whole0 || index(0) < p.vocab) m = __ldg(mb);
-        if (whole1 || index(8) < p.vocab) m |= static_cast<uint32_t>(__ldg(mb + kRun / 8)) << 8;
-      } else {
+  };
+  const bool masked = p.masks != nullptr;
+  auto allowed = [&](int j) -> uint32_t {
+    if (j >= batch) return 0u;
+    const int mi = masked ? s_mask[j] : -1;
+    if (mi < 0) return inside;
+    const uint32_t* mr = p.masks + static_cast<long long>(mi) * p.ld_mask;
+    uint32_t m = 0;
+    if (kVec) {
+      // the byte of tokens index(8 o) .. + 7 (little endian words)
+      const uint8_t* mb = reinterpret_cast<const uint8_t*>(mr) + (base >> 3) + tid;
+      if (whole0 || index(0) < p.vocab) m = __ldg(mb);
+      if (whole1 || index(8) < p.vocab) m |= static_cast<uint32_t>(__ldg(mb + kRun / 8)) << 8;
+    } else {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const int v = index(e);
-          if (v < p.vocab) m |= ((__ldg(mr + (v >> 5)) >> (v & 31)) & 1u) << e;
-        }
+      for (int e = 0; e < kPer; ++e) {
+        const int v = index(e);
+        if (v < p.vocab) m |= ((__ldg(mr + (v >> 5)) >> (v & 31)) & 1u) << e;
       }
-      return m & inside;
-    };
-    // whether the streaming pass needs run o's logits
-    auto wanted = [&](int o, uint32_t allow) {
-      const uint32_t a = (allow >> (8 * o)) & 0xffu, all = (inside >> (8 * o)) & 0xffu;
-      return a != 0 && (kArgmax || !(p.in_place && a == all));
-    };
-    // packed: word 4 o + k holds tokens 8 o + 2 k and + 1; otherwise one token a word
-    constexpr int kWords = kPacked ? 8 : 16;
-    auto fetch = [&](int j, uint32_t allow, uint32_t (&w)[kWords], bool all = false) {
-      if (j >= batch) return;
-      const TIn* lr = lg + static_cast<long long>(q0 + j0 + j) * p.ld;
+    }
+    return m & inside;
+  };
+  // whether the streaming pass needs run o's logits
+  auto wanted = [&](int o, uint32_t allow) {
+    const uint32_t a = (allow >> (8 * o)) & 0xffu, all = (inside >> (8 * o)) & 0xffu;
+    return a != 0 && (kArgmax || !(p.in_place && a == all));
+  };
+  // packed: word 4 o + k holds tokens 8 o + 2 k and + 1; otherwise one token a word
+  constexpr int kWords = kPacked ? 8 : 16;
+  auto fetch = [&](int j, uint32_t allow, uint32_t (&w)[kWords], bool all = false) {
+    if (j >= batch) return;
+    const TIn* lr = lg + static_cast<long long>(q0 + j0 + j) * p.ld;
 #pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        if (!all && !wanted(o, allow)) continue;
-        if constexpr (kPacked) {
-          if (whole(o)) {
-            const uint4 v = *reinterpret_cast<const uint4*>(lr + index(8 * o));
-            w[4 * o] = v.x;
-            w[4 * o + 1] = v.y;
-            w[4 * o + 2] = v.z;
-            w[4 * o + 3] = v.w;
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t lo = 0, hi = 0;
-              if (index(8 * o + 2 * k) < p.vocab) lo = __bfloat16_as_ushort(lr[index(8 * o + 2 * k)]);
-              if (index(8 * o + 2 * k + 1) < p.vocab) hi = __bfloat16_as_ushort(lr[index(8 * o + 2 * k + 1)]);
-              w[4 * o + k] = lo | (hi << 16);
-            }
-          }
+    for (int o = 0; o < 2; ++o) {
+      if (!all && !wanted(o, allow)) continue;
+      if constexpr (kPacked) {
+        if (whole(o)) {
+          const uint4 v = *reinterpret_cast<const uint4*>(lr + index(8 * o));
+          w[4 * o] = v.x;
+          w[4 * o + 1] = v.y;
+          w[4 * o + 2] = v.z;
+          w[4 * o + 3] = v.w;
         } else {
-          if (kVec && whole(o)) {
-            float z[8];
-            load_f32x8(reinterpret_cast<const float*>(lr) + index(8 * o), z);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[8 * o + e] = __float_as_uint(z[e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              w[8 * o + e] = index(8 * o + e) < p.vocab ? __float_as_uint(to_f32(lr[index(8 * o + e)])) : 0u;
+          for (int k = 0; k < 4; ++k) {
+            uint32_t lo = 0, hi = 0;
+            if (index(8 * o + 2 * k) < p.vocab) lo = __bfloat16_as_ushort(lr[index(8 * o + 2 * k)]);
+            if (index(8 * o + 2 * k + 1) < p.vocab) hi = __bfloat16_as_ushort(lr[index(8 * o + 2 * k + 1)]);
+            w[4 * o + k] = lo | (hi << 16);
           }
         }
-      }
-    };
-    // Pipelined by rows: while row j is decided, row j + 1's logits and row j + 2's mask words
-    // are in flight. (Row 0 is read whole, before its mask is there.)
-    uint32_t next[kWords];
-    fetch(0, inside, next, !p.in_place || p.masks);
-    uint32_t allow = allowed(0), allow1 = allowed(1);
-    if (j0 == 0) {
-      // The chunk's biases, compacted in list order (so that a token's entries add in that order);
-      // more than kListCap of them are read from the list itself.
-      int listed = 0;
-      const int nb = p.bias_ids ? min(max(p.bias_len[slot], 0), p.max_bias) : 0;
-      const int* list_id = p.bias_ids + static_cast<long long>(slot) * p.max_bias;
-      const float* list_val = p.bias_values + static_cast<long long>(slot) * p.max_bias;
-      for (int b0 = 0; b0 < nb; b0 += kThreads) {
-        const int b = b0 + tid;
-        const int id = b < nb ? list_id[b] : -1;
-        const bool in = id >= base && id < base + kChunk && id < p.vocab;
-        const unsigned ballot = __ballot_sync(0xffffffffu, in);
-        __syncthreads();
-        if (lane == 0) s_count[warp] = __popc(ballot);
-        __syncthreads();
-        int at = listed + __popc(ballot & ((1u << lane) - 1));
-        for (int w = 0; w < kThreads / 32; ++w) {
-          if (w < warp) at += s_count[w];
-          listed += s_count[w];
-        }
-        if (in && at < kListCap) {
-          s_id[at] = id;
-          s_val[at] = list_val[b];
-        }
-      }
-      const bool in_smem = listed <= kListCap;
-      const int list_n = in_smem ? listed : nb;
-      __syncthreads();
-      uint32_t biased = 0;
-      if (listed > 0) {
-        for (int k = 0; k < list_n; ++k) {
-          const int x = (in_smem ? s_id[k] : list_id[k]) - base;
-          if (x >= 0 && x < kChunk && owner(x) == tid) biased |= 1u << bit_of(x);
-        }
-        biased &= inside;
-      }
-      // Tokens that were seen or have a bias, into the list (in any order).
+      } else {
+        if (kVec && whole(o)) {
+          float z[8];
+          load_f32x8(reinterpret_cast<const float*>(lr) + index(8 * o), z);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        used |= static_cast<uint32_t>(static_cast<short>(cw[k] & 0xffffu) > 0) << (2 * k);
-        used |= static_cast<uint32_t>(static_cast<int>(cw[k]) >> 16 > 0) << (2 * k + 1);
-      }
-      changed = prompt | used | biased;
-      int at = __popc(changed);                      // the warp's entries lie behind one another
+          for (int e = 0; e < 8; ++e) w[8 * o + e] = __float_as_uint(z[e]);
+        } else {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += v;
-      }
-      int first = 0;
-      if (lane == 31 && at > 0) first = atomicAdd(&s_n, at);
-      at += __shfl_sync(0xffffffffu, first, 31) - __popc(changed);
-#pragma unroll 1
-      for (uint32_t m = changed; m != 0; m &= m - 1, ++at) {
-        const int e = __ffs(m) - 1;
-        uint32_t count = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) count = k == (e >> 1) ? cw[k] : count;
-        count = ((used >> e) & 1u) ? (count >> (16 * (e & 1))) & 0x7fffu : 0u;
-        s_list[at] = static_cast<uint32_t>(rel(e)) | (count << 12) | (((prompt >> e) & 1u) ? kEntryPrompt : 0u) |
-                     (((biased >> e) & 1u) ? kEntryBias : 0u);
-        if ((biased >> e) & 1u) {
-          float sum = 0.f;
-          for (int k = 0; k < list_n; ++k)
-            if ((in_smem ? s_id[k] : list_id[k]) == index(e)) sum = __fadd_rn(sum, in_smem ? s_val[k] : list_val[k]);
-          s_bias[at] = sum;
+          for (int e = 0; e < 8; ++e)
+            w[8 * o + e] = index(8 * o + e) < p.vocab ? __float_as_uint(to_f32(lr[index(8 * o + e)])) : 0u;
         }
       }
     }
+  };
+  uint32_t next[kWords];
+  stage();
+  // (row 0 is read whole, before its mask is there)
+  fetch(0, inside, next, !p.in_place || p.masks);
+  // The chunk's biases, compacted in list order (so that a token's entries add in that order);
+  // more than kListCap of them are read from the list itself.
+  int listed = 0;
+  const int nb = p.bias_ids ? min(max(p.bias_len[slot], 0), p.max_bias) : 0;
+  const int* list_id = p.bias_ids + static_cast<long long>(slot) * p.max_bias;
+  const float* list_val = p.bias_values + static_cast<long long>(slot) * p.max_bias;
+  for (int b0 = 0; b0 < nb; b0 += kThreads) {
+    const int b = b0 + tid;
+    const int id = b < nb ? list_id[b] : -1;
+    const bool in = id >= base && id < base + kChunk && id < p.vocab;
+    const unsigned ballot = __ballot_sync(0xffffffffu, in);
+    __syncthreads();
+    if (lane == 0) s_count[warp] = __popc(ballot);
+    __syncthreads();
+    int at = listed + __popc(ballot & ((1u << lane) - 1));
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) at += s_count[w];
+      listed += s_count[w];
+    }
+    if (in && at < kListCap) {
+      s_id[at] = id;
+      s_val[at] = list_val[b];
+    }
+  }
+  const bool in_smem = listed <= kListCap;
+  const int list_n = in_smem ? listed : nb;
+  __syncthreads();
+  uint32_t biased = 0;
+  if (listed > 0) {
+    for (int k = 0; k < list_n; ++k) {
+      const int x = (in_smem ? s_id[k] : list_id[k]) - base;
+      if (x >= 0 && x < kChunk && owner(x) == tid) biased |= 1u << bit_of(x);
+    }
+    biased &= inside;
+  }
+  // Tokens that were seen or have a bias, into the list (in any order).
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    used |= static_cast<uint32_t>(static_cast<short>(cw[k] & 0xffffu) > 0) << (2 * k);
+    used |= static_cast<uint32_t>(static_cast<int>(cw[k]) >> 16 > 0) << (2 * k + 1);
+  }
+  changed = prompt | used | biased;
+  int at = __popc(changed);                      // the warp's entries lie behind one another
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += v;
+  }
+  int first = 0;
+  if (lane == 31 && at > 0) first = atomicAdd(&s_n, at);
+  at += __shfl_sync(0xffffffffu, first, 31) - __popc(changed);
+#pragma unroll 1
+  for (uint32_t m = changed; m != 0; m &= m - 1, ++at) {
+    const int e = __ffs(m) - 1;
+    uint32_t count = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) count = k == (e >> 1) ? cw[k] : count;
+    count = ((used >> e) & 1u) ? (count >> (16 * (e & 1))) & 0x7fffu : 0u;
+    s_list[at] = static_cast<uint32_t>(rel(e)) | (count << 12) | (((prompt >> e) & 1u) ? kEntryPrompt : 0u) |
+                 (((biased >> e) & 1u) ? kEntryBias : 0u);
+    if ((biased >> e) & 1u) {
+      float sum = 0.f;
+      for (int k = 0; k < list_n; ++k)
+        if ((in_smem ? s_id[k] : list_id[k]) == index(e)) sum = __fadd_rn(sum, in_smem ? s_val[k] : list_val[k]);
+      s_bias[at] = sum;
+    }
+  }
+
+  for (; j0 < nq; j0 += kRowBatch) {
+    if (j0 > 0) {
+      stage();
+      fetch(0, inside, next, !p.in_place || p.masks);
+    }
+    // Pipelined by rows: while row j is decided, row j + 1's logits and row j + 2's mask words
+    // are in flight.
+    uint32_t allow = allowed(0), allow1 = allowed(1);
     // proposals join the list (count 0 until their row)
     for (int j = 0; j < batch; ++j) {
       const int x = s_token[j];
@@ -517,16 +525,28 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     const int n = s_n;
     const bool proposals = s_proposals != 0;
     // units of 32 entries of one row, spread over the warps
-    const int units = ((n + 31) >> 5) * batch;
+    const int units = ((n + 31) >> 5) * batch;   // (a unit past them has i >= n)
     constexpr int kAhead = 4;                    // units whose loads are in flight together
+    int row_at = warp, block_at = 0;             // this warp's next unit, stepped without divisions
+    auto step = [&](int by) {
+      row_at += by;
+      while (row_at >= batch) {
+        row_at -= batch;
+        ++block_at;
+      }
+    };
+    step(0);
     for (int u0 = warp; u0 < units; u0 += kAhead * (kThreads / 32)) {
       uint32_t entry[kAhead];
       float value[kAhead], shift[kAhead];
+      int unit_row[kAhead];
       bool ok[kAhead];
 #pragma unroll
       for (int h = 0; h < kAhead; ++h) {
-        const int u = u0 + h * (kThreads / 32), j = u % batch, i = (u / batch) * 32 + lane;
-        ok[h] = u < units && i < n;
+        const int j = row_at, i = block_at * 32 + lane;
+        unit_row[h] = j;
+        ok[h] = i < n;
+        step(kThreads / 32);
         entry[h] = ok[h] ? s_list[i] : 0u;
         shift[h] = ok[h] && (entry[h] & kEntryBias) ? s_bias[i] : 0.f;
         const int v = base + static_cast<int>(entry[h] & 0xfffu), mi = s_mask[j];
@@ -537,8 +557,8 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
       }
 #pragma unroll
       for (int h = 0; h < kAhead; ++h) {
-        const int u = u0 + h * (kThreads / 32), j = u % batch;
-        if (u >= units) break;
+        if (u0 + h * (kThreads / 32) >= units) break;
+        const int j = unit_row[h];
         const int x = static_cast<int>(entry[h] & 0xfffu), v = base + x;
         int count = static_cast<int>((entry[h] >> 12) & 0x7fffu);
         if (proposals) {
