@@ -211,7 +211,8 @@ int dspark_commit_kv(void* resident_k, void* resident_v, const void* scratch_k, 
  * of those rows. Proposals are accepted while they equal the prediction before
  * them (stopping after an accepted EOS); the first mismatch commits the target's
  * token instead and a full accept commits the bonus prediction. Committed tokens
- * are cut after their first EOS and to budget[i] (if budget is not NULL). Outputs:
+ * are cut after their first EOS and to budget[i] (if budget is not NULL). A negative
+ * pred (dspark_control_argmax, a row without an allowed token) commits nothing. Outputs:
  * accepted[i] proposals, n_commit[i] committed tokens (= verified rows to keep,
  * the n_commit input of dspark_commit_kv) and emitted[cu_q[i] + k] the committed
  * tokens (-1 after them). All pointers are device memory; int64 tokens.
@@ -451,9 +452,9 @@ int dspark_train_attn(const void* q, const void* k, const void* v, int total_q, 
  *
  * dspark_prefix_attn: q and out [total_q, 16, 128]; source s holds `rows` rows of
  * which the plan's rows start at row `off` (a layer's first row). A source that the
- * plan does not read may be NULL. bf16 (16-byte aligned pointers; workspace of
- * dspark_prefix_workspace_bytes(plan_head) bytes, 16-byte aligned, never needing a
- * clear, one per call in flight) or fp32. A device plan that is not the one plan_head
+ * plan does not read may be NULL. bf16 (tensor cores) or fp32 (CUDA cores), 16-byte
+ * aligned pointers; workspace: dspark_prefix_workspace_bytes(plan_head) bytes, 16-byte
+ * aligned, never needing a clear, one per call in flight. A device plan that is not the one plan_head
  * belongs to sets DSPARK_DEVICE_BAD_ARGUMENT and computes nothing. out may be q.
  */
 #define DSPARK_PREFIX_HEAD_WORDS 32

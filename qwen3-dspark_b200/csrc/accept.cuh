@@ -12,7 +12,8 @@
 // a full accept contributes the bonus pred[Q-1]. The committed tokens are cut
 // after their first EOS and to the request's remaining budget. n_commit is the
 // number of verified rows whose KV is kept (anchor .. newest-1), i.e. the number
-// of committed tokens, ready for dspark_commit_kv.
+// of committed tokens, ready for dspark_commit_kv. A negative prediction (a row whose
+// grammar mask allows no token) ends the request's round without a token of its own.
 #pragma once
 #include "ptx.cuh"
 
@@ -141,7 +142,7 @@ __global__ void greedy_accept_kernel(AcceptParams p) {
     const long long proposed = p.tokens[q0 + 1 + j];
     const long long correct = static_cast<long long>(p.pred[q0 + j]);
     if (proposed != correct) {
-      p.emitted[q0 + n++] = correct;
+      if (correct >= 0) p.emitted[q0 + n++] = correct;
       stop = true;
       break;
     }
@@ -149,7 +150,7 @@ __global__ void greedy_accept_kernel(AcceptParams p) {
     ++acc;
     if (is_eos(p, proposed)) stop = true;
   }
-  if (!stop) p.emitted[q0 + n++] = static_cast<long long>(p.pred[q1 - 1]);
+  if (!stop && p.pred[q1 - 1] >= 0) p.emitted[q0 + n++] = static_cast<long long>(p.pred[q1 - 1]);
   // cut after the first EOS, then to the budget
   for (int k = 0; k < n; ++k)
     if (is_eos(p, p.emitted[q0 + k])) {

@@ -85,6 +85,8 @@ int device_info(int dev, DeviceInfo* out) {
                              static_cast<int>(kAttnSmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(prefix::prefix_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(prefix::kSmemBytes)) != cudaSuccess ||
+        cudaFuncSetAttribute(prefix::prefix_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(prefix::kF32SmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(train::train_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(train::kSmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(markov::markov_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -338,6 +340,20 @@ int encode_rows_map(CUtensorMap* m, const void* base, long long rows, int heads,
 }  // namespace
 
 namespace {
+
+// The merge of a plan's partial rows. A plain launch: as a programmatic dependent its CTAs
+// could take the registers the attention's third warpgroup gives back before its softmax
+// warps draw them, and with the trigger behind that point small batches measured slower (8
+// rows behind 32768 keys: 102 us against 60).
+template <typename T>
+int launch_prefix_merge(const prefix::Params& p, const int32_t* plan_head, const float* part, cudaStream_t stream) {
+  const long long pairs = static_cast<long long>(p.total_q) * prefix::kHeads;
+  if (plan_head[prefix::kHMaxParts] > prefix::kMergeWideParts && pairs <= prefix::kMergeWidePairs)
+    prefix::prefix_merge_kernel<T, 8><<<static_cast<unsigned>(pairs), 256, 0, stream>>>(p, part);
+  else
+    prefix::prefix_merge_kernel<T, 1><<<static_cast<unsigned>((pairs + 7) / 8), 256, 0, stream>>>(p, part);
+  return launch_status();
+}
 
 bool control_params(controls::Params& p, const void* logits, long long ld, int dtype, int rows, int vocab,
                     const int32_t* cu_q, const long long* tokens, const int32_t* slots, int num_requests,
@@ -1165,7 +1181,7 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
       total_q != plan_head[kHTotalQ] || !(scale > 0.f) || (dtype != DSPARK_DTYPE_BF16 && dtype != DSPARK_DTYPE_F32))
     return DSPARK_ERR_INVALID_ARGUMENT;
   if (total_q == 0) return DSPARK_OK;
-  const size_t align = dtype == DSPARK_DTYPE_F32 ? 4 : 16;
+  const size_t align = 16;
   if (!q || !out || !aligned(q, align) || !aligned(out, align)) return DSPARK_ERR_INVALID_ARGUMENT;
   Params p{};
   p.q = q;
@@ -1195,17 +1211,20 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   DeviceInfo dev;
   const int st = current_device_info(&dev);
   if (st != DSPARK_OK) return st;
-  if (dtype == DSPARK_DTYPE_F32) {
-    const int max_q = plan_head[kHMaxQ];
-    const dim3 grid(plan_head[kHRequests], (max_q + kQBlock - 1) / kQBlock, kKVHeads);
-    if (grid.y > 65535) return DSPARK_ERR_UNSUPPORTED;
-    prefix_simple_kernel<float><<<grid, kSimpleThreads, 0, stream>>>(p);
-    return launch_status();
-  }
   if (p.slots > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < prefix::workspace_bytes(p.slots)))
     return DSPARK_ERR_INVALID_ARGUMENT;
+  int rc = DSPARK_OK;
+  float* part = static_cast<float*>(workspace);
+  if (dtype == DSPARK_DTYPE_F32) {
+    const int max_rows = std::min<int>(plan_head[kHMaxItemRows], kTileRows);
+    prefix_f32_kernel<<<dim3(plan_head[kHItems], (max_rows + kF32Sub - 1) / kF32Sub), kF32Threads2, kF32SmemBytes,
+                        stream>>>(p, part);
+    rc = launch_status();
+    if (rc != DSPARK_OK || p.slots == 0) return rc;
+    return launch_prefix_merge<float>(p, plan_head, part, stream);
+  }
   Maps maps;
-  int rc = encode_rows_map(&maps.q, q, total_q, kQHeads, 2, kHalfTile / 2);
+  rc = encode_rows_map(&maps.q, q, total_q, kQHeads, 2, kHalfTile / 2);
   if (rc != DSPARK_OK) return rc;
   for (int s = 0; s < 3; ++s) {
     const Source& x = p.src[s];
@@ -1219,20 +1238,10 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
       if ((rc = encode_block_map(&maps.block[2 * s + v], base, x.rows)) != DSPARK_OK) return rc;
     }
   }
-  float* part = static_cast<float*>(workspace);
   prefix_attn_kernel<<<p.grid, kAttThreads, prefix::kSmemBytes, stream>>>(maps, p, part);
   rc = launch_status();
   if (rc != DSPARK_OK || p.slots == 0) return rc;
-  // A plain launch: as a programmatic dependent the merge's CTAs could take the registers
-  // the attention's third warpgroup gives back before its softmax warps draw them, and
-  // with the trigger behind that point small batches measured slower (R = 8 rows behind
-  // 32768 keys: 102 us against 60).
-  const long long pairs = static_cast<long long>(total_q) * kHeads;
-  if (plan_head[kHMaxParts] > kMergeWideParts && pairs <= kMergeWidePairs)
-    prefix_merge_kernel<8><<<static_cast<unsigned>(pairs), 256, 0, stream>>>(p, part);
-  else
-    prefix_merge_kernel<1><<<static_cast<unsigned>((pairs + 7) / 8), 256, 0, stream>>>(p, part);
-  return launch_status();
+  return launch_prefix_merge<__nv_bfloat16>(p, plan_head, part, stream);
 }
 
 int dspark_control_logits(const void* logits, long long ld, int dtype, int rows, int vocab, const int32_t* cu_q,

@@ -41,122 +41,6 @@ __device__ __forceinline__ bool plan_ok(const Params& p) {
   return p.plan[kHMagic] == kPlanMagic && p.plan[kHCheck] == p.check && p.plan[kHTotalQ] == p.total_q;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_out(T* dst, float v);
-template <>
-__device__ __forceinline__ void store_out<float>(float* dst, float v) { *dst = v; }
-template <>
-__device__ __forceinline__ void store_out<__nv_bfloat16>(__nv_bfloat16* dst, float v) { *dst = __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ float load_in(const float* p) { return *p; }
-__device__ __forceinline__ float load_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-
-// CUDA-core kernel: one CTA per (request, block of 8 query rows, KV head); its 16 MMA
-// rows (2 heads x 8 query rows) walk the request's keys 32 at a time with an online
-// softmax, products and sums in fp32.
-constexpr int kSimpleThreads = 128;
-constexpr int kSimpleKeys = 32;
-
-template <typename T>
-__global__ void __launch_bounds__(kSimpleThreads) prefix_simple_kernel(const Params p) {
-  __shared__ float sq[16][kHeadDim];
-  __shared__ float sk[kSimpleKeys][kHeadDim + 1];
-  __shared__ float sv[kSimpleKeys][kHeadDim];
-  __shared__ float sp[16][kSimpleKeys];
-  const int tid = threadIdx.x;
-  if (!plan_ok(p)) {
-    if (tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
-    return;
-  }
-  const int* rec = p.plan + p.plan[kHRequestsAt] + static_cast<size_t>(blockIdx.x) * kRequestWords;
-  const int h = blockIdx.z;
-  const int q0 = rec[kRQ0], nq = rec[kRNq], r0 = blockIdx.y * kQBlock;
-  if (r0 >= nq) return;
-  const int len[3] = {rec[kRPrefixLen], rec[kROwnLen], rec[kRNewLen]};
-  const int start[3] = {rec[kRPrefixRow], rec[kROwnRow], rec[kRNewRow]};
-  const int keys = len[0] + len[1] + len[2];
-  const int rows = min(kQBlock, nq - r0);
-  const bool causal = p.plan[kHCausal] != 0;
-  const int vis = causal ? keys - nq + r0 + rows : keys;      // keys the block's last row sees
-  const T* qg = static_cast<const T*>(p.q);
-  T* og = static_cast<T*>(p.out);
-  for (int u = tid; u < 16 * kHeadDim; u += kSimpleThreads) {
-    const int m = u / kHeadDim, d = u % kHeadDim, r = m & 7, row = q0 + r0 + r;
-    sq[m][d] = r < rows && row < p.total_q
-                   ? load_in(qg + (static_cast<size_t>(row) * kQHeads + 2 * h + (m >> 3)) * kHeadDim + d)
-                   : 0.f;
-  }
-  const int m = tid >> 3, kq = tid & 7, r = m & 7;
-  float mrow = -INFINITY, lrow = 0.f;
-  float acc[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  const int row_vis = causal ? keys - nq + r0 + r + 1 : keys;
-  for (int kb0 = 0; kb0 < vis; kb0 += kSimpleKeys) {
-    __syncthreads();
-    for (int u = tid; u < kSimpleKeys * kHeadDim; u += kSimpleThreads) {
-      const int n = u / kHeadDim, d = u % kHeadDim, j = kb0 + n;
-      float kv = 0.f, vv = 0.f;
-      if (j < vis) {
-        const int s = j < len[0] ? 0 : (j < len[0] + len[1] ? 1 : 2);
-        const int at = s == 0 ? j : (s == 1 ? j - len[0] : j - len[0] - len[1]);
-        const Source& src = p.src[s];
-        const long long row = src.off + start[s] + at;
-        if (row >= 0 && row < src.rows) {
-          const size_t off = (static_cast<size_t>(row) * kKVHeads + h) * kHeadDim + d;
-          kv = load_in(static_cast<const T*>(src.k) + off);
-          vv = load_in(static_cast<const T*>(src.v) + off);
-        } else {
-          atomicOr(&g_device_status, kStatusBadArgument);
-        }
-      }
-      sk[n][d] = kv;
-      sv[n][d] = vv;
-    }
-    __syncthreads();
-    float s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = kq * 4 + i, j = kb0 + n;
-      float dot = 0.f;
-      for (int d = 0; d < kHeadDim; ++d) dot = fmaf(sq[m][d], sk[n][d], dot);
-      s[i] = j < row_vis && j < vis ? dot * p.scale : -INFINITY;
-    }
-    float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float mn = fmaxf(mrow, mx);
-    const float mu = mn == -INFINITY ? 0.f : mn;
-    const float alpha = expf(mrow - mu);
-    float ps = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float e = expf(s[i] - mu);
-      sp[m][kq * 4 + i] = e;
-      ps += e;
-    }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-    lrow = lrow * alpha + ps;
-    mrow = mn;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] *= alpha;
-    for (int n = 0; n < kSimpleKeys; ++n) {
-      const float pn = sp[m][n];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] = fmaf(pn, sv[n][kq * 16 + i], acc[i]);
-    }
-  }
-  const int row = q0 + r0 + r;
-  if (r < rows && row < p.total_q) {
-    const float inv = lrow > 0.f ? 1.f / lrow : 0.f;
-    T* dst = og + (static_cast<size_t>(row) * kQHeads + 2 * h + (m >> 3)) * kHeadDim + kq * 16;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) store_out(dst + i, acc[i] * inv);
-  }
-}
-
 // ---------------------------------------------------------------------------
 // bf16 tensor-core kernel (tcgen05), one persistent CTA per SM over the plan's items.
 //
@@ -819,6 +703,171 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   if (warp == 8) train::tmem_dealloc(tmem, 512);
 }
 
+// ---------------------------------------------------------------------------
+// fp32 kernel (CUDA cores) over the same plan: products, softmax and sums in fp32.
+//
+// CTA (item, 32 query rows of it): 64 rows of S, 32 keys at a time in shared memory. A
+// thread owns kRpt rows and one sixteenth of the keys, then of d; the 16 lanes that share
+// its rows reduce the maximum and the sum by shuffles and pass P through shared memory
+// inside their warp. The FMA rate bounds it; items of at most 8 query rows take kRpt = 1 (16
+// rows) instead of multiplying 48 empty ones. A dual item's keys all go to its first slot.
+constexpr int kF32Threads2 = 256, kF32Keys2 = 32, kF32Sub = 32;
+constexpr int kF32Pitch = kHeadDim + 4;
+constexpr size_t kF32SmemBytes = (64 * kF32Pitch + kF32Keys2 * kF32Pitch + kF32Keys2 * kHeadDim + 64 * 33) * sizeof(float);
+
+template <int kRpt>
+__device__ __forceinline__ void f32_item(const Params& p, const ItemView& x, int sub, float* smem, float* part) {
+  float* sq = smem;
+  float* sk = sq + 64 * kF32Pitch;
+  float* sv = sk + kF32Keys2 * kF32Pitch;
+  float* sp = sv + kF32Keys2 * kHeadDim;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int rows = 2 * min(kF32Sub, x.nq - sub);           // rows of S: 2 * query row + head
+  const float* qg = static_cast<const float*>(p.q);
+  for (int u = tid; u < 16 * kRpt * (kHeadDim / 4); u += kF32Threads2) {
+    const int m = u >> 5, d = (u & 31) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m < rows)
+      v = *reinterpret_cast<const float4*>(
+          qg + (static_cast<size_t>(x.q0 + sub + (m >> 1)) * kQHeads + 2 * x.head + (m & 1)) * kHeadDim + d);
+    *reinterpret_cast<float4*>(sq + m * kF32Pitch + d) = v;
+  }
+  float mrow[kRpt], lrow[kRpt], acc[kRpt][8];
+#pragma unroll
+  for (int i = 0; i < kRpt; ++i) {
+    mrow[i] = -INFINITY;
+    lrow[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) acc[i][d] = 0.f;
+  }
+#pragma unroll 1
+  for (int s = 0; s < x.nsegs; ++s) {
+    const Source& src = p.src[x.src[s]];
+    const float* kg = static_cast<const float*>(src.k);
+    const float* vg = static_cast<const float*>(src.v);
+    const long long row0 = src.off + x.row[s];
+#pragma unroll 1
+    for (int k0 = 0; k0 < x.len[s]; k0 += kF32Keys2) {
+      const int keys = min(kF32Keys2, x.len[s] - k0);
+      __syncthreads();
+      for (int u = tid; u < kF32Keys2 * (kHeadDim / 4); u += kF32Threads2) {
+        const int n = u >> 5, d = (u & 31) * 4;
+        float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
+        if (n < keys) {
+          const size_t off = (static_cast<size_t>(row0 + k0 + n) * kKVHeads + x.head) * kHeadDim + d;
+          kv = __ldg(reinterpret_cast<const float4*>(kg + off));
+          vv = __ldg(reinterpret_cast<const float4*>(vg + off));
+        }
+        *reinterpret_cast<float4*>(sk + n * kF32Pitch + d) = kv;
+        *reinterpret_cast<float4*>(sv + n * kHeadDim + d) = vv;
+      }
+      __syncthreads();
+      float dot[kRpt][2] = {};
+#pragma unroll 4
+      for (int d = 0; d < kHeadDim; d += 4) {
+        const float4 ka = *reinterpret_cast<const float4*>(sk + tx * kF32Pitch + d);
+        const float4 kb = *reinterpret_cast<const float4*>(sk + (tx + 16) * kF32Pitch + d);
+#pragma unroll
+        for (int i = 0; i < kRpt; ++i) {
+          const float4 q = *reinterpret_cast<const float4*>(sq + (ty * kRpt + i) * kF32Pitch + d);
+          dot[i][0] = fmaf(q.x, ka.x, fmaf(q.y, ka.y, fmaf(q.z, ka.z, fmaf(q.w, ka.w, dot[i][0]))));
+          dot[i][1] = fmaf(q.x, kb.x, fmaf(q.y, kb.y, fmaf(q.z, kb.z, fmaf(q.w, kb.w, dot[i][1]))));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kRpt; ++i) {
+        const int m = ty * kRpt + i;
+        const int see = min(keys, x.visible + sub + (m >> 1) - (x.pos[s] + k0));
+        const float a = tx < see ? dot[i][0] * p.scale : -INFINITY, b = tx + 16 < see ? dot[i][1] * p.scale : -INFINITY;
+        float mx = fmaxf(a, b);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float mn = fmaxf(mrow[i], mx), mu = mn == -INFINITY ? 0.f : mn;
+        const float alpha = expf(mrow[i] - mu), ea = expf(a - mu), eb = expf(b - mu);
+        float ps = ea + eb;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
+        lrow[i] = lrow[i] * alpha + ps;
+        mrow[i] = mn;
+        sp[m * 33 + tx] = ea;
+        sp[m * 33 + tx + 16] = eb;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[i][d] *= alpha;
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int n = 0; n < kF32Keys2; ++n) {
+        const float4 va = *reinterpret_cast<const float4*>(sv + n * kHeadDim + 4 * tx);
+        const float4 vb = *reinterpret_cast<const float4*>(sv + n * kHeadDim + 64 + 4 * tx);
+#pragma unroll
+        for (int i = 0; i < kRpt; ++i) {
+          const float e = sp[(ty * kRpt + i) * 33 + n];
+          acc[i][0] = fmaf(e, va.x, acc[i][0]);
+          acc[i][1] = fmaf(e, va.y, acc[i][1]);
+          acc[i][2] = fmaf(e, va.z, acc[i][2]);
+          acc[i][3] = fmaf(e, va.w, acc[i][3]);
+          acc[i][4] = fmaf(e, vb.x, acc[i][4]);
+          acc[i][5] = fmaf(e, vb.y, acc[i][5]);
+          acc[i][6] = fmaf(e, vb.z, acc[i][6]);
+          acc[i][7] = fmaf(e, vb.w, acc[i][7]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRpt; ++i) {
+    const int m = ty * kRpt + i;
+    if (m >= rows) continue;
+    const int lt = sub + (m >> 1);
+    const bool any = lrow[i] > 0.f || lrow[i] != lrow[i];   // (a NaN sum stays NaN)
+    const float inv = any ? 1.f / lrow[i] : 0.f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) acc[i][d] = any ? acc[i][d] * inv : 0.f;
+    const float4 a = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    const float4 b = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+    if (x.slot < 0) {
+      float* dst = static_cast<float*>(p.out) +
+                   (static_cast<size_t>(x.q0 + lt) * kQHeads + 2 * x.head + (m & 1)) * kHeadDim;
+      *reinterpret_cast<float4*>(dst + 4 * tx) = a;
+      *reinterpret_cast<float4*>(dst + 64 + 4 * tx) = b;
+    } else {
+      const int slot = x.slot + (x.dual ? 0 : lt >> 6), rm = 2 * (lt & 63) + (m & 1);
+      float* prow = part + static_cast<size_t>(slot) * (kSlotFloats + 128);
+      *reinterpret_cast<float4*>(prow + tx * 512 + 4 * rm) = a;
+      *reinterpret_cast<float4*>(prow + (16 + tx) * 512 + 4 * rm) = b;
+      if (tx == 0) {
+        prow[kSlotFloats + rm] = any ? mrow[i] * 1.4426950408889634f + log2f(lrow[i]) : -INFINITY;
+        if (x.dual) prow[kSlotFloats + 128 + kSlotFloats + rm] = -INFINITY;     // the second slot holds nothing
+      }
+      if (x.dual) {
+        float* empty = prow + kSlotFloats + 128;
+        *reinterpret_cast<float4*>(empty + tx * 512 + 4 * rm) = make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(empty + (16 + tx) * 512 + 4 * rm) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kF32Threads2) prefix_f32_kernel(const Params p, float* part) {
+  extern __shared__ float f32_smem[];
+  if (!plan_ok(p)) {
+    if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
+    return;
+  }
+  ItemView x;
+  const bool ok = static_cast<int>(blockIdx.x) < p.plan[kHItems] && load_item(p, blockIdx.x, x);
+  const int sub = blockIdx.y * kF32Sub;
+  if (!ok) {
+    if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
+    return;
+  }
+  if (sub >= x.nq) return;
+  if (x.nq - sub <= 8)
+    f32_item<1>(p, x, sub, f32_smem, part);
+  else
+    f32_item<4>(p, x, sub, f32_smem, part);
+}
+
 // Combines the partial rows of a query row's head pair (adjacent rows of a slot, so a lane
 // reads whole 32-byte sectors); lane l owns d = 4 l ..
 //   out = sum_c 2^(L_c - M) o_c / sum_c 2^(L_c - M),  M = max_c L_c
@@ -828,7 +877,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 // many rows the warps are there anyway (1024 rows of 8 parts: 14 us slower in CTAs).
 constexpr int kMergeWideParts = 6, kMergeWidePairs = 2048;
 
-template <int kWarps>
+template <typename T, int kWarps>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const float* part) {
   __shared__ float s_acc[kWarps > 1 ? 8 : 1][8][33];
   __shared__ float2 s_den[8];
@@ -904,10 +953,15 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const
   }
   auto inverse = [](float d) { return d > 0.f ? 1.f / d : (d != d ? d : 0.f); };
   const float i0 = inverse(den0), i1 = inverse(den1);
-  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (static_cast<size_t>(t) * kQHeads + 2 * h) * kHeadDim + 4 * lane;
-  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a[0] * i0, a[1] * i0), pack_bf16x2(a[2] * i0, a[3] * i0));
-  *reinterpret_cast<uint2*>(dst + kHeadDim) =
-      make_uint2(pack_bf16x2(a[4] * i1, a[5] * i1), pack_bf16x2(a[6] * i1, a[7] * i1));
+  T* dst = static_cast<T*>(p.out) + (static_cast<size_t>(t) * kQHeads + 2 * h) * kHeadDim + 4 * lane;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(dst) = make_float4(a[0] * i0, a[1] * i0, a[2] * i0, a[3] * i0);
+    *reinterpret_cast<float4*>(dst + kHeadDim) = make_float4(a[4] * i1, a[5] * i1, a[6] * i1, a[7] * i1);
+  } else {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a[0] * i0, a[1] * i0), pack_bf16x2(a[2] * i0, a[3] * i0));
+    *reinterpret_cast<uint2*>(dst + kHeadDim) =
+        make_uint2(pack_bf16x2(a[4] * i1, a[5] * i1), pack_bf16x2(a[6] * i1, a[7] * i1));
+  }
 }
 
 }  // namespace prefix

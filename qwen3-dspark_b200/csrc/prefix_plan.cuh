@@ -42,7 +42,7 @@ constexpr int kAllVisible = 1 << 30;
 
 enum Head {
   kHMagic = 0, kHRequests, kHTotalQ, kHGrid, kHItems, kHCtaAt, kHItemsAt, kHRequestsAt, kHSlots, kHRuns, kHRunsAt,
-  kHTokenRunAt, kHPrefixRows, kHOwnRows, kHNewRows, kHCausal, kHMaxQ, kHWords, kHCheck, kHMaxParts
+  kHTokenRunAt, kHPrefixRows, kHOwnRows, kHNewRows, kHCausal, kHMaxQ, kHWords, kHCheck, kHMaxParts, kHMaxItemRows
 };
 // Request record: first query row, query rows, then (first row, rows) of prefix, own, new.
 enum RequestField { kRQ0 = 0, kRNq, kRPrefixRow, kRPrefixLen, kROwnRow, kROwnLen, kRNewRow, kRNewLen };
@@ -388,6 +388,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   plan[kHCausal] = in.causal ? 1 : 0;
   plan[kHMaxQ] = max_q;
   plan[kHMaxParts] = max_parts;
+  for (const PlanTile& t : tiles) plan[kHMaxItemRows] = std::max(plan[kHMaxItemRows], t.nq);
   plan[kHWords] = static_cast<int32_t>(words);
   int next = 0;
   for (int c = 0; c < grid; ++c) {

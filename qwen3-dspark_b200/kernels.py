@@ -234,7 +234,7 @@ class B200SharedPrefixKernel:
     or float32 (CUDA cores). A row without a visible key gives zeros. ``out`` (default: a
     new tensor) may be ``query`` itself.
 
-    bf16 partial rows live in a workspace that each call allocates on its own stream, so
+    Partial rows live in a workspace that each call allocates on its own stream, so
     calls on different streams and in different captured graphs share nothing.
     """
     backend_name = PREFIX_BACKEND
@@ -282,7 +282,7 @@ class B200SharedPrefixKernel:
                 out = torch.empty_like(query)
             if total == 0:
                 return out
-            nbytes = layout.workspace_bytes if dtype == torch.bfloat16 else 0
+            nbytes = layout.workspace_bytes
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
             new = (new_key.data_ptr(), new_value.data_ptr()) if new_key is not None else (None, None)
             self._operator(query.data_ptr(), total, prefix_key.data_ptr(), prefix_value.data_ptr(), p_rows, prefix_off,
@@ -435,7 +435,8 @@ def merged_mlp_ready(mlp):
             and (type(mlp.act_fn).__name__ == 'SiLUActivation' or type(mlp.act_fn) is torch.nn.SiLU))
 
 
-def greedy_accept(logits, tokens, cu_query, eos_ids=(), budget=None):
+def greedy_accept(logits, tokens, cu_query, eos_ids=(), budget=None, *, controls=None, slots=None, masks=None,
+                  mask_index=None):
     """Greedy acceptance of one verify round on the GPU (cached_decode.py:84-98).
 
     ``logits`` [N, vocab] (bf16/fp32) are the target's logits of the N verified rows,
@@ -446,6 +447,12 @@ def greedy_accept(logits, tokens, cu_query, eos_ids=(), budget=None):
     caps each request's committed tokens. Returns device tensors
     ``(pred [N] int32, accepted [R] int32, n_commit [R] int32, emitted [N] int64)``
     with ``emitted[cu_query[i] + k]`` the committed tokens of request i (-1 after).
+
+    With ``controls`` (a ``TokenControls``, with the requests' ``slots`` and optionally
+    grammar ``masks`` / ``mask_index`` as in ``control_argmax``) the predictions are the
+    controlled maxima: penalties, biases and masks applied as the logits are read, each
+    row counting the chunk's own proposals. ``controls.commit(slots, emitted, cu_query,
+    n_commit)`` then counts what the round emitted.
     """
     device = logits.device
     if (logits.ndim != 2 or logits.dtype not in _DTYPES or logits.stride(1) != 1 or not logits.is_cuda
@@ -463,13 +470,21 @@ def greedy_accept(logits, tokens, cu_query, eos_ids=(), budget=None):
         eos = torch.tensor(sorted(set(int(e) for e in eos_ids)), dtype=torch.long, device=device)
     if budget is not None and (budget.shape != (r,) or budget.dtype != torch.int32 or budget.device != device):
         raise ValueError('budget must be int32 [R] on the logits device')
+    if controls is None and any(x is not None for x in (slots, masks, mask_index)):
+        raise ValueError('slots, masks and mask_index go with controls')
     n = logits.shape[0]
-    pred = torch.empty(n, dtype=torch.int32, device=device)
+    if controls is None:
+        pred = torch.empty(n, dtype=torch.int32, device=device)
+    else:
+        from .controls import control_argmax
+        pred = control_argmax(logits, controls, slots, cu_query=cu_query, tokens=tokens, masks=masks,
+                              mask_index=mask_index)
     counts = torch.empty(2 * r, dtype=torch.int32, device=device)
     emitted = torch.empty(n, dtype=torch.long, device=device)
     lib, stream = _lib.load_library(), _stream(device)
-    _lib.check(lib.dspark_row_argmax(logits.data_ptr(), logits.stride(0), n, logits.shape[1], _DTYPES[logits.dtype],
-                                     pred.data_ptr(), stream), 'dspark_row_argmax')
+    if controls is None:
+        _lib.check(lib.dspark_row_argmax(logits.data_ptr(), logits.stride(0), n, logits.shape[1],
+                                         _DTYPES[logits.dtype], pred.data_ptr(), stream), 'dspark_row_argmax')
     _lib.check(lib.dspark_greedy_accept(pred.data_ptr(), tokens.data_ptr(), cu_query.contiguous().data_ptr(), r, n,
                                         eos.data_ptr() if eos.numel() else None, eos.numel(),
                                         budget.data_ptr() if budget is not None else None, counts.data_ptr(),

@@ -61,10 +61,11 @@ def _pinned(values, dtype, device):
     return torch.tensor(values, dtype=dtype).pin_memory().to(device, non_blocking=True)
 
 
-def _accept_on_device(target, verified, ids, active, width, output, max_new_tokens, eos_ids):
+def _accept_on_device(target, verified, ids, active, width, output, max_new_tokens, eos_ids, controls=None):
     """One round's acceptance with the on-device argmax + accept kernels: the host
     reads back one small int64 vector (counts and committed tokens) per round.
-    ``ids`` [R, width] are the verified chunks (anchor, proposals) in ``active`` order."""
+    ``ids`` [R, width] are the verified chunks (anchor, proposals) in ``active`` order. The
+    second result is what ``controls.commit`` counts once the round is known to be good."""
     from .kernels import greedy_accept
     logits = target.model.get_output_embeddings()(verified.last)[0]
     tokens = ids.reshape(-1)
@@ -72,18 +73,21 @@ def _accept_on_device(target, verified, ids, active, width, output, max_new_toke
     dev = logits.device
     cu_q = _pinned(cu, torch.int32, dev)
     budget = _pinned([max_new_tokens - len(output[r]) for r in active], torch.int32, dev)
-    _pred, accepted, n_commit, emitted = greedy_accept(logits, tokens, cu_q, eos_ids, budget)
+    slots = None if controls is None else controls.slot_index(active)
+    _pred, accepted, n_commit, emitted = greedy_accept(logits, tokens, cu_q, eos_ids, budget, controls=controls,
+                                                       slots=slots)
     host = torch.cat((accepted.long(), n_commit.long(), emitted)).cpu().tolist()
     n = len(active)
     result = {}
     for i, r in enumerate(active):
         k = host[n + i]
         result[r] = (host[i], host[2 * n + cu[i]:2 * n + cu[i] + k])
-    return result
+    return result, (slots, emitted, cu_q, n_commit)
 
 
 @torch.no_grad()
-def speculative_greedy(target, draft, prompts, max_new_tokens, eos_ids=(), device_accept=True, graph=False):
+def speculative_greedy(target, draft, prompts, max_new_tokens, eos_ids=(), device_accept=True, graph=False,
+                       controls=None):
     """prompts: {request: ids [1, P]} on the target device. Returns ({request: tokens}, rounds).
 
     ``device_accept`` runs the argmax and the accept rule on the GPU (one small
@@ -92,9 +96,18 @@ def speculative_greedy(target, draft, prompts, max_new_tokens, eos_ids=(), devic
     forward from a CUDA graph captured once per set of chunk lengths (``QueryBucket``)
     and, for bf16 drafts with the fused Markov head, the draft proposal from a graph
     captured once per request count, instead of running them eagerly; the tokens are
-    the same."""
+    the same.
+
+    ``controls`` (a ``TokenControls`` that holds every request of ``prompts``, with its
+    prompt, penalties and biases) makes the output the target's own controlled greedy
+    decode: the drafts propose as before, acceptance compares with the controlled
+    predictions, and every emitted token is counted. Needs ``device_accept``."""
     if type(max_new_tokens) is not int or max_new_tokens < 0:
         raise ValueError('max_new_tokens must be a nonnegative integer')
+    if controls is not None:
+        if not device_accept:
+            raise ValueError('controls are applied by the on-device acceptance')
+        all_slots = controls.slot_index(list(prompts))
     eos_ids = set(eos_ids)
     for r in prompts:
         target.add_request(r)
@@ -103,8 +116,15 @@ def speculative_greedy(target, draft, prompts, max_new_tokens, eos_ids=(), devic
         return {r: [] for r in prompts}, []
     features = target.prefill(prompts)
     last = target.predict(features, last_only=True)
-    output = {r: [int(last[r].argmax(-1).item())] for r in prompts}
+    if controls is None:
+        output = {r: [int(last[r].argmax(-1).item())] for r in prompts}
+    else:
+        from .controls import control_argmax
+        first = control_argmax(torch.cat([last[r].reshape(1, -1) for r in prompts]), controls, all_slots)
+        output = {r: [t] for r, t in zip(prompts, first.tolist())}
     _round_status(where='prefill')
+    if controls is not None:
+        controls.commit(all_slots, first.long(), _pinned(list(range(len(prompts) + 1)), torch.int32, target.device))
     draft.append_committed({r: features.context_for(r) for r in prompts})
     active = [r for r in prompts if output[r][-1] not in eos_ids and max_new_tokens > 1]
     rounds = []
@@ -130,7 +150,8 @@ def speculative_greedy(target, draft, prompts, max_new_tokens, eos_ids=(), devic
         else:
             verified = target.verify(chunks)
         if device_accept:
-            decided = _accept_on_device(target, verified, ids, active, width, output, max_new_tokens, eos_ids)
+            decided, emitted = _accept_on_device(target, verified, ids, active, width, output, max_new_tokens,
+                                                 eos_ids, controls)
         else:
             logits = target.predict(verified)
             host_ids = ids.tolist()
@@ -139,6 +160,8 @@ def speculative_greedy(target, draft, prompts, max_new_tokens, eos_ids=(), devic
                 accepted, committed = accept_greedy(host_ids[i][1:], v[0].argmax(-1).tolist(), eos_ids)
                 decided[r] = (accepted, committed[:max_new_tokens - len(output[r])])
         _round_status(target, verified)
+        if controls is not None:
+            controls.commit(*emitted)
         commit, stats = {}, {}
         for r in active:
             accepted, committed = decided[r]
