@@ -611,29 +611,26 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
     __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) +
                           (static_cast<size_t>(q0 + (row_ok ? lt : 0)) * kQHeads + 2 * head + (rm & 1)) * kHeadDim;
     if (warp_ok) {
+      // (small code: a launch meets it cold, and unrolled over the row the first epilogue took
+      // 5,000 cycles of instruction fetches)
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r0[32], r1[32];
-        train::tmem_ld32_async(o_addr + 64 * c, r0);
-        train::tmem_ld32_async(o_addr + 64 * c + 32, r1);
-        train::tmem_ld_wait();
-        train::tmem_ld_landed(r0);
-        train::tmem_ld_landed(r1);
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        train::tmem_ld32(o_addr + 32 * c, o);
         // (without a visible key O was never written, or holds products of zeros)
-        auto o = [&](int i) {
-          return inv != 0.f ? __uint_as_float(i < 32 ? r0[i & 31] : r1[i & 31]) * inv : 0.f;
-        };
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = inv != 0.f ? o[i] * inv : 0.f;
         if (row_ok && slot < 0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(orow + 64 * c + 8 * j) =
-                make_uint4(pack_bf16x2(o(8 * j), o(8 * j + 1)), pack_bf16x2(o(8 * j + 2), o(8 * j + 3)),
-                           pack_bf16x2(o(8 * j + 4), o(8 * j + 5)), pack_bf16x2(o(8 * j + 6), o(8 * j + 7)));
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(orow + 32 * c + 8 * j) =
+                make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]),
+                           pack_bf16x2(o[8 * j + 4], o[8 * j + 5]), pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
         } else if (row_ok) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            __stcg(reinterpret_cast<float4*>(prow + (16 * c + j) * 512 + 4 * rm),
-                   make_float4(o(4 * j), o(4 * j + 1), o(4 * j + 2), o(4 * j + 3)));
+          for (int j = 0; j < 8; ++j)
+            __stcg(reinterpret_cast<float4*>(prow + (8 * c + j) * 512 + 4 * rm),
+                   make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
         }
       }
       if (row_ok && slot >= 0)
