@@ -678,12 +678,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   train::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kSmemSlot);
   // 384 threads are launched with 168 registers each (64,512). A softmax thread holds a row
-  // of 128 scores: its warpgroups grow to 208 each out of what the third one gives back
-  // (2 x 128 x 208 + 128 x 72 = 62,464); without this the row spills to local memory.
+  // of 128 scores: its warpgroups grow to 200 each out of what the third one gives back
+  // (2 x 128 x 200 + 128 x 96 = 63,488); without this the row spills to local memory (444
+  // instead of 724 us at 1024 query rows x 32768 shared keys with 512 own keys a request).
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   }
   if (warp < 8) {
     softmax_role(p, part, first, last, bars, tmem, abort_flag);
