@@ -94,15 +94,18 @@ class TokenControls:
         self._slots[request] = slot
         self.counts[slot].zero_()
         self.prompt_bits[slot].zero_()
-        self.penalties[slot].copy_(_row([repetition, frequency, presence], self.device))
-        self.bias_len[slot:slot + 1].fill_(0 if ids is None else ids.numel())
-        if ids is not None:
-            self.bias_ids[slot, :ids.numel()].copy_(ids)
-            self.bias_values[slot, :ids.numel()].copy_(values)
-        index = _upload([slot], self.device)
-        for tokens, to_counts in ((prompt, False), (output, True)):
+        n_bias = 0 if ids is None else ids.numel()
+        # one upload: the penalties' bits, the bias count, the slot and the two token ranges
+        host = torch.tensor([repetition, frequency, presence], dtype=torch.float32).view(torch.int32).tolist()
+        words = _upload(host + [n_bias, slot, 0, prompt.numel(), 0, output.numel()], self.device)
+        self.penalties[slot].copy_(words[:3].view(torch.float32))
+        self.bias_len[slot:slot + 1].copy_(words[3:4])
+        if n_bias:
+            self.bias_ids[slot, :n_bias].copy_(ids)
+            self.bias_values[slot, :n_bias].copy_(values)
+        for tokens, cu, to_counts in ((prompt, words[5:7], False), (output, words[7:9], True)):
             if tokens.numel():
-                self._add(tokens, _upload([0, tokens.numel()], self.device), None, index, to_counts)
+                self._add(tokens, cu, None, words[4:5], to_counts)
         return slot
 
     def remove_request(self, request):
@@ -140,10 +143,6 @@ class TokenControls:
             raise ValueError('commit: contiguous int32 [R] slots, int64 [N] emitted, int32 [R + 1] cu_query and int32 '
                              '[R] n_commit on the tables\' device required')
         self._add(emitted, cu_query, n_commit, slots, True)
-
-
-def _row(values, device):
-    return torch.tensor(values, dtype=torch.float32).pin_memory().to(device, non_blocking=True)
 
 
 def _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index):

@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(256) control_tokens_kernel(const TokenParams p
     return;
   }
   const int n = p.n ? min(max(p.n[r], 0), b - a) : b - a;
-  for (int k = threadIdx.x; k < n; k += blockDim.x) {
+  for (int k = blockIdx.y * blockDim.x + threadIdx.x; k < n; k += gridDim.y * blockDim.x) {
     const long long t = p.tokens[a + k];
     if (t < 0 || t >= p.vocab) {
       atomicOr(&g_device_status, kStatusBadArgument);

@@ -1318,7 +1318,9 @@ int dspark_control_tokens(const long long* tokens, int num_tokens, const int32_t
   if (!tokens || !cu || !slots) return DSPARK_ERR_INVALID_ARGUMENT;
   const controls::TokenParams tp{tokens, cu, n, slots, num_tokens, num_slots, vocab, counts, ld_counts, prompt_bits,
                                  ld_bits};
-  controls::control_tokens_kernel<<<num_requests, 256, 0, stream>>>(tp);
+  // a long history (one request's prompt) is spread over several CTAs
+  const int per = std::min(32, std::max(1, num_tokens / num_requests / 256));
+  controls::control_tokens_kernel<<<dim3(num_requests, per), 256, 0, stream>>>(tp);
   return launch_status();
 }
 
