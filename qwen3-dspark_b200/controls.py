@@ -220,7 +220,7 @@ def control_argmax(logits, controls, slots, *, cu_query=None, tokens=None, masks
     """Index of each row's largest controlled logit, int32 [N] (``dspark_control_argmax``): the
     arguments of ``control_logits``, nothing written but the indices. Ties give the lowest
     index, NaN is largest, and a row whose mask allows nothing gives -1 and sets the
-    device status bit ``DEVICE_EMPTY_MASK``."""
+    device status bit ``DEVICE_EMPTY_MASK``. Rows outside every request stay unset."""
     args = _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index)
     lib = _lib.load_library()
     with _on_device(logits.device):

@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
+#include <exception>
 #include <mutex>
 #include <numeric>
 #include <queue>
@@ -100,6 +101,14 @@ int device_info(int dev, DeviceInfo* out) {
         cudaFuncSetAttribute(append::draft_append_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(append::PairCfg::kSmemBytes)) != cudaSuccess)
       return DSPARK_ERR_CUDA;
+    {
+      // the prefix kernel's register split must fit what its CTA is launched with: a
+      // setmaxnreg.inc beyond it would wait forever
+      cudaFuncAttributes attr;
+      if (cudaFuncGetAttributes(&attr, prefix::prefix_attn_kernel) != cudaSuccess) return DSPARK_ERR_CUDA;
+      if (attr.numRegs * prefix::kAttThreads < 256 * prefix::kSoftmaxRegs + 128 * prefix::kOtherRegs)
+        return DSPARK_ERR_UNSUPPORTED;
+    }
     {
       // CTA pairs of the 2-SM append the GPU holds at once (a pair needs two SMs of
       // one GPC); a refused query leaves the single-CTA kernels in use.
@@ -1160,7 +1169,7 @@ int dspark_prefix_plan(int num_groups, const int32_t* group_size, const int32_t*
     if (plan_capacity < *plan_words) return plan == nullptr ? DSPARK_OK : DSPARK_ERR_INVALID_ARGUMENT;
     if (plan != nullptr) std::copy(words.begin(), words.end(), plan);
     return DSPARK_OK;
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {      // no memory for a plan of this size
     return DSPARK_ERR_UNSUPPORTED;
   }
 }

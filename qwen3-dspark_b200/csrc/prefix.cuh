@@ -51,8 +51,8 @@ __device__ __forceinline__ bool plan_ok(const Params& p) {
 //                   registers (no exchange between threads); P (bf16) overwrites its S
 //                   columns in TMEM; the running maximum is raised, and O rescaled, only
 //                   when it grows by more than 2^8 (exact: O / l does not depend on it);
-//   warps 8, 9      MMA issuers of tile A / B (one thread each): S = Q K^T, O += P V. The
-//                   MMAs of one thread execute in order, so S(i + 1) may follow PV(i)
+//   warps 8, 9      MMA issuers of tile A / B (an elected lane each): S = Q K^T, O += P V.
+//                   The MMAs of one thread execute in order, so S(i + 1) may follow PV(i)
 //                   over the P it reads without a wait, and the tiles alternate on the
 //                   tensor pipe: one tile's products run under the other's softmax;
 //   warp 10         TMA producer: Q per item, K and V blocks through one ring of 32 KB
@@ -62,6 +62,11 @@ __device__ __forceinline__ bool plan_ok(const Params& p) {
 // Short blocks load only boxes of 32 rows that hold keys, and multiply only N =
 // keys rounded up to 16. Every wait is bounded; a timed-out wait raises the CTA abort
 // flag, copies and MMAs in flight are drained and TMEM is released.
+//
+// Bound by the softmax chain where there are many rows (1024 rows x 32768 keys: about 270 us,
+// 1,000 TFLOP/s of 1,666; a block of both tiles takes 3,700 cycles of which the MMAs are
+// 2,048) and by DRAM and the latency of short items where there are few (8 rows x 32768 keys:
+// 40 us with the merge; the keys alone take 21).
 constexpr int kStagesN = 5;
 constexpr int kAttThreads = 12 * 32;
 constexpr uint32_t kSmemQ = 0;                             // 2 tiles x 32 KB
@@ -72,6 +77,9 @@ enum Bar {
   kBSFull = kBFixed + kStagesN, kBPFull = kBSFull + 2, kBODone = kBPFull + 2, kBOFree = kBODone + 2,
   kBTurn = kBOFree + 2, kBDrain = kBTurn + 2, kNumBars
 };
+// Registers per thread of the softmax warpgroups and of the third one after setmaxnreg; the
+// launch's own (kAttThreads x the kernel's count, checked when the device is set up) cover them.
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 96;
 constexpr uint32_t kSmemSlot = kSmemBar + kNumBars * 8;
 constexpr uint32_t kSmemAbort = kSmemSlot + 4;
 constexpr uint32_t kSmemBytes = 1024 + kSmemAbort + 4;
@@ -127,9 +135,6 @@ struct BlockWalk {
   __device__ __forceinline__ int keys(const ItemView& x) const {
     const int len = seg == 0 ? x.len[0] : (seg == 1 ? x.len[1] : x.len[2]);
     return min(kBlock, len - at);
-  }
-  __device__ __forceinline__ int pos(const ItemView& x) const {
-    return (seg == 0 ? x.pos[0] : (seg == 1 ? x.pos[1] : x.pos[2])) + at;
   }
   __device__ __forceinline__ int row(const ItemView& x) const {
     return (seg == 0 ? x.row[0] : (seg == 1 ? x.row[1] : x.row[2])) + at;
@@ -682,9 +687,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   // (2 x 128 x 200 + 128 x 96 = 63,488); without this the row spills to local memory (444
   // instead of 724 us at 1024 query rows x 32768 shared keys with 512 own keys a request).
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   }
   if (warp < 8) {
     softmax_role(p, part, first, last, bars, tmem, abort_flag);

@@ -223,6 +223,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
     r += n;
   }
   if (r != in.requests) return kPlanInvalid;
+  if (tiles.size() > 500000) return kPlanTooLarge;
 
   // Cut the chains: try several piece lengths and keep the shortest schedule. Pieces
   // are the same for the 8 KV heads, so a slot index is computed from (piece, head).

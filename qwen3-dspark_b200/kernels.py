@@ -255,8 +255,8 @@ class B200SharedPrefixKernel:
         rows = []
         for t, heads in ((query, HQ), (prefix_key, HKV), (prefix_value, HKV), (key, HKV), (value, HKV), (new_key, HKV),
                          (new_value, HKV), (out, HQ)):
-            if t is None:
-                rows.append(0)
+            if t is None and len(rows) >= 5:
+                rows.append(0)                       # new rows and out are optional
                 continue
             if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or dtype not in _DTYPES
                     or t.requires_grad or t.ndim != 3 or not t.is_contiguous()):

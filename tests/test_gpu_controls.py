@@ -217,6 +217,30 @@ def test_strided_in_place_and_untouched_rows(pkg, vocab, dtype):
     status_clean(pkg)
 
 
+def test_division_equals_torch(pkg):
+    """Every token seen: positive logits are divided by the repetition penalty, correctly rounded,
+    over penalties and logits of many magnitudes (the vocabulary's tail takes other paths)."""
+    r, vocab = 48, 8192 + 72
+    g = torch.Generator(device='cpu').manual_seed(5)
+    controls = pkg.TokenControls(r, vocab, device=dev())
+    reps = torch.cat([1 + torch.rand(20, generator=g), torch.rand(8, generator=g) * 10 + 1e-3,
+                      2.0 ** torch.randint(-60, 60, (8,), generator=g) * (1 + torch.rand(8, generator=g)),
+                      torch.nextafter(2.0 ** torch.arange(-4, 4).float(), torch.zeros(8)),
+                      torch.tensor([1.0, 3.0, 1 + 2.0 ** -23, 1e-30])])
+    for i in range(r):
+        controls.add_request(f'r{i}', repetition=float(reps[i]))
+    controls.prompt_bits.fill_(-1)
+    x = (torch.rand((r, vocab), generator=g) + 1e-3) * 2.0 ** torch.randint(-30, 30, (r, vocab), generator=g)
+    x[:, :64] *= 1e-22
+    x[:, 64:128] *= 1e25
+    x[:, 128:4000] *= -1
+    x[0, 7], x[1, 7], x[2, 7] = float('inf'), float('-inf'), 0.0
+    want = torch.where(x > 0, x / reps[:, None], x * reps[:, None])
+    got = pkg.control_logits(x.to(dev()), controls, controls.slot_index([f'r{i}' for i in range(r)])).cpu()
+    assert torch.equal(got, want)
+    status_clean(pkg)
+
+
 def test_commit_counts_emitted_tokens(pkg):
     controls = pkg.TokenControls(3, 101, device=dev())
     for n in 'abc':

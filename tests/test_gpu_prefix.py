@@ -176,7 +176,7 @@ def test_refusals(pkg):
     for bad in (dict(query=ok['query'][:2]), dict(query=ok['query'].float()), dict(query=ok['query'].cpu()),
                 dict(query=ok['query'].half()), dict(scale=0.1), dict(layout=object()), dict(key=ok['key'][:, :4]),
                 dict(value=ok['value'][:-1]), dict(prefix_key=ok['prefix_key'].transpose(0, 1)),
-                dict(prefix_key=ok['prefix_key'][:5], prefix_value=ok['prefix_value'][:5]), dict(new_key=None),
+                dict(prefix_key=ok['prefix_key'][:5], prefix_value=ok['prefix_value'][:5]), dict(new_key=None), dict(key=None), dict(prefix_value=None),
                 dict(new_key=None, new_value=None), dict(prefix_off=9), dict(prefix_off=-1), dict(own_off=1.0),
                 dict(out=torch.empty_like(ok['query'][:1])), dict(query=ok['query'].clone().requires_grad_())):
         with pytest.raises(ValueError):
