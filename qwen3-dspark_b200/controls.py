@@ -201,18 +201,21 @@ def control_logits(logits, controls, slots, *, cu_query=None, tokens=None, masks
     ``mask_value`` replaces forbidden logits: a finite one (``torch.finfo(dtype).min``) keeps
     the rows acceptable to ``stochastic_accept``, which refuses infinities."""
     args = _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index)
+    device, ld_out = controls.device, controls.vocab
     if out is None:
-        out = torch.empty(logits.shape, dtype=out_dtype or logits.dtype, device=logits.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError('out has another dtype than out_dtype')
-    if (out.shape != logits.shape or out.device != logits.device or out.stride(1) != 1
-            or (len(out) > 1 and out.stride(0) < controls.vocab)
-            or (out.dtype != logits.dtype and out.dtype != torch.float32)):
-        raise ValueError('out must be [N, vocab] rows of the logits\' dtype or float32 on their device')
-    with _on_device(logits.device):
+        if out_dtype is not None and out_dtype != logits.dtype and out_dtype != torch.float32:
+            raise ValueError("out_dtype must be the logits' dtype or float32")
+        out = torch.empty_like(logits, dtype=out_dtype, memory_format=torch.contiguous_format)
+    else:
+        if (out.shape != logits.shape or out.device != device or out.stride(1) != 1
+                or (len(out) > 1 and out.stride(0) < ld_out) or (out_dtype is not None and out.dtype != out_dtype)
+                or (out.dtype != logits.dtype and out.dtype != torch.float32)):
+            raise ValueError("out must be [N, vocab] rows of the logits' dtype or float32 on their device")
+        ld_out = max(out.stride(0), ld_out)
+    with _on_device(device):
         _lib.check(_lib.load_library().dspark_control_logits(
-            *args, float(mask_value), out.data_ptr(), max(out.stride(0), controls.vocab), _DTYPES[out.dtype],
-            _stream(logits.device)), 'dspark_control_logits')
+            *args, float(mask_value), out.data_ptr(), ld_out, _DTYPES[out.dtype], _stream(device)),
+            'dspark_control_logits')
     return out
 
 
@@ -222,11 +225,13 @@ def control_argmax(logits, controls, slots, *, cu_query=None, tokens=None, masks
     index, NaN is largest, and a row whose mask allows nothing gives -1 and sets the
     device status bit ``DEVICE_EMPTY_MASK``. Rows outside every request stay unset."""
     args = _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index)
-    lib = _lib.load_library()
-    with _on_device(logits.device):
-        pred = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
-        nbytes = int(lib.dspark_control_argmax_scratch_bytes(*logits.shape))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-        _lib.check(lib.dspark_control_argmax(*args, pred.data_ptr(), scratch.data_ptr(), nbytes,
-                                             _stream(logits.device)), 'dspark_control_argmax')
+    lib, device = _lib.load_library(), controls.device
+    with _on_device(device):
+        n = len(logits)
+        nbytes = lib.dspark_control_argmax_scratch_bytes(n, controls.vocab)
+        # one allocation: 8-byte partial maxima, then the indices
+        scratch = controls.bias_len.new_empty(nbytes // 4 + n)
+        pred = scratch[nbytes // 4:]
+        _lib.check(lib.dspark_control_argmax(*args, pred.data_ptr(), scratch.data_ptr(), nbytes, _stream(device)),
+                   'dspark_control_argmax')
     return pred

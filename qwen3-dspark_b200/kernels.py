@@ -52,7 +52,11 @@ def runtime_identity(device):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle (torch.cuda.current_stream builds a stream object first:
+    2.3 us a call against 0.1)."""
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 _NO_SWITCH = contextlib.nullcontext()
@@ -283,7 +287,7 @@ class B200SharedPrefixKernel:
             if total == 0:
                 return out
             nbytes = layout.workspace_bytes
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+            ws = query.new_empty(nbytes // query.element_size()) if nbytes else None
             new = (new_key.data_ptr(), new_value.data_ptr()) if new_key is not None else (None, None)
             self._operator(query.data_ptr(), total, prefix_key.data_ptr(), prefix_value.data_ptr(), p_rows, prefix_off,
                            key.data_ptr(), value.data_ptr(), a_rows, own_off, *new, b_rows, new_off,
