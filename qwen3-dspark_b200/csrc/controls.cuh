@@ -316,9 +316,10 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     }
   };
   uint32_t next[kWords];
-  stage();
-  // (row 0 is read whole, before its mask is there)
+  // row 0 is on its way with the tables, read whole before its mask is there
+  batch = min(kRowBatch, nq);
   fetch(0, inside, next, !p.in_place || p.masks);
+  stage();
   // The chunk's biases, compacted in list order (so that a token's entries add in that order);
   // more than kListCap of them are read from the list itself.
   int listed = 0;
