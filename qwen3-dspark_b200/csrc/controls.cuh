@@ -145,23 +145,25 @@ __device__ __forceinline__ float bf16_half(uint32_t w, int high) {
   return __uint_as_float(high ? w & 0xffff0000u : w << 16);
 }
 
-// List entry: token - base (12 bits), count (15 bits), in the prompt, has a bias.
-constexpr uint32_t kEntryPrompt = 1u << 27, kEntryBias = 1u << 28;
+// List entry: token - base (12 bits), in the prompt, has a bias.
+constexpr uint32_t kEntryPrompt = 1u << 12, kEntryBias = 1u << 13;
 
 // kVec: every row starts on a boundary of the vector accesses and a thread owns two runs of
 // 8 consecutive tokens; otherwise its tokens lie 256 apart, so that the element accesses of
 // a warp stay contiguous whatever the row's alignment.
 template <typename TIn, typename TOut, bool kArgmax, bool kVec>
 __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
-  __shared__ uint32_t s_list[kChunk];
-  __shared__ float s_bias[kChunk];
+  __shared__ uint16_t s_list[kChunk];
+  __shared__ __align__(16) uint16_t s_counts[kChunk];
+  __shared__ float s_bias[kListCap];             // of the list's first entries
   __shared__ int s_id[kListCap];
   __shared__ float s_val[kListCap];
   __shared__ int s_count[kThreads / 32];
   __shared__ unsigned long long s_best[kRowBatch][kThreads / 32], s_list_best[kRowBatch];
   __shared__ uint32_t s_top[kRowBatch];
   __shared__ int s_mask[kRowBatch], s_token[kRowBatch];
-  __shared__ int s_n, s_proposals;
+  __shared__ int s_n;
+  __shared__ uint32_t s_proposals;               // rows whose proposal lies in this chunk
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // chunks in order, so that the first ones (low token ids are the frequent ones: long lists)
   // do not start last
@@ -346,6 +348,13 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
   }
   const bool in_smem = listed <= kListCap;
   const int list_n = in_smem ? listed : nb;
+  auto bias_of = [&](int v) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < list_n; ++k)
+      if ((in_smem ? s_id[k] : list_id[k]) == v) sum = __fadd_rn(sum, in_smem ? s_val[k] : list_val[k]);
+    return sum;
+  };
   __syncthreads();
   uint32_t biased = 0;
   if (listed > 0) {
@@ -355,37 +364,45 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     }
     biased &= inside;
   }
-  // Tokens that were seen or have a bias, into the list (in any order).
+  // Counts into shared memory (a thread's own tokens, which only it will change), tokens that
+  // were seen or have a bias into the list (in any order).
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     used |= static_cast<uint32_t>(static_cast<short>(cw[k] & 0xffffu) > 0) << (2 * k);
     used |= static_cast<uint32_t>(static_cast<int>(cw[k]) >> 16 > 0) << (2 * k + 1);
   }
-  changed = prompt | used | biased;
-  int at = __popc(changed);                      // the warp's entries lie behind one another
+  if (kVec) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, at, o);
-    if (lane >= o) at += v;
+    for (int o = 0; o < 2; ++o)
+      *reinterpret_cast<uint4*>(&s_counts[rel(8 * o)]) = make_uint4(cw[4 * o], cw[4 * o + 1], cw[4 * o + 2], cw[4 * o + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) s_counts[rel(e)] = static_cast<uint16_t>(cw[e >> 1] >> (16 * (e & 1)));
   }
-  int first = 0;
-  if (lane == 31 && at > 0) first = atomicAdd(&s_n, at);
-  at += __shfl_sync(0xffffffffu, first, 31) - __popc(changed);
+  changed = prompt | used | biased;
+  // biased tokens first, so that their sums fit s_bias unless there are more than kListCap
 #pragma unroll 1
-  for (uint32_t m = changed; m != 0; m &= m - 1, ++at) {
-    const int e = __ffs(m) - 1;
-    uint32_t count = 0;
+  for (int pass = listed > 0 ? 0 : 1; pass < 2; ++pass) {
+    const uint32_t set = pass == 0 ? biased : changed & ~biased;
+    if (__any_sync(0xffffffffu, set != 0)) {
+      int at = __popc(set);                      // the warp's entries lie behind one another
 #pragma unroll
-    for (int k = 0; k < 8; ++k) count = k == (e >> 1) ? cw[k] : count;
-    count = ((used >> e) & 1u) ? (count >> (16 * (e & 1))) & 0x7fffu : 0u;
-    s_list[at] = static_cast<uint32_t>(rel(e)) | (count << 12) | (((prompt >> e) & 1u) ? kEntryPrompt : 0u) |
-                 (((biased >> e) & 1u) ? kEntryBias : 0u);
-    if ((biased >> e) & 1u) {
-      float sum = 0.f;
-      for (int k = 0; k < list_n; ++k)
-        if ((in_smem ? s_id[k] : list_id[k]) == index(e)) sum = __fadd_rn(sum, in_smem ? s_val[k] : list_val[k]);
-      s_bias[at] = sum;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += v;
+      }
+      int first = 0;
+      if (lane == 31) first = atomicAdd(&s_n, at);
+      at += __shfl_sync(0xffffffffu, first, 31) - __popc(set);
+#pragma unroll 1
+      for (uint32_t m = set; m != 0; m &= m - 1, ++at) {
+        const int e = __ffs(m) - 1;
+        s_list[at] = static_cast<uint16_t>(static_cast<uint32_t>(rel(e)) | (((prompt >> e) & 1u) * kEntryPrompt) |
+                                           (pass == 0 ? kEntryBias : 0u));
+        if (pass == 0 && at < kListCap) s_bias[at] = bias_of(index(e));
+      }
     }
+    if (pass == 0) __syncthreads();
   }
 
   for (; j0 < nq; j0 += kRowBatch) {
@@ -396,15 +413,14 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     // Pipelined by rows: while row j is decided, row j + 1's logits and row j + 2's mask words
     // are in flight.
     uint32_t allow = allowed(0), allow1 = allowed(1);
-    // proposals join the list (count 0 until their row)
+    // proposals join the list (not seen until their row)
     for (int j = 0; j < batch; ++j) {
       const int x = s_token[j];
       if (x < 0 || owner(x) != tid) continue;
-      s_proposals = 1;
+      atomicOr(&s_proposals, 1u << j);
       if (!((changed >> bit_of(x)) & 1u)) {
         changed |= 1u << bit_of(x);
-        const int at = atomicAdd(&s_n, 1);
-        s_list[at] = static_cast<uint32_t>(x);
+        s_list[atomicAdd(&s_n, 1)] = static_cast<uint16_t>(x);
       }
     }
     const uint32_t plain = inside & ~changed;    // tokens the streaming pass decides by itself
@@ -524,67 +540,69 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     }
     __syncthreads();                             // the list is complete, the streamed stores are done
     const int n = s_n;
-    const bool proposals = s_proposals != 0;
-    // units of 32 entries of one row, spread over the warps
-    const int units = ((n + 31) >> 5) * batch;   // (a unit past them has i >= n)
-    constexpr int kAhead = 4;                    // units whose loads are in flight together
-    int row_at = warp, block_at = 0;             // this warp's next unit, stepped without divisions
-    auto step = [&](int by) {
-      row_at += by;
-      while (row_at >= batch) {
-        row_at -= batch;
-        ++block_at;
-      }
-    };
-    step(0);
-    for (int u0 = warp; u0 < units; u0 += kAhead * (kThreads / 32)) {
-      uint32_t entry[kAhead];
-      float value[kAhead], shift[kAhead];
-      int unit_row[kAhead];
-      bool ok[kAhead];
+    const uint32_t proposals = s_proposals;
+    // A warp takes a row, or a slice of one where there are fewer rows than warps.
+    const int slices = batch >= kThreads / 32 ? 1 : (kThreads / 32) / batch;
+    constexpr int kAhead = 4;                    // entries of a lane whose loads are in flight together
+    for (int job = warp; job < batch * slices; job += kThreads / 32) {
+      const int slice = job / batch, j = job - slice * batch;
+      const TIn* lr = lg + static_cast<long long>(q0 + j0 + j) * p.ld + base;
+      const int mi = s_mask[j];
+      const uint32_t* mr = mi >= 0 ? p.masks + static_cast<long long>(mi) * p.ld_mask + (base >> 5) : nullptr;
+      const uint32_t before = proposals & ((2u << j) - 1u);   // rows up to this one with proposals here
+      uint32_t best = 0, best_at = 0;
+#pragma unroll 1
+      for (int i0 = slice * 32 + lane; i0 - lane < n; i0 += kAhead * 32 * slices) {
+        uint32_t entry[kAhead], word[kAhead];
+        float value[kAhead];
 #pragma unroll
-      for (int h = 0; h < kAhead; ++h) {
-        const int j = row_at, i = block_at * 32 + lane;
-        unit_row[h] = j;
-        ok[h] = i < n;
-        step(kThreads / 32);
-        entry[h] = ok[h] ? s_list[i] : 0u;
-        shift[h] = ok[h] && (entry[h] & kEntryBias) ? s_bias[i] : 0.f;
-        const int v = base + static_cast<int>(entry[h] & 0xfffu), mi = s_mask[j];
-        uint32_t word = 0xffffffffu;
-        if (ok[h] && mi >= 0) word = __ldg(p.masks + static_cast<long long>(mi) * p.ld_mask + (v >> 5));
-        value[h] = ok[h] ? to_f32(lg[static_cast<long long>(q0 + j0 + j) * p.ld + v]) : 0.f;
-        ok[h] = ok[h] && ((word >> (v & 31)) & 1u);
-      }
-#pragma unroll
-      for (int h = 0; h < kAhead; ++h) {
-        if (u0 + h * (kThreads / 32) >= units) break;
-        const int j = unit_row[h];
-        const int x = static_cast<int>(entry[h] & 0xfffu), v = base + x;
-        int count = static_cast<int>((entry[h] >> 12) & 0x7fffu);
-        if (proposals) {
-          for (int k = 0; k <= j; ++k) count += s_token[k] == x;
-          count = min(count, kMaxCount);
-        }
-        float y = value[h];
-        if (count > 0 || (entry[h] & kEntryPrompt)) y = y > 0.f ? divide(y, rep, inv_rep, rep_safe) : __fmul_rn(y, rep);
-        if (count > 0) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(count))), pres);
-        if (entry[h] & kEntryBias) y = __fadd_rn(y, shift[h]);
-        if constexpr (kArgmax) {
-          const uint32_t key = ok[h] ? order_key(y) : 0u;
-          const uint32_t best = __reduce_max_sync(0xffffffffu, key);
-          if (best != 0) {
-            const uint32_t at =
-                __reduce_min_sync(0xffffffffu, ok[h] && key == best ? static_cast<uint32_t>(v) : 0xffffffffu);
-            if (lane == 0)
-              atomicMax(&s_list_best[j], (static_cast<unsigned long long>(best) << 32) | (0xffffffffu - at));
+        for (int h = 0; h < kAhead; ++h) {
+          const int i = i0 + h * 32 * slices;
+          entry[h] = i < n ? s_list[i] : 0xffffu;
+          const int x = static_cast<int>(entry[h] & 0xfffu);
+          word[h] = 0;
+          value[h] = 0.f;
+          if (i < n) {
+            word[h] = mr ? __ldg(mr + (x >> 5)) : 0xffffffffu;
+            value[h] = to_f32(lr[x]);
           }
-        } else if (ok[h]) {
-          TOut* orow = static_cast<TOut*>(p.out) + static_cast<long long>(q0 + j0 + j) * p.ld_out;
-          if constexpr (sizeof(TOut) == 4)
-            orow[v] = y;
-          else
-            orow[v] = __float2bfloat16_rn(y);
+        }
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h) {
+          const int x = static_cast<int>(entry[h] & 0xfffu);
+          if (!((word[h] >> (x & 31)) & 1u)) continue;        // forbidden, or past the list
+          int count = max(static_cast<int>(static_cast<short>(s_counts[x])), 0);
+          for (uint32_t m = before; m != 0; m &= m - 1) count += s_token[__ffs(m) - 1] == x;
+          count = min(count, kMaxCount);
+          float y = value[h];
+          if (count > 0 || (entry[h] & kEntryPrompt))
+            y = y > 0.f ? divide(y, rep, inv_rep, rep_safe) : __fmul_rn(y, rep);
+          if (count > 0) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(count))), pres);
+          if (entry[h] & kEntryBias) {
+            const int i = i0 + h * 32 * slices;
+            y = __fadd_rn(y, i < kListCap ? s_bias[i] : bias_of(base + x));
+          }
+          if constexpr (kArgmax) {
+            const uint32_t key = order_key(y), at = static_cast<uint32_t>(base + x);
+            if (key > best || (key == best && at < best_at)) {
+              best = key;
+              best_at = at;
+            }
+          } else {
+            TOut* orow = static_cast<TOut*>(p.out) + static_cast<long long>(q0 + j0 + j) * p.ld_out + base;
+            if constexpr (sizeof(TOut) == 4)
+              orow[x] = y;
+            else
+              orow[x] = __float2bfloat16_rn(y);
+          }
+        }
+      }
+      if constexpr (kArgmax) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        if (top != 0) {
+          const uint32_t at = __reduce_min_sync(0xffffffffu, best == top ? best_at : 0xffffffffu);
+          if (lane == 0)
+            atomicMax(&s_list_best[j], (static_cast<unsigned long long>(top) << 32) | (0xffffffffu - at));
         }
       }
     }
@@ -595,12 +613,11 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
       p.part[static_cast<long long>(q0 + j0 + tid) * p.chunks + chunk] = m;
     }
     if (j0 + kRowBatch < nq && proposals) {
-      // the next batch counts this one's proposals
-      for (int i = tid; i < n; i += kThreads) {
-        const uint32_t entry = s_list[i];
-        int count = static_cast<int>((entry >> 12) & 0x7fffu);
-        for (int k = 0; k < batch; ++k) count += s_token[k] == static_cast<int>(entry & 0xfffu);
-        s_list[i] = (entry & ~(0x7fffu << 12)) | (static_cast<uint32_t>(min(count, kMaxCount)) << 12);
+      // the next batch counts this one's proposals (each by the thread that owns its token)
+      for (int j = 0; j < batch; ++j) {
+        const int x = s_token[j];
+        if (x >= 0 && owner(x) == tid)
+          s_counts[x] = static_cast<uint16_t>(min(max(static_cast<int>(static_cast<short>(s_counts[x])), 0) + 1, kMaxCount));
       }
     }
   }
