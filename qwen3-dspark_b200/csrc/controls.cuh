@@ -14,9 +14,10 @@
 // are seen or biased: they go into a list in shared memory first. Then the rows stream
 // through untouched - bf16 stays packed, masks are applied to pairs, maxima are packed - and
 // a second pass over the list computes the penalised values and stores them over, or
-// compares them. 896 rows x 151936 bf16 tokens with masks and biases take 133 us (2.4 TB/s;
-// rows beyond the first of a chunk stream at about 5), 260 rows to float32 63 us (4 TB/s): the
-// start of a CTA and the instructions per row bound it beside DRAM. With the penalties
+// compares them. 896 rows x 151936 bf16 tokens with masks and biases take 135 us (2.4 TB/s of
+// the 325 MB; 12.8 us a row of all requests, 7.9 - 8.5 or 4.6 - 5.0 TB/s without masks and
+// lists), 260 rows to float32 64 us (4 TB/s): the start of a CTA, the list pass and the
+// instructions per row bound it beside DRAM. With the penalties
 // inside the streaming pass (per token, or in loops over set bits) it took 252 and 165 us.
 #pragma once
 #include "accept.cuh"

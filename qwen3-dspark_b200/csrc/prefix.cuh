@@ -63,8 +63,8 @@ __device__ __forceinline__ bool plan_ok(const Params& p) {
 // keys rounded up to 16. Every wait is bounded; a timed-out wait raises the CTA abort
 // flag, copies and MMAs in flight are drained and TMEM is released.
 //
-// Bound by the softmax chain where there are many rows (1024 rows x 32768 keys: about 270 us,
-// 1,000 TFLOP/s of 1,666; a block of both tiles takes 3,700 cycles of which the MMAs are
+// Bound by the softmax chain where there are many rows (1024 rows x 32768 keys: 281 us,
+// 977 TFLOP/s of 1,666; a block of both tiles takes 3,700 cycles of which the MMAs are
 // 2,048) and by DRAM and the latency of short items where there are few (8 rows x 32768 keys:
 // 40 us with the merge; the keys alone take 21).
 constexpr int kStagesN = 5;
