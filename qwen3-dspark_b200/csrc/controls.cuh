@@ -14,8 +14,8 @@
 // are seen or biased: they go into a list in shared memory first. Then the rows stream
 // through untouched - bf16 stays packed, masks are applied to pairs, maxima are packed - and
 // a second pass over the list computes the penalised values and stores them over, or
-// compares them. 896 rows x 151936 bf16 tokens with masks and biases take 135 us (2.4 TB/s of
-// the 325 MB; 12.8 us a row of all requests, 7.9 - 8.5 or 4.6 - 5.0 TB/s without masks and
+// compares them. 896 rows x 151936 bf16 tokens with masks and biases take 134 us (2.4 TB/s of
+// the 325 MB; 12.8 us a row of all requests, 7.9 - 8.6 or 4.5 - 5.0 TB/s without masks and
 // lists), 260 rows to float32 64 us (4 TB/s): the start of a CTA, the list pass and the
 // instructions per row bound it beside DRAM. With the penalties
 // inside the streaming pass (per token, or in loops over set bits) it took 252 and 165 us.
@@ -543,9 +543,12 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     __syncthreads();                             // the list is complete, the streamed stores are done
     const int n = s_n;
     const uint32_t proposals = s_proposals;
-    // A warp takes a row, or a slice of one where there are fewer rows than warps.
-    const int slices = batch >= kThreads / 32 ? 1 : (kThreads / 32) / batch;
     constexpr int kAhead = 4;                    // entries of a lane whose loads are in flight together
+    // A warp takes a row, or a slice of one: where there are fewer rows than warps, and of a
+    // long list, so that rows that are no multiple of the warps leave none idle (24 requests x
+    // 5 float32 rows x 50257: 33.0 us with a warp a row, 29.0 with slices).
+    constexpr int kWarps = kThreads / 32;
+    const int slices = max(kWarps / min(batch, kWarps), min(kWarps, (n + kAhead * 32 - 1) / (kAhead * 32)));
     for (int job = warp; job < batch * slices; job += kThreads / 32) {
       const int slice = job / batch, j = job - slice * batch;
       const TIn* lr = lg + static_cast<long long>(q0 + j0 + j) * p.ld + base;
