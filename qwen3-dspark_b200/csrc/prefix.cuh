@@ -108,10 +108,7 @@ __device__ __forceinline__ bool load_item(const Params& p, int idx, ItemView& x)
   x.nsegs = b.y;
   x.dual = b.z != 0;
   x.blocks = 0;
-  bool ok = x.nq >= 1 && x.nq <= kTileRows && x.q0 >= 0 && x.q0 <= p.total_q - x.nq && x.head >= 0 &&
-            x.head < kHeads && x.nsegs >= 0 && x.nsegs <= kMaxSegs &&
-            x.slot < p.slots - (x.nq > kHalfTile || x.dual ? 1 : 0) &&
-            (!x.dual || (x.nq <= kHalfTile && x.slot >= 0));
+  bool ok = item_fits(x.q0, x.nq, x.head, x.slot, x.nsegs, x.dual, p.total_q, p.slots);
 #pragma unroll
   for (int s = 0; s < kMaxSegs; ++s) {
     const int4 g = __ldg(w + 2 + s);

@@ -60,6 +60,17 @@ enum RunField {
 };
 constexpr int kDualSlots = 3;              // two slots, both holding (part of) every row
 
+// Whether an item's own words are in range: its rows, its head, and its slots among the
+// plan's (a direct item, slot -1, needs none; a wide or dual one needs two). The kernels
+// skip an item that fails, so build_plan hands out none.
+__host__ __device__ inline bool item_fits(int q0, int nq, int head, int slot, int nsegs, bool dual, int total_q,
+                                          int slots) {
+  const bool rows = nq >= 1 && nq <= kTileRows && q0 >= 0 && q0 <= total_q - nq;
+  const bool store = slot < 0 ? slot == -1 && !dual
+                              : slot <= slots - (nq > kHalfTile || dual ? 2 : 1) && (!dual || nq <= kHalfTile);
+  return rows && store && head >= 0 && head < kHeads && nsegs >= 0 && nsegs <= kMaxSegs;
+}
+
 // Costs the schedule balances, in units of one two-tile key block.
 constexpr double kCostPair = 1.0;
 constexpr double kCostSingle = 0.9;
@@ -311,6 +322,8 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
           pos += t.segs[s].len;
         }
         it[kISegs] = n;
+        if (!item_fits(it[kIQ0], it[kINq], h, it[kISlot], n, t.dual, static_cast<int>(q0), static_cast<int>(slots)))
+          return kPlanInvalid;
         per_cta[cta[idx]].push_back({cost[idx], idx});
       }
 
