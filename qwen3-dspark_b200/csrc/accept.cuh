@@ -141,7 +141,7 @@ __global__ void greedy_accept_kernel(AcceptParams p) {
   for (int j = 0; j + 1 < q && !stop; ++j) {
     const long long proposed = p.tokens[q0 + 1 + j];
     const long long correct = static_cast<long long>(p.pred[q0 + j]);
-    if (proposed != correct) {
+    if (proposed != correct || correct < 0) {   // (a padded proposal may be negative too)
       if (correct >= 0) p.emitted[q0 + n++] = correct;
       stop = true;
       break;
