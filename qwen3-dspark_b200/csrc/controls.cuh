@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     if (tid < batch) {
       const int row = q0 + j0 + tid;
       int mi = p.masks ? p.mask_index[row] : -1, x = -1;
-      if (mi >= p.num_masks) mi = -2;
+      if (mi < -1 || mi >= p.num_masks) mi = -2;
       if (j0 + tid > 0 && p.tokens) {
         const long long t = p.tokens[row];
         if (t < 0 || t >= p.vocab)
