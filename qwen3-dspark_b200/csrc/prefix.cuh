@@ -33,9 +33,10 @@ struct Params {
 
 // Partial rows of one MMA tile: 128 x 128 fp32 (normalised) as [d / 4][row][4], so that
 // the 32 rows of a warp store 512 contiguous bytes (row by row, each store instruction
-// touched 32 lines: 7,000 cycles a tile), then 128 log2-sum-exp2.
-constexpr size_t kSlotFloats = 128 * kHeadDim;
-inline size_t workspace_bytes(int slots) { return static_cast<size_t>(slots) * (kSlotFloats + 128) * sizeof(float); }
+// touched 32 lines: 7,000 cycles a tile), then each row's maximum and sum. The two stay
+// apart: where scores are large, m + log2(l) would round away how many keys a part holds.
+constexpr size_t kRowFloats = 128 * kHeadDim, kSlotFloats = kRowFloats + 2 * 128;
+inline size_t workspace_bytes(int slots) { return static_cast<size_t>(slots) * kSlotFloats * sizeof(float); }
 
 __device__ __forceinline__ bool plan_ok(const Params& p) {
   return p.plan[kHMagic] == kPlanMagic && p.plan[kHCheck] == p.check && p.plan[kHTotalQ] == p.total_q;
@@ -470,6 +471,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
@@ -484,6 +490,51 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 struct RowState {
   float m, l;                             // running maximum (log2 units), sum of 2^(s - m)
 };
+constexpr float kNoMax = -3.402823466e38f;   // m before a visible key: below every score
+
+// O *= alpha for the warp's rows, 16 columns at a time (the rows' scores are live in registers).
+__device__ __forceinline__ void rescale_o(uint32_t o_addr, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < 8; ++c) {
+    uint32_t o[16];
+    tmem_ld16(o_addr + 16 * c, o);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+    tmem_st16(o_addr + 16 * c, o);
+  }
+  tmem_st_wait();
+}
+
+// 2^(s scale - m) is one fma and one ex2, exact in its argument; m is the rounded product, so
+// the largest score's argument is that rounding error, up to |m| 2^-24. From |m| = 2^24 on it
+// would count (at 2^31 it overflows ex2): there far_block computes the probabilities, product
+// and difference rounded one by one, as m was, so that the largest argument is 0. Few rows
+// ever come there: 16 scores at a time, read from TMEM again (P takes the columns of scores
+// already read), so that the usual path carries no code or registers for it.
+__device__ __forceinline__ bool is_far(float m) {            // 2^24 <= |m| < 2^127: not kNoMax, not infinite
+  constexpr uint32_t kLow = 0x4b800000u, kHigh = 0x7f000000u;
+  return (__float_as_uint(m) & 0x7fffffffu) - kLow < kHigh - kLow;
+}
+__device__ __noinline__ float far_block(uint32_t s_addr, uint32_t o_addr, int cols, int see, float scale_log2,
+                                        bool rescale, float alpha, float m) {
+  if (rescale) rescale_o(o_addr, alpha);
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < cols; c += 16) {
+    uint32_t v[16], pk[8];
+    tmem_ld16(s_addr + c, v);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float a = c + i < see ? ex2(__fsub_rn(__fmul_rn(__uint_as_float(v[i]), scale_log2), m)) : 0.f;
+      const float b = c + i + 1 < see ? ex2(__fsub_rn(__fmul_rn(__uint_as_float(v[i + 1]), scale_log2), m)) : 0.f;
+      sum += a + b;
+      pk[i >> 1] = pack_bf16x2(a, b);
+    }
+    tmem_st8(s_addr + (c >> 1), pk);
+  }
+  tmem_st_wait();
+  return sum;
+}
 
 // One block of a row: kCols scores from TMEM, probabilities back as packed bf16. `see`
 // scores are visible.
@@ -501,26 +552,19 @@ __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, 
 #pragma unroll
     for (int i = 0; i < kCols; ++i) s[i] = i < see ? s[i] : -INFINITY;
   }
-  const float m_new = fmaxf(st.m, max_n(s) * scale_log2);
+  const float m_new = fmaxf(st.m, __fmul_rn(max_n(s), scale_log2));
   const bool raise = m_new > st.m + 8.f;
   float alpha = 1.f;
   if (raise) {
     alpha = ex2(st.m - m_new);
     st.m = m_new;
   }
-  if (!first && __any_sync(0xffffffffu, raise)) {
-    // the block's S was committed behind the previous PV: O is complete (16 columns at a
-    // time: the row's scores are live in registers)
-#pragma unroll 1
-    for (int c = 0; c < 8; ++c) {
-      uint32_t o[16];
-      tmem_ld16(o_addr + 16 * c, o);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-      tmem_st16(o_addr + 16 * c, o);
-    }
-    tmem_st_wait();
+  if (__any_sync(0xffffffffu, is_far(st.m))) {
+    st.l = st.l * alpha + far_block(s_addr, o_addr, kCols, see, scale_log2, !first, alpha, st.m);
+    return;
   }
+  // the block's S was committed behind the previous PV: O is complete
+  if (!first && __any_sync(0xffffffffu, raise)) rescale_o(o_addr, alpha);
   float sum[2] = {0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < kCols / 32; ++c) {
@@ -561,7 +605,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
     int len0 = nx.len[0], len1 = nx.len[1], len2 = nx.len[2];
     int see0 = row_ok ? nx.visible + lt - nx.pos[0] : 0;
     if (!valid && threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
-    RowState st{-1e30f, 0.f};
+    RowState st{kNoMax, 0.f};
     if (active) {
       const int b0 = dual ? tile : 0;
 #pragma unroll 1
@@ -609,7 +653,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
       train::tc_fence_after();
     }
     const float inv = st.l > 0.f ? 1.f / st.l : (st.l != st.l ? st.l : 0.f);   // (a NaN sum stays NaN)
-    float* prow = part + static_cast<size_t>(max(slot, 0) + tile) * (kSlotFloats + 128);
+    float* prow = part + static_cast<size_t>(max(slot, 0) + tile) * kSlotFloats;
     __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) +
                           (static_cast<size_t>(q0 + (row_ok ? lt : 0)) * kQHeads + 2 * head + (rm & 1)) * kHeadDim;
     if (warp_ok) {
@@ -636,7 +680,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
         }
       }
       if (row_ok && slot >= 0)
-        __stcg(prow + kSlotFloats + rm, st.l > 0.f ? st.m + log2f(st.l) : (st.l != st.l ? st.l : -INFINITY));
+        __stcg(reinterpret_cast<float2*>(prow + kRowFloats) + rm, make_float2(st.m, st.l));
     }
     if (blocks > 0) {
       train::tc_fence_before();
@@ -832,15 +876,16 @@ __device__ __forceinline__ void f32_item(const Params& p, const ItemView& x, int
       *reinterpret_cast<float4*>(dst + 64 + 4 * tx) = b;
     } else {
       const int slot = x.slot + (x.dual ? 0 : lt >> 6), rm = 2 * (lt & 63) + (m & 1);
-      float* prow = part + static_cast<size_t>(slot) * (kSlotFloats + 128);
+      float* prow = part + static_cast<size_t>(slot) * kSlotFloats;
       *reinterpret_cast<float4*>(prow + tx * 512 + 4 * rm) = a;
       *reinterpret_cast<float4*>(prow + (16 + tx) * 512 + 4 * rm) = b;
       if (tx == 0) {
-        prow[kSlotFloats + rm] = any ? mrow[i] * 1.4426950408889634f + log2f(lrow[i]) : -INFINITY;
-        if (x.dual) prow[kSlotFloats + 128 + kSlotFloats + rm] = -INFINITY;     // the second slot holds nothing
+        reinterpret_cast<float2*>(prow + kRowFloats)[rm] = make_float2(mrow[i], lrow[i]);
+        // (the second slot holds nothing)
+        if (x.dual) reinterpret_cast<float2*>(prow + kSlotFloats + kRowFloats)[rm] = make_float2(-INFINITY, 0.f);
       }
       if (x.dual) {
-        float* empty = prow + kSlotFloats + 128;
+        float* empty = prow + kSlotFloats;
         *reinterpret_cast<float4*>(empty + tx * 512 + 4 * rm) = make_float4(0.f, 0.f, 0.f, 0.f);
         *reinterpret_cast<float4*>(empty + (16 + tx) * 512 + 4 * rm) = make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -870,7 +915,8 @@ __global__ void __launch_bounds__(kF32Threads2) prefix_f32_kernel(const Params p
 
 // Combines the partial rows of a query row's head pair (adjacent rows of a slot, so a lane
 // reads whole 32-byte sectors); lane l owns d = 4 l ..
-//   out = sum_c 2^(L_c - M) o_c / sum_c 2^(L_c - M),  M = max_c L_c
+//   out = sum_c w_c o_c / sum_c w_c,  w_c = l_c 2^(m_c - M),  M = max_c m_c
+// (m of the float32 kernel in natural units)
 // kWarps = 1: a warp per (query row, KV head), 8 to a CTA. kWarps = 8: a CTA per pair, its
 // warps taking every eighth contribution, for the many pieces of a long prefix behind few
 // rows (18 pieces of 32768 keys behind 8 rows: one warp each walked them in 16 us); with
@@ -878,7 +924,7 @@ __global__ void __launch_bounds__(kF32Threads2) prefix_f32_kernel(const Params p
 constexpr int kMergeWideParts = 6, kMergeWidePairs = 2048;
 
 template <typename T, int kWarps>
-__global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const float* part) {
+__global__ void __launch_bounds__(256, 4) prefix_merge_kernel(const Params p, const float* part) {
   __shared__ float s_acc[kWarps > 1 ? 8 : 1][8][33];
   __shared__ float2 s_den[8];
   if (!plan_ok(p)) return;
@@ -901,16 +947,17 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const
     const int4 k = first ? k0 : k1;
     const int i = first ? c : c - n0, lt = first ? lt0 : lt1;
     const int slot = dual ? k.x + ((i >> 1) * kHeads + h) * 2 + (i & 1) : k.x + (i * kHeads + h) * k.z + (lt >> 6);
-    return part + static_cast<size_t>(min(max(slot, 0), p.slots - 1)) * (kSlotFloats + 128);
+    return part + static_cast<size_t>(min(max(slot, 0), p.slots - 1)) * kSlotFloats;
   };
   auto row_of = [&](int c) { return 2 * ((c < n0 ? lt0 : lt1) & 63); };
-  auto lse = [&](int c) { return __ldcg(reinterpret_cast<const float2*>(base(c) + kSlotFloats + row_of(c))); };
+  // (m, l) of the two heads' rows
+  auto stats = [&](int c) { return __ldcg(reinterpret_cast<const float4*>(base(c) + kRowFloats + 2 * row_of(c))); };
+  constexpr float kUnit = sizeof(T) == 4 ? 1.4426950408889634f : 1.f;
   float2 top = make_float2(-INFINITY, -INFINITY);
   for (int c = lane; c < total; c += 32) {
-    const float2 v = lse(c);
-    // fmaxf drops a NaN: it comes back through the weights below
+    const float4 v = stats(c);
     top.x = fmaxf(top.x, v.x);
-    top.y = fmaxf(top.y, v.y);
+    top.y = fmaxf(top.y, v.z);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -923,10 +970,10 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const Params p, const
   const int c_first = kWarps > 1 ? warp : 0;
 #pragma unroll 4
   for (int c = c_first; c < total; c += kWarps) {
-    const float2 f = lse(c);
+    const float4 f = stats(c);
     const float4* src = reinterpret_cast<const float4*>(base(c) + static_cast<size_t>(lane) * 512 + 4 * row_of(c));
     const float4 v0 = __ldcg(src), v1 = __ldcg(src + 1);
-    const float f0 = ex2(f.x - mx), f1 = ex2(f.y - my);
+    const float f0 = ex2((f.x - mx) * kUnit) * f.y, f1 = ex2((f.z - my) * kUnit) * f.w;
     den0 += f0;
     den1 += f1;
     a[0] = fmaf(f0, v0.x, a[0]);

@@ -14,8 +14,8 @@
 //                  kChainRows query rows on average): nothing to merge then.
 //
 // A tile whose chain is one piece and holds every key of its rows writes the output;
-// any other piece leaves normalised fp32 partial rows and their log2-sum-exp2, which
-// the merge kernel combines (out = sum_c 2^(L_c - L) o_c).
+// any other piece leaves normalised fp32 partial rows with their maximum m and sum l, which
+// the merge kernel combines (out = sum_c w_c o_c / sum_c w_c, w_c = l_c 2^(m_c - max m)).
 #pragma once
 #include <algorithm>
 #include <cmath>
