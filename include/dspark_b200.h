@@ -455,7 +455,9 @@ int dspark_train_attn(const void* q, const void* k, const void* v, int total_q, 
  * plan does not read may be NULL. bf16 (tensor cores) or fp32 (CUDA cores), 16-byte
  * aligned pointers; workspace: dspark_prefix_workspace_bytes(plan_head) bytes, 16-byte
  * aligned, never needing a clear, one per call in flight. A device plan that is not the one plan_head
- * belongs to sets DSPARK_DEVICE_BAD_ARGUMENT and computes nothing. out may be q.
+ * belongs to sets DSPARK_DEVICE_BAD_ARGUMENT and computes nothing. out may be q itself;
+ * otherwise out, and the workspace, must share no byte with q or with the key and value
+ * rows that the plan reads (refused).
  */
 #define DSPARK_PREFIX_HEAD_WORDS 32
 int dspark_prefix_plan(int num_groups, const int32_t* group_size, const int32_t* prefix_start,

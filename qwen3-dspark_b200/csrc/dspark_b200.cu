@@ -350,6 +350,12 @@ int encode_rows_map(CUtensorMap* m, const void* base, long long rows, int heads,
 
 namespace {
 
+// Whether [a, + an) and [b, + bn) share a byte.
+bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return an > 0 && bn > 0 && x < y + bn && y < x + an;
+}
+
 // The merge of a plan's partial rows. A plain launch: as a programmatic dependent its CTAs
 // could take the registers the attention's third warpgroup gives back before its softmax
 // warps draw them, and with the trigger behind that point small batches measured slower (8
@@ -1217,11 +1223,25 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
         x.off > x.rows - need)
       return DSPARK_ERR_INVALID_ARGUMENT;
   }
+  const size_t ws = prefix::workspace_bytes(p.slots);
+  if (p.slots > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < ws)) return DSPARK_ERR_INVALID_ARGUMENT;
+  // CTAs write output rows while others still read: out is q itself or shares no byte with an input,
+  // and the workspace shares none with either
+  const size_t elem = dtype == DSPARK_DTYPE_F32 ? 4 : 2, q_bytes = static_cast<size_t>(total_q) * kQHeads * kHeadDim * elem;
+  if ((out != q && overlap(out, q_bytes, q, q_bytes)) || overlap(workspace, ws, out, q_bytes) ||
+      overlap(workspace, ws, q, q_bytes))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  for (int s = 0; s < 3; ++s) {
+    const size_t row = kKVHeads * kHeadDim * elem, bytes = plan_head[kHPrefixRows + s] * row;
+    for (const void* t : {p.src[s].k, p.src[s].v}) {
+      const char* base = static_cast<const char*>(t) + p.src[s].off * row;
+      if (bytes > 0 && (overlap(out, q_bytes, base, bytes) || overlap(workspace, ws, base, bytes)))
+        return DSPARK_ERR_INVALID_ARGUMENT;
+    }
+  }
   DeviceInfo dev;
   const int st = current_device_info(&dev);
   if (st != DSPARK_OK) return st;
-  if (p.slots > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < prefix::workspace_bytes(p.slots)))
-    return DSPARK_ERR_INVALID_ARGUMENT;
   int rc = DSPARK_OK;
   float* part = static_cast<float*>(workspace);
   if (dtype == DSPARK_DTYPE_F32) {
@@ -1270,11 +1290,10 @@ int dspark_control_logits(const void* logits, long long ld, int dtype, int rows,
     return DSPARK_ERR_INVALID_ARGUMENT;
   const int in_size = dtype == DSPARK_DTYPE_F32 ? 4 : 2, out_size = out_dtype == DSPARK_DTYPE_F32 ? 4 : 2;
   // the output is the input itself (same rows, same type) or shares no byte with it
-  const uintptr_t a0 = reinterpret_cast<uintptr_t>(logits), b0 = reinterpret_cast<uintptr_t>(out);
-  const uintptr_t a1 = a0 + (static_cast<uintptr_t>(rows - 1) * ld + vocab) * in_size;
-  const uintptr_t b1 = b0 + (static_cast<uintptr_t>(rows - 1) * ld_out + vocab) * out_size;
-  p.in_place = a0 == b0 && ld == ld_out && dtype == out_dtype;
-  if (!p.in_place && a0 < b1 && b0 < a1) return DSPARK_ERR_INVALID_ARGUMENT;
+  const size_t in_bytes = (static_cast<size_t>(rows - 1) * ld + vocab) * in_size;
+  const size_t out_bytes = (static_cast<size_t>(rows - 1) * ld_out + vocab) * out_size;
+  p.in_place = logits == out && ld == ld_out && dtype == out_dtype;
+  if (!p.in_place && overlap(logits, in_bytes, out, out_bytes)) return DSPARK_ERR_INVALID_ARGUMENT;
   p.mask_value = mask_value;
   p.out = out;
   p.ld_out = ld_out;

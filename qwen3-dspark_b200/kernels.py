@@ -236,7 +236,7 @@ class B200SharedPrefixKernel:
     the source rows at which the layout's row 0 lies, so one layout serves every layer
     of a store. Contiguous tensors of one dtype on the kernel's GPU: bf16 (tensor cores)
     or float32 (CUDA cores). A row without a visible key gives zeros. ``out`` (default: a
-    new tensor) may be ``query`` itself.
+    new tensor) may be ``query`` itself, and otherwise must not overlap ``query`` or the rows read.
 
     Partial rows live in a workspace that each call allocates on its own stream, so
     calls on different streams and in different captured graphs share nothing.
