@@ -38,6 +38,7 @@ struct DeviceInfo {
   bool ready = false;
   int sms = 0;
   int append_pairs = 0;   // CTA pairs of the 2-SM append kernel resident at once (0: not used)
+  int prefix_status = DSPARK_ERR_UNSUPPORTED;   // whether the shared-prefix kernels can run
   int max_smem_optin = 0;
   int cc_major = 0, cc_minor = 0;
 };
@@ -60,6 +61,25 @@ std::atomic<unsigned long long> g_launches{0};
 constexpr size_t kAttnSmemBytes = 1024 + static_cast<size_t>(kSmemBarOff) + 2 * kStages * sizeof(uint64_t) +
                                   sizeof(SchedShared);
 
+// Sets the shared-prefix kernels up. What it finds concerns them alone: no other entry
+// depends on it. The bf16 kernel's register split must fit what its CTA is launched with (a
+// setmaxnreg.inc beyond it would wait forever), which is the compiler's choice.
+int prefix_setup(int max_smem_optin) {
+  if (static_cast<size_t>(max_smem_optin) < prefix::kSmemBytes) return DSPARK_ERR_UNSUPPORTED;
+  cudaFuncAttributes attr;
+  if (cudaFuncGetAttributes(&attr, prefix::prefix_attn_kernel) != cudaSuccess ||
+      cudaFuncSetAttribute(prefix::prefix_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(prefix::kSmemBytes)) != cudaSuccess ||
+      cudaFuncSetAttribute(prefix::prefix_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(prefix::kF32SmemBytes)) != cudaSuccess) {
+    cudaGetLastError();
+    return DSPARK_ERR_CUDA;
+  }
+  return attr.numRegs * prefix::kAttThreads < 256 * prefix::kSoftmaxRegs + 128 * prefix::kOtherRegs
+             ? DSPARK_ERR_UNSUPPORTED
+             : DSPARK_OK;
+}
+
 int device_info(int dev, DeviceInfo* out) {
   if (dev < 0 || dev >= kMaxDevices) return DSPARK_ERR_INVALID_ARGUMENT;
   std::lock_guard<std::mutex> lock(g_mu);
@@ -72,8 +92,7 @@ int device_info(int dev, DeviceInfo* out) {
       return DSPARK_ERR_CUDA;
     if (d.cc_major != 10) return DSPARK_ERR_UNSUPPORTED;   // built for sm_100a only
     if (static_cast<size_t>(d.max_smem_optin) < kAttnSmemBytes ||
-        static_cast<size_t>(d.max_smem_optin) < train::kSmemBytes ||
-        static_cast<size_t>(d.max_smem_optin) < prefix::kSmemBytes)
+        static_cast<size_t>(d.max_smem_optin) < train::kSmemBytes)
       return DSPARK_ERR_UNSUPPORTED;
     int cur = -1;
     cudaGetDevice(&cur);
@@ -84,10 +103,6 @@ int device_info(int dev, DeviceInfo* out) {
                              static_cast<int>(kAttnSmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(attn_bf16_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(kAttnSmemBytes)) != cudaSuccess ||
-        cudaFuncSetAttribute(prefix::prefix_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(prefix::kSmemBytes)) != cudaSuccess ||
-        cudaFuncSetAttribute(prefix::prefix_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(prefix::kF32SmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(train::train_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(train::kSmemBytes)) != cudaSuccess ||
         cudaFuncSetAttribute(markov::markov_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -101,14 +116,7 @@ int device_info(int dev, DeviceInfo* out) {
         cudaFuncSetAttribute(append::draft_append_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(append::PairCfg::kSmemBytes)) != cudaSuccess)
       return DSPARK_ERR_CUDA;
-    {
-      // the prefix kernel's register split must fit what its CTA is launched with: a
-      // setmaxnreg.inc beyond it would wait forever
-      cudaFuncAttributes attr;
-      if (cudaFuncGetAttributes(&attr, prefix::prefix_attn_kernel) != cudaSuccess) return DSPARK_ERR_CUDA;
-      if (attr.numRegs * prefix::kAttThreads < 256 * prefix::kSoftmaxRegs + 128 * prefix::kOtherRegs)
-        return DSPARK_ERR_UNSUPPORTED;
-    }
+    d.prefix_status = prefix_setup(d.max_smem_optin);
     {
       // CTA pairs of the 2-SM append the GPU holds at once (a pair needs two SMs of
       // one GPC); a refused query leaves the single-CTA kernels in use.
@@ -1242,6 +1250,7 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   DeviceInfo dev;
   const int st = current_device_info(&dev);
   if (st != DSPARK_OK) return st;
+  if (dev.prefix_status != DSPARK_OK) return dev.prefix_status;
   int rc = DSPARK_OK;
   float* part = static_cast<float*>(workspace);
   if (dtype == DSPARK_DTYPE_F32) {
