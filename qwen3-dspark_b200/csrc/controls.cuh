@@ -29,7 +29,7 @@ constexpr int kThreads = 256;
 constexpr int kPer = 16;                       // tokens per thread: two runs of 8
 constexpr int kChunk = kThreads * kPer;
 constexpr int kRun = kThreads * 8;             // tokens between a thread's two runs
-constexpr int kListCap = 512;                  // biases of a chunk staged in shared memory
+constexpr int kStage = 2 * kThreads;           // biases of a chunk summed up at a time
 constexpr int kRowBatch = 16;                  // rows whose indices are staged at a time
 constexpr int kMaxCount = 32767;               // counts saturate here
 
@@ -157,9 +157,9 @@ template <typename TIn, typename TOut, bool kArgmax, bool kVec>
 __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
   __shared__ uint16_t s_list[kChunk];
   __shared__ __align__(16) uint16_t s_counts[kChunk];
-  __shared__ float s_bias[kListCap];             // of the list's first entries
-  __shared__ int s_id[kListCap];
-  __shared__ float s_val[kListCap];
+  __shared__ float s_bias[kChunk];               // of biased tokens (the rest is not written)
+  __shared__ int s_id[kStage];
+  __shared__ float s_val[kStage];
   __shared__ int s_count[kThreads / 32];
   __shared__ unsigned long long s_best[kRowBatch][kThreads / 32], s_list_best[kRowBatch];
   __shared__ uint32_t s_top[kRowBatch];
@@ -324,13 +324,26 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
   batch = min(kRowBatch, nq);
   fetch(0, inside, next, !p.in_place || p.masks);
   stage();
-  // The chunk's biases, compacted in list order (so that a token's entries add in that order);
-  // more than kListCap of them are read from the list itself.
-  int listed = 0;
+  // The chunk's biases, compacted in list order; each thread sums its own tokens' entries up, in
+  // that order, so a list of any length is read once.
+  uint32_t biased = 0;
+  int staged = 0;
   const int nb = p.bias_ids ? min(max(p.bias_len[slot], 0), p.max_bias) : 0;
   const int* list_id = p.bias_ids + static_cast<long long>(slot) * p.max_bias;
   const float* list_val = p.bias_values + static_cast<long long>(slot) * p.max_bias;
+  auto sum_up = [&]() {
+    __syncthreads();
+    for (int k = 0; k < staged; ++k) {
+      const int x = s_id[k] - base;
+      if (owner(x) != tid) continue;
+      const uint32_t bit = 1u << bit_of(x);
+      s_bias[x] = __fadd_rn((biased & bit) ? s_bias[x] : 0.f, s_val[k]);
+      biased |= bit;
+    }
+    staged = 0;
+  };
   for (int b0 = 0; b0 < nb; b0 += kThreads) {
+    if (staged > kStage - kThreads) sum_up();
     const int b = b0 + tid;
     const int id = b < nb ? list_id[b] : -1;
     const bool in = id >= base && id < base + kChunk && id < p.vocab;
@@ -338,34 +351,17 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     __syncthreads();
     if (lane == 0) s_count[warp] = __popc(ballot);
     __syncthreads();
-    int at = listed + __popc(ballot & ((1u << lane) - 1));
+    int at = staged + __popc(ballot & ((1u << lane) - 1));
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) at += s_count[w];
-      listed += s_count[w];
+      staged += s_count[w];
     }
-    if (in && at < kListCap) {
+    if (in) {
       s_id[at] = id;
       s_val[at] = list_val[b];
     }
   }
-  const bool in_smem = listed <= kListCap;
-  const int list_n = in_smem ? listed : nb;
-  auto bias_of = [&](int v) {
-    float sum = 0.f;
-#pragma unroll 1
-    for (int k = 0; k < list_n; ++k)
-      if ((in_smem ? s_id[k] : list_id[k]) == v) sum = __fadd_rn(sum, in_smem ? s_val[k] : list_val[k]);
-    return sum;
-  };
-  __syncthreads();
-  uint32_t biased = 0;
-  if (listed > 0) {
-    for (int k = 0; k < list_n; ++k) {
-      const int x = (in_smem ? s_id[k] : list_id[k]) - base;
-      if (x >= 0 && x < kChunk && owner(x) == tid) biased |= 1u << bit_of(x);
-    }
-    biased &= inside;
-  }
+  if (staged > 0) sum_up();
   // Counts into shared memory (a thread's own tokens, which only it will change), tokens that
   // were seen or have a bias into the list (in any order).
 #pragma unroll
@@ -382,29 +378,22 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
     for (int e = 0; e < kPer; ++e) s_counts[rel(e)] = static_cast<uint16_t>(cw[e >> 1] >> (16 * (e & 1)));
   }
   changed = prompt | used | biased;
-  // biased tokens first, so that their sums fit s_bias unless there are more than kListCap
-#pragma unroll 1
-  for (int pass = listed > 0 ? 0 : 1; pass < 2; ++pass) {
-    const uint32_t set = pass == 0 ? biased : changed & ~biased;
-    if (__any_sync(0xffffffffu, set != 0)) {
-      int at = __popc(set);                      // the warp's entries lie behind one another
+  if (__any_sync(0xffffffffu, changed != 0)) {
+    int at = __popc(changed);                    // the warp's entries lie behind one another
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += v;
-      }
-      int first = 0;
-      if (lane == 31) first = atomicAdd(&s_n, at);
-      at += __shfl_sync(0xffffffffu, first, 31) - __popc(set);
-#pragma unroll 1
-      for (uint32_t m = set; m != 0; m &= m - 1, ++at) {
-        const int e = __ffs(m) - 1;
-        s_list[at] = static_cast<uint16_t>(static_cast<uint32_t>(rel(e)) | (((prompt >> e) & 1u) * kEntryPrompt) |
-                                           (pass == 0 ? kEntryBias : 0u));
-        if (pass == 0 && at < kListCap) s_bias[at] = bias_of(index(e));
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += v;
     }
-    if (pass == 0) __syncthreads();
+    int first = 0;
+    if (lane == 31) first = atomicAdd(&s_n, at);
+    at += __shfl_sync(0xffffffffu, first, 31) - __popc(changed);
+#pragma unroll 1
+    for (uint32_t m = changed; m != 0; m &= m - 1, ++at) {
+      const int e = __ffs(m) - 1;
+      s_list[at] = static_cast<uint16_t>(static_cast<uint32_t>(rel(e)) | (((prompt >> e) & 1u) * kEntryPrompt) |
+                                         (((biased >> e) & 1u) * kEntryBias));
+    }
   }
 
   for (; j0 < nq; j0 += kRowBatch) {
@@ -583,10 +572,7 @@ __global__ void __launch_bounds__(kThreads, 4) control_kernel(const Params p) {
           if (count > 0 || (entry[h] & kEntryPrompt))
             y = y > 0.f ? divide(y, rep, inv_rep, rep_safe) : __fmul_rn(y, rep);
           if (count > 0) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(count))), pres);
-          if (entry[h] & kEntryBias) {
-            const int i = i0 + h * 32 * slices;
-            y = __fadd_rn(y, i < kListCap ? s_bias[i] : bias_of(base + x));
-          }
+          if (entry[h] & kEntryBias) y = __fadd_rn(y, s_bias[x]);
           if constexpr (kArgmax) {
             const uint32_t key = order_key(y), at = static_cast<uint32_t>(base + x);
             if (key > best || (key == best && at < best_at)) {
