@@ -1190,7 +1190,7 @@ int dspark_prefix_plan(int num_groups, const int32_t* group_size, const int32_t*
 
 size_t dspark_prefix_workspace_bytes(const int32_t* plan_head) {
   if (plan_head == nullptr || plan_head[prefix::kHMagic] != prefix::kPlanMagic) return 0;
-  return prefix::workspace_bytes(plan_head[prefix::kHSlots]);
+  return prefix::workspace_bytes(plan_head[prefix::kHPartRows]);
 }
 
 int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const void* prefix_v,
@@ -1214,6 +1214,8 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   p.total_q = total_q;
   p.grid = plan_head[kHGrid];
   p.slots = plan_head[kHSlots];
+  p.part_rows = plan_head[kHPartRows];
+  p.parts_at = plan_head[kHPartsAt];
   p.items_at = plan_head[kHItemsAt];
   p.runs = plan_head[kHRuns];
   p.runs_at = plan_head[kHRunsAt];
@@ -1231,7 +1233,7 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
         x.off > x.rows - need)
       return DSPARK_ERR_INVALID_ARGUMENT;
   }
-  const size_t ws = prefix::workspace_bytes(p.slots);
+  const size_t ws = prefix::workspace_bytes(p.part_rows);
   if (p.slots > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < ws)) return DSPARK_ERR_INVALID_ARGUMENT;
   // CTAs write output rows while others still read: out is q itself or shares no byte with an input,
   // and the workspace shares none with either

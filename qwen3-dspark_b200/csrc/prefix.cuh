@@ -26,17 +26,19 @@ struct Params {
   const void* q;     // [total_q, 16, 128]
   void* out;
   const int* plan;
-  int check, total_q, grid, slots, items_at, runs, runs_at, token_run_at;
+  int check, total_q, grid, slots, part_rows, items_at, runs, runs_at, parts_at, token_run_at;
   Source src[3];     // prefix, own, new
   float scale, scale_log2;
 };
 
-// Partial rows of one MMA tile: 128 x 128 fp32 (normalised) as [d / 4][row][4], so that
-// the 32 rows of a warp store 512 contiguous bytes (row by row, each store instruction
-// touched 32 lines: 7,000 cycles a tile), then each row's maximum and sum. The two stay
-// apart: where scores are large, m + log2(l) would round away how many keys a part holds.
-constexpr size_t kRowFloats = 128 * kHeadDim, kSlotFloats = kRowFloats + 2 * 128;
-inline size_t workspace_bytes(int slots) { return static_cast<size_t>(slots) * kSlotFloats * sizeof(float); }
+// Partial rows of one MMA tile, a slot of R = part_pitch workspace rows: R x 128 fp32
+// (normalised) as [d / 4][row][4], so that the 32 rows of a warp store 512 contiguous bytes
+// (row by row, each store instruction touched 32 lines: 7,000 cycles a tile), then each row's
+// maximum and sum. The two stay apart: where scores are large, m + log2(l) would round away
+// how many keys a part holds.
+constexpr int kPartRowFloats = kHeadDim + 2;
+inline size_t workspace_bytes(int part_rows) { return static_cast<size_t>(part_rows) * kPartRowFloats * sizeof(float); }
+__device__ __forceinline__ size_t part_at(int row) { return static_cast<size_t>(row) * kPartRowFloats; }
 
 __device__ __forceinline__ bool plan_ok(const Params& p) {
   return p.plan[kHMagic] == kPlanMagic && p.plan[kHCheck] == p.check && p.plan[kHTotalQ] == p.total_q;
@@ -93,7 +95,7 @@ struct Maps {
 };
 
 struct ItemView {
-  int q0, nq, head, slot, visible, nsegs, blocks;
+  int q0, nq, head, slot, part, visible, nsegs, blocks;
   bool dual;
   int src[kMaxSegs], row[kMaxSegs], len[kMaxSegs], pos[kMaxSegs];
 };
@@ -108,8 +110,9 @@ __device__ __forceinline__ bool load_item(const Params& p, int idx, ItemView& x)
   x.visible = b.x;
   x.nsegs = b.y;
   x.dual = b.z != 0;
+  x.part = b.w;
   x.blocks = 0;
-  bool ok = item_fits(x.q0, x.nq, x.head, x.slot, x.nsegs, x.dual, p.total_q, p.slots);
+  bool ok = item_fits(x.q0, x.nq, x.head, x.slot, x.part, x.nsegs, x.dual, p.total_q, p.slots, p.part_rows);
 #pragma unroll
   for (int s = 0; s < kMaxSegs; ++s) {
     const int4 g = __ldg(w + 2 + s);
@@ -653,7 +656,10 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
       train::tc_fence_after();
     }
     const float inv = st.l > 0.f ? 1.f / st.l : (st.l != st.l ? st.l : 0.f);   // (a NaN sum stays NaN)
-    float* prow = part + static_cast<size_t>(max(slot, 0) + tile) * kSlotFloats;
+    const int pitch = part_pitch(nq);
+    float* prow = part;
+    if (slot >= 0)
+      prow += part_at(__ldg(p.plan + p.items_at + static_cast<size_t>(idx) * kItemWords + kIPart) + tile * pitch);
     __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) +
                           (static_cast<size_t>(q0 + (row_ok ? lt : 0)) * kQHeads + 2 * head + (rm & 1)) * kHeadDim;
     if (warp_ok) {
@@ -675,12 +681,12 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
         } else if (row_ok) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            __stcg(reinterpret_cast<float4*>(prow + (8 * c + j) * 512 + 4 * rm),
+            __stcg(reinterpret_cast<float4*>(prow + 4 * ((8 * c + j) * pitch + rm)),
                    make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
         }
       }
       if (row_ok && slot >= 0)
-        __stcg(reinterpret_cast<float2*>(prow + kRowFloats) + rm, make_float2(st.m, st.l));
+        __stcg(reinterpret_cast<float2*>(prow + kHeadDim * pitch) + rm, make_float2(st.m, st.l));
     }
     if (blocks > 0) {
       train::tc_fence_before();
@@ -875,19 +881,16 @@ __device__ __forceinline__ void f32_item(const Params& p, const ItemView& x, int
       *reinterpret_cast<float4*>(dst + 4 * tx) = a;
       *reinterpret_cast<float4*>(dst + 64 + 4 * tx) = b;
     } else {
-      const int slot = x.slot + (x.dual ? 0 : lt >> 6), rm = 2 * (lt & 63) + (m & 1);
-      float* prow = part + static_cast<size_t>(slot) * kSlotFloats;
-      *reinterpret_cast<float4*>(prow + tx * 512 + 4 * rm) = a;
-      *reinterpret_cast<float4*>(prow + (16 + tx) * 512 + 4 * rm) = b;
-      if (tx == 0) {
-        reinterpret_cast<float2*>(prow + kRowFloats)[rm] = make_float2(mrow[i], lrow[i]);
-        // (the second slot holds nothing)
-        if (x.dual) reinterpret_cast<float2*>(prow + kSlotFloats + kRowFloats)[rm] = make_float2(-INFINITY, 0.f);
-      }
-      if (x.dual) {
-        float* empty = prow + kSlotFloats;
-        *reinterpret_cast<float4*>(empty + tx * 512 + 4 * rm) = make_float4(0.f, 0.f, 0.f, 0.f);
-        *reinterpret_cast<float4*>(empty + (16 + tx) * 512 + 4 * rm) = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int rm = 2 * (lt & 63) + (m & 1), pitch = part_pitch(x.nq);
+      float* prow = part + part_at(x.part + (x.dual ? 0 : lt >> 6) * pitch);
+      *reinterpret_cast<float4*>(prow + 4 * (tx * pitch + rm)) = a;
+      *reinterpret_cast<float4*>(prow + 4 * ((16 + tx) * pitch + rm)) = b;
+      if (tx == 0) reinterpret_cast<float2*>(prow + kHeadDim * pitch)[rm] = make_float2(mrow[i], lrow[i]);
+      if (x.dual) {                              // the second slot holds nothing
+        float* empty = prow + part_at(pitch);
+        *reinterpret_cast<float4*>(empty + 4 * (tx * pitch + rm)) = make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(empty + 4 * ((16 + tx) * pitch + rm)) = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tx == 0) reinterpret_cast<float2*>(empty + kHeadDim * pitch)[rm] = make_float2(-INFINITY, 0.f);
       }
     }
   }
@@ -937,6 +940,7 @@ __global__ void __launch_bounds__(256, 4) prefix_merge_kernel(const Params p, co
   const int* w = p.plan + p.runs_at + static_cast<size_t>(run) * kRunWords;
   const int4 k0 = *reinterpret_cast<const int4*>(w + kRunTile0);
   const int4 k1 = *reinterpret_cast<const int4*>(w + kRunTile0 + kRunTileWords);
+  const int4 at = *reinterpret_cast<const int4*>(p.plan + p.parts_at + static_cast<size_t>(run) * kPartWords);
   // (a dual tile's pieces are two contributions each, in consecutive slots)
   const bool d0 = k0.z == kDualSlots, d1 = k1.z == kDualSlots;
   const int n0 = k0.y << d0, total = n0 + (w[kRunTiles] > 1 ? k1.y << d1 : 0);
@@ -946,12 +950,14 @@ __global__ void __launch_bounds__(256, 4) prefix_merge_kernel(const Params p, co
     const bool dual = first ? d0 : d1;
     const int4 k = first ? k0 : k1;
     const int i = first ? c : c - n0, lt = first ? lt0 : lt1;
-    const int slot = dual ? k.x + ((i >> 1) * kHeads + h) * 2 + (i & 1) : k.x + (i * kHeads + h) * k.z + (lt >> 6);
-    return part + static_cast<size_t>(min(max(slot, 0), p.slots - 1)) * kSlotFloats;
+    const int slot = dual ? ((i >> 1) * kHeads + h) * 2 + (i & 1) : (i * kHeads + h) * k.z + (lt >> 6);
+    const int pitch = first ? at.y : at.w, row = (first ? at.x : at.z) + slot * pitch;
+    return part + part_at(min(max(row, 0), p.part_rows - pitch));
   };
+  auto pitch_of = [&](int c) { return c < n0 ? at.y : at.w; };
   auto row_of = [&](int c) { return 2 * ((c < n0 ? lt0 : lt1) & 63); };
   // (m, l) of the two heads' rows
-  auto stats = [&](int c) { return __ldcg(reinterpret_cast<const float4*>(base(c) + kRowFloats + 2 * row_of(c))); };
+  auto stats = [&](int c) { return __ldcg(reinterpret_cast<const float4*>(base(c) + kHeadDim * pitch_of(c) + 2 * row_of(c))); };
   constexpr float kUnit = sizeof(T) == 4 ? 1.4426950408889634f : 1.f;
   float2 top = make_float2(-INFINITY, -INFINITY);
   for (int c = lane; c < total; c += 32) {
@@ -971,7 +977,7 @@ __global__ void __launch_bounds__(256, 4) prefix_merge_kernel(const Params p, co
 #pragma unroll 4
   for (int c = c_first; c < total; c += kWarps) {
     const float4 f = stats(c);
-    const float4* src = reinterpret_cast<const float4*>(base(c) + static_cast<size_t>(lane) * 512 + 4 * row_of(c));
+    const float4* src = reinterpret_cast<const float4*>(base(c) + 4 * (lane * pitch_of(c) + row_of(c)));
     const float4 v0 = __ldcg(src), v1 = __ldcg(src + 1);
     const float f0 = ex2((f.x - mx) * kUnit) * f.y, f1 = ex2((f.z - my) * kUnit) * f.w;
     den0 += f0;

@@ -42,7 +42,8 @@ constexpr int kAllVisible = 1 << 30;
 
 enum Head {
   kHMagic = 0, kHRequests, kHTotalQ, kHGrid, kHItems, kHCtaAt, kHItemsAt, kHRequestsAt, kHSlots, kHRuns, kHRunsAt,
-  kHTokenRunAt, kHPrefixRows, kHOwnRows, kHNewRows, kHCausal, kHMaxQ, kHWords, kHCheck, kHMaxParts, kHMaxItemRows
+  kHTokenRunAt, kHPrefixRows, kHOwnRows, kHNewRows, kHCausal, kHMaxQ, kHWords, kHCheck, kHMaxParts, kHMaxItemRows,
+  kHPartRows, kHPartsAt
 };
 // Request record: first query row, query rows, then (first row, rows) of prefix, own, new.
 enum RequestField { kRQ0 = 0, kRNq, kRPrefixRow, kRPrefixLen, kROwnRow, kROwnLen, kRNewRow, kRNewLen };
@@ -50,7 +51,8 @@ enum RequestField { kRQ0 = 0, kRNq, kRPrefixRow, kRPrefixLen, kROwnRow, kROwnLen
 // the item sees the keys whose chain position is below kIVisible + t.
 enum ItemField {
   kIQ0 = 0, kINq, kIHead, kISlot /* -1: write the output */, kIVisible, kISegs,
-  kIDual /* one MMA tile's rows, even key blocks on tile A and odd ones on tile B */, kISeg0 = 8,
+  kIDual /* one MMA tile's rows, even key blocks on tile A and odd ones on tile B */,
+  kIPart /* workspace row at which the item's first slot begins */, kISeg0 = 8,
   kISegWords = 4 /* source (0 prefix, 1 own, 2 new), first row, keys, chain position of the first key */
 };
 // Run record: query rows [kRunQ0, + kRunNq) merge the same tiles' partials.
@@ -59,15 +61,24 @@ enum RunField {
   kRunTileWords = 4 /* slot, pieces, slots per (piece, head): 1, 2 or kDualSlots, q0 */
 };
 constexpr int kDualSlots = 3;              // two slots, both holding (part of) every row
+// Behind the runs, the workspace of a run's tiles: (first row of the tile's slots, rows of a
+// slot) for each of the two. Slots follow one another as (piece, head, slot).
+constexpr int kPartWords = 4;
+
+// Workspace rows of a slot: an MMA tile's rows (query row, head). An even number, so every slot
+// starts on 16 bytes. (128 rows throughout took 1.1 GB for 1024 one-row requests.)
+__host__ __device__ inline int part_pitch(int nq) { return 2 * (nq > kHalfTile ? kHalfTile : nq); }
 
 // Whether an item's own words are in range: its rows, its head, and its slots among the
-// plan's (a direct item, slot -1, needs none; a wide or dual one needs two). The kernels
-// skip an item that fails, so build_plan hands out none.
-__host__ __device__ inline bool item_fits(int q0, int nq, int head, int slot, int nsegs, bool dual, int total_q,
-                                          int slots) {
+// plan's (a direct item, slot -1, needs none; a wide or dual one needs two) and in the
+// workspace. The kernels skip an item that fails, so build_plan hands out none.
+__host__ __device__ inline bool item_fits(int q0, int nq, int head, int slot, int part, int nsegs, bool dual,
+                                          int total_q, int slots, int part_rows) {
   const bool rows = nq >= 1 && nq <= kTileRows && q0 >= 0 && q0 <= total_q - nq;
+  const int need = nq > kHalfTile || dual ? 2 : 1;
   const bool store = slot < 0 ? slot == -1 && !dual
-                              : slot <= slots - (nq > kHalfTile || dual ? 2 : 1) && (!dual || nq <= kHalfTile);
+                              : slot <= slots - need && (!dual || nq <= kHalfTile) && part >= 0 &&
+                                    part <= part_rows - need * part_pitch(nq);
   return rows && store && head >= 0 && head < kHeads && nsegs >= 0 && nsegs <= kMaxSegs;
 }
 
@@ -90,7 +101,7 @@ struct PlanTile {
   int nsegs;
   bool complete;      // holds every key of its rows
   int blocks;
-  int pieces, slot;
+  int pieces, slot, part;
   bool dual;
   int slots() const { return dual || nq > kHalfTile ? 2 : 1; }
 };
@@ -274,16 +285,19 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
       best = pieces;
     }
   }
-  long long slots = 0;
+  long long slots = 0, part_rows = 0;
   for (size_t i = 0; i < tiles.size(); ++i) {
     PlanTile& t = tiles[i];
     t.pieces = best[i];
     t.slot = -1;
     t.dual = dual_piece(t.nq, t.complete, t.blocks, t.pieces);
     if (!(t.complete && t.pieces == 1 && !t.dual)) {
+      const long long n = static_cast<long long>(t.pieces) * kHeads * t.slots();
       t.slot = static_cast<int>(slots);
-      slots += static_cast<long long>(t.pieces) * kHeads * t.slots();
-      if (slots > kLimit) return kPlanTooLarge;
+      t.part = static_cast<int>(part_rows);
+      slots += n;
+      part_rows += n * part_pitch(t.nq);
+      if (part_rows > kLimit) return kPlanTooLarge;
     }
   }
   costs(best, cost);
@@ -305,6 +319,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
         it[kIHead] = h;
         it[kISlot] = t.slot < 0 ? -1 : t.slot + (p * kHeads + h) * t.slots();
         it[kIDual] = t.dual ? 1 : 0;
+        it[kIPart] = t.slot < 0 ? 0 : t.part + (p * kHeads + h) * t.slots() * part_pitch(t.nq);
         it[kIVisible] = t.visible;
         int at = 0, pos = 0, n = 0;
         for (int s = 0; s < t.nsegs; ++s) {
@@ -322,13 +337,14 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
           pos += t.segs[s].len;
         }
         it[kISegs] = n;
-        if (!item_fits(it[kIQ0], it[kINq], h, it[kISlot], n, t.dual, static_cast<int>(q0), static_cast<int>(slots)))
+        if (!item_fits(it[kIQ0], it[kINq], h, it[kISlot], it[kIPart], n, t.dual, static_cast<int>(q0),
+                       static_cast<int>(slots), static_cast<int>(part_rows)))
           return kPlanInvalid;
         per_cta[cta[idx]].push_back({cost[idx], idx});
       }
 
   // Merge runs: maximal row ranges whose rows merge the same tiles.
-  std::vector<int32_t> runs, token_run;
+  std::vector<int32_t> runs, parts, token_run;
   int max_parts = 0;                             // partial rows that one output row merges
   if (slots > 0) {
     token_run.assign(q0, -1);
@@ -336,10 +352,11 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
       if (a >= b) return;
       const int id = static_cast<int>(runs.size()) / kRunWords;
       runs.resize(runs.size() + kRunWords, 0);
+      parts.resize(parts.size() + kPartWords, 0);
       int32_t* w = runs.data() + static_cast<size_t>(id) * kRunWords;
       w[kRunQ0] = a;
       w[kRunNq] = b - a;
-      int n = 0, parts = 0;
+      int n = 0, count = 0;
       for (const PlanTile* t : {x, y})
         if (t) {
           int32_t* k = w + kRunTile0 + kRunTileWords * n++;
@@ -347,9 +364,11 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
           k[1] = t->pieces;
           k[2] = t->dual ? kDualSlots : t->slots();
           k[3] = t->q0;
-          parts += t->pieces * (t->dual ? 2 : 1);
+          parts[parts.size() - kPartWords + 2 * n - 2] = t->part;
+          parts[parts.size() - kPartWords + 2 * n - 1] = part_pitch(t->nq);
+          count += t->pieces * (t->dual ? 2 : 1);
         }
-      max_parts = std::max(max_parts, parts);
+      max_parts = std::max(max_parts, count);
       w[kRunTiles] = n;
       std::fill(token_run.begin() + a, token_run.begin() + b, id);
     };
@@ -380,7 +399,8 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   const long long cta_at = kHeadWords, requests_at = round4(cta_at + grid + 1),
                   items_at = requests_at + static_cast<long long>(in.requests) * kRequestWords,
                   runs_at = items_at + static_cast<long long>(items.size()),
-                  token_at = runs_at + static_cast<long long>(runs.size()),
+                  parts_at = runs_at + static_cast<long long>(runs.size()),
+                  token_at = parts_at + static_cast<long long>(parts.size()),
                   words = round4(token_at + static_cast<long long>(token_run.size()));
   if (words > kLimit) return kPlanTooLarge;
   plan.assign(words, 0);
@@ -395,6 +415,8 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   plan[kHSlots] = static_cast<int32_t>(slots);
   plan[kHRuns] = static_cast<int32_t>(runs.size() / kRunWords);
   plan[kHRunsAt] = static_cast<int32_t>(runs_at);
+  plan[kHPartsAt] = static_cast<int32_t>(parts_at);
+  plan[kHPartRows] = static_cast<int32_t>(part_rows);
   plan[kHTokenRunAt] = static_cast<int32_t>(token_at);
   plan[kHPrefixRows] = static_cast<int32_t>(prefix_rows);
   plan[kHOwnRows] = static_cast<int32_t>(own_rows);
@@ -429,6 +451,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
     w[kRNewLen] = in.new_len ? in.new_len[i] : 0;
   }
   std::copy(runs.begin(), runs.end(), plan.begin() + runs_at);
+  std::copy(parts.begin(), parts.end(), plan.begin() + parts_at);
   std::copy(token_run.begin(), token_run.end(), plan.begin() + token_at);
   plan[kHCheck] = plan_check(plan);
   return kPlanOk;
