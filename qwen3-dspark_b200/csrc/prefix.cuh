@@ -668,6 +668,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         float o[32];
+        float* prow_c = prow + 4 * (8 * c * pitch + rm);
         train::tmem_ld32(o_addr + 32 * c, o);
         // (without a visible key O was never written, or holds products of zeros)
 #pragma unroll
@@ -681,7 +682,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, float* part, int f
         } else if (row_ok) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            __stcg(reinterpret_cast<float4*>(prow + 4 * ((8 * c + j) * pitch + rm)),
+            __stcg(reinterpret_cast<float4*>(prow_c + 4 * j * pitch),
                    make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
         }
       }
