@@ -501,6 +501,11 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
  * sets DSPARK_DEVICE_EMPTY_MASK. scratch: dspark_control_argmax_scratch_bytes(rows,
  * vocab) bytes, 8-byte aligned, never needing a clear, one per call in flight.
  *
+ * dspark_control_logits does not look for such rows: one comes out as mask_value
+ * throughout, and dspark_stochastic_accept would draw any token from a finite one.
+ * dspark_control_check_masks (the same masks, mask_index, rows and requests) sets
+ * DSPARK_DEVICE_EMPTY_MASK where a request's row has a mask that allows nothing.
+ *
  * dspark_control_tokens adds tokens[cu[i] .. cu[i+1]), cut to n[i] where n is not NULL,
  * to table row slots[i]: to the counts, or (counts NULL) to the prompt bits; with
  * dspark_greedy_accept's emitted, cu_q and n_commit it commits a round's tokens.
@@ -520,6 +525,8 @@ int dspark_control_argmax(const void* logits, long long ld, int dtype, int rows,
                           int max_bias, const uint32_t* masks, long long ld_mask, int num_masks,
                           const int32_t* mask_index, int32_t* pred, void* scratch, size_t scratch_bytes,
                           cudaStream_t stream);
+int dspark_control_check_masks(const uint32_t* masks, long long ld_mask, int num_masks, const int32_t* mask_index,
+                               int rows, int vocab, const int32_t* cu_q, int num_requests, cudaStream_t stream);
 int dspark_control_tokens(const long long* tokens, int num_tokens, const int32_t* cu, const int32_t* n,
                           const int32_t* slots, int num_requests, int vocab, int num_slots, int16_t* counts,
                           long long ld_counts, uint32_t* prompt_bits, long long ld_bits, cudaStream_t stream);

@@ -66,6 +66,7 @@ SIGNATURES = {
     'dspark_control_logits': (_i, _CONTROL_ARGS + [_f, _vp, _ll, _i, _vp]),
     'dspark_control_argmax_scratch_bytes': (_sz, [_i, _i]),
     'dspark_control_argmax': (_i, _CONTROL_ARGS + [_vp, _vp, _sz, _vp]),
+    'dspark_control_check_masks': (_i, [_vp, _ll, _i, _vp, _i, _i, _vp, _i, _vp]),
     'dspark_control_tokens': (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _ll, _vp, _ll, _vp]),
     'dspark_draft_append': (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _vp, _vp, _ll, _ll,
                                  _vp]),

@@ -10,8 +10,8 @@ row j counts proposals 1 .. j on top of the table.
 
 The arithmetic (float32, one rounding per step; ``dspark_control_logits``):
 seen tokens (in the prompt, or emitted) are divided (positive) or multiplied by
-``repetition``; emitted ones lose ``frequency * count + presence``; biases are added in
-list order; tokens the row's mask forbids become ``mask_value``.
+``repetition``; emitted ones lose ``frequency * count + presence``; the sum of a token's
+biases (added up in list order) is added; tokens the row's mask forbids become ``mask_value``.
 """
 import math
 
@@ -189,7 +189,7 @@ def _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index):
 
 
 def control_logits(logits, controls, slots, *, cu_query=None, tokens=None, masks=None, mask_index=None,
-                   mask_value=float('-inf'), out=None, out_dtype=None):
+                   mask_value=float('-inf'), out=None, out_dtype=None, flag_empty=False):
     """Controlled logits of a verify round or decode step (``dspark_control_logits``).
 
     ``logits`` [N, vocab] bf16/fp32 (rows may be strided); ``slots`` int32 [R] from
@@ -199,7 +199,10 @@ def control_logits(logits, controls, slots, *, cu_query=None, tokens=None, masks
     and ``mask_index`` int32 [N] the row of each logits row, -1 for none. Returns [N, vocab] in
     ``out_dtype`` (the logits' dtype or float32); ``out=logits`` changes them in place.
     ``mask_value`` replaces forbidden logits: a finite one (``torch.finfo(dtype).min``) keeps
-    the rows acceptable to ``stochastic_accept``, which refuses infinities."""
+    the rows acceptable to ``stochastic_accept``, which refuses infinities. A row whose mask
+    allows nothing is ``mask_value`` throughout, and sampling from it gives any token: with
+    ``flag_empty`` such a row sets the device status bit ``DEVICE_EMPTY_MASK`` (one more small
+    launch). Rows outside every request are not written."""
     args = _arguments(logits, controls, slots, cu_query, tokens, masks, mask_index)
     device, ld_out = controls.device, controls.vocab
     if out is None:
@@ -216,6 +219,10 @@ def control_logits(logits, controls, slots, *, cu_query=None, tokens=None, masks
         _lib.check(_lib.load_library().dspark_control_logits(
             *args, float(mask_value), out.data_ptr(), ld_out, _DTYPES[out.dtype], _stream(device)),
             'dspark_control_logits')
+        if flag_empty and masks is not None:
+            # masks, ld_mask, num_masks, mask_index; rows and vocab; cu_q; requests
+            _lib.check(_lib.load_library().dspark_control_check_masks(*args[-4:], args[3], args[4], args[5], args[8],
+                                                                      _stream(device)), 'dspark_control_check_masks')
     return out
 
 

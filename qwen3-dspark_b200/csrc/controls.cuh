@@ -636,6 +636,37 @@ __global__ void __launch_bounds__(128) control_argmax_finish_kernel(const Params
   }
 }
 
+// Sets the status bit where a row's mask allows no token of the vocabulary: a warp per row,
+// 16 words a lane in flight, done at the first word with a bit.
+__global__ void __launch_bounds__(256) control_masks_kernel(const uint32_t* masks, long long ld_mask, int num_masks,
+                                                            const int* mask_index, int rows, int vocab,
+                                                            const int* cu_q) {
+  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int q0 = cu_q ? cu_q[r] : r, q1 = cu_q ? cu_q[r + 1] : r + 1;
+  if (q0 < 0 || q1 < q0 || q1 > rows) {
+    if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
+    return;
+  }
+  const int words = (vocab + 31) / 32;
+  const uint32_t last = 0xffffffffu >> (31 - ((vocab - 1) & 31));
+  for (int j = q0 + warp; j < q1; j += 8) {
+    const int mi = mask_index[j];
+    if (mi < 0 || mi >= num_masks) continue;     // no mask, or refused by the controls
+    const uint32_t* m = masks + static_cast<long long>(mi) * ld_mask;
+    bool any = false;
+    for (int w0 = 0; w0 < words && !any; w0 += 512) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int w = w0 + 32 * k + lane;
+        if (w < words) bits |= __ldg(m + w) & (w == words - 1 ? last : 0xffffffffu);
+      }
+      any = __any_sync(0xffffffffu, bits != 0);
+    }
+    if (!any && lane == 0) atomicOr(&g_device_status, kStatusEmptyMask);
+  }
+}
+
 // Adds tokens to the tables: counts[slot][token] += 1 (saturating), or the prompt bit.
 // Request i's tokens are tokens[cu[i] .. cu[i + 1]), cut to n[i] where n is not null.
 struct TokenParams {

@@ -1346,6 +1346,16 @@ int dspark_control_argmax(const void* logits, long long ld, int dtype, int rows,
   return launch_status();
 }
 
+int dspark_control_check_masks(const uint32_t* masks, long long ld_mask, int num_masks, const int32_t* mask_index,
+                               int rows, int vocab, const int32_t* cu_q, int num_requests, cudaStream_t stream) {
+  if (!masks || !mask_index || vocab < 1 || vocab > (1 << 30) || ld_mask < (vocab + 31) / 32 || num_masks < 1 ||
+      rows < 0 || num_requests < 1 || (!cu_q && num_requests > rows))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  controls::control_masks_kernel<<<num_requests, 256, 0, stream>>>(masks, ld_mask, num_masks, mask_index, rows, vocab,
+                                                                   cu_q);
+  return launch_status();
+}
+
 int dspark_control_tokens(const long long* tokens, int num_tokens, const int32_t* cu, const int32_t* n,
                           const int32_t* slots, int num_requests, int vocab, int num_slots, int16_t* counts,
                           long long ld_counts, uint32_t* prompt_bits, long long ld_bits, cudaStream_t stream) {
