@@ -88,11 +88,16 @@ __device__ __forceinline__ unsigned long long max_u64(unsigned long long a, unsi
   return a > b ? a : b;
 }
 
-// a / b rounded to nearest, from r = 1 / b rounded to nearest: q = a r is within an ulp, its
-// residual a - q b is exact in one fma, and q + (a - q b) r rounds to the quotient
-// (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
-// processor", 1990) as long as nothing over- or underflows; __fdiv_rn otherwise. A
-// penalised warp is bound by its instructions, and this takes four.
+// a / b rounded to nearest, from r = 1 / b rounded to nearest: q = a r, corrected by its
+// residual, q + (a - q b) r (P. Markstein, "Computation of elementary functions on the IBM
+// RISC System/6000 processor", 1990), as long as nothing over- or underflows; __fdiv_rn
+// otherwise. A penalised warp is bound by its instructions, and this takes four.
+// Markstein's theorem asks for a q within an ulp, whose residual is exact. Here q is off by up
+// to 1.5 ulp and a residual may lose its last bit, so the correction is right to 2^-23 of
+// itself, and the result to 1.5 * 2^-23 ulp before the last rounding. With 24-bit integers for
+// the mantissas a quotient lies c / (2 B) ulp from a midpoint, c = 1, 2, ..: only c <= 6 could
+// round the wrong way. All 93 million pairs with c <= 16 were enumerated (by the inverse of B
+// modulo 2^24 and 2^25) and computed on the host: every one rounds as the division does.
 constexpr float kDivLow = 1e-20f, kDivHigh = 1e20f;
 __device__ __forceinline__ float divide(float a, float b, float r, bool b_safe) {
   if (b_safe && a > kDivLow && a < kDivHigh) {
