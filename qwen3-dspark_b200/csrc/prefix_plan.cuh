@@ -30,7 +30,6 @@ namespace prefix {
 
 constexpr int kPlanMagic = 0x44535046;     // "DSPF"
 constexpr int kHeadWords = 32;
-constexpr int kRequestWords = 8;
 constexpr int kItemWords = 20;
 constexpr int kRunWords = 12;
 constexpr int kHeads = 8;                  // KV heads
@@ -41,12 +40,9 @@ constexpr int kMaxSegs = 3;
 constexpr int kAllVisible = 1 << 30;
 
 enum Head {
-  kHMagic = 0, kHRequests, kHTotalQ, kHGrid, kHItems, kHCtaAt, kHItemsAt, kHRequestsAt, kHSlots, kHRuns, kHRunsAt,
-  kHTokenRunAt, kHPrefixRows, kHOwnRows, kHNewRows, kHCausal, kHMaxQ, kHWords, kHCheck, kHMaxParts, kHMaxItemRows,
-  kHPartRows, kHPartsAt
+  kHMagic = 0, kHTotalQ = 2, kHGrid, kHItems, kHCtaAt, kHItemsAt, kHSlots = 8, kHRuns, kHRunsAt, kHTokenRunAt,
+  kHPrefixRows, kHOwnRows, kHNewRows, kHCheck = 18, kHMaxParts, kHMaxItemRows, kHPartRows, kHPartsAt
 };
-// Request record: first query row, query rows, then (first row, rows) of prefix, own, new.
-enum RequestField { kRQ0 = 0, kRNq, kRPrefixRow, kRPrefixLen, kROwnRow, kROwnLen, kRNewRow, kRNewLen };
 // Item record: a tile, a KV head and a piece of the tile's key chain. Query row t of
 // the item sees the keys whose chain position is below kIVisible + t.
 enum ItemField {
@@ -199,7 +195,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   std::vector<Req> reqs(in.requests);
   std::vector<Group> groups(in.groups);
   long long q0 = 0, prefix_rows = 0, own_rows = 0, new_rows = 0;
-  int r = 0, max_q = 0;
+  int r = 0;
   for (int g = 0; g < in.groups; ++g) {
     const int n = in.group_size[g];
     if (n < 1 || n > in.requests - r || in.prefix_len[g] < 0 || in.prefix_start[g] < 0) return kPlanInvalid;
@@ -216,7 +212,6 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
       if (al > 0) own_rows = std::max(own_rows, as + al);
       if (bl > 0) new_rows = std::max(new_rows, bs + bl);
       reqs[i] = Req{static_cast<int>(q0 + tokens), static_cast<int>(q), 0, 0};
-      max_q = std::max(max_q, static_cast<int>(q));
       tokens += q;
     }
     Group& gr = groups[g];
@@ -396,8 +391,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   }
 
   auto round4 = [](long long v) { return (v + 3) & ~3ll; };
-  const long long cta_at = kHeadWords, requests_at = round4(cta_at + grid + 1),
-                  items_at = requests_at + static_cast<long long>(in.requests) * kRequestWords,
+  const long long cta_at = kHeadWords, items_at = round4(cta_at + grid + 1),
                   runs_at = items_at + static_cast<long long>(items.size()),
                   parts_at = runs_at + static_cast<long long>(runs.size()),
                   token_at = parts_at + static_cast<long long>(parts.size()),
@@ -405,13 +399,11 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   if (words > kLimit) return kPlanTooLarge;
   plan.assign(words, 0);
   plan[kHMagic] = kPlanMagic;
-  plan[kHRequests] = in.requests;
   plan[kHTotalQ] = static_cast<int32_t>(q0);
   plan[kHGrid] = grid;
   plan[kHItems] = n_items;
   plan[kHCtaAt] = static_cast<int32_t>(cta_at);
   plan[kHItemsAt] = static_cast<int32_t>(items_at);
-  plan[kHRequestsAt] = static_cast<int32_t>(requests_at);
   plan[kHSlots] = static_cast<int32_t>(slots);
   plan[kHRuns] = static_cast<int32_t>(runs.size() / kRunWords);
   plan[kHRunsAt] = static_cast<int32_t>(runs_at);
@@ -421,11 +413,8 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   plan[kHPrefixRows] = static_cast<int32_t>(prefix_rows);
   plan[kHOwnRows] = static_cast<int32_t>(own_rows);
   plan[kHNewRows] = static_cast<int32_t>(new_rows);
-  plan[kHCausal] = in.causal ? 1 : 0;
-  plan[kHMaxQ] = max_q;
   plan[kHMaxParts] = max_parts;
   for (const PlanTile& t : tiles) plan[kHMaxItemRows] = std::max(plan[kHMaxItemRows], t.nq);
-  plan[kHWords] = static_cast<int32_t>(words);
   int next = 0;
   for (int c = 0; c < grid; ++c) {
     plan[cta_at + c] = next;
@@ -436,20 +425,6 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
                   plan.begin() + items_at + static_cast<long long>(next++) * kItemWords);
   }
   plan[cta_at + grid] = next;
-  int g = 0, left = in.groups ? in.group_size[0] : 0;
-  for (int i = 0; i < in.requests; ++i) {
-    while (left == 0) left = in.group_size[++g];
-    --left;
-    int32_t* w = plan.data() + requests_at + static_cast<long long>(i) * kRequestWords;
-    w[kRQ0] = reqs[i].q0;
-    w[kRNq] = reqs[i].nq;
-    w[kRPrefixRow] = in.prefix_start[g];
-    w[kRPrefixLen] = in.prefix_len[g];
-    w[kROwnRow] = in.own_start[i];
-    w[kROwnLen] = in.own_len[i];
-    w[kRNewRow] = in.new_len ? in.new_start[i] : 0;
-    w[kRNewLen] = in.new_len ? in.new_len[i] : 0;
-  }
   std::copy(runs.begin(), runs.end(), plan.begin() + runs_at);
   std::copy(parts.begin(), parts.end(), plan.begin() + parts_at);
   std::copy(token_run.begin(), token_run.end(), plan.begin() + token_at);
