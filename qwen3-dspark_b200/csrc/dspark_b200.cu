@@ -364,14 +364,13 @@ bool overlap(const void* a, size_t an, const void* b, size_t bn) {
   return an > 0 && bn > 0 && x < y + bn && y < x + an;
 }
 
-// The merge of a plan's partial rows. A plain launch: as a programmatic dependent its CTAs
-// could take the registers the attention's third warpgroup gives back before its softmax
-// warps draw them, and with the trigger behind that point small batches measured slower (8
-// rows behind 32768 keys: 102 us against 60).
+// The merge of a plan's partial rows. A plain launch: as a programmatic dependent one, with
+// the trigger behind the attention's register split, small batches measured slower (8 rows
+// behind 32768 keys: 102 us against 60).
 template <typename T>
-int launch_prefix_merge(const prefix::Params& p, const int32_t* plan_head, const float* part, cudaStream_t stream) {
+int launch_prefix_merge(const prefix::Params& p, const float* part, cudaStream_t stream) {
   const long long pairs = static_cast<long long>(p.total_q) * prefix::kHeads;
-  if (plan_head[prefix::kHMaxParts] > prefix::kMergeWideParts && pairs <= prefix::kMergeWidePairs)
+  if (pairs <= prefix::kMergeWidePairs)
     prefix::prefix_merge_kernel<T, 8><<<static_cast<unsigned>(pairs), 256, 0, stream>>>(p, part);
   else
     prefix::prefix_merge_kernel<T, 1><<<static_cast<unsigned>((pairs + 7) / 8), 256, 0, stream>>>(p, part);
@@ -1261,7 +1260,7 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
                         stream>>>(p, part);
     rc = launch_status();
     if (rc != DSPARK_OK || p.slots == 0) return rc;
-    return launch_prefix_merge<float>(p, plan_head, part, stream);
+    return launch_prefix_merge<float>(p, part, stream);
   }
   Maps maps;
   rc = encode_rows_map(&maps.q, q, total_q, kQHeads, 2, kHalfTile / 2);
@@ -1281,7 +1280,7 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
   prefix_attn_kernel<<<p.grid, kAttThreads, prefix::kSmemBytes, stream>>>(maps, p, part);
   rc = launch_status();
   if (rc != DSPARK_OK || p.slots == 0) return rc;
-  return launch_prefix_merge<__nv_bfloat16>(p, plan_head, part, stream);
+  return launch_prefix_merge<__nv_bfloat16>(p, part, stream);
 }
 
 int dspark_control_logits(const void* logits, long long ld, int dtype, int rows, int vocab, const int32_t* cu_q,

@@ -922,10 +922,11 @@ __global__ void __launch_bounds__(kF32Threads2) prefix_f32_kernel(const Params p
 //   out = sum_c w_c o_c / sum_c w_c,  w_c = l_c 2^(m_c - M),  M = max_c m_c
 // (m of the float32 kernel in natural units)
 // kWarps = 1: a warp per (query row, KV head), 8 to a CTA. kWarps = 8: a CTA per pair, its
-// warps taking every eighth contribution, for the many pieces of a long prefix behind few
-// rows (18 pieces of 32768 keys behind 8 rows: one warp each walked them in 16 us); with
-// many rows the warps are there anyway (1024 rows of 8 parts: 14 us slower in CTAs).
-constexpr int kMergeWideParts = 6, kMergeWidePairs = 2048;
+// warps taking every eighth contribution, for few rows, whose warps alone would not fill the
+// GPU (CTA against warp a pair, whole call: 4 rows of 32 parts 27 / 35 us, of 7 parts 16.5 /
+// 18.6; 32 rows of 38 parts 41 / 49, of 4 parts 24.1 / 24.7; 64 rows equal; 96 rows of 3
+// parts 51.4 / 49.8, 256 rows 121 / 115).
+constexpr int kMergeWidePairs = 64 * kHeads;
 
 template <typename T, int kWarps>
 __global__ void __launch_bounds__(256, 4) prefix_merge_kernel(const Params p, const float* part) {

@@ -41,7 +41,7 @@ constexpr int kAllVisible = 1 << 30;
 
 enum Head {
   kHMagic = 0, kHTotalQ = 2, kHGrid, kHItems, kHCtaAt, kHItemsAt, kHSlots = 8, kHRuns, kHRunsAt, kHTokenRunAt,
-  kHPrefixRows, kHOwnRows, kHNewRows, kHCheck = 18, kHMaxParts, kHMaxItemRows, kHPartRows, kHPartsAt
+  kHPrefixRows, kHOwnRows, kHNewRows, kHCheck = 18, kHMaxItemRows = 20, kHPartRows, kHPartsAt
 };
 // Item record: a tile, a KV head and a piece of the tile's key chain. Query row t of
 // the item sees the keys whose chain position is below kIVisible + t.
@@ -84,7 +84,11 @@ constexpr double kCostSingle = 0.9;
 constexpr double kCostDual = 0.6;
 constexpr double kCostItem = 1.6;
 constexpr double kCostPartial = 0.5;       // writing one MMA tile's partial rows (and reading them back)
-constexpr int kChainRows = 96;             // mean query rows from which a group's requests get chain tiles
+// Mean query rows from which a group's requests get chain tiles instead of a share of the
+// group's. Behind 8192 shared keys, chain against shared: 16 requests of 64 rows 115 / 91 us,
+// 96 139 / 129, 112 140 / 153, 128 139 / 155; behind 1024: 64 rows 37 / 43, 96 31 / 46. With
+// few requests the shared tiles spread better (4 x 128 rows behind 1024: 35 / 27).
+constexpr int kChainRows = 96;
 
 struct Seg {
   int src, row, len;
@@ -104,8 +108,10 @@ struct PlanTile {
 
 // Whether a one-tile piece runs its blocks on both MMA tiles: a single tile's chain
 // (product, softmax, product) is bound by its latency, two of them overlap. A complete
-// tile pays with a merge, which is worth it from kDualBlocks blocks.
-constexpr int kDualBlocks = 8;
+// tile pays with a merge, which is worth it from kDualBlocks blocks (400 requests of 8 rows
+// and no prefix, on both tiles against one: 2 blocks 201 / 181 us, 3 248 / 236, 4 263 / 279,
+// 8 377 / 455; 40 requests: 2 32 / 31, 4 39 / 45).
+constexpr int kDualBlocks = 4;
 inline bool dual_piece(int nq, bool complete, int blocks, int pieces) {
   return nq <= kHalfTile && blocks / pieces >= 2 && (!complete || pieces > 1 || blocks >= kDualBlocks);
 }
@@ -340,7 +346,6 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
 
   // Merge runs: maximal row ranges whose rows merge the same tiles.
   std::vector<int32_t> runs, parts, token_run;
-  int max_parts = 0;                             // partial rows that one output row merges
   if (slots > 0) {
     token_run.assign(q0, -1);
     auto add_run = [&](int a, int b, const PlanTile* x, const PlanTile* y) {
@@ -351,7 +356,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
       int32_t* w = runs.data() + static_cast<size_t>(id) * kRunWords;
       w[kRunQ0] = a;
       w[kRunNq] = b - a;
-      int n = 0, count = 0;
+      int n = 0;
       for (const PlanTile* t : {x, y})
         if (t) {
           int32_t* k = w + kRunTile0 + kRunTileWords * n++;
@@ -361,9 +366,7 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
           k[3] = t->q0;
           parts[parts.size() - kPartWords + 2 * n - 2] = t->part;
           parts[parts.size() - kPartWords + 2 * n - 1] = part_pitch(t->nq);
-          count += t->pieces * (t->dual ? 2 : 1);
         }
-      max_parts = std::max(max_parts, count);
       w[kRunTiles] = n;
       std::fill(token_run.begin() + a, token_run.begin() + b, id);
     };
@@ -413,7 +416,6 @@ inline int build_plan(const PlanInput& in, std::vector<int32_t>& plan) {
   plan[kHPrefixRows] = static_cast<int32_t>(prefix_rows);
   plan[kHOwnRows] = static_cast<int32_t>(own_rows);
   plan[kHNewRows] = static_cast<int32_t>(new_rows);
-  plan[kHMaxParts] = max_parts;
   for (const PlanTile& t : tiles) plan[kHMaxItemRows] = std::max(plan[kHMaxItemRows], t.nq);
   int next = 0;
   for (int c = 0; c < grid; ++c) {
