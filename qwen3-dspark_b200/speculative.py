@@ -107,6 +107,9 @@ def speculative_greedy(target, draft, prompts, max_new_tokens, eos_ids=(), devic
     if controls is not None:
         if not device_accept:
             raise ValueError('controls are applied by the on-device acceptance')
+        head = target.model.get_output_embeddings().weight
+        if controls.vocab != head.shape[0] or controls.device != head.device:     # before any request is added
+            raise ValueError("controls must cover the target's vocabulary on its device")
         all_slots = controls.slot_index(list(prompts))
     eos_ids = set(eos_ids)
     for r in prompts:
