@@ -74,7 +74,8 @@ class TokenControls:
         """Take a free slot for ``request``. ``prompt`` / ``output``: its prompt tokens and the
         tokens emitted so far (ids on the host, or integer tensors; on-device ids outside the
         vocabulary are skipped and flagged in the device status). ``bias``: {token: value},
-        or (ids, values) whose duplicates add in order. Returns the slot."""
+        or (ids, values) whose duplicates add in order (on-device ids outside the vocabulary
+        are skipped). Returns the slot."""
         if not isinstance(request, str) or not request or request in self._slots:
             raise ValueError('Require a fresh nonempty request name')
         if not self._free:
@@ -90,8 +91,7 @@ class TokenControls:
             values = torch.as_tensor(values, dtype=torch.float32).to(self.device)
             if values.shape != ids.shape or ids.numel() > self.max_bias:
                 raise ValueError(f'bias: one value per token and at most max_bias = {self.max_bias} entries required')
-        slot = self._free.pop(0)
-        self._slots[request] = slot
+        slot = self._free[0]
         self.counts[slot].zero_()
         self.prompt_bits[slot].zero_()
         n_bias = 0 if ids is None else ids.numel()
@@ -106,6 +106,7 @@ class TokenControls:
         for tokens, cu, to_counts in ((prompt, words[5:7], False), (output, words[7:9], True)):
             if tokens.numel():
                 self._add(tokens, cu, None, words[4:5], to_counts)
+        self._slots[request] = self._free.pop(0)       # taken once its tables are filled
         return slot
 
     def remove_request(self, request):

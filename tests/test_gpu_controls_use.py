@@ -98,3 +98,14 @@ def test_every_token_proposed_seen_and_biased(pkg):
     assert np.array_equal(pkg.control_logits(xd, controls, slots, **args).cpu().numpy(), want)
     assert (pkg.control_argmax(xd, controls, slots, **args).cpu().numpy() == want.argmax(-1)).all()
     status_clean(pkg)
+
+
+def test_a_failed_request_takes_no_slot(pkg, monkeypatch):
+    controls = pkg.TokenControls(1, 100, device=dev())
+    with monkeypatch.context() as m:
+        m.setattr(pkg.TokenControls, '_add', lambda self, *a: (_ for _ in ()).throw(RuntimeError('native failure')))
+        with pytest.raises(RuntimeError):
+            controls.add_request('a', output=[3])
+    assert controls.add_request('a', output=[4]) == 0
+    assert int(controls.counts[0, 3]) == 0 and int(controls.counts[0, 4]) == 1
+    status_clean(pkg)
