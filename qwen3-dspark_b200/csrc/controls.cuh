@@ -14,11 +14,13 @@
 // are seen or biased: they go into a list in shared memory first. Then the rows stream
 // through untouched - bf16 stays packed, masks are applied to pairs, maxima are packed - and
 // a second pass over the list computes the penalised values and stores them over, or
-// compares them. 896 rows x 151936 bf16 tokens with masks and biases take 134 us (2.4 TB/s of
-// the 325 MB; 12.8 us a row of all requests, 7.9 - 8.6 or 4.5 - 5.0 TB/s without masks and
-// lists), 260 rows to float32 64 us (4 TB/s): the start of a CTA, the list pass and the
-// instructions per row bound it beside DRAM. With the penalties
-// inside the streaming pass (per token, or in loops over set bits) it took 252 and 165 us.
+// compares them. 896 rows (7 of each of 128 requests) x 151936 bf16 tokens with masks and
+// biases take 129 us (2.5 TB/s of the 325 MB), 260 rows to float32 62 us (4.1 TB/s). The start
+// of the CTAs, the list pass and the instructions per row bound it beside DRAM: one row a
+// request takes 54 us and each further one 12.5; without masks and lists 37 us and 8.1, which
+// is 4.8 TB/s of a row's 38.9 MB. With the penalties inside the streaming pass (per token, or in
+// loops over set bits) the 896 rows took 252 and 165 us. Four CTAs an SM leave a thread 64
+// registers: the forms that read float32 or unaligned rows spill 12 to 96 bytes.
 #pragma once
 #include "accept.cuh"
 

@@ -6,7 +6,8 @@
 // over the visible keys j of row t's request: its group's prefix rows, then its own
 // cached rows, then its new rows, read in place from three sources. With `causal`, row
 // x of a request with q rows and n keys sees keys j <= n - q + x. A row without a
-// visible key gives zeros.
+// visible key gives zeros. Keys behind a row's limit may hold anything; values there are
+// multiplied by zero weights, so an infinity or NaN in a later row of the request shows.
 #pragma once
 #include "attention.cuh"
 #include "prefix_plan.cuh"
@@ -66,10 +67,14 @@ __device__ __forceinline__ bool plan_ok(const Params& p) {
 // keys rounded up to 16. Every wait is bounded; a timed-out wait raises the CTA abort
 // flag, copies and MMAs in flight are drained and TMEM is released.
 //
-// Bound by the softmax chain where there are many rows (1024 rows x 32768 keys: 281 us,
-// 977 TFLOP/s of 1,666; a block of both tiles takes 3,700 cycles of which the MMAs are
+// The probabilities are rounded to bf16 for the second product (the MMA takes both operands
+// in one type; their sum l is of the unrounded ones): at most 2^-8 of each weight, which takes
+// the relative error of an output from 0.0017 (its own rounding) to 0.0023.
+//
+// Bound by the softmax chain where there are many rows (1024 rows x 32768 keys: 269 us,
+// 1,021 TFLOP/s of 1,666; a block of both tiles takes 3,700 cycles of which the MMAs are
 // 2,048) and by DRAM and the latency of short items where there are few (8 rows x 32768 keys:
-// 40 us with the merge; the keys alone take 21).
+// 40 us with the merge; the keys alone take 21). 28 bytes of a softmax thread spill.
 constexpr int kStagesN = 5;
 constexpr int kAttThreads = 12 * 32;
 constexpr uint32_t kSmemQ = 0;                             // 2 tiles x 32 KB
