@@ -439,7 +439,8 @@ int dspark_train_attn(const void* q, const void* k, const void* v, int total_q, 
  * and n keys sees keys j <= n - q + x (own + new rows must then number at least q).
  * A prefix row is read once per 128 query rows of its group instead of once per
  * request. A row without a visible key gives zeros; values behind a row's causal limit
- * (later rows of its request) get zero weights and have to be finite. No reference counterpart: the reference gathers every request's keys
+ * (later rows of its request) get zero weights and have to be finite. No reference
+ * counterpart: the reference gathers every request's keys
  * (persistent_target_kv.py:441-460).
  *
  * dspark_prefix_plan runs on the host only (all pointers HOST memory): group_size,
@@ -449,7 +450,8 @@ int dspark_train_attn(const void* q, const void* k, const void* v, int total_q, 
  * plan == NULL it returns the plan size in int32 words in *plan_words. The plan is
  * copied to the device once and serves every call with these lengths (all layers of
  * a round); its first DSPARK_PREFIX_HEAD_WORDS words also stay on the host as
- * plan_head. A captured launch keeps its plan: once a length has changed, capture again. DSPARK_ERR_UNSUPPORTED when a row index or a plan offset reaches 2^30.
+ * plan_head. A captured launch keeps its plan: once a length has changed, capture again.
+ * DSPARK_ERR_UNSUPPORTED when a row index or a plan offset reaches 2^30.
  *
  * dspark_prefix_attn: q and out [total_q, 16, 128]; source s holds `rows` rows of
  * which the plan's rows start at row `off` (a layer's first row). A source that the

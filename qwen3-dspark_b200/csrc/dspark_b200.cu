@@ -1242,9 +1242,10 @@ int dspark_prefix_attn(const void* q, int total_q, const void* prefix_k, const v
     return DSPARK_ERR_INVALID_ARGUMENT;
   for (int s = 0; s < 3; ++s) {
     const size_t row = kKVHeads * kHeadDim * elem, bytes = plan_head[kHPrefixRows + s] * row;
+    if (bytes == 0) continue;
     for (const void* t : {p.src[s].k, p.src[s].v}) {
       const char* base = static_cast<const char*>(t) + p.src[s].off * row;
-      if (bytes > 0 && (overlap(out, q_bytes, base, bytes) || overlap(workspace, ws, base, bytes)))
+      if (overlap(out, q_bytes, base, bytes) || overlap(workspace, ws, base, bytes))
         return DSPARK_ERR_INVALID_ARGUMENT;
     }
   }

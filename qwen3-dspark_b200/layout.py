@@ -202,7 +202,8 @@ class SharedPrefixLayout:
     and its own + new rows must number at least q. Lengths may be zero.
 
     ``plan`` is the kernel's work plan (``dspark_prefix_plan``), built once on the host and
-    kept on the device: build the layout once per round and use it for every layer.
+    kept on the device: build the layout once per round and use it for every layer. It is
+    uploaded on the device's current stream, and a captured call keeps the plan of its capture.
     ``head`` holds the plan's first words on the host.
     """
     prefix_lengths: tuple
