@@ -36,6 +36,10 @@ extern "C" {
 #define DSPARK_DTYPE_BF16 0
 #define DSPARK_DTYPE_F32 1
 
+/* Codes of the paged 8-bit cache: signed integers, or e4m3 floating point. */
+#define DSPARK_CODE_INT8 0
+#define DSPARK_CODE_E4M3 1
+
 /* Device status bits (set by kernels, read with dspark_read_device_status). */
 #define DSPARK_DEVICE_WAIT_TIMEOUT 1u
 #define DSPARK_DEVICE_BAD_SCHEDULE 2u
@@ -182,6 +186,17 @@ int dspark_verify_strided(const void* q_raw, long long ld_q, const void* k_raw, 
                           void* resident_v, long long rows_per_layer, void* scratch_k, void* scratch_v,
                           int scratch_rows, int num_layers, int layer, float scale, int path, void* out,
                           void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/*
+ * The preparation of a verify layer by itself (step 1 and 2 of dspark_verify_fused):
+ * q_norm/k_norm + RoPE of the raw projections' rows, written to q_out [total_q, 16, 128],
+ * and roped k and raw v to k_out / v_out [total_q, 8, 128]. Strides as in
+ * dspark_verify_strided; 16-byte aligned pointers. For hosts whose cache is not the
+ * resident rows of that entry (the paged 8-bit cache).
+ */
+int dspark_verify_prep(const void* q_raw, long long ld_q, const void* k_raw, long long ld_k, const void* v_raw,
+                       long long ld_v, const void* q_norm_weight, const void* k_norm_weight, const void* rope_table,
+                       float eps, int total_q, void* q_out, void* k_out, void* v_out, cudaStream_t stream);
 
 /*
  * Commit / rollback for all layers in one launch: for every request copy
@@ -554,6 +569,65 @@ size_t dspark_varlen_attn_noalloc_scratch_bytes(void);
 int dspark_varlen_attn_noalloc(const void* q, const void* k, const void* v, const int32_t* cu_q,
                                const int32_t* cu_k, int num_requests, int total_q, long long key_rows, int max_q,
                                int max_k, float scale, void* out, cudaStream_t stream);
+
+/*
+ * Paged KV cache in 8 bits (no reference counterpart). A page holds 64 tokens; of one layer
+ * and KV head, 64 x 128 codes of K and of V (DSPARK_CODE_INT8 or DSPARK_CODE_E4M3) and one
+ * float32 scale each: value = scale * code. Storage, per layer:
+ *   key [pages][8][2][64][64] (head, half of the head dim, token, dim),
+ *   value [pages][8][128][64] (head, dim, token), key_scale / value_scale [pages][8],
+ *   tail_key / tail_value [slots][2][64][8][128] rows in `dtype` (bf16 or f32).
+ * Request i has ctx_len[i] tokens: ctx_len[i] / 64 pages, the first entries of row i of
+ * `table` [num_requests][table_width] (an id in [0, num_pages)), and ctx_len[i] % 64 open
+ * rows in block (ctx_len[i] / 64) % 2 of tail slot slots[i]. Its new rows are rows
+ * [cu_q[i], cu_q[i + 1]) of q / new_k / new_v, of total_q in all. Values of the device arrays
+ * are checked by the kernels: a request or page that does not fit is skipped and sets
+ * DSPARK_DEVICE_BAD_ARGUMENT. Tensors are 16-byte aligned.
+ *
+ * dspark_quant_plan writes the work plan of a batch (dspark_quant_plan_words words, for
+ * num_requests requests and total_q rows) from the device's cu_q and ctx_len: one small launch
+ * per batch that every layer's attention reuses. After a change of cu_q or ctx_len it has to
+ * be made again. Only the bf16 attention reads it.
+ *
+ * dspark_quant_attn: bottom-right causal attention of one layer. Keys of request i are its
+ * pages' tokens, its open rows and its new rows, of which query row r sees those up to its
+ * own. q and out [total_q, 16, 128], new_k / new_v [total_q, 8, 128] in `dtype`; out may be q
+ * and otherwise overlaps nothing that is read. max_q: no fewer than the longest request's new
+ * rows. bf16 needs the plan and a workspace of dspark_quant_workspace_size bytes, used
+ * by this call alone until it is done. A NaN or infinity in a new row reaches only the
+ * rows that see it.
+ *
+ * dspark_quant_append: the first counts[i] (null: all) new rows of request i follow its
+ * ctx_len[i] tokens, in all layers: new_k / new_v [num_layers][new_rows][8][128]. A block of
+ * 64 rows that gets full becomes page table[i][block], which must not be in use by another
+ * reader; per head, scale = a / qmax and code = round(x * qmax / a) with a = max |x| of the
+ * block (qmax 127 or 448, to nearest, ties to even; a = 0: scale and codes 0; an infinity or
+ * NaN becomes the scale). Rows of the block that stays open go to the tail. ctx_len
+ * itself is not changed.
+ *
+ * dspark_quant_copy: in all layers, pages src[k] -> dst[k] (codes and scales; num of them)
+ * and the open rows (tail_len[k] % 64 of them) of a request of tail_len[k] tokens from tail
+ * slot tail_src[k] to tail_dst[k]. Targets must be distinct, and no source a target.
+ */
+int dspark_quant_plan_words(int device, int num_requests, long long total_q, long long* words);
+int dspark_quant_workspace_size(int device, size_t* bytes);
+int dspark_quant_plan(const int32_t* cu_q, const int32_t* ctx_len, int num_requests, int total_q, int table_width,
+                      int32_t* plan, long long plan_words, cudaStream_t stream);
+int dspark_quant_attn(const void* q, int total_q, const void* new_k, const void* new_v, const void* key,
+                      const void* value, const float* key_scale, const float* value_scale, const void* tail_key,
+                      const void* tail_value, int num_pages, int num_slots, int code, const int32_t* cu_q,
+                      const int32_t* ctx_len, const int32_t* table, int table_width, const int32_t* slots,
+                      int num_requests, int max_q, const int32_t* plan, float scale, int dtype, void* out,
+                      void* workspace, size_t workspace_bytes, cudaStream_t stream);
+int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows, void* key, void* value,
+                        float* key_scale, float* value_scale, void* tail_key, void* tail_value, int num_layers,
+                        int num_pages, int num_slots, int code, const int32_t* cu_q, const int32_t* ctx_len,
+                        const int32_t* table, int table_width, const int32_t* slots, const int32_t* counts,
+                        int num_requests, int total_q, int max_q, int dtype, cudaStream_t stream);
+int dspark_quant_copy(void* key, void* value, float* key_scale, float* value_scale, void* tail_key, void* tail_value,
+                      int num_layers, int num_pages, int num_slots, int dtype, const int32_t* src, const int32_t* dst,
+                      int num, const int32_t* tail_src, const int32_t* tail_dst, const int32_t* tail_len, int num_tails,
+                      cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,7 @@ from .build import LIB_PATH
 
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F32 = 0, 1
+CODE_INT8, CODE_E4M3 = 0, 1
 DEVICE_WAIT_TIMEOUT, DEVICE_BAD_SCHEDULE, DEVICE_BAD_ARGUMENT, DEVICE_EMPTY_MASK = 1, 2, 4, 8
 VERIFY_PATHS = {'auto': -1, 'fused': 0, 'prep': 1}
 
@@ -38,6 +39,7 @@ SIGNATURES = {
     'dspark_verify_strided': (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _f, _vp, _vp, _vp, _i, _i, _i, _vp,
                                    _vp, _ll, _vp, _vp, _i, _i, _i, _f, _i, _vp, _vp, _sz, _vp]),
     'dspark_rope_table': (_i, [_vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
+    'dspark_verify_prep': (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _f, _i, _vp, _vp, _vp, _vp]),
     'dspark_commit_kv': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _ll, _i, _i, _vp]),
     'dspark_train_plan': (_i, [_i, _vp, _vp, _vp, _i, _i, _vp, _ll, ctypes.POINTER(_ll)]),
     'dspark_row_argmax': (_i, [_vp, _ll, _i, _i, _i, _vp, _vp]),
@@ -68,6 +70,14 @@ SIGNATURES = {
     'dspark_control_argmax': (_i, _CONTROL_ARGS + [_vp, _vp, _sz, _vp]),
     'dspark_control_check_masks': (_i, [_vp, _ll, _i, _vp, _i, _i, _vp, _i, _vp]),
     'dspark_control_tokens': (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _ll, _vp, _ll, _vp]),
+    'dspark_quant_plan_words': (_i, [_i, _i, _ll, ctypes.POINTER(_ll)]),
+    'dspark_quant_workspace_size': (_i, [_i, ctypes.POINTER(_sz)]),
+    'dspark_quant_plan': (_i, [_vp, _vp, _i, _i, _i, _vp, _ll, _vp]),
+    'dspark_quant_attn': (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i,
+                               _i, _vp, _f, _i, _vp, _vp, _sz, _vp]),
+    'dspark_quant_append': (_i, [_vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp,
+                                 _vp, _i, _i, _i, _i, _vp]),
+    'dspark_quant_copy': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp]),
     'dspark_draft_append': (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _vp, _vp, _ll, _ll,
                                  _vp]),
 }

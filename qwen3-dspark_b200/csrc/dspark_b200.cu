@@ -23,6 +23,7 @@
 #include "markov.cuh"
 #include "norm.cuh"
 #include "prefix.cuh"
+#include "quant_attn.cuh"
 #include "sampling.cuh"
 #include "train.cuh"
 #include "verify.cuh"
@@ -39,6 +40,7 @@ struct DeviceInfo {
   int sms = 0;
   int append_pairs = 0;   // CTA pairs of the 2-SM append kernel resident at once (0: not used)
   int prefix_status = DSPARK_ERR_UNSUPPORTED;   // whether the shared-prefix kernels can run
+  int quant_status = DSPARK_ERR_UNSUPPORTED;    // whether the kernels of the paged 8-bit cache can run
   int max_smem_optin = 0;
   int cc_major = 0, cc_minor = 0;
 };
@@ -80,6 +82,21 @@ int prefix_setup(int max_smem_optin) {
              : DSPARK_OK;
 }
 
+// Sets the kernels of the paged 8-bit cache up; what it finds concerns them alone.
+int quant_setup(int max_smem_optin) {
+  if (static_cast<size_t>(max_smem_optin) < quant::kAttnSmemQ) return DSPARK_ERR_UNSUPPORTED;
+  const int bytes = static_cast<int>(quant::kAttnSmemQ), f32_bytes = static_cast<int>(quant::kF32AttnSmem);
+  const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  if (cudaFuncSetAttribute(quant::quant_attn_kernel<quant::kInt8>, attr, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(quant::quant_attn_kernel<quant::kE4M3>, attr, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(quant::f32_attn_kernel<quant::kInt8>, attr, f32_bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(quant::f32_attn_kernel<quant::kE4M3>, attr, f32_bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return DSPARK_ERR_CUDA;
+  }
+  return DSPARK_OK;
+}
+
 int device_info(int dev, DeviceInfo* out) {
   if (dev < 0 || dev >= kMaxDevices) return DSPARK_ERR_INVALID_ARGUMENT;
   std::lock_guard<std::mutex> lock(g_mu);
@@ -117,6 +134,7 @@ int device_info(int dev, DeviceInfo* out) {
                              static_cast<int>(append::PairCfg::kSmemBytes)) != cudaSuccess)
       return DSPARK_ERR_CUDA;
     d.prefix_status = prefix_setup(d.max_smem_optin);
+    d.quant_status = quant_setup(d.max_smem_optin);
     {
       // CTA pairs of the 2-SM append the GPU holds at once (a pair needs two SMs of
       // one GPC); a refused query leaves the single-CTA kernels in use.
@@ -432,6 +450,68 @@ int launch_control(const controls::Params& p, bool vec, cudaStream_t stream) {
   return launch_status();
 }
 
+// ---------------------------------------------------------------------------
+// Paged 8-bit cache
+
+size_t row_bytes(int dtype) { return static_cast<size_t>(quant::kRowElems) * (dtype == DSPARK_DTYPE_F32 ? 4 : 2); }
+
+bool quant_cache(quant::Cache& c, void* key, void* value, float* key_scale, float* value_scale, void* tail_key,
+                 void* tail_value, int pages, int slots, int code, int dtype) {
+  c = quant::Cache{static_cast<uint8_t*>(key), static_cast<uint8_t*>(value), key_scale, value_scale, tail_key,
+                   tail_value, pages, slots};
+  return key && value && key_scale && value_scale && tail_key && tail_value && aligned(key, 16) && aligned(value, 16) &&
+         aligned(key_scale, 4) && aligned(value_scale, 4) && aligned(tail_key, 16) && aligned(tail_value, 16) &&
+         pages >= 1 && slots >= 1 && (code == DSPARK_CODE_INT8 || code == DSPARK_CODE_E4M3) &&
+         (dtype == DSPARK_DTYPE_BF16 || dtype == DSPARK_DTYPE_F32);
+}
+
+bool quant_batch(quant::Batch& b, const int32_t* cu_q, const int32_t* ctx_len, const int32_t* table,
+                 const int32_t* slots, int requests, int rows, int width) {
+  b = quant::Batch{cu_q, ctx_len, table, slots, requests, rows, width};
+  return cu_q && ctx_len && table && slots && aligned(cu_q, 4) && aligned(ctx_len, 4) && aligned(table, 4) &&
+         aligned(slots, 4) && requests >= 1 && rows >= 0 && width >= 1;
+}
+
+// The status of the current device, and its SM count.
+int quant_device(int* sms) {
+  DeviceInfo dev;
+  const int st = current_device_info(&dev);
+  if (st != DSPARK_OK) return st;
+  *sms = dev.sms;
+  return dev.quant_status;
+}
+
+// `kernel` on `stream` as a programmatic dependent of the launch before it (it waits in
+// griddepcontrol.wait); a plain launch where the attribute is refused.
+template <typename P>
+int launch_dependent(void (*kernel)(P), dim3 grid, int threads, const P& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    cfg.numAttrs = 0;
+    if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return DSPARK_ERR_CUDA;
+  }
+  return launch_status();
+}
+
+template <typename T>
+int launch_append(const quant::AppendParams& ap, int code, cudaStream_t stream) {
+  const dim3 grid(ap.batch.requests * ap.blocks, ap.layers, 4);
+  if (code == DSPARK_CODE_INT8)
+    quant::append_kernel<T, quant::kInt8, 2><<<grid, 256, 0, stream>>>(ap);
+  else
+    quant::append_kernel<T, quant::kE4M3, 2><<<grid, 256, 0, stream>>>(ap);
+  return launch_status();
+}
+
 }  // namespace
 
 extern "C" {
@@ -632,6 +712,25 @@ int dspark_verify_strided(const void* q_raw, long long ld_q, const void* k_raw, 
                      slot_row, ctx_len, num_requests, total_q, max_q, resident_k, resident_v, rows_per_layer,
                      scratch_k, scratch_v, scratch_rows, num_layers, layer, scale, path, out, workspace,
                      workspace_bytes, stream);
+}
+
+int dspark_verify_prep(const void* q_raw, long long ld_q, const void* k_raw, long long ld_k, const void* v_raw,
+                       long long ld_v, const void* q_norm_weight, const void* k_norm_weight, const void* rope_table,
+                       float eps, int total_q, void* q_out, void* k_out, void* v_out, cudaStream_t stream) {
+  const long long q_row = static_cast<long long>(kQHeads) * kHeadDim, kv_row = static_cast<long long>(kKVHeads) * kHeadDim;
+  if (ld_q < q_row || ld_k < kv_row || ld_v < kv_row || ld_q % 8 != 0 || ld_k % 8 != 0 || ld_v % 8 != 0 || total_q < 1 ||
+      total_q > (1 << 26) || !(eps > 0.f))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  for (const void* x : {q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, rope_table, static_cast<const void*>(q_out),
+                        static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
+    if (x == nullptr || !aligned(x, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
+  const VerifyPrepParams vp{static_cast<const __nv_bfloat16*>(q_raw), static_cast<const __nv_bfloat16*>(k_raw),
+                            static_cast<const __nv_bfloat16*>(v_raw), static_cast<const __nv_bfloat16*>(q_norm_weight),
+                            static_cast<const __nv_bfloat16*>(k_norm_weight), static_cast<const uint32_t*>(rope_table),
+                            static_cast<__nv_bfloat16*>(q_out), static_cast<__nv_bfloat16*>(k_out),
+                            static_cast<__nv_bfloat16*>(v_out), total_q, eps, ld_q, ld_k, ld_v};
+  verify_prep_kernel<<<static_cast<unsigned>((static_cast<long long>(total_q) * 32 + 7) / 8), 256, 0, stream>>>(vp);
+  return launch_status();
 }
 
 int dspark_commit_kv(void* resident_k, void* resident_v, const void* scratch_k, const void* scratch_v,
@@ -1370,6 +1469,145 @@ int dspark_control_tokens(const long long* tokens, int num_tokens, const int32_t
   // a long history (one request's prompt) is spread over several CTAs
   const int per = std::min(32, std::max(1, num_tokens / num_requests / 256));
   controls::control_tokens_kernel<<<dim3(num_requests, per), 256, 0, stream>>>(tp);
+  return launch_status();
+}
+
+int dspark_quant_plan_words(int device, int num_requests, long long total_q, long long* words) {
+  if (words == nullptr || num_requests < 1 || total_q < 0 || total_q >= (1ll << 31)) return DSPARK_ERR_INVALID_ARGUMENT;
+  DeviceInfo d;
+  const int st = device_info(device, &d);
+  if (st != DSPARK_OK) return st;
+  *words = quant::plan_words(d.sms, num_requests, total_q);
+  return DSPARK_OK;
+}
+
+int dspark_quant_workspace_size(int device, size_t* bytes) {
+  if (bytes == nullptr) return DSPARK_ERR_INVALID_ARGUMENT;
+  DeviceInfo d;
+  const int st = device_info(device, &d);
+  if (st != DSPARK_OK) return st;
+  *bytes = quant::attn_workspace(d.sms);
+  return DSPARK_OK;
+}
+
+int dspark_quant_plan(const int32_t* cu_q, const int32_t* ctx_len, int num_requests, int total_q, int table_width,
+                      int32_t* plan, long long plan_words, cudaStream_t stream) {
+  if (!cu_q || !ctx_len || !plan || !aligned(cu_q, 4) || !aligned(ctx_len, 4) || !aligned(plan, 16) ||
+      num_requests < 1 || total_q < 0 || table_width < 1)
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  const int st = quant_device(&sms);
+  if (st != DSPARK_OK) return st;
+  if (plan_words < quant::plan_words(sms, num_requests, total_q)) return DSPARK_ERR_INVALID_ARGUMENT;
+  const quant::PlanParams pp{cu_q, ctx_len, num_requests, total_q, table_width, sms, plan};
+  quant::plan_kernel<<<1, quant::kPlanThreads, 0, stream>>>(pp);
+  return launch_status();
+}
+
+int dspark_quant_attn(const void* q, int total_q, const void* new_k, const void* new_v, const void* key,
+                      const void* value, const float* key_scale, const float* value_scale, const void* tail_key,
+                      const void* tail_value, int num_pages, int num_slots, int code, const int32_t* cu_q,
+                      const int32_t* ctx_len, const int32_t* table, int table_width, const int32_t* slots,
+                      int num_requests, int max_q, const int32_t* plan, float scale, int dtype, void* out,
+                      void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  quant::Cache c;
+  quant::Batch b;
+  if (!quant_cache(c, const_cast<void*>(key), const_cast<void*>(value), const_cast<float*>(key_scale),
+                   const_cast<float*>(value_scale), const_cast<void*>(tail_key), const_cast<void*>(tail_value), num_pages,
+                   num_slots, code, dtype) ||
+      !quant_batch(b, cu_q, ctx_len, table, slots, num_requests, total_q, table_width) || !(scale > 0.f) || max_q < 0 ||
+      max_q > total_q)
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  if (total_q == 0) return DSPARK_OK;
+  if (!q || !new_k || !new_v || !out || !aligned(q, 16) || !aligned(new_k, 16) || !aligned(new_v, 16) || !aligned(out, 16))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  // rows are written while others are still read: out is q itself or shares no byte with what is read
+  const size_t out_bytes = 2 * row_bytes(dtype) * total_q, new_bytes = row_bytes(dtype) * total_q;
+  const size_t tail_bytes = row_bytes(dtype) * num_slots * 2 * quant::kPage, code_bytes = num_pages * quant::kPageBytes;
+  if ((out != q && overlap(out, out_bytes, q, out_bytes)) || overlap(out, out_bytes, new_k, new_bytes) ||
+      overlap(out, out_bytes, new_v, new_bytes) || overlap(out, out_bytes, tail_key, tail_bytes) ||
+      overlap(out, out_bytes, tail_value, tail_bytes) || overlap(out, out_bytes, key, code_bytes) ||
+      overlap(out, out_bytes, value, code_bytes))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  int st = quant_device(&sms);
+  if (st != DSPARK_OK) return st;
+  if (dtype == DSPARK_DTYPE_F32) {
+    const quant::F32Params fp{static_cast<const float*>(q), static_cast<const float*>(new_k),
+                              static_cast<const float*>(new_v), static_cast<float*>(out), c, b, scale};
+    const dim3 grid(num_requests, (max_q + kQBlock - 1) / kQBlock, kKVHeads);
+    if (grid.y > 65535) return DSPARK_ERR_UNSUPPORTED;
+    if (grid.y == 0) return DSPARK_OK;
+    if (code == DSPARK_CODE_INT8)
+      quant::f32_attn_kernel<quant::kInt8><<<grid, quant::kF32AttnThreads, quant::kF32AttnSmem, stream>>>(fp);
+    else
+      quant::f32_attn_kernel<quant::kE4M3><<<grid, quant::kF32AttnThreads, quant::kF32AttnSmem, stream>>>(fp);
+    return launch_status();
+  }
+  if (!plan || !aligned(plan, 16) || !workspace || !aligned(workspace, 16) || workspace_bytes < quant::attn_workspace(sms) ||
+      overlap(workspace, workspace_bytes, out, out_bytes) || overlap(workspace, workspace_bytes, q, out_bytes))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  const quant::AttnParamsQ ap{static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(new_k),
+                              static_cast<const __nv_bfloat16*>(new_v), static_cast<__nv_bfloat16*>(out), c, b, plan, sms,
+                              scale * 1.4426950408889634f, static_cast<float*>(workspace)};
+  if (code == DSPARK_CODE_INT8)
+    quant::quant_attn_kernel<quant::kInt8><<<sms, quant::kAttnThreadsQ, quant::kAttnSmemQ, stream>>>(ap);
+  else
+    quant::quant_attn_kernel<quant::kE4M3><<<sms, quant::kAttnThreadsQ, quant::kAttnSmemQ, stream>>>(ap);
+  st = launch_status();
+  if (st != DSPARK_OK) return st;
+  return launch_dependent(quant::quant_merge_kernel, dim3(sms, kKVHeads), 128, ap, stream);
+}
+
+int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows, void* key, void* value,
+                        float* key_scale, float* value_scale, void* tail_key, void* tail_value, int num_layers,
+                        int num_pages, int num_slots, int code, const int32_t* cu_q, const int32_t* ctx_len,
+                        const int32_t* table, int table_width, const int32_t* slots, const int32_t* counts,
+                        int num_requests, int total_q, int max_q, int dtype, cudaStream_t stream) {
+  quant::AppendParams ap{};
+  if (!quant_cache(ap.cache, key, value, key_scale, value_scale, tail_key, tail_value, num_pages, num_slots, code, dtype) ||
+      !quant_batch(ap.batch, cu_q, ctx_len, table, slots, num_requests, total_q, table_width) || num_layers < 1 ||
+      num_layers > 65535 || new_rows < total_q || max_q < 0 || max_q > total_q || (counts && !aligned(counts, 4)))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  if (max_q == 0) return DSPARK_OK;
+  if (!new_k || !new_v || !aligned(new_k, 16) || !aligned(new_v, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  const int st = quant_device(&sms);
+  if (st != DSPARK_OK) return st;
+  ap.new_k = new_k;
+  ap.new_v = new_v;
+  ap.new_rows = new_rows;
+  ap.layers = num_layers;
+  ap.blocks = (max_q + quant::kPage - 1) / quant::kPage;
+  ap.counts = counts;
+  if (static_cast<long long>(num_requests) * ap.blocks >= (1ll << 31)) return DSPARK_ERR_UNSUPPORTED;
+  return dtype == DSPARK_DTYPE_F32 ? launch_append<float>(ap, code, stream) : launch_append<__nv_bfloat16>(ap, code, stream);
+}
+
+int dspark_quant_copy(void* key, void* value, float* key_scale, float* value_scale, void* tail_key, void* tail_value,
+                      int num_layers, int num_pages, int num_slots, int dtype, const int32_t* src, const int32_t* dst,
+                      int num, const int32_t* tail_src, const int32_t* tail_dst, const int32_t* tail_len, int num_tails,
+                      cudaStream_t stream) {
+  quant::CopyParams cp{};
+  if (!quant_cache(cp.cache, key, value, key_scale, value_scale, tail_key, tail_value, num_pages, num_slots,
+                   DSPARK_CODE_INT8, dtype) ||
+      num_layers < 1 || num_layers > 65535 || num < 0 || num_tails < 0 || num > (1 << 26) || num_tails > (1 << 26) ||
+      (num > 0 && (!src || !dst)) || (num_tails > 0 && (!tail_src || !tail_dst || !tail_len)))
+    return DSPARK_ERR_INVALID_ARGUMENT;
+  if (num == 0 && num_tails == 0) return DSPARK_OK;
+  int sms = 0;
+  const int st = quant_device(&sms);
+  if (st != DSPARK_OK) return st;
+  cp.layers = num_layers;
+  cp.num = num;
+  cp.tails = num_tails;
+  cp.row_bytes = static_cast<int>(row_bytes(dtype));
+  cp.src = src;
+  cp.dst = dst;
+  cp.tail_src = tail_src;
+  cp.tail_dst = tail_dst;
+  cp.tail_len = tail_len;
+  quant::copy_kernel<<<dim3(num * quant::kCopyParts + 2 * num_tails, num_layers), 256, 0, stream>>>(cp);
   return launch_status();
 }
 

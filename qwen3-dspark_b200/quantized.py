@@ -1,0 +1,360 @@
+"""Paged KV cache in 8 bits: its storage, a batch's layout and the attention over it.
+
+``QuantizedPages`` holds the pages of every layer: 64 tokens each, int8 or e4m3 codes with
+one float32 scale per (page, KV head) of K and of V. A request's last, open block of
+tokens waits unquantised in a tail slot until it is full, so that every block is
+quantised once, over all of its tokens, whatever the rounds it came in.
+
+* ``B200QuantizedKernel`` - bottom-right causal attention over pages, open rows and new rows
+* ``QuantizedPages.append`` - new rows of a round into the tail, full blocks into pages
+* ``QuantizedPages.copy`` - pages moved (compaction), open rows copied (forks)
+* ``QuantizedPages.allocate`` / ``share`` / ``free`` - the pages' owners, on the host
+
+bf16 rows run on the tensor cores, float32 rows (the exact configuration) on CUDA cores.
+``B200QuantizedTargetKV`` (quantized_store.py) is the target's KV store over these pages.
+"""
+import ctypes
+import heapq
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .kernels import _DTYPES, HEAD_DIM, HKV, HQ, SCALE, _on_device, _stream, runtime_identity
+from .layout import cumulative
+
+PAGE = 64
+QUANT_BACKEND = 'b200_sm100a_paged_8bit_causal_v1'
+_CODES = {torch.int8: (_lib.CODE_INT8, 127.0), torch.float8_e4m3fn: (_lib.CODE_E4M3, 448.0)}
+CACHE_TYPES = {'int8': torch.int8, 'e4m3': torch.float8_e4m3fn}
+
+
+def _int_list(values, what, low, high):
+    out = [int(x) for x in values]
+    if any(not low <= x < high for x in out):
+        raise ValueError(f'{what}: integers in [{low}, {high}) required')
+    return out
+
+
+@dataclass
+class QuantizedLayout:
+    """A batch over the cache: ``query_lengths[i]`` new rows of request i behind
+    ``context_lengths[i]`` tokens, its pages in row i of ``table`` and its open rows in
+    tail slot ``slots[i]``. The tensors are int32 on the cache's device and are read
+    when a kernel runs. ``context_lengths`` is None where only the device knows them.
+
+    ``plan`` is the attention's work plan, made from the device's ``cu_query`` and ``context``
+    by one small launch (``replan``) and used by every layer: call ``replan`` after changing
+    either in place. It can be captured in a graph in front of the layers.
+    """
+    query_lengths: tuple
+    context_lengths: tuple
+    cu_query: torch.Tensor     # [R + 1]
+    context: torch.Tensor      # [R]
+    table: torch.Tensor        # [R, pages of the longest request]
+    slots: torch.Tensor        # [R]
+    plan: torch.Tensor
+    query_tokens: int
+    max_query: int
+
+    @classmethod
+    def from_lengths(cls, query_lengths, context_lengths, table, slots):
+        """``table`` int32 [R, width] and ``slots`` int32 [R], contiguous on the cache's device."""
+        q = tuple(_int_list(query_lengths, 'query_lengths', 0, 2 ** 30))
+        n = tuple(_int_list(context_lengths, 'context_lengths', 0, 2 ** 30))
+        if not q or len(n) != len(q):
+            raise ValueError('One query and one context length per request required')
+        if not isinstance(table, torch.Tensor) or not table.is_cuda or table.ndim != 2:
+            raise ValueError('table must be a CUDA tensor [requests, pages]')
+        if max(n) // PAGE > table.shape[1]:
+            raise ValueError('table holds fewer pages than a request has full blocks')
+        device = table.device
+        host = torch.tensor(n, dtype=torch.int32)
+        return cls.on_device(q, cumulative(q, device), host.to(device), table, slots, context_lengths=n)
+
+    @classmethod
+    def on_device(cls, query_lengths, cu_query, context, table, slots, *, context_lengths=None, plan=None, replan=True):
+        """A layout over tensors that are on the device already (and may change there)."""
+        q = tuple(query_lengths)
+        r = len(q)
+        device = table.device
+        for t, shape in ((cu_query, (r + 1,)), (context, (r,)), (slots, (r,)), (table, (r, None))):
+            if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or not t.is_contiguous()
+                    or t.ndim != len(shape) or any(s is not None and s != x for s, x in zip(shape, t.shape))):
+                raise ValueError('cu_query [R + 1], context [R], table [R, pages] and slots [R] must be contiguous int32 '
+                                 'tensors on one device')
+        if table.shape[1] < 1:
+            raise ValueError('table needs at least one column')
+        total = sum(q)
+        with _on_device(device):
+            words = plan_words(device, r, total)
+            if plan is None:
+                plan = torch.empty(words, dtype=torch.int32, device=device)
+            elif plan.dtype != torch.int32 or plan.device != device or not plan.is_contiguous() or plan.numel() < words:
+                raise ValueError(f'plan must be a contiguous int32 tensor of at least {words} words on the device')
+        out = cls(q, context_lengths, cu_query, context, table, slots, plan, total, max(q))
+        if replan:
+            out.replan()
+        return out
+
+    def replan(self):
+        device = self.plan.device
+        with _on_device(device):
+            _lib.check(_lib.load_library().dspark_quant_plan(
+                self.cu_query.data_ptr(), self.context.data_ptr(), len(self.query_lengths), self.query_tokens,
+                self.table.shape[1], self.plan.data_ptr(), self.plan.numel(), _stream(device)), 'dspark_quant_plan')
+
+
+def plan_words(device, requests, rows):
+    words = ctypes.c_longlong(0)
+    _lib.check(_lib.load_library().dspark_quant_plan_words(device.index, requests, rows, ctypes.byref(words)),
+               'dspark_quant_plan_words')
+    return words.value
+
+
+_workspace_bytes = {}
+
+
+class QuantizedPages:
+    """Pages of a KV cache in 8 bits, of every layer, and the open rows of its requests.
+
+    ``key`` [layers, pages, 8, 2, 64, 64] (KV head, half of the head dim, token, dim) and
+    ``value`` [layers, pages, 8, 128, 64] (KV head, dim, token): int8 or float8_e4m3fn codes in
+    the order in which the attention reads them; ``key_scale`` / ``value_scale`` float32
+    [layers, pages, 8]; ``tail_key`` / ``tail_value`` [layers, slots, 2, 64, 8, 128] bf16 or
+    float32: block b of a request that is still open lies in tail block b % 2 of its slot.
+    A full block is immutable, so requests may share its page.
+    """
+
+    def __init__(self, key, value, key_scale, value_scale, tail_key, tail_value):
+        tensors = (key, value, key_scale, value_scale, tail_key, tail_value)
+        if any(not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != key.device or not t.is_contiguous()
+               or t.requires_grad for t in tensors):
+            raise ValueError('Pages, scales and tails must be contiguous tensors without autograd on one CUDA device')
+        if key.ndim != 6 or tail_key.ndim != 6:
+            raise ValueError('key must be [layers, pages, 8, 2, 64, 64] and tail_key [layers, slots, 2, 64, 8, 128]')
+        layers, pages, slots = key.shape[0], key.shape[1], tail_key.shape[1]
+        tail = (layers, slots, 2, PAGE, HKV, HEAD_DIM)
+        shapes = ((layers, pages, HKV, 2, PAGE, HEAD_DIM // 2), (layers, pages, HKV, HEAD_DIM, PAGE),
+                  (layers, pages, HKV), (layers, pages, HKV), tail, tail)
+        if any(tuple(t.shape) != s for t, s in zip(tensors, shapes)) or min(layers, pages, slots) < 1:
+            raise ValueError('Page, scale and tail shapes do not match')
+        if (key.dtype not in _CODES or value.dtype != key.dtype or key_scale.dtype != torch.float32
+                or value_scale.dtype != torch.float32 or tail_key.dtype not in _DTYPES
+                or tail_value.dtype != tail_key.dtype):
+            raise ValueError('Codes must be int8 or float8_e4m3fn, scales float32, tails bf16 or float32')
+        if any(t.data_ptr() % 16 for t in tensors):
+            raise ValueError('Pages, scales and tails must be 16-byte aligned')
+        self.key, self.value, self.key_scale, self.value_scale = key, value, key_scale, value_scale
+        self.tail_key, self.tail_value = tail_key, tail_value
+        self.layers, self.pages, self.slots = layers, pages, slots
+        self.device, self.dtype, self.row_dtype = key.device, key.dtype, tail_key.dtype
+        self.runtime = runtime_identity(self.device)
+        self._code, self.qmax = _CODES[key.dtype]
+        self.users = [0] * pages             # requests that hold each page (host)
+        self._free = list(range(pages))      # min-heap
+
+    @classmethod
+    def empty(cls, *, layers, pages, slots, dtype=torch.int8, row_dtype=torch.bfloat16, device='cuda'):
+        if any(type(n) is not int or n < 1 for n in (layers, pages, slots)):
+            raise ValueError('layers, pages and slots must be positive integers')
+        if dtype not in _CODES or row_dtype not in _DTYPES:
+            raise ValueError('Codes must be int8 or float8_e4m3fn, rows bf16 or float32')
+        zeros = lambda shape, t: torch.zeros(shape, dtype=t, device=device)  # noqa: E731
+        tail = (layers, slots, 2, PAGE, HKV, HEAD_DIM)
+        return cls(zeros((layers, pages, HKV, 2, PAGE, HEAD_DIM // 2), torch.int8).view(dtype),
+                   zeros((layers, pages, HKV, HEAD_DIM, PAGE), torch.int8).view(dtype),
+                   zeros((layers, pages, HKV), torch.float32), zeros((layers, pages, HKV), torch.float32),
+                   zeros(tail, row_dtype), zeros(tail, row_dtype))
+
+    # -- owners of pages (host) -------------------------------------------------------
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def allocate(self, count):
+        """``count`` free pages, the lowest ids first, with one user each."""
+        if type(count) is not int or count < 0:
+            raise ValueError('A page count must be a nonnegative integer')
+        if count > len(self._free):
+            raise ValueError(f'{count} pages asked for, {len(self._free)} free')
+        ids = [heapq.heappop(self._free) for _ in range(count)]
+        for x in ids:
+            self.users[x] = 1
+        return ids
+
+    def _held(self, ids):
+        ids = _int_list(ids, 'page ids', 0, self.pages)
+        if any(self.users[x] < 1 for x in ids):
+            raise ValueError('A page that no request holds')
+        return ids
+
+    def share(self, ids):
+        """One more user of each page (a fork)."""
+        for x in self._held(ids):
+            self.users[x] += 1
+
+    def free(self, ids):
+        """One user fewer of each page; a page without users is free."""
+        ids = self._held(ids)
+        if any(self.users[x] < n for x, n in ((x, ids.count(x)) for x in set(ids)) if n > 1):
+            raise ValueError('A page that no request holds')
+        for x in ids:
+            self.users[x] -= 1
+            if not self.users[x]:
+                heapq.heappush(self._free, x)
+
+    # -- device work --------------------------------------------------------------------
+    def _pointers(self, layer=0):
+        return tuple(t[layer].data_ptr() for t in (self.key, self.value, self.key_scale, self.value_scale,
+                                                   self.tail_key, self.tail_value))
+
+    def _layout(self, layout):
+        if not isinstance(layout, QuantizedLayout) or layout.table.device != self.device:
+            raise ValueError('A QuantizedLayout on the cache\'s device is required')
+
+    @torch.no_grad()
+    def append(self, key, value, layout, counts=None):
+        """The first ``counts[i]`` (int32 [R] on the device; None: all) new rows of request i
+        follow its tokens, in all layers in one launch: ``key`` / ``value`` [layers, rows, 8, 128]
+        in the tails' dtype, of which the layout's rows are the first. A block of 64 that gets
+        full is quantised into the page that the table holds for it; the rest waits in the
+        tail. The layout's context lengths are the caller's to advance."""
+        self._layout(layout)
+        for t in (key, value):
+            if (not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != self.row_dtype or t.ndim != 4
+                    or tuple(t.shape[2:]) != (HKV, HEAD_DIM) or t.shape != key.shape or not t.is_contiguous()
+                    or t.requires_grad):
+                raise ValueError(f'append requires contiguous {self.row_dtype} rows [layers, rows, 8, 128] on '
+                                 f'{self.device} without autograd')
+        if key.shape[0] != self.layers or key.shape[1] < layout.query_tokens:
+            raise ValueError('append requires the rows of every layer and of every request')
+        if counts is not None and (not isinstance(counts, torch.Tensor) or counts.device != self.device
+                                   or counts.dtype != torch.int32 or not counts.is_contiguous()
+                                   or counts.shape != (len(layout.query_lengths),)):
+            raise ValueError('counts must be contiguous int32 [requests] on the device')
+        with _on_device(self.device):
+            _lib.check(_lib.load_library().dspark_quant_append(
+                key.data_ptr(), value.data_ptr(), key.shape[1], *self._pointers(), self.layers, self.pages, self.slots,
+                self._code, layout.cu_query.data_ptr(), layout.context.data_ptr(), layout.table.data_ptr(),
+                layout.table.shape[1], layout.slots.data_ptr(), None if counts is None else counts.data_ptr(),
+                len(layout.query_lengths), layout.query_tokens, layout.max_query, _DTYPES[self.row_dtype],
+                _stream(self.device)), 'dspark_quant_append')
+
+    def _index(self, values, limit, what, distinct=False):
+        if isinstance(values, torch.Tensor):
+            if values.device != self.device or values.dtype != torch.int32 or values.ndim != 1 or not values.is_contiguous():
+                raise ValueError(f'{what} must be contiguous int32 [n] on the device')
+            return values
+        values = _int_list(values, what, 0, limit)
+        if distinct and len(set(values)) != len(values):
+            raise ValueError(f'{what} must be distinct')
+        host = torch.tensor(values, dtype=torch.int32)
+        return host.pin_memory().to(self.device, non_blocking=True) if values else host.to(self.device)
+
+    @torch.no_grad()
+    def copy(self, src=(), dst=(), *, tail_src=(), tail_dst=(), tail_lengths=()):
+        """In all layers in one launch: pages ``src[k]`` -> ``dst[k]``, codes and scales, and the
+        open rows of a request of ``tail_lengths[k]`` tokens from tail slot ``tail_src[k]`` to
+        ``tail_dst[k]`` (its full pages are shared instead). Targets must be distinct and no
+        source a target: checked for lists; int32 device tensors are taken at their word,
+        except that an id out of range is skipped and flagged. Users of pages do not change."""
+        for a, b in ((src, dst), (tail_src, tail_dst)):
+            if len(a) != len(b):
+                raise ValueError('One target per source required')
+            if not isinstance(a, torch.Tensor) and not isinstance(b, torch.Tensor) and set(a) & set(b):
+                raise ValueError('A source must not be a target')
+        if len(tail_lengths) != len(tail_src):
+            raise ValueError('One length per tail required')
+        s, d = self._index(src, self.pages, 'src'), self._index(dst, self.pages, 'dst', True)
+        ts, td = self._index(tail_src, self.slots, 'tail_src'), self._index(tail_dst, self.slots, 'tail_dst', True)
+        tn = self._index(tail_lengths, 2 ** 30, 'tail_lengths')
+        with _on_device(self.device):
+            _lib.check(_lib.load_library().dspark_quant_copy(
+                *self._pointers(), self.layers, self.pages, self.slots, _DTYPES[self.row_dtype], s.data_ptr(),
+                d.data_ptr(), s.numel(), ts.data_ptr(), td.data_ptr(), tn.data_ptr(), ts.numel(), _stream(self.device)),
+                'dspark_quant_copy')
+
+    @torch.no_grad()
+    def values(self, ids):
+        """The float32 values of pages ``ids``: (key, value), each [layers, n, 64, 8, 128]."""
+        at = torch.as_tensor(ids, dtype=torch.long, device=self.device)
+        scale = lambda s: s[:, at][..., None, None]  # noqa: E731
+        k = self.key[:, at].float().permute(0, 1, 2, 4, 3, 5).reshape(self.layers, -1, HKV, PAGE, HEAD_DIM)
+        v = self.value[:, at].float().transpose(3, 4)
+        return ((k * scale(self.key_scale)).transpose(2, 3).contiguous(),
+                (v * scale(self.value_scale)).transpose(2, 3).contiguous())
+
+    def open_rows(self, slot, length):
+        """The unquantised last ``length % 64`` tokens of a request: (key, value) views
+        [layers, rows, 8, 128] of its tail."""
+        block, n = length // PAGE % 2, length % PAGE
+        return self.tail_key[:, slot, block, :n], self.tail_value[:, slot, block, :n]
+
+    def bytes(self):
+        """Bytes of the pages with their scales, and of the tails."""
+        size = lambda *ts: sum(t.numel() * t.element_size() for t in ts)  # noqa: E731
+        return (size(self.key, self.value, self.key_scale, self.value_scale), size(self.tail_key, self.tail_value))
+
+
+class B200QuantizedKernel:
+    """Bottom-right causal attention over a paged 8-bit cache (``dspark_quant_attn``).
+
+    ``kernel(query, key, value, layout, *, scale, pages, layer=0, out=None)`` with a
+    ``QuantizedLayout`` and ``QuantizedPages``: ``query`` [sum q, 16, 128], ``key`` / ``value`` the
+    requests' new rows [sum q, 8, 128], contiguous, all in the tails' dtype on the kernel's GPU.
+    Request i's keys are its full pages, its open rows and its new rows; new row r sees
+    everything up to itself. ``out`` (default: a new tensor) may be ``query`` itself and
+    otherwise must not overlap what is read.
+
+    bf16 partial rows live in a workspace that each call allocates on its own stream, so
+    calls on different streams and in different captured graphs share nothing.
+    """
+    backend_name = QUANT_BACKEND
+    native_varlen_calls_per_layer = 1
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+        if self.device.type == 'cuda' and self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
+        self.runtime = runtime_identity(self.device)
+
+    def __call__(self, query, key, value, layout, *, scale, pages, layer=0, out=None):
+        device = self.device
+        if not isinstance(pages, QuantizedPages) or pages.device != device:
+            raise ValueError('B200 quantized attention requires QuantizedPages on its GPU')
+        pages._layout(layout)
+        dtype, n = pages.row_dtype, layout.query_tokens
+        for t, heads in ((query, HQ), (key, HKV), (value, HKV)) + (((out, HQ),) if out is not None else ()):
+            if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or t.requires_grad
+                    or t.ndim != 3 or not t.is_contiguous()):
+                raise ValueError(f'B200 quantized attention requires no-autograd contiguous {dtype} THD tensors on its GPU')
+            if tuple(t.shape) != (n, heads, HEAD_DIM):
+                raise ValueError('Rows must match the layout, with Hq16/Hkv8/D128 heads')
+        if not isinstance(scale, (float, int)) or not math.isfinite(scale) or scale != SCALE:
+            raise ValueError('B200 quantized attention requires the 1/sqrt(128) scale')
+        if type(layer) is not int or not 0 <= layer < pages.layers:
+            raise ValueError('No such layer in the cache')
+        with _on_device(device):
+            if out is None:
+                out = torch.empty_like(query)
+            if n == 0:
+                return out
+            lib = _lib.load_library()
+            ws, nbytes = None, 0
+            if dtype == torch.bfloat16:
+                nbytes = _workspace_bytes.get(device.index)
+                if nbytes is None:
+                    size = ctypes.c_size_t(0)
+                    _lib.check(lib.dspark_quant_workspace_size(device.index, ctypes.byref(size)),
+                               'dspark_quant_workspace_size')
+                    nbytes = _workspace_bytes[device.index] = size.value
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            _lib.check(lib.dspark_quant_attn(
+                query.data_ptr(), n, key.data_ptr(), value.data_ptr(), *pages._pointers(layer), pages.pages, pages.slots,
+                pages._code, layout.cu_query.data_ptr(), layout.context.data_ptr(), layout.table.data_ptr(),
+                layout.table.shape[1], layout.slots.data_ptr(), len(layout.query_lengths), layout.max_query,
+                layout.plan.data_ptr(), float(scale), _DTYPES[dtype], out.data_ptr(),
+                None if ws is None else ws.data_ptr(), nbytes, _stream(device)), 'dspark_quant_attn')
+        return out

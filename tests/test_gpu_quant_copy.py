@@ -1,0 +1,38 @@
+"""Copies of pages and open rows of the paged 8-bit cache: bit for bit, and nothing else changes."""
+import pytest
+import torch
+
+import quant_util as U
+from gpu_util import status_clean
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('row_dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+@pytest.mark.parametrize('src,dst,tails', [
+    ([0], [5], []),
+    ([7, 2, 3], [1, 9, 0], [(0, 3, 130), (0, 1, 130), (2, 4, 64), (0, 5, 0)]),
+    ([], [], [(1, 0, 63)]),
+    ([], [], []),
+])
+def test_copy(pkg, src, dst, tails, row_dtype):
+    x, _ = U.make(3, [1] * 4, [64 * 2, 70, 0, 64], torch.int8, row_dtype, layers=3, spare=8)
+    x['tail_key'].normal_()
+    x['tail_value'].normal_()
+    pages = pkg.QuantizedPages(**{k: v.cuda() for k, v in x.items()})
+    for as_tensor in (False, True):
+        lists = [src, dst] + [[t[k] for t in tails] for k in range(3)]
+        if as_tensor:
+            lists = [torch.tensor(v, dtype=torch.int32, device='cuda') for v in lists]
+        pages.copy(lists[0], lists[1], tail_src=lists[2], tail_dst=lists[3], tail_lengths=lists[4])
+        status_clean(pkg)
+    want = {k: v.clone() for k, v in x.items()}
+    for name in ('key', 'value', 'key_scale', 'value_scale'):
+        want[name][:, dst] = x[name][:, src]
+    for a, b, n in tails:
+        for name in ('tail_key', 'tail_value'):
+            want[name][:, b, n // 64 % 2, :n % 64] = x[name][:, a, n // 64 % 2, :n % 64]
+    for name, w in want.items():
+        got = getattr(pages, name).cpu()
+        view = lambda t: t.contiguous().view(torch.int8)  # noqa: E731
+        assert torch.equal(view(got), view(w)), name
