@@ -582,7 +582,8 @@ int dspark_varlen_attn_noalloc(const void* q, const void* k, const void* v, cons
  * rows in block (ctx_len[i] / 64) % 2 of tail slot slots[i]. Its new rows are rows
  * [cu_q[i], cu_q[i + 1]) of q / new_k / new_v, of total_q in all. Values of the device arrays
  * are checked by the kernels: a request or page that does not fit is skipped and sets
- * DSPARK_DEVICE_BAD_ARGUMENT. Tensors are 16-byte aligned.
+ * DSPARK_DEVICE_BAD_ARGUMENT. Tensors are 16-byte aligned. max_q: no fewer than the longest
+ * request's new rows. The structures themselves are HOST memory, read during the call.
  *
  * dspark_quant_plan writes the work plan of a batch (dspark_quant_plan_words words, for
  * num_requests requests and total_q rows) from the device's cu_q and ctx_len: one small launch
@@ -592,10 +593,9 @@ int dspark_varlen_attn_noalloc(const void* q, const void* k, const void* v, cons
  * dspark_quant_attn: bottom-right causal attention of one layer. Keys of request i are its
  * pages' tokens, its open rows and its new rows, of which query row r sees those up to its
  * own. q and out [total_q, 16, 128], new_k / new_v [total_q, 8, 128] in `dtype`; out may be q
- * and otherwise overlaps nothing that is read. max_q: no fewer than the longest request's new
- * rows. bf16 needs the plan and a workspace of dspark_quant_workspace_size bytes, used
- * by this call alone until it is done. A NaN or infinity in a new row reaches only the
- * rows that see it.
+ * and otherwise overlaps nothing that is read. bf16 needs the plan and a workspace of
+ * dspark_quant_workspace_size bytes, used by this call alone until it is done. A NaN or
+ * infinity in a new row reaches only the rows that see it.
  *
  * dspark_quant_append: the first counts[i] (null: all) new rows of request i follow its
  * ctx_len[i] tokens, in all layers: new_k / new_v [num_layers][new_rows][8][128]. A block of
@@ -609,24 +609,34 @@ int dspark_varlen_attn_noalloc(const void* q, const void* k, const void* v, cons
  * and the open rows (tail_len[k] % 64 of them) of a request of tail_len[k] tokens from tail
  * slot tail_src[k] to tail_dst[k]. Targets must be distinct, and no source a target.
  */
+typedef struct {
+  void* key;
+  void* value;
+  float* key_scale;
+  float* value_scale;
+  void* tail_key;
+  void* tail_value;
+  int num_layers, num_pages, num_slots;
+  int code;                 /* DSPARK_CODE_* */
+  int dtype;                /* DSPARK_DTYPE_*, of the tails and of every row */
+} dspark_quant_cache;
+typedef struct {
+  const int32_t* cu_q;      /* [num_requests + 1] */
+  const int32_t* ctx_len;   /* [num_requests] */
+  const int32_t* table;     /* [num_requests][table_width] */
+  const int32_t* slots;     /* [num_requests] */
+  int num_requests, total_q, max_q, table_width;
+} dspark_quant_batch;
 int dspark_quant_plan_words(int device, int num_requests, long long total_q, long long* words);
 int dspark_quant_workspace_size(int device, size_t* bytes);
-int dspark_quant_plan(const int32_t* cu_q, const int32_t* ctx_len, int num_requests, int total_q, int table_width,
-                      int32_t* plan, long long plan_words, cudaStream_t stream);
-int dspark_quant_attn(const void* q, int total_q, const void* new_k, const void* new_v, const void* key,
-                      const void* value, const float* key_scale, const float* value_scale, const void* tail_key,
-                      const void* tail_value, int num_pages, int num_slots, int code, const int32_t* cu_q,
-                      const int32_t* ctx_len, const int32_t* table, int table_width, const int32_t* slots,
-                      int num_requests, int max_q, const int32_t* plan, float scale, int dtype, void* out,
-                      void* workspace, size_t workspace_bytes, cudaStream_t stream);
-int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows, void* key, void* value,
-                        float* key_scale, float* value_scale, void* tail_key, void* tail_value, int num_layers,
-                        int num_pages, int num_slots, int code, const int32_t* cu_q, const int32_t* ctx_len,
-                        const int32_t* table, int table_width, const int32_t* slots, const int32_t* counts,
-                        int num_requests, int total_q, int max_q, int dtype, cudaStream_t stream);
-int dspark_quant_copy(void* key, void* value, float* key_scale, float* value_scale, void* tail_key, void* tail_value,
-                      int num_layers, int num_pages, int num_slots, int dtype, const int32_t* src, const int32_t* dst,
-                      int num, const int32_t* tail_src, const int32_t* tail_dst, const int32_t* tail_len, int num_tails,
+int dspark_quant_plan(const dspark_quant_batch* batch, int32_t* plan, long long plan_words, cudaStream_t stream);
+int dspark_quant_attn(const void* q, const void* new_k, const void* new_v, const dspark_quant_cache* cache, int layer,
+                      const dspark_quant_batch* batch, const int32_t* plan, float scale, void* out, void* workspace,
+                      size_t workspace_bytes, cudaStream_t stream);
+int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows, const dspark_quant_cache* cache,
+                        const dspark_quant_batch* batch, const int32_t* counts, cudaStream_t stream);
+int dspark_quant_copy(const dspark_quant_cache* cache, const int32_t* src, const int32_t* dst, int num,
+                      const int32_t* tail_src, const int32_t* tail_dst, const int32_t* tail_len, int num_tails,
                       cudaStream_t stream);
 
 #ifdef __cplusplus

@@ -22,6 +22,19 @@ _vp, _i, _ll, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes
 _CONTROL_ARGS = [_vp, _ll, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _ll, _vp, _ll, _vp, _i, _vp, _vp, _vp, _i, _vp, _ll, _i,
                  _vp]
 
+
+class QuantCache(ctypes.Structure):
+    """dspark_quant_cache"""
+    _fields_ = [(n, _vp) for n in ('key', 'value', 'key_scale', 'value_scale', 'tail_key', 'tail_value')] + \
+               [(n, _i) for n in ('num_layers', 'num_pages', 'num_slots', 'code', 'dtype')]
+
+
+class QuantBatch(ctypes.Structure):
+    """dspark_quant_batch"""
+    _fields_ = [(n, _vp) for n in ('cu_q', 'ctx_len', 'table', 'slots')] + \
+               [(n, _i) for n in ('num_requests', 'total_q', 'max_q', 'table_width')]
+
+
 # name -> (restype, argtypes); mirrors include/dspark_b200.h
 SIGNATURES = {
     'dspark_abi_version': (_i, []),
@@ -72,12 +85,10 @@ SIGNATURES = {
     'dspark_control_tokens': (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _ll, _vp, _ll, _vp]),
     'dspark_quant_plan_words': (_i, [_i, _i, _ll, ctypes.POINTER(_ll)]),
     'dspark_quant_workspace_size': (_i, [_i, ctypes.POINTER(_sz)]),
-    'dspark_quant_plan': (_i, [_vp, _vp, _i, _i, _i, _vp, _ll, _vp]),
-    'dspark_quant_attn': (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i,
-                               _i, _vp, _f, _i, _vp, _vp, _sz, _vp]),
-    'dspark_quant_append': (_i, [_vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp,
-                                 _vp, _i, _i, _i, _i, _vp]),
-    'dspark_quant_copy': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp]),
+    'dspark_quant_plan': (_i, [_vp, _vp, _ll, _vp]),
+    'dspark_quant_attn': (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _f, _vp, _vp, _sz, _vp]),
+    'dspark_quant_append': (_i, [_vp, _vp, _ll, _vp, _vp, _vp, _vp]),
+    'dspark_quant_copy': (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp]),
     'dspark_draft_append': (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _vp, _vp, _ll, _ll,
                                  _vp]),
 }

@@ -94,6 +94,13 @@ int quant_setup(int max_smem_optin) {
     cudaGetLastError();
     return DSPARK_ERR_CUDA;
   }
+  // the register split must fit what the CTA is launched with (a setmaxnreg.inc beyond it would wait forever)
+  for (const void* k : {reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kInt8>),
+                        reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kE4M3>)}) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, k) != cudaSuccess) return DSPARK_ERR_CUDA;
+    if (a.numRegs * quant::kAttnThreadsQ < 256 * quant::kHeadRegs + 128 * quant::kFetchRegs) return DSPARK_ERR_UNSUPPORTED;
+  }
   return DSPARK_OK;
 }
 
@@ -455,21 +462,24 @@ int launch_control(const controls::Params& p, bool vec, cudaStream_t stream) {
 
 size_t row_bytes(int dtype) { return static_cast<size_t>(quant::kRowElems) * (dtype == DSPARK_DTYPE_F32 ? 4 : 2); }
 
-bool quant_cache(quant::Cache& c, void* key, void* value, float* key_scale, float* value_scale, void* tail_key,
-                 void* tail_value, int pages, int slots, int code, int dtype) {
-  c = quant::Cache{static_cast<uint8_t*>(key), static_cast<uint8_t*>(value), key_scale, value_scale, tail_key,
-                   tail_value, pages, slots};
-  return key && value && key_scale && value_scale && tail_key && tail_value && aligned(key, 16) && aligned(value, 16) &&
-         aligned(key_scale, 4) && aligned(value_scale, 4) && aligned(tail_key, 16) && aligned(tail_value, 16) &&
-         pages >= 1 && slots >= 1 && (code == DSPARK_CODE_INT8 || code == DSPARK_CODE_E4M3) &&
-         (dtype == DSPARK_DTYPE_BF16 || dtype == DSPARK_DTYPE_F32);
+bool quant_cache(quant::Cache& c, const dspark_quant_cache* x) {
+  if (x == nullptr) return false;
+  c = quant::Cache{static_cast<uint8_t*>(x->key), static_cast<uint8_t*>(x->value), x->key_scale, x->value_scale,
+                   x->tail_key, x->tail_value, x->num_pages, x->num_slots};
+  for (const void* t : {x->key, x->value, static_cast<void*>(x->key_scale), static_cast<void*>(x->value_scale),
+                        x->tail_key, x->tail_value})
+    if (t == nullptr || !aligned(t, 16)) return false;
+  return x->num_layers >= 1 && x->num_layers <= 65535 && x->num_pages >= 1 && x->num_slots >= 1 &&
+         (x->code == DSPARK_CODE_INT8 || x->code == DSPARK_CODE_E4M3) &&
+         (x->dtype == DSPARK_DTYPE_BF16 || x->dtype == DSPARK_DTYPE_F32);
 }
 
-bool quant_batch(quant::Batch& b, const int32_t* cu_q, const int32_t* ctx_len, const int32_t* table,
-                 const int32_t* slots, int requests, int rows, int width) {
-  b = quant::Batch{cu_q, ctx_len, table, slots, requests, rows, width};
-  return cu_q && ctx_len && table && slots && aligned(cu_q, 4) && aligned(ctx_len, 4) && aligned(table, 4) &&
-         aligned(slots, 4) && requests >= 1 && rows >= 0 && width >= 1;
+bool quant_batch(quant::Batch& b, const dspark_quant_batch* x) {
+  if (x == nullptr) return false;
+  b = quant::Batch{x->cu_q, x->ctx_len, x->table, x->slots, x->num_requests, x->total_q, x->table_width};
+  for (const int32_t* t : {x->cu_q, x->ctx_len, x->table, x->slots})
+    if (t == nullptr || !aligned(t, 4)) return false;
+  return x->num_requests >= 1 && x->total_q >= 0 && x->max_q >= 0 && x->max_q <= x->total_q && x->table_width >= 1;
 }
 
 // The status of the current device, and its SM count.
@@ -483,23 +493,38 @@ int quant_device(int* sms) {
 
 // `kernel` on `stream` as a programmatic dependent of the launch before it (it waits in
 // griddepcontrol.wait); a plain launch where the attribute is refused.
-template <typename P>
-int launch_dependent(void (*kernel)(P), dim3 grid, int threads, const P& p, cudaStream_t stream) {
+template <typename... P>
+int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const P&... p) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, p...) != cudaSuccess) {
     cudaGetLastError();
     cfg.numAttrs = 0;
-    if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return DSPARK_ERR_CUDA;
+    if (cudaLaunchKernelEx(&cfg, kernel, p...) != cudaSuccess) return DSPARK_ERR_CUDA;
   }
   return launch_status();
+}
+
+// K or V rows [rows, 8, 128] bf16 as dims (d, row, head): a box of 8 rows lands head by head.
+int encode_unit_map(CUtensorMap* m, const void* base, long long rows) {
+  if (rows < 1 || rows >= (1ll << 31)) return DSPARK_ERR_INVALID_ARGUMENT;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(kHeadDim), static_cast<cuuint64_t>(rows),
+                        static_cast<cuuint64_t>(kKVHeads)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(kKVHeads * kHeadDim * 2), static_cast<cuuint64_t>(kHeadDim * 2)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(kHeadDim), 8, static_cast<cuuint32_t>(kKVHeads)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DSPARK_OK : DSPARK_ERR_CUDA;
 }
 
 template <typename T>
@@ -1490,55 +1515,52 @@ int dspark_quant_workspace_size(int device, size_t* bytes) {
   return DSPARK_OK;
 }
 
-int dspark_quant_plan(const int32_t* cu_q, const int32_t* ctx_len, int num_requests, int total_q, int table_width,
-                      int32_t* plan, long long plan_words, cudaStream_t stream) {
-  if (!cu_q || !ctx_len || !plan || !aligned(cu_q, 4) || !aligned(ctx_len, 4) || !aligned(plan, 16) ||
-      num_requests < 1 || total_q < 0 || table_width < 1)
-    return DSPARK_ERR_INVALID_ARGUMENT;
+int dspark_quant_plan(const dspark_quant_batch* batch, int32_t* plan, long long plan_words, cudaStream_t stream) {
+  quant::Batch b;
+  if (!quant_batch(b, batch) || !plan || !aligned(plan, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
   int sms = 0;
   const int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;
-  if (plan_words < quant::plan_words(sms, num_requests, total_q)) return DSPARK_ERR_INVALID_ARGUMENT;
-  const quant::PlanParams pp{cu_q, ctx_len, num_requests, total_q, table_width, sms, plan};
+  if (plan_words < quant::plan_words(sms, b.requests, b.rows)) return DSPARK_ERR_INVALID_ARGUMENT;
+  const quant::PlanParams pp{b.cu_q, b.ctx, b.slot, b.requests, b.rows, b.width, sms, plan};
   quant::plan_kernel<<<1, quant::kPlanThreads, 0, stream>>>(pp);
   return launch_status();
 }
 
-int dspark_quant_attn(const void* q, int total_q, const void* new_k, const void* new_v, const void* key,
-                      const void* value, const float* key_scale, const float* value_scale, const void* tail_key,
-                      const void* tail_value, int num_pages, int num_slots, int code, const int32_t* cu_q,
-                      const int32_t* ctx_len, const int32_t* table, int table_width, const int32_t* slots,
-                      int num_requests, int max_q, const int32_t* plan, float scale, int dtype, void* out,
-                      void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+int dspark_quant_attn(const void* q, const void* new_k, const void* new_v, const dspark_quant_cache* cache, int layer,
+                      const dspark_quant_batch* batch, const int32_t* plan, float scale, void* out, void* workspace,
+                      size_t workspace_bytes, cudaStream_t stream) {
   quant::Cache c;
   quant::Batch b;
-  if (!quant_cache(c, const_cast<void*>(key), const_cast<void*>(value), const_cast<float*>(key_scale),
-                   const_cast<float*>(value_scale), const_cast<void*>(tail_key), const_cast<void*>(tail_value), num_pages,
-                   num_slots, code, dtype) ||
-      !quant_batch(b, cu_q, ctx_len, table, slots, num_requests, total_q, table_width) || !(scale > 0.f) || max_q < 0 ||
-      max_q > total_q)
+  if (!quant_cache(c, cache) || !quant_batch(b, batch) || layer < 0 || layer >= cache->num_layers || !(scale > 0.f))
     return DSPARK_ERR_INVALID_ARGUMENT;
-  if (total_q == 0) return DSPARK_OK;
-  if (!q || !new_k || !new_v || !out || !aligned(q, 16) || !aligned(new_k, 16) || !aligned(new_v, 16) || !aligned(out, 16))
-    return DSPARK_ERR_INVALID_ARGUMENT;
+  if (b.rows == 0 || batch->max_q == 0) return DSPARK_OK;
+  for (const void* t : {q, new_k, new_v, static_cast<const void*>(out)})
+    if (t == nullptr || !aligned(t, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
+  const size_t row = row_bytes(cache->dtype), code_bytes = c.pages * quant::kPageBytes;
+  const size_t tail_bytes = row * c.slots * 2 * quant::kPage, scales = static_cast<size_t>(c.pages) * kKVHeads;
+  c.key += layer * code_bytes;
+  c.value += layer * code_bytes;
+  c.key_scale += layer * scales;
+  c.value_scale += layer * scales;
+  c.tail_key = static_cast<uint8_t*>(c.tail_key) + layer * tail_bytes;
+  c.tail_value = static_cast<uint8_t*>(c.tail_value) + layer * tail_bytes;
   // rows are written while others are still read: out is q itself or shares no byte with what is read
-  const size_t out_bytes = 2 * row_bytes(dtype) * total_q, new_bytes = row_bytes(dtype) * total_q;
-  const size_t tail_bytes = row_bytes(dtype) * num_slots * 2 * quant::kPage, code_bytes = num_pages * quant::kPageBytes;
+  const size_t out_bytes = 2 * row * b.rows, new_bytes = row * b.rows;
   if ((out != q && overlap(out, out_bytes, q, out_bytes)) || overlap(out, out_bytes, new_k, new_bytes) ||
-      overlap(out, out_bytes, new_v, new_bytes) || overlap(out, out_bytes, tail_key, tail_bytes) ||
-      overlap(out, out_bytes, tail_value, tail_bytes) || overlap(out, out_bytes, key, code_bytes) ||
-      overlap(out, out_bytes, value, code_bytes))
+      overlap(out, out_bytes, new_v, new_bytes) || overlap(out, out_bytes, c.tail_key, tail_bytes) ||
+      overlap(out, out_bytes, c.tail_value, tail_bytes) || overlap(out, out_bytes, c.key, code_bytes) ||
+      overlap(out, out_bytes, c.value, code_bytes))
     return DSPARK_ERR_INVALID_ARGUMENT;
   int sms = 0;
   int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;
-  if (dtype == DSPARK_DTYPE_F32) {
+  if (cache->dtype == DSPARK_DTYPE_F32) {
     const quant::F32Params fp{static_cast<const float*>(q), static_cast<const float*>(new_k),
                               static_cast<const float*>(new_v), static_cast<float*>(out), c, b, scale};
-    const dim3 grid(num_requests, (max_q + kQBlock - 1) / kQBlock, kKVHeads);
+    const dim3 grid(b.requests, (batch->max_q + kQBlock - 1) / kQBlock, kKVHeads);
     if (grid.y > 65535) return DSPARK_ERR_UNSUPPORTED;
-    if (grid.y == 0) return DSPARK_OK;
-    if (code == DSPARK_CODE_INT8)
+    if (cache->code == DSPARK_CODE_INT8)
       quant::f32_attn_kernel<quant::kInt8><<<grid, quant::kF32AttnThreads, quant::kF32AttnSmem, stream>>>(fp);
     else
       quant::f32_attn_kernel<quant::kE4M3><<<grid, quant::kF32AttnThreads, quant::kF32AttnSmem, stream>>>(fp);
@@ -1550,26 +1572,27 @@ int dspark_quant_attn(const void* q, int total_q, const void* new_k, const void*
   const quant::AttnParamsQ ap{static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(new_k),
                               static_cast<const __nv_bfloat16*>(new_v), static_cast<__nv_bfloat16*>(out), c, b, plan, sms,
                               scale * 1.4426950408889634f, static_cast<float*>(workspace)};
-  if (code == DSPARK_CODE_INT8)
-    quant::quant_attn_kernel<quant::kInt8><<<sms, quant::kAttnThreadsQ, quant::kAttnSmemQ, stream>>>(ap);
-  else
-    quant::quant_attn_kernel<quant::kE4M3><<<sms, quant::kAttnThreadsQ, quant::kAttnSmemQ, stream>>>(ap);
-  st = launch_status();
+  quant::MapsQ maps;
+  const long long tail_rows = static_cast<long long>(c.slots) * 2 * quant::kPage;
+  if ((st = encode_unit_map(&maps.tail_k, c.tail_key, tail_rows)) != DSPARK_OK ||
+      (st = encode_unit_map(&maps.tail_v, c.tail_value, tail_rows)) != DSPARK_OK ||
+      (st = encode_unit_map(&maps.new_k, new_k, b.rows)) != DSPARK_OK ||
+      (st = encode_unit_map(&maps.new_v, new_v, b.rows)) != DSPARK_OK)
+    return st;
+  st = launch_dependent(cache->code == DSPARK_CODE_INT8 ? quant::quant_attn_kernel<quant::kInt8>
+                                                        : quant::quant_attn_kernel<quant::kE4M3>,
+                        dim3(sms), quant::kAttnThreadsQ, quant::kAttnSmemQ, stream, maps, ap);
   if (st != DSPARK_OK) return st;
-  return launch_dependent(quant::quant_merge_kernel, dim3(sms, kKVHeads), 128, ap, stream);
+  return launch_dependent(quant::quant_merge_kernel, dim3(sms, kKVHeads), 256, 0, stream, ap);
 }
 
-int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows, void* key, void* value,
-                        float* key_scale, float* value_scale, void* tail_key, void* tail_value, int num_layers,
-                        int num_pages, int num_slots, int code, const int32_t* cu_q, const int32_t* ctx_len,
-                        const int32_t* table, int table_width, const int32_t* slots, const int32_t* counts,
-                        int num_requests, int total_q, int max_q, int dtype, cudaStream_t stream) {
+int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows, const dspark_quant_cache* cache,
+                        const dspark_quant_batch* batch, const int32_t* counts, cudaStream_t stream) {
   quant::AppendParams ap{};
-  if (!quant_cache(ap.cache, key, value, key_scale, value_scale, tail_key, tail_value, num_pages, num_slots, code, dtype) ||
-      !quant_batch(ap.batch, cu_q, ctx_len, table, slots, num_requests, total_q, table_width) || num_layers < 1 ||
-      num_layers > 65535 || new_rows < total_q || max_q < 0 || max_q > total_q || (counts && !aligned(counts, 4)))
+  if (!quant_cache(ap.cache, cache) || !quant_batch(ap.batch, batch) || new_rows < ap.batch.rows ||
+      (counts && !aligned(counts, 4)))
     return DSPARK_ERR_INVALID_ARGUMENT;
-  if (max_q == 0) return DSPARK_OK;
+  if (batch->max_q == 0) return DSPARK_OK;
   if (!new_k || !new_v || !aligned(new_k, 16) || !aligned(new_v, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
   int sms = 0;
   const int st = quant_device(&sms);
@@ -1577,37 +1600,35 @@ int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows
   ap.new_k = new_k;
   ap.new_v = new_v;
   ap.new_rows = new_rows;
-  ap.layers = num_layers;
-  ap.blocks = (max_q + quant::kPage - 1) / quant::kPage;
+  ap.layers = cache->num_layers;
+  ap.blocks = (batch->max_q + quant::kPage - 1) / quant::kPage;
   ap.counts = counts;
-  if (static_cast<long long>(num_requests) * ap.blocks >= (1ll << 31)) return DSPARK_ERR_UNSUPPORTED;
-  return dtype == DSPARK_DTYPE_F32 ? launch_append<float>(ap, code, stream) : launch_append<__nv_bfloat16>(ap, code, stream);
+  if (static_cast<long long>(ap.batch.requests) * ap.blocks >= (1ll << 31)) return DSPARK_ERR_UNSUPPORTED;
+  return cache->dtype == DSPARK_DTYPE_F32 ? launch_append<float>(ap, cache->code, stream)
+                                          : launch_append<__nv_bfloat16>(ap, cache->code, stream);
 }
 
-int dspark_quant_copy(void* key, void* value, float* key_scale, float* value_scale, void* tail_key, void* tail_value,
-                      int num_layers, int num_pages, int num_slots, int dtype, const int32_t* src, const int32_t* dst,
-                      int num, const int32_t* tail_src, const int32_t* tail_dst, const int32_t* tail_len, int num_tails,
+int dspark_quant_copy(const dspark_quant_cache* cache, const int32_t* src, const int32_t* dst, int num,
+                      const int32_t* tail_src, const int32_t* tail_dst, const int32_t* tail_len, int num_tails,
                       cudaStream_t stream) {
   quant::CopyParams cp{};
-  if (!quant_cache(cp.cache, key, value, key_scale, value_scale, tail_key, tail_value, num_pages, num_slots,
-                   DSPARK_CODE_INT8, dtype) ||
-      num_layers < 1 || num_layers > 65535 || num < 0 || num_tails < 0 || num > (1 << 26) || num_tails > (1 << 26) ||
+  if (!quant_cache(cp.cache, cache) || num < 0 || num_tails < 0 || num > (1 << 26) || num_tails > (1 << 26) ||
       (num > 0 && (!src || !dst)) || (num_tails > 0 && (!tail_src || !tail_dst || !tail_len)))
     return DSPARK_ERR_INVALID_ARGUMENT;
   if (num == 0 && num_tails == 0) return DSPARK_OK;
   int sms = 0;
   const int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;
-  cp.layers = num_layers;
+  cp.layers = cache->num_layers;
   cp.num = num;
   cp.tails = num_tails;
-  cp.row_bytes = static_cast<int>(row_bytes(dtype));
+  cp.row_bytes = static_cast<int>(row_bytes(cache->dtype));
   cp.src = src;
   cp.dst = dst;
   cp.tail_src = tail_src;
   cp.tail_dst = tail_dst;
   cp.tail_len = tail_len;
-  quant::copy_kernel<<<dim3(num * quant::kCopyParts + 2 * num_tails, num_layers), 256, 0, stream>>>(cp);
+  quant::copy_kernel<<<dim3(num * quant::kCopyParts + 2 * num_tails, cp.layers), 256, 0, stream>>>(cp);
   return launch_status();
 }
 

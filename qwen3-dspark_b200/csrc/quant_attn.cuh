@@ -7,41 +7,48 @@
 //
 // An item is up to 8 query rows of a request: with the 2 query heads of a KV head they are the
 // 16 rows of an m16n8k16 MMA (row m = 8 * head + row, so that both rows of a thread end at the
-// same key). Its keys are cut into units of equal bytes, 32 unquantised rows or one page, the
-// rows first. A plan (one small launch per batch, reused by every layer) numbers the units of
+// same key). Its keys are cut into units of at most 16 KB a head: 32 open rows, 32 new rows or one
+// page, in this order. A plan (one small launch per batch, reused by every layer) numbers the units of
 // all items and gives every CTA an equal contiguous range; warp h of a CTA computes KV head h
-// of its range on its own. A page's 16 KB of a head come by bulk copies of 4 KB (half of the
-// dims of K, half of the dims of V) into the warp's own ring of 7 stages, so no warp ever
-// waits for another one. Items cut by ranges leave fp32 partial rows that a dependent launch
-// merges.
+// of its range. A ninth warp fetches the units, K or V of all heads as one bulk copy of 64 KB (rows:
+// TMA boxes of 8), into a ring of 3 stages, across items. Items cut by ranges leave fp32 partial
+// rows that a dependent launch merges.
 //
-// Codes become halves in registers (int8: the byte under the exponent of 1024, minus 1152;
-// e4m3: one conversion), both exactly. So does Q: bf16 has 8 significant bits, a half 11, and
-// each query row is scaled by the power of two that takes its largest value to 2^14, so that
-// only values below 2^-38 of it lose bits; the scale is undone in the scores. Probabilities are
-// rounded to halves relative to 2^7 of the running maximum (2^-11 of each; below 2^-31 of
-// the maximum they vanish), their sum is of the unrounded ones. The V scale multiplies a page's
-// product when it is added to the float32 accumulator.
+// Codes become halves in registers, exactly: e4m3 by one conversion, int8 as the byte under the
+// exponent of 1024, from which 1152 is taken (V), or which the scores' sums start 1152 sum(q)
+// below (K: in float32 that costs 2^-20 of sum |q| 127 at most). So does Q: bf16 has 8
+// significant bits, a half 11, and each query row is scaled by the power of two that takes its
+// largest value to 2^14, so that only values below 2^-38 of it lose bits; the scale is undone in
+// the scores. Probabilities are rounded to halves (2^-11 of each; what is below 2^-30 of the
+// largest vanishes), their sum is of the unrounded ones. Against unquantised rows Q, P and the
+// products are bf16.
 #pragma once
 #include "quant.cuh"
+#include "train.cuh"
 
 namespace dspark {
 namespace quant {
 
-constexpr int kStagesA = 7, kStageA = 4096;
-constexpr int kWarpRing = kStagesA * kStageA;
-constexpr int kAttnThreadsQ = kKVHeads * 32;
-constexpr size_t kAttnSmemQ = 1024 + static_cast<size_t>(kKVHeads) * kWarpRing + kKVHeads * kStagesA * 8;
+constexpr int kStagesA = 3;
+constexpr int kStageA = static_cast<int>(kPageBytes);       // K or V of a unit, all heads
+constexpr int kAttnThreadsQ = 12 * 32;                      // 8 warps of heads, one that fetches, 3 idle
+// Registers of a thread of the head warps and of the others after setmaxnreg; the launch's own
+// (kAttnThreadsQ x the kernel's count, checked when the device is set up) cover them.
+constexpr int kHeadRegs = 216, kFetchRegs = 72;
 constexpr int kRowUnit = 32;                                // unquantised keys of a unit
+constexpr int kRowBox = 8 * kRowElems * 2;                  // bytes of 8 of them, all heads
+constexpr int kChunk = 32;                                  // units whose ids and scales a warp holds at a time
 
 // ---------------------------------------------------------------------------
 // Plan: int32 words [head | CTA ranges | merges | items].
 constexpr int kPlanMagicQ = 0x51a77e11;
 enum PlanWord { kQMagic = 0, kQGrid, kQItems, kQRequests, kQRows, kQHeadWords = 8 };
-constexpr int kCtaWords = 4;                                // first item, its first unit, last item, its end unit
-constexpr int kMergeWords = 4;                              // item (-1: none), last contributor, slot of the first
-constexpr int kItemWordsQ = 8;
-// item: first global row | rows | row in the request | request | row units | pages | start | cost
+constexpr int kCtaWords = 12;       // first item, its first unit, last item, its end unit, the first item's 8 words
+constexpr int kMergeWords = 4;      // item (-1: none), last contributor, slot of the first
+constexpr int kItemWordsQ = 12;
+// item: first global row | rows | row in the request | request | row units | pages | tokens | tail slot |
+//       start and cost in the plan's numbering
+enum ItemWord { kIRow = 0, kIRows, kIR0, kIRequest, kIRowUnits, kIPages, kICtx, kISlot, kIStart, kICost };
 __host__ __device__ constexpr int plan_cta_at() { return kQHeadWords; }
 __host__ __device__ constexpr int plan_merge_at(int grid) { return kQHeadWords + grid * kCtaWords; }
 __host__ __device__ constexpr int plan_items_at(int grid) { return kQHeadWords + grid * (kCtaWords + kMergeWords); }
@@ -55,13 +62,16 @@ constexpr int kItemCost = 1, kMinUnits = 2;
 struct PlanParams {
   const int* cu_q;
   const int* ctx;
+  const int* slot;
   int requests, rows, width, grid;
   int* plan;
 };
 
 constexpr int kPlanThreads = 1024;
+__device__ __forceinline__ int units_of(int keys) { return (keys + kRowUnit - 1) / kRowUnit; }
+// of the open rows and of the new rows that an item sees
 __device__ __forceinline__ int row_units(int ctx, int q_len, int r0) {
-  return (ctx % kPage + min(r0 + kQBlock, q_len) + kRowUnit - 1) / kRowUnit;
+  return units_of(ctx % kPage) + units_of(min(r0 + kQBlock, q_len));
 }
 
 // One CTA. Requests whose lengths do not fit the batch have no items (the status is set).
@@ -79,12 +89,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   __syncthreads();
   for (int base = 0; base < p.requests; base += kPlanThreads) {
     const int i = base + tid;
-    int q0 = 0, q_len = 0, ctx = 0, n = 0;
+    int q0 = 0, q_len = 0, ctx = 0, slot = 0, n = 0;
     long long cost = 0;
     if (i < p.requests) {
       q0 = p.cu_q[i];
       q_len = p.cu_q[i + 1] - q0;
       ctx = p.ctx[i];
+      slot = p.slot[i];
       if (q0 >= 0 && q_len >= 0 && q0 <= p.rows - q_len && ctx >= 0 && ctx / kPage <= p.width) {
         n = (q_len + kQBlock - 1) / kQBlock;
         for (int x = 0; x < n; ++x) cost += kItemCost + ctx / kPage + row_units(ctx, q_len, x * kQBlock);
@@ -131,7 +142,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       const int ru = row_units(ctx, q_len, x * kQBlock), full = ctx / kPage, total = kItemCost + full + ru;
       int4* w = reinterpret_cast<int4*>(items + static_cast<size_t>(idx) * kItemWordsQ);
       w[0] = make_int4(q0 + x * kQBlock, min(kQBlock, q_len - x * kQBlock), x * kQBlock, i);
-      w[1] = make_int4(ru, full, static_cast<int>(at), total);
+      w[1] = make_int4(ru, full, ctx, slot);
+      w[2] = make_int4(static_cast<int>(at), total, 0, 0);
       at += total;
     }
     __syncthreads();
@@ -154,9 +166,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     int lo = 0, hi = count - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (items[static_cast<size_t>(mid) * kItemWordsQ + 6] <= pos) lo = mid; else hi = mid - 1;
+      if (items[static_cast<size_t>(mid) * kItemWordsQ + kIStart] <= pos) lo = mid; else hi = mid - 1;
     }
-    const long long u = pos - items[static_cast<size_t>(lo) * kItemWordsQ + 6] - kItemCost;
+    const long long u = pos - items[static_cast<size_t>(lo) * kItemWordsQ + kIStart] - kItemCost;
     item = lo;
     unit = u > 0 ? static_cast<int>(u) : 0;
   };
@@ -176,17 +188,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       }
       if (u1 == 0) {                                         // ends with the item before
         --i1;
-        u1 = items[static_cast<size_t>(i1) * kItemWordsQ + 4] + items[static_cast<size_t>(i1) * kItemWordsQ + 5];
+        const int* w = items + static_cast<size_t>(i1) * kItemWordsQ;
+        u1 = w[kIRowUnits] + w[kIPages];
       } else if (i1 > i0 || u0 == 0) {                       // the first of the last item's contributors
-        const long long stop = items[static_cast<size_t>(i1) * kItemWordsQ + 6] +
-                               static_cast<long long>(items[static_cast<size_t>(i1) * kItemWordsQ + 7]);
+        const int* w = items + static_cast<size_t>(i1) * kItemWordsQ;
+        const long long stop = static_cast<long long>(w[kIStart]) + w[kICost];
         // the last range k with floor(total k / ranges) < stop
         const int last = static_cast<int>(min(static_cast<long long>(ranges - 1), (stop * ranges - 1) / total));
         merge = make_int4(i1, last, i1 > i0 ? 1 : 0, 0);
       }
       if (i1 >= i0) range = make_int4(i0, u0, i1, u1);
     }
-    ctas[c] = range;
+    ctas[3 * c] = range;
+    if (range.z >= range.x) {
+      const int4* w = reinterpret_cast<const int4*>(items + static_cast<size_t>(range.x) * kItemWordsQ);
+      ctas[3 * c + 1] = w[0];
+      ctas[3 * c + 2] = w[1];
+    }
     merges[c] = merge;
   }
   if (tid == 0) {
@@ -219,31 +237,59 @@ __host__ __device__ inline size_t part_index(int cta, int slot, int head) {
 inline size_t attn_workspace(int grid) { return part_index(grid, 0, 0) * sizeof(float); }
 
 struct ItemQ {
-  int q0, rows, r0, request, row_units, pages;
+  int q0, rows, r0, request, row_units, pages, ctx, slot;
 };
+__device__ __forceinline__ ItemQ item_of(const int4& a, const int4& b) {
+  return ItemQ{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
 __device__ __forceinline__ ItemQ load_item_q(const AttnParamsQ& p, int idx) {
   const int4* w = reinterpret_cast<const int4*>(p.plan + plan_items_at(p.grid) + static_cast<size_t>(idx) * kItemWordsQ);
-  const int4 a = __ldg(w), b = __ldg(w + 1);
-  return ItemQ{a.x, a.y, a.z, a.w, b.x, b.y};
+  return item_of(__ldg(w), __ldg(w + 1));
 }
 
-// D(16x8 f32) += A(16x16 f16, row) * B(16x8 f16, col)
+// A unit. A page: its id (-1: left out). Rows: the first one in its source, their number, and the
+// first new row of them (-1: open rows).
+struct UnitQ {
+  int a, b, c, d;
+};
+// Up to 32 consecutive units of an item, with the scales of their pages.
+struct ChunkQ {
+  UnitQ unit[kChunk];
+  float ks[kChunk][kKVHeads], vs[kChunk][kKVHeads];
+  ItemQ item;
+  int u0, u1;                                               // units
+  int begin, end;                                           // the range's units of the item
+};
+enum BarQ { kQFull = 0, kQEmpty = kQFull + kStagesA, kQChunk = kQEmpty + kStagesA, kQChunkFree = kQChunk + 2, kQBars = kQChunkFree + 2 };
+constexpr uint32_t kSmemChunks = kStagesA * kStageA;
+constexpr uint32_t kSmemBarsQ = kSmemChunks + 2 * sizeof(ChunkQ);
+constexpr uint32_t kSmemAbortQ = kSmemBarsQ + kQBars * 8;
+constexpr size_t kAttnSmemQ = 1024 + kSmemAbortQ + 4;
+struct MapsQ {
+  CUtensorMap tail_k, tail_v, new_k, new_v;                 // boxes of 8 rows of every head, head by head
+};
+
+// D(16x8 f32) += A(16x16 f16, row) * B(16x8 f16, col). Not volatile: the compiler moves the next
+// tile's loads and conversions between the products of this one.
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 4 codes of a word as two pairs of halves.
-template <int kCode>
+// 4 codes of a word as two pairs of halves; int8 with kBiased: 1152 more each.
+constexpr float kBias = 1152.f;
+template <int kCode, bool kBiased>
 __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (kCode == kInt8) {
     w ^= 0x80808080u;                                        // code + 128
-    const __half2 bias = __floats2half2_rn(-1152.f, -1152.f);
-    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);   // 1024 + that
-    __half2 x = __hadd2(*reinterpret_cast<__half2*>(&a), bias), y = __hadd2(*reinterpret_cast<__half2*>(&b), bias);
+    lo = __byte_perm(w, 0x64646464u, 0x4140);                // 1024 + that
+    hi = __byte_perm(w, 0x64646464u, 0x4342);
+    if (kBiased) return;
+    const __half2 bias = __floats2half2_rn(-kBias, -kBias);
+    __half2 x = __hadd2(*reinterpret_cast<__half2*>(&lo), bias), y = __hadd2(*reinterpret_cast<__half2*>(&hi), bias);
     lo = *reinterpret_cast<uint32_t*>(&x);
     hi = *reinterpret_cast<uint32_t*>(&y);
   } else {
@@ -252,10 +298,8 @@ __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) 
   }
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
+__device__ __forceinline__ uint32_t word_of(const uint4& w, int x) {
+  return x == 0 ? w.x : (x == 1 ? w.y : (x == 2 ? w.z : w.w));
 }
 __device__ __forceinline__ uint32_t movm(uint32_t x) {
   uint32_t y;
@@ -275,11 +319,23 @@ __device__ __forceinline__ float quad_max(float x) {
 // 2 h) and g + 8 (head 2 h + 1) of the same query row. Column n of output tile (j, r) is dim
 // 64 j + 16 (n / 2) + 2 r + n % 2, so a thread's columns of a half j are 16 consecutive dims.
 constexpr float kNoMaxQ = -3.402823466e38f;
-constexpr float kLift = 7.f, kSlack = 15.f;                 // p = 2^(s - m), m between max - 15 and max - 7
+constexpr float kLift = 8.f, kSlack = 13.f;                 // p = 2^(s - m), m between max - 13 and max - 8
 struct RowsQ {
-  float o[2][8][4];
-  float m[2], l[2];
+  float o[2][8][4];                                         // in units of `unit`, a power of two
+  float m[2], l[2], unit, inv_unit;
+  __device__ __forceinline__ void scale(float a0, float a1) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        o[j][r][0] *= a0;
+        o[j][r][1] *= a0;
+        o[j][r][2] *= a1;
+        o[j][r][3] *= a1;
+      }
+  }
   __device__ __forceinline__ void clear() {
+    unit = inv_unit = 1.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -288,6 +344,18 @@ struct RowsQ {
         for (int e = 0; e < 4; ++e) o[j][r][e] = 0.f;
     m[0] = m[1] = kNoMaxQ;
     l[0] = l[1] = 0.f;
+  }
+  // The power of two next below `vs` as the unit; returns vs in it. Exponents are kept within
+  // [-100, 100]; a zero block keeps the unit (its codes are zero), and a NaN or infinite scale makes
+  // every value NaN whatever the unit.
+  __device__ __forceinline__ float change_unit(float vs) {
+    if (vs == 0.f) return 1.f;
+    const int e = min(max(static_cast<int>((__float_as_uint(vs) >> 23) & 0xff) - 127, -100), 100);
+    const float was = unit;
+    unit = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    inv_unit = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    scale(was * inv_unit, was * inv_unit);
+    return vs * inv_unit;
   }
   // Raises m where the new maxima need it, and rescales what was added up relative to the old.
   // Rarely: only past kSlack. The result does not depend on m.
@@ -300,46 +368,33 @@ struct RowsQ {
     m[1] = n1;
     l[0] *= a0;
     l[1] *= a1;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        o[j][r][0] *= a0;
-        o[j][r][1] *= a0;
-        o[j][r][2] *= a1;
-        o[j][r][3] *= a1;
-      }
+    scale(a0, a1);
   }
 };
 
-// 16 unquantised keys from key t0 of the item: scores, probabilities and their product with V.
-// qa: bf16 A fragments, k-step (j, w) = dims 64 j + 16 c + 4 w .. + 3. Keys are read straight
-// into B fragments: lane n reads key n's 32 bytes of each half; V is transposed 8 x 8 at a time
-// in registers.
-struct RowSource {
-  const __nv_bfloat16 *tk, *tv, *nk, *nv;                   // tail and new rows of this head
-  int tail, count;                                          // tail rows; keys in all
-};
+// Keys t0 .. t0 + 15 of a row unit (of `count`), at k and v 8 rows of 256 bytes a box: scores,
+// probabilities and their product with V. A row sees the keys below its `limit`; from `diagonal`
+// on not every row does. qa: bf16 A fragments, k-step (j, w) = dims
+// 64 j + 16 c + 4 w .. + 3. Lane n reads key n's dims straight into B fragments; V is transposed
+// 8 x 8 at a time in registers.
 __device__ __forceinline__ bool not_finite(uint32_t w) {    // either bf16 of a word
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
-__device__ __forceinline__ void row_step(RowsQ& st, const uint32_t (&qa)[32], const RowSource& src, int t0, int limit,
-                                         int diagonal, float f) {
+__device__ __forceinline__ void row_step(RowsQ& st, const uint32_t (&qa)[32], const uint8_t* k, const uint8_t* v, int t0,
+                                         int count, int limit, int diagonal, float f) {
   const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
   uint32_t kw[2][2][8], vw[2][2][8];                        // [keys 8 u + n][half][word]
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int t = t0 + 8 * u + n;
-    const bool in = t < src.count, old = t < src.tail;
-    const size_t at = static_cast<size_t>(old ? t : t - src.tail) * kRowElems + 16 * c;
-    const uint4* k = reinterpret_cast<const uint4*>((old ? src.tk : src.nk) + (in ? at : 0));
-    const uint4* v = reinterpret_cast<const uint4*>((old ? src.tv : src.nv) + (in ? at : 0));
+    const bool in = t0 + 8 * u + n < count;                 // (what lies behind the last key may be anything)
+    const uint4* kr = reinterpret_cast<const uint4*>(k + u * kRowBox + n * 256 + 32 * c);
+    const uint4* vr = reinterpret_cast<const uint4*>(v + u * kRowBox + n * 256 + 32 * c);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        const uint4 a = in ? k[8 * j + x] : zero, b = in ? v[8 * j + x] : zero;
+        const uint4 a = in ? kr[8 * j + x] : zero, b = in ? vr[8 * j + x] : zero;
         kw[u][j][4 * x] = a.x;
         kw[u][j][4 * x + 1] = a.y;
         kw[u][j][4 * x + 2] = a.z;
@@ -406,14 +461,12 @@ __device__ __forceinline__ void row_step(RowsQ& st, const uint32_t (&qa)[32], co
             vw[u][j][w] = x;
           }
 #pragma unroll 1
-      for (int t = t0; t < min(min(t0 + 16, src.count), limit); ++t) {
-        const bool old = t < src.tail;
-        const __nv_bfloat16* v = (old ? src.tv : src.nv) + static_cast<size_t>(old ? t : t - src.tail) * kRowElems + 16 * c;
+      for (int t = t0; t < min(t0 + 16, min(count, limit)); ++t) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(v + 64 * j + 2 * r);
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(v + ((t - t0) >> 3) * kRowBox + (t & 7) * 256 + 128 * j + 32 * c + 4 * r);
             const float a = (x & 0x7f80u) == 0x7f80u ? __uint_as_float(x << 16) : 0.f;
             const float b = (x & 0x7f800000u) == 0x7f800000u ? __uint_as_float(x & 0xffff0000u) : 0.f;
             st.o[j][r][0] += a;
@@ -431,101 +484,171 @@ __device__ __forceinline__ void row_step(RowsQ& st, const uint32_t (&qa)[32], co
     for (int r = 0; r < 8; ++r) mma_bf16(st.o[j][r], pa, movm(vw[0][j][r]), movm(vw[1][j][r]));
 }
 
-// A warp's ring: 4 KB stages, filled in the order K low, K high, V low, V high of page after page.
 struct RingQ {
-  uint32_t base, bars;
   int stage = 0;
-  uint32_t parity = 0;                                       // of the stage's next use
-  __device__ __forceinline__ uint32_t addr() const { return base + stage * kStageA; }
-  __device__ __forceinline__ uint32_t bar() const { return bars + 8 * stage; }
+  uint32_t phase = 0;
   __device__ __forceinline__ void next() {
     if (++stage == kStagesA) {
       stage = 0;
-      parity ^= 1;
+      phase ^= 1;
     }
   }
 };
 
+// Fetches the range's units, K and then V of each, chunk by chunk (one warp).
+__device__ __forceinline__ void quant_producer(const AttnParamsQ& p, const MapsQ& maps, const int4& range, const int4& first_a,
+                                               const int4& first_b, ChunkQ* chunks, uint32_t sbase, volatile int* abort_flag) {
+  const int lane = threadIdx.x & 31;
+  auto bar = [&](int i) { return sbase + kSmemBarsQ + 8u * i; };
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  RingQ ring;
+  int ci = range.x, cu = range.y, uses = 0;
+  bool ok = true;
+#pragma unroll 1
+  for (int k = 0; ci <= range.z && ok; ++k) {
+    ChunkQ& ck = chunks[k & 1];
+    const ItemQ it = ci == range.x ? item_of(first_a, first_b) : load_item_q(p, ci);
+    const int end = ci == range.z ? range.w : it.row_units + it.pages;
+    const int u1 = min(end, cu + kChunk), unit = cu + lane, page = unit - it.row_units;
+    UnitQ x{-1, 0, 0, 0};
+    float4 ks[2] = {}, vs[2] = {};
+    if (unit < u1) {
+      const int tail = it.ctx % kPage, tails = units_of(tail), news = it.r0 + it.rows;
+      if (page >= 0) {
+        x.a = __ldg(p.batch.table + static_cast<size_t>(it.request) * p.batch.width + page);
+        if (x.a < 0 || x.a >= p.cache.pages) {
+          x.a = -1;
+        } else {
+          const float4* sk = reinterpret_cast<const float4*>(p.cache.key_scale + static_cast<size_t>(x.a) * kKVHeads);
+          const float4* sv = reinterpret_cast<const float4*>(p.cache.value_scale + static_cast<size_t>(x.a) * kKVHeads);
+          ks[0] = __ldg(sk);
+          ks[1] = __ldg(sk + 1);
+          vs[0] = __ldg(sv);
+          vs[1] = __ldg(sv + 1);
+        }
+      } else if (unit >= tails) {
+        const int j = (unit - tails) * kRowUnit;
+        x = UnitQ{it.q0 - it.r0 + j, min(kRowUnit, news - j), j, 0};
+      } else if (it.slot >= 0 && it.slot < p.cache.slots) {
+        x = UnitQ{static_cast<int>(tail_row(it.slot, it.ctx - tail)) + unit * kRowUnit, min(kRowUnit, tail - unit * kRowUnit), -1, 0};
+      }
+      if (x.a < 0) atomicOr(&g_device_status, kStatusBadArgument);
+    }
+    if (!(ok = wait(kQChunkFree + (k & 1), ((k >> 1) & 1) ^ 1))) break;
+    ck.unit[lane] = x;
+    if (lane == 0) {
+      ck.item = it;
+      ck.u0 = cu;
+      ck.u1 = u1;
+      ck.begin = ci == range.x ? range.y : 0;
+      ck.end = end;
+    }
+    *reinterpret_cast<float4*>(&ck.ks[lane][0]) = ks[0];
+    *reinterpret_cast<float4*>(&ck.ks[lane][4]) = ks[1];
+    *reinterpret_cast<float4*>(&ck.vs[lane][0]) = vs[0];
+    *reinterpret_cast<float4*>(&ck.vs[lane][4]) = vs[1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kQChunk + (k & 1)));
+    const int num = u1 - cu, rows = it.row_units - cu;
+#pragma unroll 1
+    for (int i = 0; i < num && ok; ++i) {
+      const UnitQ y = ck.unit[i];
+      if (y.a < 0) continue;                                 // (a page that is not there is left out)
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {
+        if (!(ok = wait(kQEmpty + ring.stage, ring.phase ^ 1))) break;
+        const uint32_t dst = sbase + ring.stage * kStageA, full = bar(kQFull + ring.stage);
+        if (i >= rows) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full, kStageA);
+            bulk_load(dst, (v ? p.cache.value : p.cache.key) + static_cast<size_t>(y.a) * kPageBytes, kStageA, full);
+          }
+        } else {
+          const int boxes = (y.b + 7) >> 3;
+          const CUtensorMap* map = y.c < 0 ? (v ? &maps.tail_v : &maps.tail_k) : (v ? &maps.new_v : &maps.new_k);
+          if (lane == 0) mbar_arrive_expect_tx(full, boxes * kRowBox);
+          __syncwarp();
+          if (lane < boxes) tma_load_3d(dst + lane * kRowBox, map, 0, y.a + 8 * lane, 0, full);
+        }
+        ++uses;
+        ring.next();
+      }
+    }
+    cu = u1;
+    if (u1 == end) {
+      ++ci;
+      cu = 0;
+    }
+  }
+  // Copies in flight land before the CTA can exit (a no-op when all were consumed).
+  volatile int never = 0;
+  if (!ok)
+    for (int s = 0; s < kStagesA && s < uses; ++s) {
+      const int last_use = uses - 1 - (uses - 1 - s) % kStagesA;
+      train::wait_or_abort(bar(kQFull + s), (last_use / kStagesA) & 1, &never);
+    }
+}
+
 template <int kCode>
-__global__ void __launch_bounds__(kAttnThreadsQ, 1) quant_attn_kernel(const AttnParamsQ p) {
+__global__ void __launch_bounds__(kAttnThreadsQ, 1)
+    quant_attn_kernel(const __grid_constant__ MapsQ maps, const AttnParamsQ p) {
   extern __shared__ uint8_t smem_q[];
   const int h = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
-  const uint32_t sbase = (smem_u32(smem_q) + 1023u) & ~1023u;
-  RingQ fill, use;
-  fill.base = use.base = sbase + h * kWarpRing;
-  fill.bars = use.bars = sbase + kKVHeads * kWarpRing + h * kStagesA * 8;
-  if (lane == 0) {
-    for (int s = 0; s < kStagesA; ++s) mbar_init(use.bars + 8 * s, 1);
+  const uint32_t sraw = smem_u32(smem_q), sbase = (sraw + 1023u) & ~1023u;
+  uint8_t* smem = smem_q + (sbase - sraw);
+  ChunkQ* chunks = reinterpret_cast<ChunkQ*>(smem + kSmemChunks);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemAbortQ);
+  auto bar = [&](int i) { return sbase + kSmemBarsQ + 8u * i; };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kQBars; ++i)
+      mbar_init(bar(i), (i >= kQEmpty && i < kQChunk) || i >= kQChunkFree ? kKVHeads : 1);
+    *abort_flag = 0;
     fence_barrier_init();
   }
-  __syncwarp();
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  if (p.plan[kQMagic] != kPlanMagicQ || p.plan[kQGrid] != p.grid || p.plan[kQRequests] != p.batch.requests ||
-      p.plan[kQRows] != p.batch.rows) {
+  const int4* cta = reinterpret_cast<const int4*>(p.plan + plan_cta_at()) + 3 * blockIdx.x;
+  const int4 head = __ldg(reinterpret_cast<const int4*>(p.plan));
+  const int head_rows = __ldg(p.plan + kQRows);
+  const int4 range = __ldg(cta);
+  if (head.x != kPlanMagicQ || head.y != p.grid || head.w != p.batch.requests || head_rows != p.batch.rows) {
     if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
     return;
   }
-  const int4 range = __ldg(reinterpret_cast<const int4*>(p.plan + plan_cta_at()) + blockIdx.x);
-  const uint8_t* key = p.cache.key + static_cast<size_t>(h) * kHeadBytes;
-  const uint8_t* value = p.cache.value + static_cast<size_t>(h) * kHeadBytes;
-  bool alive = true;                                         // no wait ran out
+  // A head warp holds O (64), Q (32) and the scores (32) of its rows: with the 168 registers of a
+  // launch of 9 warps it spilled.
+  if (h >= kKVHeads) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
+    if (h == kKVHeads) quant_producer(p, maps, range, __ldg(cta + 1), __ldg(cta + 2), chunks, sbase, abort_flag);
+    return;
+  }
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHeadRegs));
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  RingQ ring;
+  const uint8_t* base = smem + h * kHeadBytes;
+  auto release = [&]() {                                     // every lane has read the stage
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kQEmpty + ring.stage));
+    ring.next();
+  };
+  const uint32_t k_at = (16 * (n >> 1) + (n & 1)) * 64 + 16 * c;
   RowsQ st;
+  uint32_t qa[32];
+  float f[2] = {0.f, 0.f}, start[2] = {0.f, 0.f};            // scores: scale and first value of the sum
+  bool halves = false, ok = true;                            // halves: qa holds halves
 #pragma unroll 1
-  for (int idx = range.x; idx <= range.z && alive; ++idx) {
-    const ItemQ it = load_item_q(p, idx);
-    const Request req = load_request(p.batch, p.cache, it.request);
-    const int units = it.row_units + it.pages;
-    const int ub = idx == range.x ? range.y : 0, ue = idx == range.z ? range.w : units;
-    // what a stale plan says of another batch is not followed
-    if (!req.ok || it.pages != req.ctx / kPage || it.q0 != req.q0 + it.r0 || it.r0 + it.rows > req.q_len ||
-        it.row_units != row_units(req.ctx, req.q_len, it.r0)) {
-      if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
-      continue;
-    }
-    // pages [pb, pe) of the request; lane l knows the id of page chunk + l
-    const int pb = max(ub - it.row_units, 0), pe = max(ue - it.row_units, 0);
-    int chunk = pb, id = -1;
-    float ks = 0.f, vs = 0.f;
-    auto load_ids = [&](int first) {
-      chunk = first;
-      id = first + lane < pe ? __ldg(req.table + first + lane) : 0;
-      const bool good = id >= 0 && id < p.cache.pages;
-      if (!good) {
-        atomicOr(&g_device_status, kStatusBadArgument);
-        id = -1;
-      }
-      const size_t at = static_cast<size_t>(good ? id : 0) * kKVHeads + h;
-      ks = good ? __ldg(p.cache.key_scale + at) : 0.f;
-      vs = good ? __ldg(p.cache.value_scale + at) : 0.f;
-    };
-    // copies of the stages are issued one by one: piece x of page fp
-    int fp = pb, piece = 0, ahead = 0;                       // ahead: stages filled and not yet used
-    auto fill_one = [&]() {
-      const int pid = __shfl_sync(0xffffffffu, id, fp - chunk);
-      if (pid >= 0) {
-        if (lane == 0) {
-          mbar_arrive_expect_tx(fill.bar(), kStageA);
-          bulk_load(fill.addr(), (piece < 2 ? key : value) + static_cast<size_t>(pid) * kPageBytes + (piece & 1) * kStageA,
-                    kStageA, fill.bar());
-        }
-        fill.next();
-        ++ahead;
-      } else {
-        piece = 3;                                           // (a page that is not there is left out)
-      }
-      if (++piece == 4) {
-        piece = 0;
-        ++fp;
-      }
-    };
-    if (pb < pe) {
-      load_ids(pb);
-      while (ahead < kStagesA && fp < min(pe, chunk + 32)) fill_one();
-    }
-    // Q: k-step (j, w) of row n holds dims 64 j + 16 c + 4 w .. + 3, words 2 w and 2 w + 1
-    uint32_t qa[32];
-    {
-      const __nv_bfloat16* q = p.q + (static_cast<size_t>(it.q0 + min(n, it.rows - 1)) * kQHeads + 2 * h) * kHeadDim + 16 * c;
+  for (int idx = range.x, k = 0; idx <= range.z; ++k) {
+    if (!(ok = wait(kQChunk + (k & 1), (k >> 1) & 1))) break;
+    const ChunkQ& ck = chunks[k & 1];
+    const int u0 = ck.u0, num = ck.u1 - u0, row_units = ck.item.row_units, rows = min(num, row_units - u0);
+    if (u0 == ck.begin) {
+      // Q: k-step (j, w) of row n holds dims 64 j + 16 c + 4 w .. + 3, words 2 w and 2 w + 1
+      const __nv_bfloat16* q = p.q + (static_cast<size_t>(ck.item.q0 + min(n, ck.item.rows - 1)) * kQHeads + 2 * h) * kHeadDim + 16 * c;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -538,215 +661,247 @@ __global__ void __launch_bounds__(kAttnThreadsQ, 1) quant_attn_kernel(const Attn
             qa[16 * j + 8 * y + 4 + x] = w.z;
             qa[16 * j + 8 * y + 6 + x] = w.w;
           }
+      st.clear();
+      halves = false;
     }
-    st.clear();
-    if (ub < it.row_units) {
-      const int tail = req.ctx % kPage;
-      const size_t tail_at = tail_row(req.slot, req.ctx - tail) * kRowElems + h * kHeadDim;
-      const size_t new_at = static_cast<size_t>(req.q0) * kRowElems + h * kHeadDim;
-      const RowSource src{static_cast<const __nv_bfloat16*>(p.cache.tail_key) + tail_at,
-                          static_cast<const __nv_bfloat16*>(p.cache.tail_value) + tail_at, p.new_k + new_at,
-                          p.new_v + new_at, tail, tail + it.r0 + it.rows};
-      const int end = min(min(ue, it.row_units) * kRowUnit, src.count);
-      const int diagonal = tail + it.r0 + 1;                 // keys from here on are not seen by every row
+    int unit = 0;
 #pragma unroll 1
-      for (int t = ub * kRowUnit; t < end; t += 16)
-        row_step(st, qa, src, t, diagonal + n, diagonal, p.scale_log2);
+    for (; unit < rows; ++unit) {
+      const UnitQ x = ck.unit[unit];
+      if (x.a < 0) continue;
+      const int see = x.c < 0 ? kPage : ck.item.r0 + 1 - x.c;     // keys that row 0 sees: all open ones
+      const RingQ kr = ring;
+      ring.next();
+      if (!(ok = wait(kQFull + kr.stage, kr.phase)) || !(ok = wait(kQFull + ring.stage, ring.phase))) break;
+      // a box of 8 rows holds them head by head
+      const uint8_t* kb = smem + kr.stage * kStageA + h * 2048;
+      const uint8_t* vb = smem + ring.stage * kStageA + h * 2048;
+#pragma unroll 1
+      for (int t0 = 0; t0 < x.b; t0 += 16)
+        row_step(st, qa, kb + (t0 >> 3) * kRowBox, vb + (t0 >> 3) * kRowBox, t0, x.b, min(see + n, x.b), see, p.scale_log2);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kQEmpty + kr.stage));
+      release();
     }
-    if (pb < pe) {
-      // Q to halves: rows n and n + 8, each times 2^(14 - e)
-      float f[2];
+    if (!ok) break;
+    if (unit < num) {
+      if (!halves) {
+        // Q to halves: rows n and n + 8, each times 2^(14 - e)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        uint32_t top = 0;
+        for (int x = 0; x < 2; ++x) {
+          uint32_t top = 0;
 #pragma unroll
-        for (int i = x; i < 32; i += 2) top = max(top, max(qa[i] & 0x7fffu, (qa[i] >> 16) & 0x7fffu));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 120);
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-        f[x] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+          for (int i = x; i < 32; i += 2) top = max(top, max(qa[i] & 0x7fffu, (qa[i] >> 16) & 0x7fffu));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 120);
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+          f[x] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+          float sum = 0.f;
 #pragma unroll
-        for (int i = x; i < 32; i += 2)
-          qa[i] = pack_f16x2(__uint_as_float(qa[i] << 16) * up, __uint_as_float(qa[i] & 0xffff0000u) * up);
+          for (int i = x; i < 32; i += 2) {
+            qa[i] = pack_f16x2(__uint_as_float(qa[i] << 16) * up, __uint_as_float(qa[i] & 0xffff0000u) * up);
+            const float2 q2 = __half22float2(*reinterpret_cast<const __half2*>(&qa[i]));
+            sum += q2.x + q2.y;
+          }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          start[x] = kCode == kInt8 ? -kBias * sum : 0.f;
+        }
+        halves = true;
       }
 #pragma unroll 1
-      for (int page = pb; page < pe && alive; ++page) {
-        if (page - chunk == 32) {
-          load_ids(page);
-          fp = page;                                         // (a chunk's stages are all used: none is ahead)
-          while (ahead < kStagesA && fp < min(pe, chunk + 32)) fill_one();
-        }
-        if (__shfl_sync(0xffffffffu, id, page - chunk) < 0) continue;
-        const float pks = __shfl_sync(0xffffffffu, ks, page - chunk), pvs = __shfl_sync(0xffffffffu, vs, page - chunk);
-        const int stop = min(pe, chunk + 32);
-        auto wait = [&]() {
-          alive = __all_sync(0xffffffffu, mbar_wait(use.bar(), use.parity)) != 0;
-          return alive;
-        };
-        auto release = [&]() {                               // every lane has read the stage
-          use.next();
-          --ahead;
-          __syncwarp();
-          if (fp < stop) fill_one();
-        };
+      for (; unit < num; ++unit) {
+        if (ck.unit[unit].a < 0) continue;
+        const float pks = ck.ks[unit][h], pvs = ck.vs[unit][h];
+        // p = 2^(s f - m) r with r = vs / unit, so that the product with the codes of V adds straight
+        // to O; r stays within [1 / 8, 4] (or O changes its unit), which p's range has room for.
+        float f0 = f[0] * pks, f1 = f[1] * pks, r = pvs * st.inv_unit;
+        if (!(r >= 0.125f && r <= 4.f)) r = st.change_unit(pvs);
+        const float lr = __log2f(r), ir = __frcp_rn(r);
         float s[8][4];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+        for (int u = 0; u < 8; ++u) {
+          s[u][0] = s[u][1] = start[0];
+          s[u][2] = s[u][3] = start[1];
+        }
         // S: column n of tile u = 2 t + x is key 16 (n / 2) + 4 t + 2 x + n % 2
-        const uint32_t k_at = (16 * (n >> 1) + (n & 1)) * 64 + 16 * c;
+        if (!(ok = wait(kQFull + ring.stage, ring.phase))) break;
+        const uint8_t* k_stage = base + ring.stage * kStageA + k_at;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if (!wait()) break;
-          const uint32_t at = use.addr() + k_at;
+          const uint8_t* at = k_stage + j * (kHeadBytes / 2);
+          // four tiles take turns: the products of one depend on each other
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const uint4 w = lds128(at + 2 * u * 64);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          for (int g = 0; g < 8; g += 4) {
+            uint4 w[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint32_t b0, b1;
-              decode4<kCode>(ww[x], b0, b1);
-              mma_f16(s[u], *reinterpret_cast<const uint32_t(*)[4]>(&qa[16 * j + 4 * x]), b0, b1);
-            }
+            for (int u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const uint4*>(at + 2 * (g + u) * 64);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                uint32_t b0, b1;
+                decode4<kCode, true>(word_of(w[u], x), b0, b1);
+                mma_f16(s[g + u], *reinterpret_cast<const uint32_t(*)[4]>(&qa[16 * j + 4 * x]), b0, b1);
+              }
           }
-          release();
         }
-        if (!alive) break;
-        const float f0 = f[0] * pks, f1 = f[1] * pks;
-        float m0 = -INFINITY, m1 = -INFINITY;
+        release();
+        float mx[2][4];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          s[u][0] *= f0;
-          s[u][1] *= f0;
-          s[u][2] *= f1;
-          s[u][3] *= f1;
-          m0 = fmaxf(m0, fmaxf(s[u][0], s[u][1]));
-          m1 = fmaxf(m1, fmaxf(s[u][2], s[u][3]));
+          const float a = fmaxf(s[u][0], s[u][1]), b = fmaxf(s[u][2], s[u][3]);
+          mx[0][u & 3] = u < 4 ? a : fmaxf(mx[0][u & 3], a);
+          mx[1][u & 3] = u < 4 ? b : fmaxf(mx[1][u & 3], b);
         }
-        st.raise(quad_max(m0), quad_max(m1));
+        st.raise(quad_max(fmaxf(fmaxf(mx[0][0], mx[0][1]), fmaxf(mx[0][2], mx[0][3]))) * f0,
+                 quad_max(fmaxf(fmaxf(mx[1][0], mx[1][1]), fmaxf(mx[1][2], mx[1][3]))) * f1);
+        float base0 = lr - st.m[0], base1 = lr - st.m[1];
+        // One fma a score, whose sum lr - m is off by 2^-24 |m|. Scores of thousands are scaled and
+        // shifted first, one by one, so that the largest keeps its place whatever its size.
+        if (__any_sync(0xffffffffu, fabsf(st.m[0]) > 1024.f || fabsf(st.m[1]) > 1024.f)) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u][e] = __fsub_rn(__fmul_rn(s[u][e], e < 2 ? f0 : f1), st.m[e >> 1]);
+          f0 = f1 = 1.f;
+          base0 = base1 = lr;
+        }
         uint32_t pa[4][4];
+        float sum[2][4];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[u][e] = ex2(s[u][e] - st.m[e >> 1]);
-            st.l[e >> 1] += s[u][e];
-          }
+          s[u][0] = ex2(fmaf(s[u][0], f0, base0));
+          s[u][1] = ex2(fmaf(s[u][1], f0, base0));
+          s[u][2] = ex2(fmaf(s[u][2], f1, base1));
+          s[u][3] = ex2(fmaf(s[u][3], f1, base1));
+          const float a = s[u][0] + s[u][1], b = s[u][2] + s[u][3];
+          sum[0][u & 3] = u < 4 ? a : sum[0][u & 3] + a;
+          sum[1][u & 3] = u < 4 ? b : sum[1][u & 3] + b;
           pa[u >> 1][2 * (u & 1)] = pack_f16x2(s[u][0], s[u][1]);
           pa[u >> 1][2 * (u & 1) + 1] = pack_f16x2(s[u][2], s[u][3]);
         }
+        st.l[0] = fmaf((sum[0][0] + sum[0][1]) + (sum[0][2] + sum[0][3]), ir, st.l[0]);
+        st.l[1] = fmaf((sum[1][0] + sum[1][1]) + (sum[1][2] + sum[1][3]), ir, st.l[1]);
         // O: column n of tile (j, r) is dim 64 j + 16 (n / 2) + 2 r + n % 2
+        if (!(ok = wait(kQFull + ring.stage, ring.phase))) break;
+        const uint8_t* v_stage = base + ring.stage * kStageA + k_at;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if (!wait()) break;
-          const uint32_t at = use.addr() + k_at;
+          const uint8_t* at = v_stage + j * (kHeadBytes / 2);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const uint4 w = lds128(at + 2 * r * 64);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-            float t[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int g = 0; g < 8; g += 4) {
+            uint4 w[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint32_t b0, b1;
-              decode4<kCode>(ww[x], b0, b1);
-              mma_f16(t, pa[x], b0, b1);
-            }
+            for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(at + 2 * (g + i) * 64);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[j][r][e] = fmaf(t[e], pvs, st.o[j][r][e]);
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t b0, b1;
+                decode4<kCode, false>(word_of(w[i], x), b0, b1);
+                mma_f16(st.o[j][g + i], pa[x], b0, b1);
+              }
           }
-          release();
         }
+        release();
       }
-      if (!alive) break;
     }
-    float l0 = st.l[0], l1 = st.l[1];
+    if (!ok) break;
+    if (ck.u1 == ck.end) {                                   // the range's last unit of the item
+      float l0 = st.l[0], l1 = st.l[1];
 #pragma unroll
-    for (int x = 1; x < 4; x <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-    }
-    if (ub > 0 || ue < units) {
-      float* part = p.part + part_index(blockIdx.x, idx == range.x ? 0 : 1, h);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            __stcg(reinterpret_cast<float4*>(part + (n + 8 * x) * kHeadDim + 64 * j + 16 * c + 4 * r),
-                   make_float4(st.o[j][2 * r][2 * x], st.o[j][2 * r][2 * x + 1], st.o[j][2 * r + 1][2 * x],
-                               st.o[j][2 * r + 1][2 * x + 1]));
-        if (c == 0)
-          __stcg(reinterpret_cast<float2*>(part + 16 * kHeadDim) + n + 8 * x, make_float2(st.m[x], x ? l1 : l0));
+      for (int x = 1; x < 4; x <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, x);
       }
-    } else if (n < it.rows) {
+      if (ck.begin > 0 || ck.end < row_units + ck.item.pages) {
+        float* part = p.part + part_index(blockIdx.x, idx == range.x ? 0 : 1, h);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float inv = 1.f / (x ? l1 : l0);
-        __nv_bfloat16* out = p.out + (static_cast<size_t>(it.q0 + n) * kQHeads + 2 * h + x) * kHeadDim + 16 * c;
+        for (int x = 0; x < 2; ++x) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            uint32_t w[4];
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              w[r] = pack_bf16x2(st.o[j][4 * y + r][2 * x] * inv, st.o[j][4 * y + r][2 * x + 1] * inv);
-            *reinterpret_cast<uint4*>(out + 64 * j + 8 * y) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+              __stcg(reinterpret_cast<float4*>(part + (n + 8 * x) * kHeadDim + 64 * j + 16 * c + 4 * r),
+                     make_float4(st.o[j][2 * r][2 * x] * st.unit, st.o[j][2 * r][2 * x + 1] * st.unit,
+                                 st.o[j][2 * r + 1][2 * x] * st.unit, st.o[j][2 * r + 1][2 * x + 1] * st.unit));
+          if (c == 0)
+            __stcg(reinterpret_cast<float2*>(part + 16 * kHeadDim) + n + 8 * x, make_float2(st.m[x], x ? l1 : l0));
+        }
+      } else if (n < ck.item.rows) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float inv = st.unit / (x ? l1 : l0);
+          __nv_bfloat16* out = p.out + (static_cast<size_t>(ck.item.q0 + n) * kQHeads + 2 * h + x) * kHeadDim + 16 * c;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              uint32_t w[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                w[r] = pack_bf16x2(st.o[j][4 * y + r][2 * x] * inv, st.o[j][4 * y + r][2 * x + 1] * inv);
+              *reinterpret_cast<uint4*>(out + 64 * j + 8 * y) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
       }
+      ++idx;
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kQChunkFree + (k & 1)));
   }
-  if (!alive) {                                              // copies in flight land before the CTA exits
-    for (int s = 0; s < kStagesA; ++s)
-      if (use.stage != fill.stage || use.parity != fill.parity) {
-        mbar_wait(use.bar(), use.parity);
-        use.next();
-      }
-  }
+  if (!ok) *abort_flag = 1;
 }
 
-// Grid (CTAs, 8): CTA (c, h) merges head h of the cut item whose first contributor is c.
-// Thread (row, part) = (tid / 8, tid % 8) holds dims 16 part .. + 15 of a row.
-__global__ void __launch_bounds__(128) quant_merge_kernel(const AttnParamsQ p) {
+// Grid (CTAs, 8), 256 threads: CTA (c, h) merges head h of the cut item whose first contributor
+// is c. Warp w takes rows w and w + 8 (the same query row); lane l holds dims 4 l .. 4 l + 3 and
+// the weights of contributors l, l + 32, ..
+__global__ void __launch_bounds__(256) quant_merge_kernel(const AttnParamsQ p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c0 = blockIdx.x, h = blockIdx.y, row = threadIdx.x >> 3, d0 = 16 * (threadIdx.x & 7);
-  if (p.plan[kQMagic] != kPlanMagicQ || p.plan[kQGrid] != p.grid) return;
+  const int c0 = blockIdx.x, h = blockIdx.y, r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 head = __ldg(reinterpret_cast<const int4*>(p.plan));
   const int4 merge = __ldg(reinterpret_cast<const int4*>(p.plan + plan_merge_at(p.grid)) + c0);
-  if (merge.x < 0 || merge.x >= p.plan[kQItems] || merge.y <= c0 || merge.y >= p.grid) return;
+  if (head.x != kPlanMagicQ || head.y != p.grid || merge.x < 0 || merge.x >= head.z || merge.y <= c0 || merge.y >= p.grid)
+    return;
+  const int parts = merge.y - c0 + 1;
+  auto at = [&](int k) { return p.part + part_index(c0 + k, k == 0 ? (merge.z & 1) : 0, h); };
   const ItemQ it = load_item_q(p, merge.x);
-  const int x = row >> 3, r = row & 7;
   if (r >= it.rows || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return;
-  auto at = [&](int k) { return p.part + part_index(k, k == c0 ? (merge.z & 1) : 0, h); };
-  auto stat = [&](int k) { return __ldcg(reinterpret_cast<const float2*>(at(k) + 16 * kHeadDim) + row); };
-  float m = kNoMaxQ;
-  for (int k = c0; k <= merge.y; ++k) m = fmaxf(m, stat(k).x);
-  float l = 0.f, o[16];
+#pragma unroll 1
+  for (int x = 0; x < 2; ++x) {
+    const int row = r + 8 * x;
+    float m = kNoMaxQ;
+    for (int k = lane; k < parts; k += 32) m = fmaxf(m, __ldcg(reinterpret_cast<const float2*>(at(k) + 16 * kHeadDim) + row).x);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = 0.f;
-#pragma unroll 2
-  for (int k = c0; k <= merge.y; ++k) {
-    const float2 ml = stat(k);
-    const float w = ex2(ml.x - m);
-    l = fmaf(ml.y, w, l);
-    const float4* src = reinterpret_cast<const float4*>(at(k) + row * kHeadDim + d0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 v = __ldcg(src + i);
-      o[4 * i] = fmaf(v.x, w, o[4 * i]);
-      o[4 * i + 1] = fmaf(v.y, w, o[4 * i + 1]);
-      o[4 * i + 2] = fmaf(v.z, w, o[4 * i + 2]);
-      o[4 * i + 3] = fmaf(v.w, w, o[4 * i + 3]);
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      float w = 0.f;
+      if (k0 + lane < parts) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(at(k0 + lane) + 16 * kHeadDim) + row);
+        w = ex2(ml.x - m);
+        l = fmaf(ml.y, w, l);
+      }
+      const int stop = min(32, parts - k0);
+#pragma unroll 8
+      for (int k = 0; k < stop; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, k);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(at(k0 + k) + row * kHeadDim) + lane);
+        o[0] = fmaf(v.x, wk, o[0]);
+        o[1] = fmaf(v.y, wk, o[1]);
+        o[2] = fmaf(v.z, wk, o[2]);
+        o[3] = fmaf(v.w, wk, o[3]);
+      }
     }
-  }
-  const float inv = 1.f / l;
-  uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
-  uint4* out = reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(it.q0 + r) * kQHeads + 2 * h + x) * kHeadDim + d0);
-  out[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  out[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    const float inv = 1.f / l;
+    reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(it.q0 + r) * kQHeads + 2 * h + x) * kHeadDim)[lane] =
+        make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+  }
 }
 
 }  // namespace quant

@@ -37,7 +37,7 @@ def _int_list(values, what, low, high):
     return out
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class QuantizedLayout:
     """A batch over the cache: ``query_lengths[i]`` new rows of request i behind
     ``context_lengths[i]`` tokens, its pages in row i of ``table`` and its open rows in
@@ -94,6 +94,10 @@ class QuantizedLayout:
             elif plan.dtype != torch.int32 or plan.device != device or not plan.is_contiguous() or plan.numel() < words:
                 raise ValueError(f'plan must be a contiguous int32 tensor of at least {words} words on the device')
         out = cls(q, context_lengths, cu_query, context, table, slots, plan, total, max(q))
+        object.__setattr__(out, '_struct', _lib.QuantBatch(
+            cu_query.data_ptr(), context.data_ptr(), table.data_ptr(), slots.data_ptr(), r, total, out.max_query,
+            table.shape[1]))
+        object.__setattr__(out, '_address', ctypes.addressof(out._struct))
         if replan:
             out.replan()
         return out
@@ -101,9 +105,8 @@ class QuantizedLayout:
     def replan(self):
         device = self.plan.device
         with _on_device(device):
-            _lib.check(_lib.load_library().dspark_quant_plan(
-                self.cu_query.data_ptr(), self.context.data_ptr(), len(self.query_lengths), self.query_tokens,
-                self.table.shape[1], self.plan.data_ptr(), self.plan.numel(), _stream(device)), 'dspark_quant_plan')
+            _lib.check(_lib.load_library().dspark_quant_plan(self._address, self.plan.data_ptr(), self.plan.numel(),
+                                                             _stream(device)), 'dspark_quant_plan')
 
 
 def plan_words(device, requests, rows):
@@ -114,6 +117,14 @@ def plan_words(device, requests, rows):
 
 
 _workspace_bytes = {}
+
+
+def workspace_bytes(device):
+    size = ctypes.c_size_t(0)
+    _lib.check(_lib.load_library().dspark_quant_workspace_size(device.index, ctypes.byref(size)),
+               'dspark_quant_workspace_size')
+    _workspace_bytes[device.index] = size.value
+    return size.value
 
 
 class QuantizedPages:
@@ -151,7 +162,10 @@ class QuantizedPages:
         self.layers, self.pages, self.slots = layers, pages, slots
         self.device, self.dtype, self.row_dtype = key.device, key.dtype, tail_key.dtype
         self.runtime = runtime_identity(self.device)
-        self._code, self.qmax = _CODES[key.dtype]
+        code, self.qmax = _CODES[key.dtype]
+        self._struct = _lib.QuantCache(*(t.data_ptr() for t in tensors), layers, pages, slots, code,
+                                       _DTYPES[self.row_dtype])
+        self._address = ctypes.addressof(self._struct)
         self.users = [0] * pages             # requests that hold each page (host)
         self._free = list(range(pages))      # min-heap
 
@@ -206,10 +220,6 @@ class QuantizedPages:
                 heapq.heappush(self._free, x)
 
     # -- device work --------------------------------------------------------------------
-    def _pointers(self, layer=0):
-        return tuple(t[layer].data_ptr() for t in (self.key, self.value, self.key_scale, self.value_scale,
-                                                   self.tail_key, self.tail_value))
-
     def _layout(self, layout):
         if not isinstance(layout, QuantizedLayout) or layout.table.device != self.device:
             raise ValueError('A QuantizedLayout on the cache\'s device is required')
@@ -236,11 +246,8 @@ class QuantizedPages:
             raise ValueError('counts must be contiguous int32 [requests] on the device')
         with _on_device(self.device):
             _lib.check(_lib.load_library().dspark_quant_append(
-                key.data_ptr(), value.data_ptr(), key.shape[1], *self._pointers(), self.layers, self.pages, self.slots,
-                self._code, layout.cu_query.data_ptr(), layout.context.data_ptr(), layout.table.data_ptr(),
-                layout.table.shape[1], layout.slots.data_ptr(), None if counts is None else counts.data_ptr(),
-                len(layout.query_lengths), layout.query_tokens, layout.max_query, _DTYPES[self.row_dtype],
-                _stream(self.device)), 'dspark_quant_append')
+                key.data_ptr(), value.data_ptr(), key.shape[1], self._address, layout._address,
+                None if counts is None else counts.data_ptr(), _stream(self.device)), 'dspark_quant_append')
 
     def _index(self, values, limit, what, distinct=False):
         if isinstance(values, torch.Tensor):
@@ -272,9 +279,8 @@ class QuantizedPages:
         tn = self._index(tail_lengths, 2 ** 30, 'tail_lengths')
         with _on_device(self.device):
             _lib.check(_lib.load_library().dspark_quant_copy(
-                *self._pointers(), self.layers, self.pages, self.slots, _DTYPES[self.row_dtype], s.data_ptr(),
-                d.data_ptr(), s.numel(), ts.data_ptr(), td.data_ptr(), tn.data_ptr(), ts.numel(), _stream(self.device)),
-                'dspark_quant_copy')
+                self._address, s.data_ptr(), d.data_ptr(), s.numel(), ts.data_ptr(), td.data_ptr(), tn.data_ptr(),
+                ts.numel(), _stream(self.device)), 'dspark_quant_copy')
 
     @torch.no_grad()
     def values(self, ids):
@@ -326,11 +332,12 @@ class B200QuantizedKernel:
             raise ValueError('B200 quantized attention requires QuantizedPages on its GPU')
         pages._layout(layout)
         dtype, n = pages.row_dtype, layout.query_tokens
-        for t, heads in ((query, HQ), (key, HKV), (value, HKV)) + (((out, HQ),) if out is not None else ()):
+        rows, kv = (n, HQ, HEAD_DIM), (n, HKV, HEAD_DIM)
+        for t, shape in ((query, rows), (key, kv), (value, kv)) + (((out, rows),) if out is not None else ()):
             if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or t.requires_grad
-                    or t.ndim != 3 or not t.is_contiguous()):
+                    or not t.is_contiguous()):
                 raise ValueError(f'B200 quantized attention requires no-autograd contiguous {dtype} THD tensors on its GPU')
-            if tuple(t.shape) != (n, heads, HEAD_DIM):
+            if t.shape != shape:
                 raise ValueError('Rows must match the layout, with Hq16/Hkv8/D128 heads')
         if not isinstance(scale, (float, int)) or not math.isfinite(scale) or scale != SCALE:
             raise ValueError('B200 quantized attention requires the 1/sqrt(128) scale')
@@ -341,20 +348,12 @@ class B200QuantizedKernel:
                 out = torch.empty_like(query)
             if n == 0:
                 return out
-            lib = _lib.load_library()
             ws, nbytes = None, 0
             if dtype == torch.bfloat16:
-                nbytes = _workspace_bytes.get(device.index)
-                if nbytes is None:
-                    size = ctypes.c_size_t(0)
-                    _lib.check(lib.dspark_quant_workspace_size(device.index, ctypes.byref(size)),
-                               'dspark_quant_workspace_size')
-                    nbytes = _workspace_bytes[device.index] = size.value
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            _lib.check(lib.dspark_quant_attn(
-                query.data_ptr(), n, key.data_ptr(), value.data_ptr(), *pages._pointers(layer), pages.pages, pages.slots,
-                pages._code, layout.cu_query.data_ptr(), layout.context.data_ptr(), layout.table.data_ptr(),
-                layout.table.shape[1], layout.slots.data_ptr(), len(layout.query_lengths), layout.max_query,
-                layout.plan.data_ptr(), float(scale), _DTYPES[dtype], out.data_ptr(),
-                None if ws is None else ws.data_ptr(), nbytes, _stream(device)), 'dspark_quant_attn')
+                nbytes = _workspace_bytes.get(device.index) or workspace_bytes(device)
+                ws = query.new_empty(nbytes // 2)
+            _lib.check(_lib.load_library().dspark_quant_attn(
+                query.data_ptr(), key.data_ptr(), value.data_ptr(), pages._address, layer, layout._address,
+                layout.plan.data_ptr(), scale, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                _stream(device)), 'dspark_quant_attn')
         return out
