@@ -513,20 +513,6 @@ int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, 
   return launch_status();
 }
 
-// K or V rows [rows, 8, 128] bf16 as dims (d, row, head): a box of 8 rows lands head by head.
-int encode_unit_map(CUtensorMap* m, const void* base, long long rows) {
-  if (rows < 1 || rows >= (1ll << 31)) return DSPARK_ERR_INVALID_ARGUMENT;
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(kHeadDim), static_cast<cuuint64_t>(rows),
-                        static_cast<cuuint64_t>(kKVHeads)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(kKVHeads * kHeadDim * 2), static_cast<cuuint64_t>(kHeadDim * 2)};
-  cuuint32_t box[3] = {static_cast<cuuint32_t>(kHeadDim), 8, static_cast<cuuint32_t>(kKVHeads)};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? DSPARK_OK : DSPARK_ERR_CUDA;
-}
-
 template <typename T>
 int launch_append(const quant::AppendParams& ap, int code, cudaStream_t stream) {
   const dim3 grid(ap.batch.requests * ap.blocks, ap.layers, 4);
@@ -1572,16 +1558,9 @@ int dspark_quant_attn(const void* q, const void* new_k, const void* new_v, const
   const quant::AttnParamsQ ap{static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(new_k),
                               static_cast<const __nv_bfloat16*>(new_v), static_cast<__nv_bfloat16*>(out), c, b, plan, sms,
                               scale * 1.4426950408889634f, static_cast<float*>(workspace)};
-  quant::MapsQ maps;
-  const long long tail_rows = static_cast<long long>(c.slots) * 2 * quant::kPage;
-  if ((st = encode_unit_map(&maps.tail_k, c.tail_key, tail_rows)) != DSPARK_OK ||
-      (st = encode_unit_map(&maps.tail_v, c.tail_value, tail_rows)) != DSPARK_OK ||
-      (st = encode_unit_map(&maps.new_k, new_k, b.rows)) != DSPARK_OK ||
-      (st = encode_unit_map(&maps.new_v, new_v, b.rows)) != DSPARK_OK)
-    return st;
   st = launch_dependent(cache->code == DSPARK_CODE_INT8 ? quant::quant_attn_kernel<quant::kInt8>
                                                         : quant::quant_attn_kernel<quant::kE4M3>,
-                        dim3(sms), quant::kAttnThreadsQ, quant::kAttnSmemQ, stream, maps, ap);
+                        dim3(sms), quant::kAttnThreadsQ, quant::kAttnSmemQ, stream, ap);
   if (st != DSPARK_OK) return st;
   return launch_dependent(quant::quant_merge_kernel, dim3(sms, kKVHeads), 256, 0, stream, ap);
 }

@@ -67,18 +67,19 @@ __device__ __forceinline__ size_t tail_row(int slot, int token) {
   return (static_cast<size_t>(slot) * 2 + ((token / kPage) & 1)) * kPage + (token & (kPage - 1));
 }
 
-// Two e4m3 codes (the low one first) as two halves; every e4m3 value is a half.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  uint32_t h;
-  asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(h) : "r"(two));
-  return h;
+// Four e4m3 codes of a word as two pairs of halves; every e4m3 value is a half.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 p, q;\n\tmov.b32 {p, q}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, p;\n\tcvt.rn.f16x2.e4m3x2 %1, q;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 template <int kCode>
 __device__ __forceinline__ float2 decode2(uint32_t two) {
   if (kCode == kInt8)
     return make_float2(static_cast<float>(static_cast<int8_t>(two & 0xff)),
                        static_cast<float>(static_cast<int8_t>((two >> 8) & 0xff)));
-  const uint32_t h = e4m3x2_to_f16x2(two & 0xffffu);
+  uint32_t h, unused;
+  e4m3x4_to_f16x4(two, h, unused);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 

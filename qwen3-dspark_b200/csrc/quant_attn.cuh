@@ -10,8 +10,8 @@
 // same key). Its keys are cut into units of at most 16 KB a head: 32 open rows, 32 new rows or one
 // page, in this order. A plan (one small launch per batch, reused by every layer) numbers the units of
 // all items and gives every CTA an equal contiguous range; warp h of a CTA computes KV head h
-// of its range. A ninth warp fetches the units, K or V of all heads as one bulk copy of 64 KB (rows:
-// TMA boxes of 8), into a ring of 3 stages, across items. Items cut by ranges leave fp32 partial
+// of its range. A ninth warp fetches the units, K or V of all heads as one bulk copy of up to 64 KB, into
+// a ring of 3 stages, across items. Items cut by ranges leave fp32 partial
 // rows that a dependent launch merges.
 //
 // Codes become halves in registers, exactly: e4m3 by one conversion, int8 as the byte under the
@@ -36,7 +36,7 @@ constexpr int kAttnThreadsQ = 12 * 32;                      // 8 warps of heads,
 // (kAttnThreadsQ x the kernel's count, checked when the device is set up) cover them.
 constexpr int kHeadRegs = 216, kFetchRegs = 72;
 constexpr int kRowUnit = 32;                                // unquantised keys of a unit
-constexpr int kRowBox = 8 * kRowElems * 2;                  // bytes of 8 of them, all heads
+constexpr int kRowBytes = kRowElems * 2;                    // a key's bytes, all heads
 constexpr int kChunk = 32;                                  // units whose ids and scales a warp holds at a time
 
 // ---------------------------------------------------------------------------
@@ -57,7 +57,7 @@ __host__ __device__ inline long long plan_words(int grid, long long requests, lo
 }
 
 // Units' worth of a new item (its queries, a partial row) and the least range of a CTA.
-constexpr int kItemCost = 1, kMinUnits = 2;
+constexpr int kItemCost = 0, kMinUnits = 1;
 
 struct PlanParams {
   const int* cu_q;
@@ -265,9 +265,6 @@ constexpr uint32_t kSmemChunks = kStagesA * kStageA;
 constexpr uint32_t kSmemBarsQ = kSmemChunks + 2 * sizeof(ChunkQ);
 constexpr uint32_t kSmemAbortQ = kSmemBarsQ + kQBars * 8;
 constexpr size_t kAttnSmemQ = 1024 + kSmemAbortQ + 4;
-struct MapsQ {
-  CUtensorMap tail_k, tail_v, new_k, new_v;                 // boxes of 8 rows of every head, head by head
-};
 
 // D(16x8 f32) += A(16x16 f16, row) * B(16x8 f16, col). Not volatile: the compiler moves the next
 // tile's loads and conversions between the products of this one.
@@ -293,8 +290,7 @@ __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) 
     lo = *reinterpret_cast<uint32_t*>(&x);
     hi = *reinterpret_cast<uint32_t*>(&y);
   } else {
-    lo = e4m3x2_to_f16x2(w & 0xffffu);
-    hi = e4m3x2_to_f16x2(w >> 16);
+    e4m3x4_to_f16x4(w, lo, hi);
   }
 }
 
@@ -372,7 +368,7 @@ struct RowsQ {
   }
 };
 
-// Keys t0 .. t0 + 15 of a row unit (of `count`), at k and v 8 rows of 256 bytes a box: scores,
+// Keys t0 .. t0 + 15 of a row unit (of `count`), whose rows of this head lie at k and v: scores,
 // probabilities and their product with V. A row sees the keys below its `limit`; from `diagonal`
 // on not every row does. qa: bf16 A fragments, k-step (j, w) = dims
 // 64 j + 16 c + 4 w .. + 3. Lane n reads key n's dims straight into B fragments; V is transposed
@@ -387,8 +383,8 @@ __device__ __forceinline__ void row_step(RowsQ& st, const uint32_t (&qa)[32], co
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const bool in = t0 + 8 * u + n < count;                 // (what lies behind the last key may be anything)
-    const uint4* kr = reinterpret_cast<const uint4*>(k + u * kRowBox + n * 256 + 32 * c);
-    const uint4* vr = reinterpret_cast<const uint4*>(v + u * kRowBox + n * 256 + 32 * c);
+    const uint4* kr = reinterpret_cast<const uint4*>(k + (8 * u + n) * kRowBytes + 32 * c);
+    const uint4* vr = reinterpret_cast<const uint4*>(v + (8 * u + n) * kRowBytes + 32 * c);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -466,7 +462,7 @@ __device__ __forceinline__ void row_step(RowsQ& st, const uint32_t (&qa)[32], co
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(v + ((t - t0) >> 3) * kRowBox + (t & 7) * 256 + 128 * j + 32 * c + 4 * r);
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(v + (t - t0) * kRowBytes + 128 * j + 32 * c + 4 * r);
             const float a = (x & 0x7f80u) == 0x7f80u ? __uint_as_float(x << 16) : 0.f;
             const float b = (x & 0x7f800000u) == 0x7f800000u ? __uint_as_float(x & 0xffff0000u) : 0.f;
             st.o[j][r][0] += a;
@@ -496,7 +492,7 @@ struct RingQ {
 };
 
 // Fetches the range's units, K and then V of each, chunk by chunk (one warp).
-__device__ __forceinline__ void quant_producer(const AttnParamsQ& p, const MapsQ& maps, const int4& range, const int4& first_a,
+__device__ __forceinline__ void quant_producer(const AttnParamsQ& p, const int4& range, const int4& first_a,
                                                const int4& first_b, ChunkQ* chunks, uint32_t sbase, volatile int* abort_flag) {
   const int lane = threadIdx.x & 31;
   auto bar = [&](int i) { return sbase + kSmemBarsQ + 8u * i; };
@@ -560,18 +556,20 @@ __device__ __forceinline__ void quant_producer(const AttnParamsQ& p, const MapsQ
       for (int v = 0; v < 2; ++v) {
         if (!(ok = wait(kQEmpty + ring.stage, ring.phase ^ 1))) break;
         const uint32_t dst = sbase + ring.stage * kStageA, full = bar(kQFull + ring.stage);
-        if (i >= rows) {
-          if (lane == 0) {
-            mbar_arrive_expect_tx(full, kStageA);
-            bulk_load(dst, (v ? p.cache.value : p.cache.key) + static_cast<size_t>(y.a) * kPageBytes, kStageA, full);
-          }
-        } else {
-          const int boxes = (y.b + 7) >> 3;
-          const CUtensorMap* map = y.c < 0 ? (v ? &maps.tail_v : &maps.tail_k) : (v ? &maps.new_v : &maps.new_k);
-          if (lane == 0) mbar_arrive_expect_tx(full, boxes * kRowBox);
-          __syncwarp();
-          if (lane < boxes) tma_load_3d(dst + lane * kRowBox, map, 0, y.a + 8 * lane, 0, full);
+        // a page's K or V of all heads, and a unit's rows, are contiguous
+        if (lane == 0) {
+          const void* src;
+          if (i >= rows)
+            src = (v ? p.cache.value : p.cache.key) + static_cast<size_t>(y.a) * kPageBytes;
+          else
+            src = static_cast<const uint8_t*>(y.c < 0 ? (v ? p.cache.tail_value : p.cache.tail_key)
+                                                      : static_cast<const void*>(v ? p.new_v : p.new_k)) +
+                  static_cast<size_t>(y.a) * kRowBytes;
+          const uint32_t bytes = i >= rows ? kStageA : y.b * kRowBytes;
+          mbar_arrive_expect_tx(full, bytes);
+          bulk_load(dst, src, bytes, full);
         }
+        __syncwarp();
         ++uses;
         ring.next();
       }
@@ -592,8 +590,7 @@ __device__ __forceinline__ void quant_producer(const AttnParamsQ& p, const MapsQ
 }
 
 template <int kCode>
-__global__ void __launch_bounds__(kAttnThreadsQ, 1)
-    quant_attn_kernel(const __grid_constant__ MapsQ maps, const AttnParamsQ p) {
+__global__ void __launch_bounds__(kAttnThreadsQ, 1) quant_attn_kernel(const AttnParamsQ p) {
   extern __shared__ uint8_t smem_q[];
   const int h = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
   const uint32_t sraw = smem_u32(smem_q), sbase = (sraw + 1023u) & ~1023u;
@@ -622,7 +619,7 @@ __global__ void __launch_bounds__(kAttnThreadsQ, 1)
   // launch of 9 warps it spilled.
   if (h >= kKVHeads) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
-    if (h == kKVHeads) quant_producer(p, maps, range, __ldg(cta + 1), __ldg(cta + 2), chunks, sbase, abort_flag);
+    if (h == kKVHeads) quant_producer(p, range, __ldg(cta + 1), __ldg(cta + 2), chunks, sbase, abort_flag);
     return;
   }
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHeadRegs));
@@ -673,12 +670,11 @@ __global__ void __launch_bounds__(kAttnThreadsQ, 1)
       const RingQ kr = ring;
       ring.next();
       if (!(ok = wait(kQFull + kr.stage, kr.phase)) || !(ok = wait(kQFull + ring.stage, ring.phase))) break;
-      // a box of 8 rows holds them head by head
-      const uint8_t* kb = smem + kr.stage * kStageA + h * 2048;
-      const uint8_t* vb = smem + ring.stage * kStageA + h * 2048;
+      const uint8_t* kb = smem + kr.stage * kStageA + h * (kHeadDim * 2);
+      const uint8_t* vb = smem + ring.stage * kStageA + h * (kHeadDim * 2);
 #pragma unroll 1
       for (int t0 = 0; t0 < x.b; t0 += 16)
-        row_step(st, qa, kb + (t0 >> 3) * kRowBox, vb + (t0 >> 3) * kRowBox, t0, x.b, min(see + n, x.b), see, p.scale_log2);
+        row_step(st, qa, kb + t0 * kRowBytes, vb + t0 * kRowBytes, t0, x.b, min(see + n, x.b), see, p.scale_log2);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kQEmpty + kr.stage));
       release();
@@ -856,51 +852,67 @@ __global__ void __launch_bounds__(kAttnThreadsQ, 1)
 }
 
 // Grid (CTAs, 8), 256 threads: CTA (c, h) merges head h of the cut item whose first contributor
-// is c. Warp w takes rows w and w + 8 (the same query row); lane l holds dims 4 l .. 4 l + 3 and
-// the weights of contributors l, l + 32, ..
+// is c. Warp w takes rows w and w + 8 (the same query row); lane l holds dims 4 l .. 4 l + 3. The
+// plan is read before the wait: the attention let this launch start after its own wait for it.
+constexpr int kMergeAhead = 4;
 __global__ void __launch_bounds__(256) quant_merge_kernel(const AttnParamsQ p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c0 = blockIdx.x, h = blockIdx.y, r = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 head = __ldg(reinterpret_cast<const int4*>(p.plan));
   const int4 merge = __ldg(reinterpret_cast<const int4*>(p.plan + plan_merge_at(p.grid)) + c0);
   if (head.x != kPlanMagicQ || head.y != p.grid || merge.x < 0 || merge.x >= head.z || merge.y <= c0 || merge.y >= p.grid)
     return;
-  const int parts = merge.y - c0 + 1;
-  auto at = [&](int k) { return p.part + part_index(c0 + k, k == 0 ? (merge.z & 1) : 0, h); };
   const ItemQ it = load_item_q(p, merge.x);
   if (r >= it.rows || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return;
+  const int parts = merge.y - c0 + 1;
+  const float* first = p.part + part_index(c0, merge.z & 1, h);
+  const float* rest = p.part + part_index(c0, 0, h);
+  const size_t pitch = part_index(1, 0, 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // parts k0 .. k0 + 3 of both rows at a time: statistics and values in one round trip
+  float m[2] = {kNoMaxQ, kNoMaxQ}, l[2] = {0.f, 0.f}, o[2][4] = {};
 #pragma unroll 1
-  for (int x = 0; x < 2; ++x) {
-    const int row = r + 8 * x;
-    float m = kNoMaxQ;
-    for (int k = lane; k < parts; k += 32) m = fmaxf(m, __ldcg(reinterpret_cast<const float2*>(at(k) + 16 * kHeadDim) + row).x);
+  for (int k0 = 0; k0 < parts; k0 += kMergeAhead) {
+    float2 ml[2][kMergeAhead];
+    float4 v[2][kMergeAhead];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-      float w = 0.f;
-      if (k0 + lane < parts) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(at(k0 + lane) + 16 * kHeadDim) + row);
-        w = ex2(ml.x - m);
-        l = fmaf(ml.y, w, l);
-      }
-      const int stop = min(32, parts - k0);
-#pragma unroll 8
-      for (int k = 0; k < stop; ++k) {
-        const float wk = __shfl_sync(0xffffffffu, w, k);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(at(k0 + k) + row * kHeadDim) + lane);
-        o[0] = fmaf(v.x, wk, o[0]);
-        o[1] = fmaf(v.y, wk, o[1]);
-        o[2] = fmaf(v.z, wk, o[2]);
-        o[3] = fmaf(v.w, wk, o[3]);
+    for (int k = 0; k < kMergeAhead; ++k) {
+      const float* at = k0 + k == 0 ? first : rest + min(k0 + k, parts - 1) * pitch;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        ml[x][k] = __ldcg(reinterpret_cast<const float2*>(at + 16 * kHeadDim) + r + 8 * x);
+        v[x][k] = __ldcg(reinterpret_cast<const float4*>(at + (r + 8 * x) * kHeadDim) + lane);
       }
     }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    const float inv = 1.f / l;
+    for (int x = 0; x < 2; ++x) {
+      float top = m[x];
+#pragma unroll
+      for (int k = 0; k < kMergeAhead; ++k) {
+        if (k0 + k >= parts) ml[x][k] = make_float2(kNoMaxQ, 0.f);
+        top = fmaxf(top, ml[x][k].x);
+      }
+      const float a = ex2(m[x] - top);
+      m[x] = top;
+      l[x] *= a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[x][i] *= a;
+#pragma unroll
+      for (int k = 0; k < kMergeAhead; ++k) {
+        if (k0 + k >= parts) break;
+        const float w = ex2(ml[x][k].x - top);
+        l[x] = fmaf(ml[x][k].y, w, l[x]);
+        o[x][0] = fmaf(v[x][k].x, w, o[x][0]);
+        o[x][1] = fmaf(v[x][k].y, w, o[x][1]);
+        o[x][2] = fmaf(v[x][k].z, w, o[x][2]);
+        o[x][3] = fmaf(v[x][k].w, w, o[x][3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const float inv = 1.f / l[x];
     reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(it.q0 + r) * kQHeads + 2 * h + x) * kHeadDim)[lane] =
-        make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+        make_uint2(pack_bf16x2(o[x][0] * inv, o[x][1] * inv), pack_bf16x2(o[x][2] * inv, o[x][3] * inv));
   }
 }
 
