@@ -10,7 +10,8 @@ Drop-in replacements for the two attention hot paths of qwen3-dspark:
 Beside them: attention of requests that share long prefixes (``B200SharedPrefixKernel``
 with ``SharedPrefixLayout``) and penalties, biases and grammar masks on the logits
 (``TokenControls``, ``control_logits``, ``control_argmax``); and a paged KV cache in 8 bits
-(``QuantizedPages``, ``QuantizedLayout``, ``B200QuantizedKernel``).
+(``QuantizedPages``, ``QuantizedLayout``, ``B200QuantizedKernel``, and the target's store
+over it, ``B200QuantizedTargetKV``).
 
 The kernels live in ``lib/libdspark_b200.so`` (C ABI, include/dspark_b200.h),
 built from ``csrc/`` by ``build.py``. Importing this package does not touch
@@ -26,6 +27,7 @@ from .kernels import (add_rms_norm, BACKEND, CAPACITY_BACKEND, DRAFT_BACKEND, SC
 from .kv_store import B200PersistentTargetKV, Slot, Transaction, rope_inv_freq
 from .controls import TokenControls, control_argmax, control_logits
 from .quantized import B200QuantizedKernel, QuantizedLayout, QuantizedPages
+from .quantized_store import B200QuantizedTargetKV
 from .layout import PackedLayout, PersistentAttentionLayout, SharedPrefixLayout, TrainingLayout
 
 
@@ -53,4 +55,5 @@ __all__ = ['add_rms_norm', 'BACKEND', 'CAPACITY_BACKEND', 'DRAFT_BACKEND', 'SCAL
            'DSparkDraftModel', 'DraftSpec', 'B200Qwen3Target', 'speculative_greedy', 'speculative_greedy_pipelined', 'speculative_sample', 'accept_greedy', 'build',
            'draft_append', 'float64_law', 'greedy_accept', 'markov_greedy', 'qk_norm_rope', 'rms_norm', 'silu_mul', 'sample_rows', 'stochastic_accept', 'stochastic_propose', 'launch_count', 'load_library', 'read_device_status', 'rope_inv_freq', 'runtime_identity',
            'segment_attention', 'B200SharedPrefixKernel', 'SharedPrefixLayout', 'TokenControls', 'control_argmax',
-           'control_logits', 'B200QuantizedKernel', 'QuantizedLayout', 'QuantizedPages']
+           'control_logits', 'B200QuantizedKernel', 'QuantizedLayout', 'QuantizedPages',
+           'B200QuantizedTargetKV']

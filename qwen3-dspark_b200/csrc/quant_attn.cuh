@@ -852,62 +852,95 @@ __global__ void __launch_bounds__(kAttnThreadsQ, 1) quant_attn_kernel(const Attn
 }
 
 // Grid (CTAs, 8), 256 threads: CTA (c, h) merges head h of the cut item whose first contributor
-// is c. Warp w takes rows w and w + 8 (the same query row); lane l holds dims 4 l .. 4 l + 3. The
-// plan is read before the wait: the attention let this launch start after its own wait for it.
-constexpr int kMergeAhead = 4;
+// is c. The item's query rows (both query heads of each) take 1, 2, 4 or 8 warps a piece, which
+// share the parts; lane l holds dims 4 l .. 4 l + 3. Each warp asks for 8 parts' statistics and
+// values in one round trip. The plan is read before the wait: the attention lets this launch
+// start after its own wait for it.
+constexpr int kMergeAhead = 8;
 __global__ void __launch_bounds__(256) quant_merge_kernel(const AttnParamsQ p) {
-  const int c0 = blockIdx.x, h = blockIdx.y, r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float4 s_o[8][2][32];
+  __shared__ float2 s_ml[8][2];
+  const int c0 = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 head = __ldg(reinterpret_cast<const int4*>(p.plan));
   const int4 merge = __ldg(reinterpret_cast<const int4*>(p.plan + plan_merge_at(p.grid)) + c0);
   if (head.x != kPlanMagicQ || head.y != p.grid || merge.x < 0 || merge.x >= head.z || merge.y <= c0 || merge.y >= p.grid)
     return;
   const ItemQ it = load_item_q(p, merge.x);
-  if (r >= it.rows || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return;
+  if (it.rows < 1 || it.rows > kQBlock || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return;
+  const int shift = it.rows > 4 ? 3 : (it.rows > 2 ? 2 : it.rows - 1);     // 2^shift rows, 8 >> shift warps each
+  const int r = warp & ((1 << shift) - 1), group = warp >> shift, step = 8 >> shift;
+  const bool live = r < it.rows;
   const int parts = merge.y - c0 + 1;
   const float* first = p.part + part_index(c0, merge.z & 1, h);
   const float* rest = p.part + part_index(c0, 0, h);
   const size_t pitch = part_index(1, 0, 0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  // parts k0 .. k0 + 3 of both rows at a time: statistics and values in one round trip
   float m[2] = {kNoMaxQ, kNoMaxQ}, l[2] = {0.f, 0.f}, o[2][4] = {};
 #pragma unroll 1
-  for (int k0 = 0; k0 < parts; k0 += kMergeAhead) {
+  for (int k0 = group; k0 < parts && live; k0 += kMergeAhead * step) {
     float2 ml[2][kMergeAhead];
     float4 v[2][kMergeAhead];
 #pragma unroll
-    for (int k = 0; k < kMergeAhead; ++k) {
-      const float* at = k0 + k == 0 ? first : rest + min(k0 + k, parts - 1) * pitch;
+    for (int i = 0; i < kMergeAhead; ++i) {
+      const int k = k0 + i * step;
+      const float* at = k == 0 ? first : rest + k * pitch;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        ml[x][k] = __ldcg(reinterpret_cast<const float2*>(at + 16 * kHeadDim) + r + 8 * x);
-        v[x][k] = __ldcg(reinterpret_cast<const float4*>(at + (r + 8 * x) * kHeadDim) + lane);
+        ml[x][i] = make_float2(kNoMaxQ, 0.f);
+        v[x][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < parts) {
+          ml[x][i] = __ldcg(reinterpret_cast<const float2*>(at + 16 * kHeadDim) + r + 8 * x);
+          v[x][i] = __ldcg(reinterpret_cast<const float4*>(at + (r + 8 * x) * kHeadDim) + lane);
+        }
       }
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       float top = m[x];
 #pragma unroll
-      for (int k = 0; k < kMergeAhead; ++k) {
-        if (k0 + k >= parts) ml[x][k] = make_float2(kNoMaxQ, 0.f);
-        top = fmaxf(top, ml[x][k].x);
-      }
+      for (int i = 0; i < kMergeAhead; ++i) top = fmaxf(top, ml[x][i].x);
       const float a = ex2(m[x] - top);
       m[x] = top;
       l[x] *= a;
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[x][i] *= a;
 #pragma unroll
-      for (int k = 0; k < kMergeAhead; ++k) {
-        if (k0 + k >= parts) break;
-        const float w = ex2(ml[x][k].x - top);
-        l[x] = fmaf(ml[x][k].y, w, l[x]);
-        o[x][0] = fmaf(v[x][k].x, w, o[x][0]);
-        o[x][1] = fmaf(v[x][k].y, w, o[x][1]);
-        o[x][2] = fmaf(v[x][k].z, w, o[x][2]);
-        o[x][3] = fmaf(v[x][k].w, w, o[x][3]);
+      for (int i = 0; i < kMergeAhead; ++i) {
+        const float w = ex2(ml[x][i].x - top);
+        l[x] = fmaf(ml[x][i].y, w, l[x]);
+        o[x][0] = fmaf(v[x][i].x, w, o[x][0]);
+        o[x][1] = fmaf(v[x][i].y, w, o[x][1]);
+        o[x][2] = fmaf(v[x][i].z, w, o[x][2]);
+        o[x][3] = fmaf(v[x][i].w, w, o[x][3]);
       }
     }
   }
+  if (step > 1) {                                            // the warps of a row: group 0 adds them up in order
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      s_o[warp][x][lane] = make_float4(o[x][0], o[x][1], o[x][2], o[x][3]);
+      if (lane == 0) s_ml[warp][x] = make_float2(m[x], l[x]);
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float top = kNoMaxQ;
+      for (int g = 0; g < step; ++g) top = fmaxf(top, s_ml[r + (g << shift)][x].x);
+      l[x] = o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+      for (int g = 0; g < step; ++g) {
+        const float2 ml = s_ml[r + (g << shift)][x];
+        const float4 v = s_o[r + (g << shift)][x][lane];
+        const float w = ex2(ml.x - top);
+        l[x] = fmaf(ml.y, w, l[x]);
+        o[x][0] = fmaf(v.x, w, o[x][0]);
+        o[x][1] = fmaf(v.y, w, o[x][1]);
+        o[x][2] = fmaf(v.z, w, o[x][2]);
+        o[x][3] = fmaf(v.w, w, o[x][3]);
+      }
+    }
+  }
+  if (!live) return;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const float inv = 1.f / l[x];

@@ -95,6 +95,7 @@ class Transaction:
     rope: dict = None           # inv_freq tensor -> [sum Q, 64] cos/sin table, built once per transaction
     table: torch.Tensor = None  # fixed cos/sin buffer of a bound bucket (graph capture/replay)
     capture: bool = False       # the placeholder transaction a CUDA graph is captured under
+    layout: object = None       # QuantizedLayout of a paged 8-bit store
 
     @property
     def query_tokens(self):
@@ -177,6 +178,10 @@ class B200PersistentTargetKV:
     def _slot_rows_view(self, x, i, start, n):
         r0 = self.slot_rows[i] + start
         return x.view(self.layers, self.rows_per_layer, self.heads, self.dim)[:, r0:r0 + n]
+
+    def _prefix_rows(self, i, n):
+        """K and V of the first n committed tokens of slot i, [layers, n, heads, dim]."""
+        return self._slot_rows_view(self._keys, i, 0, n), self._slot_rows_view(self._values, i, 0, n)
 
     # -- slot lifecycle ----------------------------------------------------------
     # Observable contract of the reference store (persistent_target_kv.py:204-265):
@@ -294,13 +299,8 @@ class B200PersistentTargetKV:
         self._staged = set(range(self.layers))
 
     # -- transactions -----------------------------------------------------------
-    @torch.no_grad()
-    def begin(self, handles, bucket=None, *, query_lengths=None):
-        """Metadata for one verify round (persistent_target_kv.py:369-415).
-
-        ``query_lengths`` (or ``bucket.query_lengths``) gives each request's new rows.
-        One host->device copy of [cu_q | slot_row | ctx_len | slot_cap] as int32.
-        """
+    def _round(self, handles, bucket, query_lengths):
+        """The checked (handles, slot indices, query lengths, context lengths) of a new transaction."""
         self._usable(idle=True)
         handles = tuple(handles)
         if query_lengths is None:
@@ -319,6 +319,16 @@ class B200PersistentTargetKV:
             raise ValueError('Actual context exceeds declared bucket applicability')
         if bucket is not None and hasattr(bucket, 'accepts') and not bucket.accepts(query_lengths, contexts):
             raise ValueError('Actual context exceeds declared bucket applicability')
+        return handles, indices, query_lengths, contexts
+
+    @torch.no_grad()
+    def begin(self, handles, bucket=None, *, query_lengths=None):
+        """Metadata for one verify round (persistent_target_kv.py:369-415).
+
+        ``query_lengths`` (or ``bucket.query_lengths``) gives each request's new rows.
+        One host->device copy of [cu_q | slot_row | ctx_len | slot_cap] as int32.
+        """
+        handles, indices, query_lengths, contexts = self._round(handles, bucket, query_lengths)
         cu = [0]
         for q in query_lengths:
             cu.append(cu[-1] + q)
@@ -359,21 +369,8 @@ class B200PersistentTargetKV:
             self._rotary[key] = cache
         return cache
 
-    @torch.no_grad()
-    def verify_layer(self, tx, layer, q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, *, inv_freq,
-                     eps=1e-6, scale=SCALE, out=None, path='auto'):
-        """Fused verify for one decoder layer; returns attention output [sum Q, 16, 128].
-
-        ``q_raw``/``k_raw``/``v_raw`` are the layer's q/k/v projections of the new
-        tokens before q_norm/k_norm/RoPE ([sum Q, 16|8, 128] bf16); norm weights [128]
-        bf16; ``inv_freq`` [64] float32 on this device (see ``rope_inv_freq``).
-        ``path``: 'fused' (norm/RoPE/append inside the attention kernel), 'prep' (a
-        prep kernel per layer, then the attention kernel) or 'auto' (prep below 512
-        new rows or for chunks longer than 16 rows); all give the same values.
-        q/k/v may be row-strided views (heads and head dims packed, row stride a
-        multiple of 8), e.g. column blocks of one merged q|k|v projection; strided
-        rows take the prep path.
-        """
+    def _verify_inputs(self, tx, layer, q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, inv_freq, scale):
+        """Checks of a verify layer's inputs; returns the new rows and the three row strides."""
         self._transaction(tx)
         if type(layer) is not int or not 0 <= layer < self.layers or layer in self._staged:
             raise ValueError('Each model layer must stage exactly once')
@@ -398,19 +395,43 @@ class B200PersistentTargetKV:
         if (not isinstance(inv_freq, torch.Tensor) or inv_freq.shape != (HEAD_DIM // 2,)
                 or inv_freq.dtype != torch.float32 or inv_freq.device != self.device):
             raise ValueError('inv_freq must be float32 [64] on the store device')
-        if out is None:
-            out = torch.empty((n, HQ, HEAD_DIM), dtype=self.dtype, device=self.device)
-        cu_q, slot_row, ctx, _cap = self._meta(tx)
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        lib = _lib.load_library()
+        return n, lds
+
+    def _rope_rows(self, tx, inv_freq, cu_q, ctx):
+        """The transaction's cos/sin table, gathered on its first layer."""
         key = (inv_freq.data_ptr(), inv_freq._version)
         table = tx.rope.get(key)
         if table is None:
             # cos/sin of every new row's position, gathered once for all layers of this
             # transaction from the rotary cache of these frequencies
-            table = rope_table(self.rotary_cache(inv_freq), cu_q, ctx, len(tx.query_lengths), n, out=tx.table)
+            table = rope_table(self.rotary_cache(inv_freq), cu_q, ctx, len(tx.query_lengths), tx.query_tokens,
+                               out=tx.table)
             tx.rope.clear()
             tx.rope[key] = table
+        return table
+
+    @torch.no_grad()
+    def verify_layer(self, tx, layer, q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, *, inv_freq,
+                     eps=1e-6, scale=SCALE, out=None, path='auto'):
+        """Fused verify for one decoder layer; returns attention output [sum Q, 16, 128].
+
+        ``q_raw``/``k_raw``/``v_raw`` are the layer's q/k/v projections of the new
+        tokens before q_norm/k_norm/RoPE ([sum Q, 16|8, 128] bf16); norm weights [128]
+        bf16; ``inv_freq`` [64] float32 on this device (see ``rope_inv_freq``).
+        ``path``: 'fused' (norm/RoPE/append inside the attention kernel), 'prep' (a
+        prep kernel per layer, then the attention kernel) or 'auto' (prep below 512
+        new rows or for chunks longer than 16 rows); all give the same values.
+        q/k/v may be row-strided views (heads and head dims packed, row stride a
+        multiple of 8), e.g. column blocks of one merged q|k|v projection; strided
+        rows take the prep path.
+        """
+        n, lds = self._verify_inputs(tx, layer, q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, inv_freq, scale)
+        if out is None:
+            out = torch.empty((n, HQ, HEAD_DIM), dtype=self.dtype, device=self.device)
+        cu_q, slot_row, ctx, _cap = self._meta(tx)
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        lib = _lib.load_library()
+        table = self._rope_rows(tx, inv_freq, cu_q, ctx)
         ws = _lib.workspace(self.device, stream)
         _lib.check(lib.dspark_verify_strided(
             q_raw.data_ptr(), lds[0], k_raw.data_ptr(), lds[1], v_raw.data_ptr(), lds[2], q_norm_weight.data_ptr(),
@@ -469,9 +490,9 @@ class B200PersistentTargetKV:
         ck, positions, o, qo = [0], [], 0, 0
         base = layer * self.max_query_tokens
         for h, c, n in zip(tx.slots, tx.context_lengths, tx.query_lengths):
-            i = h.index
-            keys[o:o + c] = self._slot_rows_view(self._keys, i, 0, c)[layer]
-            values[o:o + c] = self._slot_rows_view(self._values, i, 0, c)[layer]
+            held_k, held_v = self._prefix_rows(h.index, c)
+            keys[o:o + c] = held_k[layer]
+            values[o:o + c] = held_v[layer]
             keys[o + c:o + c + n] = self.scratch_keys[base + qo:base + qo + n]
             values[o + c:o + c + n] = self.scratch_values[base + qo:base + qo + n]
             positions.extend(range(c, c + n))
@@ -481,6 +502,40 @@ class B200PersistentTargetKV:
         cu_q = self._meta(tx)[0]
         return (keys, values, cu_q, torch.tensor(ck, dtype=torch.int32, device=self.device),
                 torch.tensor(positions, dtype=torch.long, device=self.device))
+
+    def _commit_rows(self, tx, counts):
+        """The commit of ``counts`` (int32 [R] on the device) rows of each request, all layers, one launch."""
+        cu_q, slot_row, ctx, cap = self._meta(tx)
+        _lib.check(_lib.load_library().dspark_commit_kv(
+            self._keys.data_ptr(), self._values.data_ptr(), self.scratch_keys.data_ptr(),
+            self.scratch_values.data_ptr(), cu_q.data_ptr(), slot_row.data_ptr(), ctx.data_ptr(), cap.data_ptr(),
+            counts.data_ptr(), len(tx.query_lengths), self.layers, self.rows_per_layer, self.max_query_tokens,
+            _lib.DTYPE_F32 if self.dtype == torch.float32 else _lib.DTYPE_BF16,
+            torch.cuda.current_stream(self.device).cuda_stream), 'dspark_commit_kv')
+
+    @torch.no_grad()
+    def device_rounds(self, handles, bucket, room):
+        """For a loop that keeps the round state on the GPU: fills the bound ``bucket``'s
+        metadata for ``handles``, whose contexts may grow by ``room`` tokens. Returns
+        ``(context, commit)``: the int32 [R] context lengths that the bucket's captured program
+        reads and the loop advances, and ``commit(counts)``, which commits that many of the
+        program's scratch rows. ``mirror_lengths`` ends the loop."""
+        self._usable(idle=True)
+        tx = self._device_round(tuple(handles), bucket, room)
+        return self._meta(tx)[2], lambda counts: self._commit_rows(tx, counts)
+
+    def _device_round(self, handles, bucket, room):
+        slots = [self._slot(h) for h in handles]
+        lengths = [self._lengths[i] for i in slots]
+        if any(c + room > self.capacities[i] for c, i in zip(lengths, slots)):
+            raise ValueError('Request slots cannot hold max_new_tokens plus one verify chunk')
+        buffers, qlens = self.bind_bucket(bucket), tuple(bucket.query_lengths)
+        cu = [0]
+        for q in qlens:
+            cu.append(cu[-1] + q)
+        buffers.meta.copy_(torch.tensor(cu + [self.slot_rows[i] for i in slots] + lengths
+                                        + [self.capacities[i] for i in slots], dtype=torch.int32))
+        return Transaction(0, handles, tuple(lengths), qlens, buffers.meta, {}, buffers.table)
 
     @torch.no_grad()
     def commit(self, tx, committed_query_lengths: Mapping):
@@ -498,14 +553,7 @@ class B200PersistentTargetKV:
             counts.append(n)
         try:
             ncommit = _upload(counts, self.device)
-            cu_q, slot_row, ctx, cap = self._meta(tx)
-            stream = torch.cuda.current_stream(self.device).cuda_stream
-            _lib.check(_lib.load_library().dspark_commit_kv(
-                self._keys.data_ptr(), self._values.data_ptr(), self.scratch_keys.data_ptr(),
-                self.scratch_values.data_ptr(), cu_q.data_ptr(), slot_row.data_ptr(), ctx.data_ptr(),
-                cap.data_ptr(), ncommit.data_ptr(), len(tx.slots), self.layers, self.rows_per_layer,
-                self.max_query_tokens, _lib.DTYPE_F32 if self.dtype == torch.float32 else _lib.DTYPE_BF16, stream),
-                'dspark_commit_kv')
+            self._commit_rows(tx, ncommit)
             for h, n in zip(tx.slots, counts):
                 self._lengths[h.index] += n
         except Exception:
@@ -513,7 +561,8 @@ class B200PersistentTargetKV:
             raise
         self._pending, self._staged = None, set()
         return dict(committed_tokens=sum(counts),
-                    copied_kv_bytes=2 * self.layers * self.heads * self.dim * self._keys.element_size() * sum(counts))
+                    copied_kv_bytes=2 * self.layers * self.heads * self.dim * self.scratch_keys.element_size()
+                    * sum(counts))
 
     def abort(self, tx):
         """Drop the transaction; scratch rows are simply never copied (persistent_target_kv.py:493-499)."""
@@ -523,7 +572,7 @@ class B200PersistentTargetKV:
     def request_kv(self, handle):
         i = self._slot(handle)
         n = self._lengths[i]
-        return (self._slot_rows_view(self._keys, i, 0, n).clone(), self._slot_rows_view(self._values, i, 0, n).clone())
+        return tuple(x.clone() for x in self._prefix_rows(i, n))
 
     def pointers(self):
         return dict(committed_keys=self._keys.data_ptr(), committed_values=self._values.data_ptr(),

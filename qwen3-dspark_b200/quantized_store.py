@@ -1,0 +1,330 @@
+"""Persistent target KV store over 8-bit pages.
+
+``B200QuantizedTargetKV`` has the transaction API of ``B200PersistentTargetKV``: slot
+handles, ``load_prefix``, ``begin`` / ``verify_layer`` (or ``stage_layer`` + ``attend``) /
+``commit`` / ``abort``, bound buckets and captured programs. What differs is where
+committed tokens go: full blocks of 64 into pages of a pool, in int8 or e4m3 with a scale
+per block and KV head, the rest unquantised into the request's tail slot. Requests hold
+pages as they grow, so the pool needs no more of them than the tokens that are resident;
+``fork`` starts continuations that share a request's full pages, and ``compact`` moves the
+pages in use to the lowest ids.
+"""
+import torch
+
+from . import _lib
+from .kernels import HEAD_DIM, HKV, HQ, SCALE, runtime_identity
+from .kv_store import B200PersistentTargetKV, Transaction, _BucketBuffers, _SlotTable, _upload
+from .quantized import CACHE_TYPES, PAGE, B200QuantizedKernel, QuantizedLayout, QuantizedPages, plan_words
+
+
+class B200QuantizedTargetKV(B200PersistentTargetKV):
+    def __init__(self, *, layers, slots, context_capacity, max_query_tokens, cache='int8', pages=None, heads=HKV,
+                 dim=HEAD_DIM, dtype=torch.bfloat16, device='cuda', slot_capacities=None):
+        """``cache``: 'int8' or 'e4m3'. ``pages``: pool size, by default enough for every slot at its
+        capacity. ``dtype`` is that of the new and the open rows."""
+        dims = (layers, slots, context_capacity, max_query_tokens, heads, dim)
+        if any(type(n) is not int or n < 1 for n in dims) or (pages is not None and (type(pages) is not int or pages < 1)):
+            raise ValueError('All capacities and dimensions must be positive integers')
+        if (heads, dim) != (HKV, HEAD_DIM) or dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError('B200 store holds bf16 (or exact-path fp32) Qwen3 KV: 8 heads x 128')
+        if cache not in CACHE_TYPES:
+            raise ValueError(f'cache must be one of {sorted(CACHE_TYPES)}')
+        caps = [context_capacity] * slots if slot_capacities is None else [int(c) for c in slot_capacities]
+        if len(caps) != slots or any(c < 1 or c > context_capacity for c in caps):
+            raise ValueError('One positive capacity <= context_capacity per slot required')
+        self.device = torch.device(device)
+        if self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
+        self.runtime = runtime_identity(self.device)
+        self.layers, self.slot_capacity, self.context_capacity = layers, slots, context_capacity
+        self.max_query_tokens, self.heads, self.dim, self.dtype = max_query_tokens, heads, dim, dtype
+        self.capacities = tuple(caps)
+        self.cache = cache
+        self.pages = QuantizedPages.empty(layers=layers, pages=pages or max(1, sum(c // PAGE for c in caps)), slots=slots,
+                                          dtype=CACHE_TYPES[cache], row_dtype=dtype, device=self.device)
+        self.table_width = max(1, context_capacity // PAGE)
+        self.scratch_keys = torch.zeros((layers * max_query_tokens, heads, dim), dtype=dtype, device=self.device)
+        self.scratch_values = torch.zeros_like(self.scratch_keys)
+        self._kernel = B200QuantizedKernel(self.device)
+        self._table = _SlotTable(slots)
+        self._lengths = self._table.length
+        self._held = [[] for _ in range(slots)]      # page ids of each slot's blocks, in order
+        self._sequence = 0
+        self._pending = None
+        self._staged = set()
+        self._buckets = {}
+        self._rotary = {}
+        self.failed = False
+
+    @property
+    def keys(self):
+        raise AttributeError('an 8-bit store keeps its tokens in pages; see pages, request_kv')
+
+    values = keys
+
+    # -- slot lifecycle ----------------------------------------------------------------
+    def remove_request(self, handle):
+        """Free the request's slot, and those of its pages that no fork holds."""
+        self._usable(idle=True)
+        i = self._table.index_of(handle)
+        self._table.release(i)
+        self.pages.free(self._held[i])
+        self._held[i] = []
+
+    def fork(self, handle, requests):
+        """Admit ``requests`` (ids) as continuations of ``handle``: they hold its full pages
+        together with it and get copies of its open rows (one launch). Returns their handles."""
+        self._usable(idle=True)
+        i = self._slot(handle)
+        requests = [requests] if isinstance(requests, str) else list(requests)
+        n = self._lengths[i]
+        handles = []
+        try:
+            for r in requests:
+                h = self._table.admit(r)
+                handles.append(h)
+                if n > self.capacities[h.index]:
+                    raise ValueError('A fork does not fit its slot')
+        except ValueError:
+            for h in handles:
+                self._table.release(h.index)
+            raise
+        # a parent's pages behind its last full block are only reserved: they stay its own
+        full = self._held[i][:n // PAGE]
+        for h in handles:
+            self.pages.share(full)
+            self._held[h.index] = list(full)
+            self._lengths[h.index] = n
+        if n % PAGE and handles:
+            self._poisoned(lambda: self.pages.copy(tail_src=[i] * len(handles), tail_dst=[h.index for h in handles],
+                                                   tail_lengths=[n] * len(handles)))
+        return handles
+
+    def compact(self):
+        """Move the pages in use to the lowest ids; returns the number moved. Captured programs
+        stay valid: they read the tables that ``begin`` writes."""
+        self._usable(idle=True)
+        pool = self.pages
+        used = sum(1 for u in pool.users if u)
+        src = [x for x in range(used, pool.pages) if pool.users[x]]
+        dst = [x for x in range(used) if not pool.users[x]]
+        if not src:
+            return 0
+        self._poisoned(lambda: pool.copy(src, dst))
+        to = dict(zip(src, dst))
+        for held in self._held:
+            held[:] = [to.get(x, x) for x in held]
+        for a, b in to.items():
+            pool.users[b], pool.users[a] = pool.users[a], 0
+        pool._free = list(range(used, pool.pages))
+        return len(src)
+
+    def _poisoned(self, launch):
+        try:
+            return launch()
+        except Exception:
+            self.failed = True
+            raise
+
+    def _reserve(self, indices, lengths):
+        """Pages for the blocks that get full when slots ``indices`` reach ``lengths``."""
+        need = [max(0, n // PAGE - len(self._held[i])) for i, n in zip(indices, lengths)]
+        if sum(need) > self.pages.free_pages:
+            raise ValueError(f'{sum(need)} pages needed, {self.pages.free_pages} free in the pool')
+        for i, k in zip(indices, need):
+            self._held[i] += self.pages.allocate(k)
+
+    def _host_meta(self, indices, query_lengths, contexts):
+        cu = [0]
+        for q in query_lengths:
+            cu.append(cu[-1] + q)
+        host = cu + list(contexts) + list(indices)
+        for i in indices:
+            held = self._held[i][:self.table_width]
+            host += held + [-1] * (self.table_width - len(held))
+        return host
+
+    def _views(self, meta, r):
+        """cu_q, context, tail slot and page table of a transaction's metadata."""
+        return (meta[:r + 1], meta[r + 1:2 * r + 1], meta[2 * r + 1:3 * r + 1],
+                meta[3 * r + 1:3 * r + 1 + r * self.table_width].view(r, self.table_width))
+
+    def _layout(self, meta, query_lengths, plan=None):
+        cu, ctx, slot, table = self._views(meta, len(query_lengths))
+        return QuantizedLayout.on_device(query_lengths, cu, ctx, table, slot, plan=plan, replan=False)
+
+    def _meta(self, tx):
+        cu, ctx, slot, _table = self._views(tx.meta, len(tx.query_lengths))
+        return cu, slot, ctx, None
+
+    @torch.no_grad()
+    def load_prefix(self, handle, keys, values):
+        """Bootstrap committed KV [L, n, H, D] into an empty slot (full blocks are quantised)."""
+        self._usable(idle=True)
+        i = self._slot(handle)
+        if self._lengths[i]:
+            raise ValueError('prefix load needs an empty slot')
+        if not isinstance(keys, torch.Tensor) or keys.ndim != 4 or not 0 <= keys.shape[1] <= self.capacities[i]:
+            raise ValueError('prefix K/V must be [layers, n, heads, dim] with n within the slot capacity')
+        n = keys.shape[1]
+        self._kv(keys, values, (self.layers, n, self.heads, self.dim))
+        self._reserve([i], [n])
+        if n:
+            meta = _upload(self._host_meta([i], [n], [0]), self.device)
+            layout = self._layout(meta, (n,))
+            self._poisoned(lambda: self.pages.append(keys.contiguous(), values.contiguous(), layout))
+        self._lengths[i] = n
+
+    # -- buckets -----------------------------------------------------------------------
+    def bind_bucket(self, bucket):
+        """Fixed-address metadata, cos/sin and work-plan buffers of ``bucket`` (see
+        ``B200PersistentTargetKV.bind_bucket``); the captured program makes the plan of
+        each replay from the metadata."""
+        self._usable()
+        qlens = tuple(bucket.query_lengths)
+        if (not qlens or any(type(q) is not int or q < 1 for q in qlens) or sum(qlens) > self.max_query_tokens
+                or len(qlens) > self.slot_capacity):
+            raise ValueError('Bucket query lengths must be positive and fit the store')
+        if bucket not in self._buckets:
+            r, n = len(qlens), sum(qlens)
+            buffers = _BucketBuffers(
+                torch.zeros(3 * r + 1 + r * self.table_width, dtype=torch.int32, device=self.device),
+                torch.zeros((n, HEAD_DIM // 2), dtype=torch.int32, device=self.device))
+            buffers.plan = torch.zeros(plan_words(self.device, r, n), dtype=torch.int32, device=self.device)
+            self._buckets[bucket] = buffers
+        return self._buckets[bucket]
+
+    @torch.no_grad()
+    def capture_transaction(self, bucket):
+        self._usable(idle=True)
+        buffers = self.bind_bucket(bucket)
+        qlens = tuple(bucket.query_lengths)
+        cu = [0]
+        for q in qlens:
+            cu.append(cu[-1] + q)
+        r = len(qlens)
+        # empty contexts: every request reads only its new rows
+        host = cu + [0] * (2 * r) + [-1] * (r * self.table_width)
+        buffers.meta.copy_(torch.tensor(host, dtype=torch.int32))
+        self._sequence += 1
+        tx = Transaction(self._sequence, (), (0,) * r, qlens, buffers.meta, {}, buffers.table, True,
+                         self._layout(buffers.meta, qlens, buffers.plan))
+        self._pending, self._staged = tx, set()
+        return tx
+
+    # -- transactions ------------------------------------------------------------------
+    @torch.no_grad()
+    def begin(self, handles, bucket=None, *, query_lengths=None):
+        """Metadata for one verify round, as in ``B200PersistentTargetKV.begin``; pages for every
+        block that the round can fill are taken from the pool first, and a pool without
+        them refuses the round with ``ValueError``, nothing changed."""
+        handles, indices, query_lengths, contexts = self._round(handles, bucket, query_lengths)
+        self._reserve(indices, [c + q for c, q in zip(contexts, query_lengths)])
+        host = self._host_meta(indices, query_lengths, contexts)
+        buffers = self._buckets.get(bucket) if bucket is not None else None
+        if buffers is not None and query_lengths == tuple(bucket.query_lengths):
+            meta, table, plan = buffers.meta, buffers.table, buffers.plan
+            meta.copy_(torch.tensor(host, dtype=torch.int32).pin_memory(), non_blocking=True)
+        else:
+            meta, table, plan = _upload(host, self.device), None, None
+        self._sequence += 1
+        tx = Transaction(self._sequence, handles, contexts, query_lengths, meta, {}, table,
+                         layout=self._layout(meta, query_lengths, plan))
+        self._pending, self._staged = tx, set()
+        return tx
+
+    def _planned(self, tx):
+        """The transaction's layout, its plan made by the first layer that needs it."""
+        if not tx.rope.get('planned'):
+            tx.layout.replan()
+            tx.rope['planned'] = True
+        return tx.layout
+
+    def _scratch(self, layer, n):
+        base = layer * self.max_query_tokens
+        return self.scratch_keys[base:base + n], self.scratch_values[base:base + n]
+
+    @torch.no_grad()
+    def verify_layer(self, tx, layer, q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, *, inv_freq,
+                     eps=1e-6, scale=SCALE, out=None, path='auto'):
+        """One decoder layer's verify attention from the raw projections (see
+        ``B200PersistentTargetKV.verify_layer``): q_norm/k_norm, RoPE and the scratch append in one
+        launch, then the attention over pages, open rows and scratch. ``path`` may be 'auto' or
+        'prep'."""
+        n, lds = self._verify_inputs(tx, layer, q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, inv_freq, scale)
+        if path not in ('auto', 'prep'):
+            raise ValueError('An 8-bit store has the prep path only')
+        if out is None:
+            out = torch.empty((n, HQ, HEAD_DIM), dtype=self.dtype, device=self.device)
+        layout = self._planned(tx)
+        table = self._rope_rows(tx, inv_freq, layout.cu_query, layout.context)
+        tx.rope['planned'] = True                    # (a new table starts the dict over)
+        keys, values = self._scratch(layer, n)
+        _lib.check(_lib.load_library().dspark_verify_prep(
+            q_raw.data_ptr(), lds[0], k_raw.data_ptr(), lds[1], v_raw.data_ptr(), lds[2], q_norm_weight.data_ptr(),
+            k_norm_weight.data_ptr(), table.data_ptr(), float(eps), n, out.data_ptr(), keys.data_ptr(),
+            values.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream), 'dspark_verify_prep')
+        self._kernel(out, keys, values, layout, scale=scale, pages=self.pages, layer=layer, out=out)
+        self._staged.add(layer)
+        return out
+
+    @torch.no_grad()
+    def attend(self, tx, layer, query, *, scale=SCALE):
+        """Bottom-right causal attention of already-roped ``query`` over the committed tokens and
+        the staged scratch rows."""
+        self._transaction(tx)
+        if layer not in self._staged:
+            raise ValueError('Layer scratch missing')
+        keys, values = self._scratch(layer, tx.query_tokens)
+        return self._kernel(query, keys, values, self._planned(tx), scale=scale, pages=self.pages, layer=layer)
+
+    def _commit_rows(self, tx, counts):
+        rows = (self.layers, self.max_query_tokens, self.heads, self.dim)
+        self.pages.append(self.scratch_keys.view(rows), self.scratch_values.view(rows), tx.layout, counts)
+
+    def mirror_lengths(self, handles, lengths):
+        """See ``B200PersistentTargetKV.mirror_lengths``; pages for the lengths are taken too."""
+        self._reserve([self._slot(h) for h in handles], [int(n) for n in lengths])
+        super().mirror_lengths(handles, lengths)
+
+    def _device_round(self, handles, bucket, room):
+        indices = [self._slot(h) for h in handles]
+        lengths = [self._lengths[i] for i in indices]
+        if any(c + room > self.capacities[i] for c, i in zip(lengths, indices)):
+            raise ValueError('Request slots cannot hold max_new_tokens plus one verify chunk')
+        self._reserve(indices, [c + room for c in lengths])
+        buffers, qlens = self.bind_bucket(bucket), tuple(bucket.query_lengths)
+        buffers.meta.copy_(torch.tensor(self._host_meta(indices, qlens, lengths), dtype=torch.int32))
+        return Transaction(0, handles, tuple(lengths), qlens, buffers.meta, {}, buffers.table,
+                           layout=self._layout(buffers.meta, qlens, buffers.plan))
+
+    # -- views -------------------------------------------------------------------------
+    def _prefix_rows(self, i, n):
+        """K and V of slot i's first n committed tokens in the store's dtype, pages as the values
+        that their codes stand for (rounded to that dtype)."""
+        parts = [x.reshape(self.layers, -1, self.heads, self.dim).to(self.dtype)
+                 for x in self.pages.values(self._held[i][:n // PAGE])]
+        return tuple(torch.cat((p, t), 1) for p, t in zip(parts, self.pages.open_rows(i, n)))
+
+    def pointers(self):
+        return dict(committed_keys=self.pages.key.data_ptr(), committed_values=self.pages.value.data_ptr(),
+                    scratch_keys=self.scratch_keys.data_ptr(), scratch_values=self.scratch_values.data_ptr())
+
+    def work(self, tx):
+        self._transaction(tx)
+        q = tx.query_tokens
+        actual_k = sum(tx.context_lengths) + q
+        row = 2 * self.heads * self.dim * self.scratch_keys.element_size()
+        page = 2 * self.heads * (PAGE * self.dim + 4)
+        pages = sum(c // PAGE for c in tx.context_lengths)
+        held, tails = self.pages.bytes()
+        return dict(active_requests=len(tx.slots), logical_query_tokens=q, physical_query_tokens=q,
+                    logical_active_key_tokens=actual_k, physical_key_capacity=actual_k, padded_key_capacity=0,
+                    inactive_resident_key_tokens=sum(self._lengths) - sum(tx.context_lengths),
+                    gather_rows_per_kv_per_layer=0, staging_output_rows_per_layer=0,
+                    attention_kv_bytes_per_layer=pages * page + (actual_k - pages * PAGE) * row,
+                    allowed_causal_pairs=sum(c * n + n * (n + 1) // 2
+                                             for c, n in zip(tx.context_lengths, tx.query_lengths)),
+                    query_lengths=list(tx.query_lengths), queried_context_lengths=list(tx.context_lengths),
+                    resident_allocated_kv_bytes=held + tails,
+                    scratch_allocated_kv_bytes=2 * self.scratch_keys.numel() * self.scratch_keys.element_size())

@@ -349,13 +349,11 @@ def speculative_greedy_pipelined(target, draft, prompts, max_new_tokens, eos_ids
     width = size + 1
     store = target.pool
     handles = [target._handles[r] for r in requests]
-    slots = [h.index for h in handles]
     # -- fixed buffers of the three captured programs -----------------------------------
     bucket = QueryBucket((width,) * R)
     if bucket not in target._graphs:
         target.capture(bucket)
     tg = target._graphs[bucket]
-    tmeta = store.bind_bucket(bucket).meta
     if R not in draft.__dict__.get('_graphs', {}):
         draft.capture_propose(R)
     pg = draft._graphs[R]
@@ -364,18 +362,13 @@ def speculative_greedy_pipelined(target, draft, prompts, max_new_tokens, eos_ids
     ag = draft._append_graphs[(R, width)]
     i32 = torch.int32
     cu_t = [width * i for i in range(R + 1)]
-    ctx0 = [store.length(h) for h in handles]
     dlen0 = [draft._lengths[r] for r in requests]
-    if any(c + max_new_tokens + width > store.capacities[s] for c, s in zip(ctx0, slots)):
-        raise ValueError('Request slots cannot hold max_new_tokens plus one verify chunk')
-    tmeta.copy_(torch.tensor(cu_t + [store.slot_rows[s] for s in slots] + ctx0
-                             + [store.capacities[s] for s in slots], dtype=i32))
+    ctx, commit_rows = store.device_rounds(handles, bucket, max_new_tokens + width)   # target lengths (device state)
     pg['meta'].copy_(torch.tensor([size * i for i in range(R + 1)]
                                   + [draft.slot_rows[draft._slots[r]] for r in requests] + dlen0 + [size] * R,
                                   dtype=i32))
     ag['meta'].copy_(torch.tensor(cu_t + [draft.slot_rows[draft._slots[r]] for r in requests] + dlen0 + [0] * R,
                                   dtype=i32))
-    ctx = tmeta[2 * R + 1:3 * R + 1]                  # target context lengths (device state)
     dlen = pg['meta'][2 * R + 1:3 * R + 1]            # draft context lengths (device state)
     anchors = torch.tensor([output[r][-1] for r in requests], dtype=torch.long, device=dev)
     budget = torch.tensor([max_new_tokens - 1 if output[r][-1] not in eos_ids else 0 for r in requests],
@@ -405,12 +398,7 @@ def speculative_greedy_pipelined(target, draft, prompts, max_new_tokens, eos_ids
         logits = lm_head(tg['last'])[0]
         _pred, accepted, n_commit, emitted = greedy_accept(logits, tg['ids'][0], cu_dev, eos_dev, budget)
         # commit the verified prefixes (rollback of the rest), all layers, one launch
-        _lib.check(lib.dspark_commit_kv(
-            store._keys.data_ptr(), store._values.data_ptr(), store.scratch_keys.data_ptr(),
-            store.scratch_values.data_ptr(), tmeta.data_ptr(), tmeta[R + 1:].data_ptr(), ctx.data_ptr(),
-            tmeta[3 * R + 1:].data_ptr(), n_commit.data_ptr(), R, store.layers, store.rows_per_layer,
-            store.max_query_tokens, _lib.DTYPE_F32 if store.dtype == torch.float32 else _lib.DTYPE_BF16,
-            stream.cuda_stream), 'dspark_commit_kv')
+        commit_rows(n_commit)
         ctx.add_(n_commit)
         # the draft projects the committed rows of every verified chunk
         ag['feat'].copy_(tg['context'])

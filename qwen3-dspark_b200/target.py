@@ -34,6 +34,7 @@ from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
 
 from .kernels import HEAD_DIM, HKV, HQ, add_rms_norm, merged_mlp_ready, rms_norm, silu_mul
 from .kv_store import B200PersistentTargetKV
+from .quantized_store import B200QuantizedTargetKV
 
 
 @dataclass
@@ -88,7 +89,10 @@ def _merged_mlp_forward(mlp):
 
 
 class B200Qwen3Target:
-    def __init__(self, model, layer_ids=(), *, slots, context_capacity, max_query_tokens, slot_capacities=None):
+    def __init__(self, model, layer_ids=(), *, slots, context_capacity, max_query_tokens, slot_capacities=None,
+                 cache=None, cache_pages=None):
+        """``cache``: None keeps committed KV in the model's dtype (``B200PersistentTargetKV``); 'int8' or
+        'e4m3' keeps it in 8-bit pages (``B200QuantizedTargetKV``), ``cache_pages`` of them."""
         config = model.config
         if (config.model_type != 'qwen3' or getattr(config, 'use_sliding_window', False)
                 or any(kind != 'full_attention' for kind in config.layer_types)
@@ -105,9 +109,15 @@ class B200Qwen3Target:
             raise ValueError('B200 target needs a bf16 (or exact-path float32) model on a CUDA device')
         self.model = model.eval().requires_grad_(False)
         self.dtype = weight.dtype
-        self.pool = B200PersistentTargetKV(layers=config.num_hidden_layers, slots=slots,
-                                           context_capacity=context_capacity, max_query_tokens=max_query_tokens,
-                                           dtype=self.dtype, device=weight.device, slot_capacities=slot_capacities)
+        sizes = dict(layers=config.num_hidden_layers, slots=slots, context_capacity=context_capacity,
+                     max_query_tokens=max_query_tokens, dtype=self.dtype, device=weight.device,
+                     slot_capacities=slot_capacities)
+        if cache is None:
+            if cache_pages is not None:
+                raise ValueError('cache_pages goes with an 8-bit cache')
+            self.pool = B200PersistentTargetKV(**sizes)
+        else:
+            self.pool = B200QuantizedTargetKV(cache=cache, pages=cache_pages, **sizes)
         self.inv_freq = model.model.rotary_emb.inv_freq.float().contiguous()
         self.eps = config.rms_norm_eps
         self._handles = {}
@@ -193,6 +203,19 @@ class B200Qwen3Target:
         handle = self.pool.add_request(request)
         self._handles[request] = handle
         return handle
+
+    def fork_request(self, request, children):
+        """Continuations of a resident request (8-bit cache): each of the ids ``children``
+        starts with its committed KV, the full pages shared and the open rows copied."""
+        if self._pending is not None:
+            raise RuntimeError('Finish the outstanding verification first')
+        if not isinstance(self.pool, B200QuantizedTargetKV):
+            raise ValueError('Forks need an 8-bit paged cache')
+        if request not in self._handles:
+            raise ValueError('Request not resident')
+        handles = self.pool.fork(self._handles[request], children)
+        self._handles.update((h.request, h) for h in handles)
+        return handles
 
     def remove_request(self, request):
         if self._pending is not None:

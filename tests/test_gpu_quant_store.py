@@ -1,0 +1,218 @@
+"""The target's KV store over 8-bit pages: rounds, forks, compaction, captured programs and the
+decode loops on it."""
+import numpy as np
+import pytest
+import torch
+
+import inputs as I
+import quant_util as U
+from gpu_util import dev, status_clean
+from test_gpu_graph import _Bucket, tiny_bf16_model
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(g, layers, n, heads, dtype):
+    return torch.randn((layers, n, heads, 128), generator=g).to(dtype)
+
+
+def state_of(store, handles, contexts, qlens, q, k, v):
+    """The store's cache and a round as quant_util holds them."""
+    p = store.pages
+    x = {n: getattr(p, n).cpu() for n in ('key', 'value', 'key_scale', 'value_scale', 'tail_key', 'tail_value')}
+    table = torch.full((len(handles), store.table_width), -1, dtype=torch.int32)
+    for r, h in enumerate(handles):
+        held = store._held[h.index]
+        table[r, :len(held)] = torch.tensor(held, dtype=torch.int32)
+    return x, dict(table=table, slots=torch.tensor([h.index for h in handles]), rows=qlens, contexts=contexts, query=q,
+                   new_key=k, new_value=v)
+
+
+def one_round(store, handles, qlens, counts, g, truth, dtype):
+    """Stage, attend and commit a round; the attention against float64 on the store's own
+    contents, and the committed rows against what went in."""
+    layers, n = store.layers, sum(qlens)
+    contexts = [store.length(h) for h in handles]
+    q, k, v = (rows(g, layers, n, h, dtype) for h in (16, 8, 8))
+    tx = store.begin(handles, query_lengths=qlens)
+    for layer in range(layers):
+        store.stage_layer(tx, layer, k[layer].cuda(), v[layer].cuda())
+        got = store.attend(tx, layer, q[layer].cuda()).double().cpu()
+        x, b = state_of(store, handles, contexts, list(qlens), q, k, v)
+        out, weight, size = U.attention(x, b, layer)
+        assert bool(((got - out).abs() <= U.attention_tolerance(out, weight, size, dtype)).all())
+    store.commit(tx, dict(zip(handles, counts)))
+    t = 0
+    for h, m, c in zip(handles, qlens, counts):
+        truth[h] = tuple(torch.cat((old, x[:, t:t + c]), 1) for old, x in zip(truth[h], (k, v)))
+        t += m
+
+
+def check_rows(store, handle, truth, cache):
+    """Committed rows: open ones as they were, quantised ones within half a step of their block."""
+    got = store.request_kv(handle)
+    n = store.length(handle)
+    for a, b in zip(got, truth[handle]):
+        a, b = a.cpu().double(), b.double()
+        assert a.shape == b.shape
+        full = n // 64 * 64
+        assert torch.equal(a[:, full:], b[:, full:])
+        if not full:
+            continue
+        blocks = b[:, :full].reshape(store.layers, -1, 64, 8, 128)
+        top = blocks.abs().amax((2, 4), keepdim=True)
+        # int8: half a step of a / 127. e4m3: half a step of 2^-3 of the value, or of its subnormals
+        # (2^-10 of a / 448). And the value rounded to the rows' dtype.
+        step = (top / 127 / 2).expand(blocks.shape) if cache == 'int8' else \
+            torch.maximum(blocks.abs() * 2.0 ** -4, top / 448 * 2.0 ** -10)
+        tol = step * (1 + 2.0 ** -7) + 2.0 ** -8 * blocks.abs()
+        assert bool(((a[:, :full].reshape(blocks.shape) - blocks).abs() <= tol).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=['bf16', 'fp32'])
+@pytest.mark.parametrize('cache', ['int8', 'e4m3'])
+def test_rounds_forks_and_compaction(pkg, cache, dtype):
+    g = torch.Generator().manual_seed(9)
+    r = np.random.Generator(np.random.PCG64(3))
+    store = pkg.B200QuantizedTargetKV(layers=2, slots=5, context_capacity=400, max_query_tokens=300, cache=cache,
+                                      dtype=dtype, pages=16)
+    truth = {}
+    handles = [store.add_request(n) for n in 'abc']
+    for h, n in zip(handles, (0, 63, 130)):
+        k, v = (rows(g, 2, n, 8, dtype) for _ in range(2))
+        store.load_prefix(h, k.cuda(), v.cuda())
+        truth[h] = (k, v)
+        check_rows(store, h, truth, cache)
+    one_round(store, handles, (150, 1, 3), (150, 1, 0), g, truth, dtype)     # a prompt, a block that fills, nothing
+    for _ in range(4):
+        q = [int(x) for x in r.integers(1, 9, 3)]
+        one_round(store, handles, tuple(q), tuple(int(r.integers(0, x + 1)) for x in q), g, truth, dtype)
+    kids = store.fork(handles[2], ['d', 'e'])
+    for h in kids:
+        truth[h] = truth[handles[2]]
+        check_rows(store, h, truth, cache)
+    free = store.pages.free_pages
+    one_round(store, [*kids, handles[2]], (60, 70, 9), (60, 70, 5), g, truth, dtype)
+    assert store.pages.free_pages < free                                    # the forks grow pages of their own
+    store.remove_request(handles[0])
+    store.remove_request(handles[2])                                         # its shared pages stay
+    moved = store.compact()
+    assert moved > 0 and store.compact() == 0
+    used = [x for x, u in enumerate(store.pages.users) if u]
+    assert used == list(range(len(used)))
+    for h in (handles[1], *kids):
+        check_rows(store, h, truth, cache)
+    one_round(store, [kids[0], handles[1], kids[1]], (2, 5, 1), (2, 5, 1), g, truth, dtype)
+    for h in (handles[1], *kids):
+        check_rows(store, h, truth, cache)
+        store.remove_request(h)
+    assert store.pages.free_pages == 16 and not any(store.pages.users)
+    status_clean(pkg)
+
+
+def test_abort_and_refusals(pkg):
+    store = pkg.B200QuantizedTargetKV(layers=1, slots=2, context_capacity=200, max_query_tokens=130, pages=1)
+    a, b = store.add_request('a'), store.add_request('b')
+    with pytest.raises(ValueError):
+        store.begin([a, b], query_lengths=(64, 64))                          # two pages, one in the pool
+    assert store.pages.free_pages == 1 and store._pending is None
+    tx = store.begin([a, b], query_lengths=(64, 1))
+    with pytest.raises(RuntimeError):
+        store.fork(a, 'c')
+    store.abort(tx)
+    assert store.length(a) == 0
+    with pytest.raises(ValueError):
+        store.fork(a, ['c'])                                                 # no slot left
+    with pytest.raises(ValueError):
+        store.pages.free([0, 0])
+    store.remove_request(b)
+    c, = store.fork(a, 'c')
+    assert store.length(c) == 0
+    with pytest.raises(ValueError):
+        store.begin([a], query_lengths=(201,))
+    with pytest.raises(AttributeError):
+        store.keys
+
+
+@pytest.mark.parametrize('cache', ['int8', 'e4m3'])
+def test_target_graph_equals_eager(pkg, cache):
+    model = tiny_bf16_model()
+    prompts = [torch.from_numpy(ids)[None].to(dev()) for ids in I.greedy_prompts()[:3]]
+    target = pkg.B200Qwen3Target(model, (1, 2), slots=4, context_capacity=2400, max_query_tokens=2500, cache=cache)
+    for i in range(3):
+        target.add_request(f'r{i}')
+    target.prefill({f'r{i}': p for i, p in enumerate(prompts)})
+    bucket = _Bucket((8, 8, 8))
+    target.capture(bucket)
+    g = np.random.Generator(np.random.PCG64(77))
+    for rnd in range(12):                                                    # (some blocks get full on the way)
+        chunks = {f'r{i}': torch.from_numpy(g.integers(0, 1000, (1, 8))).to(dev()) for i in range(3)}
+        ref = target.verify(chunks)
+        want = {r: v.clone() for r, v in target.predict(ref).items()}
+        target.abort(ref)
+        got = target.verify_graph(chunks, bucket)
+        logits = target.predict(got)
+        for r in chunks:
+            assert torch.equal(logits[r], want[r]), (rnd, r)
+        target.commit(got, {f'r{i}': int(x) for i, x in enumerate(g.integers(1, 9, 3))})
+    target.fork_request('r0', ['child'])
+    same = {r: torch.arange(5, device=dev())[None] for r in ('r0', 'child')}
+    out = target.predict(target.verify(same))
+    torch.testing.assert_close(out['child'], out['r0'], rtol=0, atol=0.25)   # cut into other partial rows
+    target.close()
+    status_clean(pkg)
+
+
+def test_short_requests_equal_the_unquantised_target(pkg):
+    """Below 64 tokens nothing is quantised: the float32 target gives the same tokens either way."""
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+    torch.backends.cuda.matmul.allow_tf32 = False
+    cfg = Qwen3Config(**I.TINY_TARGET)
+    cfg._attn_implementation = 'sdpa'
+    model = Qwen3ForCausalLM(cfg).eval()
+    shapes = {k: tuple(v.shape) for k, v in model.state_dict().items()}
+    model.load_state_dict({k: torch.from_numpy(v) for k, v in I.deterministic_state(shapes, 1).items()})
+    model = model.to(dev())
+    prompts = {f'r{i}': torch.arange(3 + 7 * i, device=dev())[None] for i in range(4)}
+    logits = []
+    for cache in (None, 'int8'):
+        target = pkg.B200Qwen3Target(model, (), slots=4, context_capacity=64, max_query_tokens=128, cache=cache)
+        for r in prompts:
+            target.add_request(r)
+        target.prefill(prompts)
+        seen = []
+        for step in range(6):
+            f = target.verify({r: torch.full((1, 4), 11 * step + 1, device=dev()) for r in prompts})
+            seen.append(torch.cat(list(target.predict(f).values()), 1))
+            target.commit(f, {r: 1 + (step + i) % 4 for i, r in enumerate(prompts)})
+        logits.append(torch.cat(seen, 1))
+        target.close()
+    torch.testing.assert_close(logits[1], logits[0], rtol=1e-4, atol=1e-4)
+    status_clean(pkg)
+
+
+@pytest.mark.parametrize('cache', ['int8', 'e4m3'])
+def test_decode_loops_agree(pkg, cache):
+    """Eager, captured and pipelined greedy decoding over an 8-bit cache: the same tokens."""
+    model = tiny_bf16_model()
+    spec = pkg.DraftSpec(**dict(I.TINY_DRAFT, markov_rank=64))
+    outs = []
+    for loop in ('eager', 'graph', 'pipelined'):
+        draft = pkg.DSparkDraftModel(model, spec).eval()
+        dshapes = {k: tuple(v.shape) for k, v in draft.state_dict().items() if not k.startswith(('embedding.', 'lm_head.'))}
+        draft.load_state_dict({k: torch.from_numpy(v) for k, v in I.deterministic_state(dshapes, 2).items()}, strict=False)
+        draft = draft.to(dev(), torch.bfloat16)
+        prompts = {f'r{i}': torch.arange(5 + 61 * i, device=dev())[None] % 900 for i in range(3)}
+        cap = 5 + 61 * 2 + 64 + 16
+        target = pkg.B200Qwen3Target(model, spec.layer_ids, slots=3, context_capacity=cap, max_query_tokens=3 * cap,
+                                     cache=cache)
+        pdraft = pkg.B200PackedDraft(draft, max_requests=3, context_capacity=cap)
+        if loop == 'pipelined':
+            out, _ = pkg.speculative_greedy_pipelined(target, pdraft, prompts, 64)
+        else:
+            out, _ = pkg.speculative_greedy(target, pdraft, prompts, 64, graph=loop == 'graph')
+        outs.append(out)
+        target.close()
+    assert outs[0] == outs[1] == outs[2]
+    assert all(len(v) == 64 for v in outs[0].values())
+    status_clean(pkg)
