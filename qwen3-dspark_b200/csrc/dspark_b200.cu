@@ -513,13 +513,18 @@ int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, 
   return launch_status();
 }
 
+// Every SM full, or as many CTAs as there can be items of full blocks or groups of 8 open rows, in
+// whole rounds over the heads and kinds.
 template <typename T>
-int launch_append(const quant::AppendParams& ap, int code, cudaStream_t stream) {
-  const dim3 grid(ap.batch.requests * ap.blocks, ap.layers, 4);
+int launch_append(const quant::AppendParams& ap, int code, int max_q, int sms, cudaStream_t stream) {
+  const long long blocks = static_cast<long long>(ap.batch.requests) * ((max_q + quant::kPage - 1) / quant::kPage);
+  const long long items = std::max(blocks * quant::kAppendKinds, (static_cast<long long>(ap.batch.rows) + 7) / 8) * ap.layers;
+  const long long most = static_cast<long long>(quant::kAppendCtas<T>) * sms;
+  const unsigned grid = static_cast<unsigned>(std::max(std::min(items, most) / quant::kAppendKinds, 1ll) * quant::kAppendKinds);
   if (code == DSPARK_CODE_INT8)
-    quant::append_kernel<T, quant::kInt8, 2><<<grid, 256, 0, stream>>>(ap);
+    quant::append_kernel<T, quant::kInt8><<<grid, quant::kAppendThreads, 0, stream>>>(ap);
   else
-    quant::append_kernel<T, quant::kE4M3, 2><<<grid, 256, 0, stream>>>(ap);
+    quant::append_kernel<T, quant::kE4M3><<<grid, quant::kAppendThreads, 0, stream>>>(ap);
   return launch_status();
 }
 
@@ -1580,11 +1585,9 @@ int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows
   ap.new_v = new_v;
   ap.new_rows = new_rows;
   ap.layers = cache->num_layers;
-  ap.blocks = (batch->max_q + quant::kPage - 1) / quant::kPage;
   ap.counts = counts;
-  if (static_cast<long long>(ap.batch.requests) * ap.blocks >= (1ll << 31)) return DSPARK_ERR_UNSUPPORTED;
-  return cache->dtype == DSPARK_DTYPE_F32 ? launch_append<float>(ap, cache->code, stream)
-                                          : launch_append<__nv_bfloat16>(ap, cache->code, stream);
+  return cache->dtype == DSPARK_DTYPE_F32 ? launch_append<float>(ap, cache->code, batch->max_q, sms, stream)
+                                          : launch_append<__nv_bfloat16>(ap, cache->code, batch->max_q, sms, stream);
 }
 
 int dspark_quant_copy(const dspark_quant_cache* cache, const int32_t* src, const int32_t* dst, int num,

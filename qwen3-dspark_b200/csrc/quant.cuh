@@ -226,7 +226,7 @@ struct AppendParams {
   const void* new_v;
   long long new_rows;        // rows between the layers of new_k / new_v
   Cache cache;               // layer 0
-  int layers, blocks;        // blocks: full blocks a request can get (grid x / requests)
+  int layers;
   Batch batch;
   const int* counts;         // [R], or null: every new row
 };
@@ -246,6 +246,12 @@ struct Vec8<__nv_bfloat16> {
       x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
+  // The larger of `top` and the largest bits without the sign: of both halves here, of a float below.
+  __device__ __forceinline__ uint32_t top(uint32_t top) const {
+    const uint32_t m = 0x7fff7fffu;
+    return __vmaxu2(__vmaxu2(__vmaxu2(a.x & m, a.y & m), __vmaxu2(a.z & m, a.w & m)), top);
+  }
+  static __device__ __forceinline__ uint32_t top_float(uint32_t top) { return max(top << 16, top & 0xffff0000u); }
 };
 template <>
 struct Vec8<float> {
@@ -261,171 +267,300 @@ struct Vec8<float> {
   __device__ __forceinline__ void get(float (&x)[8]) const {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
+  __device__ __forceinline__ uint32_t top(uint32_t top) const {
+    float x[8];
+    get(x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    return top;
+  }
+  static __device__ __forceinline__ uint32_t top_float(uint32_t top) { return top; }
 };
 
-// Codes of one block and head. Small maxima are scaled up first, or qmax / a would overflow.
+// Codes of one block and head. Blocks of tiny values (a < 2^-100) are scaled by 2^100 first, or
+// qmax / a would overflow.
 template <typename T, int kCode>
 struct Quantizer {
-  float a, pre, inv, scale;
+  float a, inv, scale;
+  bool tiny;
   __device__ __forceinline__ explicit Quantizer(uint32_t max_bits) {
     a = __uint_as_float(max_bits);
     scale = __fdiv_rn(a, code_max<kCode>());
-    pre = a < 0x1p-64f ? 0x1p64f : 1.f;
-    a *= pre;
+    tiny = a < 0x1p-100f;
+    if (tiny) a *= 0x1p100f;
     inv = a > 0.f ? __fdiv_rn(code_max<kCode>(), a) : 0.f;
   }
   __device__ __forceinline__ float quotient(float x) const {
     if (sizeof(T) == 4) {
-      const double q = static_cast<double>(x * pre) * static_cast<double>(code_max<kCode>()) / static_cast<double>(a);
+      const double q = static_cast<double>(tiny ? x * 0x1p100f : x) * static_cast<double>(code_max<kCode>()) / static_cast<double>(a);
       if (kCode == kInt8) return static_cast<float>(rint(q));
       // to odd, so that the second rounding (to e4m3) is the only one that counts
       float f = __double2float_rz(q);
       if (static_cast<double>(f) != q) f = __uint_as_float(__float_as_uint(f) | 1u);
       return f;
     }
-    return __uint_as_float((__float_as_uint(x * pre * inv) + 8u) & ~15u);
+    return __uint_as_float((__float_as_uint(x * inv) + 8u) & ~15u);
   }
   // 4 codes in a word, x[0] lowest
   __device__ __forceinline__ uint32_t code4(float x0, float x1, float x2, float x3) const {
     if (!(a > 0.f)) return 0u;                                // a zero block; a NaN one, whose scale says so
-    const float q[4] = {quotient(x0), quotient(x1), quotient(x2), quotient(x3)};
-    if (kCode == kInt8) {
-      uint32_t w = 0;                                         // rint by adding 1.5 * 2^23: the low byte is the code
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w |= (__float_as_uint(__fadd_rn(q[i], 12582912.f)) & 0xffu) << (8 * i);
-      return w;
+    if (sizeof(T) == 2 && tiny) {
+      x0 *= 0x1p100f;
+      x1 *= 0x1p100f;
+      x2 *= 0x1p100f;
+      x3 *= 0x1p100f;
     }
-    uint32_t lo, hi;
-    asm("{\n\t.reg .b16 x;\n\tcvt.rn.satfinite.e4m3x2.f32 x, %2, %1;\n\tcvt.u32.u16 %0, x;\n\t}" : "=r"(lo) : "f"(q[0]), "f"(q[1]));
-    asm("{\n\t.reg .b16 x;\n\tcvt.rn.satfinite.e4m3x2.f32 x, %2, %1;\n\tcvt.u32.u16 %0, x;\n\t}" : "=r"(hi) : "f"(q[2]), "f"(q[3]));
-    return lo | (hi << 16);
+    const float q[4] = {quotient(x0), quotient(x1), quotient(x2), quotient(x3)};
+    uint32_t w[4];
+    if (kCode == kInt8) {
+      // rint by adding 1.5 * 2^23: the low byte is the code
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(__fadd_rn(q[i], 12582912.f));
+      return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+    }
+    asm("{\n\t.reg .b16 p, q;\n\tcvt.rn.satfinite.e4m3x2.f32 p, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 q, %4, %3;\n\t"
+        "mov.b32 %0, {p, q};\n\t}"
+        : "=r"(w[0])
+        : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+    return w[0];
   }
 };
 
-// Quantises K and V of one (block, head): rows base(t) for t = 0 .. 63. Thread (g, c) of the
-// 256 takes rows 4 g .. 4 g + 3 (g = 2 warp + lane / 16) and dims 8 c .. 8 c + 7, so that a
-// warp's loads are whole 256-byte rows and a thread holds four tokens of a dim, one word of V.
-struct QuantSmem {
-  uint32_t top[2][8];
+// Persistent CTAs (256 threads). Each looks at the batch itself, 256 requests at a time: how many
+// blocks get full and which rows stay open. Then all of them share two lists. First the full
+// blocks: an item is K or V of one (block, head, layer), 64 x 128 values; a CTA keeps its head and
+// kind, so that 16 neighbours read whole rows. Thread (g, c) takes rows 4 g .. 4 g + 3
+// (g = 2 warp + lane / 16) and dims 8 c .. 8 c + 7, so that a warp's loads are whole 256 bytes of a
+// head and a thread holds four tokens of a dim, one word of V; the next item's loads are issued
+// before this one is reduced. Then the open rows, K and V of one (row, layer) a
+// warp. Bound by the bytes where blocks get full; a round of a few rows by the look at the batch
+// and one pass over its rows.
+//
+// An item that reads the tail and open rows that are written there lie in different tail blocks,
+// unless two (four, ..) blocks of the request get full in one append. Then the items of its
+// first block write their head's open rows themselves, behind the values that they have read.
+constexpr int kAppendThreads = 256, kAppendKinds = 2 * kKVHeads;
+template <typename T>
+constexpr int kAppendCtas = sizeof(T) == 2 ? 4 : 2;            // of an SM
+struct AppendSmem {
+  uint32_t top[8];
+  int sum[2][8];
   uint32_t v[kHeadDim * 16];                                  // [dim][token / 4], columns rotated by dim / 8
+  int full[kAppendThreads], open[kAppendThreads];             // inclusive sums over the requests
+  int q0[kAppendThreads], ctx[kAppendThreads], slot[kAppendThreads], n[kAppendThreads];
 };
-template <typename T, int kCode, typename RowOf>
-__device__ __forceinline__ void quantize_block(const Cache& c, size_t page_head, const RowOf& row_of, QuantSmem& sm) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = 2 * warp + (lane >> 4), d0 = 8 * (lane & 15);
-  Vec8<T> x[2][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const T *k, *v;
-    row_of(4 * g + i, k, v);
-    x[0][i].load(k + d0);
-    x[1][i].load(v + d0);
+struct AppendItem {
+  int request, layer, block;                                  // block: of the request; request: of the 256
+};
+
+// Index of the first of `num` sums above x.
+__device__ __forceinline__ int find_above(const int* sums, int num, int x) {
+  int lo = 0, hi = num - 1;
+#pragma unroll 1
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] > x) hi = mid; else lo = mid + 1;
   }
-  uint32_t top[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    top[s] = 0u;                                              // of the bits without the sign: a NaN is the largest
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[8];
-      x[s][i].get(f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top[s] = max(top[s], __float_as_uint(f[e]) & 0x7fffffffu);
-    }
-    top[s] = __reduce_max_sync(0xffffffffu, top[s]);
-    if (lane == 0) sm.top[s][warp] = top[s];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top[s] = max(top[s], sm.top[s][w]);
-  }
-  const Quantizer<T, kCode> qk(top[0]), qv(top[1]);
-  uint8_t* kd = c.key + page_head * kHeadBytes + (d0 >> 6) * (kPage * 64) + (d0 & 63);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float f[8];
-    x[0][i].get(f);
-    *reinterpret_cast<uint2*>(kd + (4 * g + i) * 64) =
-        make_uint2(qk.code4(f[0], f[1], f[2], f[3]), qk.code4(f[4], f[5], f[6], f[7]));
-  }
-  float f[4][8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[1][i].get(f[i]);
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    sm.v[(d0 + e) * 16 + (g ^ (lane & 15))] = qv.code4(f[0][e], f[1][e], f[2][e], f[3][e]);
-  __syncthreads();
-  uint4* vd = reinterpret_cast<uint4*>(c.value + page_head * kHeadBytes);
-#pragma unroll
-  for (int u = tid; u < kHeadDim * 4; u += 256) {
-    const int d = u >> 2, w = 4 * (u & 3);
-    const uint32_t* s = sm.v + d * 16;
-    const int rot = (d >> 3) & 15;
-    vd[u] = make_uint4(s[w ^ rot], s[(w + 1) ^ rot], s[(w + 2) ^ rot], s[(w + 3) ^ rot]);
-  }
-  if (tid == 0) {
-    c.key_scale[page_head] = qk.scale;
-    c.value_scale[page_head] = qv.scale;
-  }
-  __syncthreads();                                            // sm is written again
+  return lo;
+}
+__device__ __forceinline__ bool tails_collide(int ctx, int n) {
+  const int full = (ctx + n) / kPage - ctx / kPage;
+  return full >= 2 && (full & 1) == 0 && ctx % kPage != 0;
 }
 
-// Grid (requests x blocks, layers, 8 / kHeads): CTA b of a request quantises its b-th block
-// that gets full; the first one also copies the rows that stay open, behind the block that it
-// reads (with 128 or more new rows both may lie in the same tail block).
-template <typename T, int kCode, int kHeads>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  __shared__ QuantSmem sm;
-  const int i = blockIdx.x / p.blocks, b = blockIdx.x % p.blocks, layer = blockIdx.y, h0 = blockIdx.z * kHeads;
-  const Request r = load_request(p.batch, p.cache, i);
-  const int n = p.counts != nullptr ? p.counts[i] : r.q_len;
-  const int first = r.ctx / kPage, end = r.ok && n >= 0 ? (r.ctx + n) / kPage : 0;
-  if (!r.ok || n < 0 || n > r.q_len || end > p.batch.width || end - first > p.blocks) {
-    if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
-    return;
-  }
-  if (n == 0 || (b > 0 && first + b >= end)) return;
-  Cache c = p.cache;
-  c.key += static_cast<size_t>(layer) * c.pages * kPageBytes;
-  c.value += static_cast<size_t>(layer) * c.pages * kPageBytes;
-  c.key_scale += static_cast<size_t>(layer) * c.pages * kKVHeads;
-  c.value_scale += static_cast<size_t>(layer) * c.pages * kKVHeads;
-  const size_t tail_layer = static_cast<size_t>(layer) * c.slots * 2 * kPage;
-  T* tk = static_cast<T*>(c.tail_key) + tail_layer * kRowElems;
-  T* tv = static_cast<T*>(c.tail_value) + tail_layer * kRowElems;
-  const size_t new0 = (static_cast<size_t>(layer) * p.new_rows + r.q0) * kRowElems;
-  const T* nk = static_cast<const T*>(p.new_k) + new0;
-  const T* nv = static_cast<const T*>(p.new_v) + new0;
-  if (first + b < end) {
-    const int id = r.table[first + b];
-    if (id < 0 || id >= c.pages) {
-      if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
-      return;
+template <typename T>
+struct AppendRows {
+  const T *tail, *fresh;                                      // of the layer: tail blocks, the batch's new rows
+};
+template <typename T>
+__device__ __forceinline__ AppendRows<T> rows_of(const AppendParams& p, int layer, bool value) {
+  const size_t tail = static_cast<size_t>(layer) * p.cache.slots * 2 * kPage * kRowElems;
+  return {static_cast<const T*>(value ? p.cache.tail_value : p.cache.tail_key) + tail,
+          static_cast<const T*>(value ? p.new_v : p.new_k) + static_cast<size_t>(layer) * p.new_rows * kRowElems};
+}
+
+template <typename T, int kCode>
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T>) append_kernel(const AppendParams p) {
+  __shared__ AppendSmem sm;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = 2 * warp + (lane >> 4), d0 = 8 * (lane & 15);
+#pragma unroll 1
+  for (int base = 0; base < p.batch.requests; base += kAppendThreads) {
+    int full = 0, open = 0, q0 = 0, ctx = 0, slot = 0, n = 0;
+    if (base + tid < p.batch.requests) {
+      const Request r = load_request(p.batch, p.cache, base + tid);
+      n = p.counts != nullptr ? p.counts[base + tid] : r.q_len;
+      if (!r.ok || n < 0 || n > r.q_len || (r.ctx + n) / kPage > p.batch.width) {
+        n = 0;
+        if (blockIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
+      } else {
+        q0 = r.q0;
+        ctx = r.ctx;
+        slot = r.slot;
+        full = (ctx + n) / kPage - ctx / kPage;
+        open = tails_collide(ctx, n) ? 0 : (full > 0 ? (ctx + n) % kPage : n);
+      }
+    }
+    sm.q0[tid] = q0;
+    sm.ctx[tid] = ctx;
+    sm.slot[tid] = slot;
+    sm.n[tid] = n;
+    int f = full, o = open;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int fu = __shfl_up_sync(0xffffffffu, f, d), ou = __shfl_up_sync(0xffffffffu, o, d);
+      if (lane >= d) {
+        f += fu;
+        o += ou;
+      }
+    }
+    if (lane == 31) {
+      sm.sum[0][warp] = f;
+      sm.sum[1][warp] = o;
+    }
+    __syncthreads();
+    int fulls = 0, opens = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) {
+        f += sm.sum[0][w];
+        o += sm.sum[1][w];
+      }
+      fulls += sm.sum[0][w];
+      opens += sm.sum[1][w];
+    }
+    sm.full[tid] = f;
+    sm.open[tid] = o;
+    __syncthreads();
+    const int num = min(kAppendThreads, p.batch.requests - base);
+    // full blocks: items (layer, block), the grid a multiple of the 16 heads and kinds
+    const int kind = blockIdx.x % kAppendKinds, head = kind >> 1, step = gridDim.x / kAppendKinds;
+    const bool value = kind & 1;
+    const int step_block = fulls > 0 ? step % fulls : 0, step_layer = fulls > 0 ? step / fulls : 0;
+    int block = 0, layer = p.layers;                          // of the item that is loaded next
+    if (fulls > 0) {
+      block = blockIdx.x / kAppendKinds % fulls;
+      layer = blockIdx.x / kAppendKinds / fulls;
+    }
+    auto take = [&]() {
+      AppendItem x;
+      x.layer = layer;
+      x.request = find_above(sm.full, num, block);
+      x.block = block - (x.request > 0 ? sm.full[x.request - 1] : 0);
+      block += step_block;
+      layer += step_layer;
+      if (block >= fulls) {
+        block -= fulls;
+        ++layer;
+      }
+      return x;
+    };
+    auto load = [&](const AppendItem& x, Vec8<T>(&v)[4]) {
+      const AppendRows<T> rows = rows_of<T>(p, x.layer, value);
+      const int c = sm.ctx[x.request], t0 = (c / kPage + x.block) * kPage + 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i;
+        const size_t row = t < c ? tail_row(sm.slot[x.request], t) : static_cast<size_t>(sm.q0[x.request] + t - c);
+        v[i].load((t < c ? rows.tail : rows.fresh) + row * kRowElems + head * kHeadDim + d0);
+      }
+    };
+    Vec8<T> next[4];
+    AppendItem x{};
+    bool more = layer < p.layers;
+    if (more) {
+      x = take();
+      load(x, next);
     }
 #pragma unroll 1
-    for (int h = h0; h < h0 + kHeads; ++h) {
-      quantize_block<T, kCode>(c, static_cast<size_t>(id) * kKVHeads + h, [&](int t, const T*& k, const T*& v) {
-        const int token = (first + b) * kPage + t;
-        const bool old = token < r.ctx;
-        const size_t at = (old ? tail_row(r.slot, token) : static_cast<size_t>(token - r.ctx)) * kRowElems + h * kHeadDim;
-        k = (old ? tk : nk) + at;
-        v = (old ? tv : nv) + at;
-      }, sm);
+    while (more) {
+      Vec8<T> cur[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cur[i] = next[i];
+      const AppendItem me = x;
+      const int c = sm.ctx[me.request];
+      const int id = p.batch.table[static_cast<size_t>(base + me.request) * p.batch.width + c / kPage + me.block];
+      more = layer < p.layers;
+      if (more) {
+        x = take();
+        load(x, next);
+      }
+      uint32_t top = 0;                                       // of the bits without the sign: a NaN is the largest
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = cur[i].top(top);
+      top = __reduce_max_sync(0xffffffffu, Vec8<T>::top_float(top));
+      if (lane == 0) sm.top[warp] = top;
+      __syncthreads();                                        // (and the last item's codes have left sm.v)
+#pragma unroll
+      for (int w = 0; w < 8; ++w) top = max(top, sm.top[w]);
+      const Quantizer<T, kCode> q(top);
+      const bool ok = id >= 0 && id < p.cache.pages;          // (uniform over the CTA)
+      if (!ok && tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
+      const size_t page = (static_cast<size_t>(me.layer) * p.cache.pages + (ok ? id : 0)) * kKVHeads + head;
+      if (!value) {
+        uint8_t* kd = p.cache.key + page * kHeadBytes + (d0 >> 6) * (kPage * 64) + (d0 & 63);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float e[8];
+          cur[i].get(e);
+          if (ok)
+            *reinterpret_cast<uint2*>(kd + (4 * g + i) * 64) =
+                make_uint2(q.code4(e[0], e[1], e[2], e[3]), q.code4(e[4], e[5], e[6], e[7]));
+        }
+        if (ok && tid == 0) p.cache.key_scale[page] = q.scale;
+        __syncthreads();
+      } else {
+        float e[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cur[i].get(e[i]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sm.v[(d0 + k) * 16 + (g ^ (lane & 15))] = q.code4(e[0][k], e[1][k], e[2][k], e[3][k]);
+        __syncthreads();
+        uint4* vd = reinterpret_cast<uint4*>(p.cache.value + page * kHeadBytes);
+#pragma unroll
+        for (int u = tid; u < kHeadDim * 4; u += kAppendThreads) {
+          const uint32_t* w = sm.v + (u >> 2) * 16;
+          const int j = 4 * (u & 3), rot = (u >> 5) & 15;
+          if (ok) vd[u] = make_uint4(w[j ^ rot], w[(j + 1) ^ rot], w[(j + 2) ^ rot], w[(j + 3) ^ rot]);
+        }
+        if (ok && tid == 0) p.cache.value_scale[page] = q.scale;
+      }
+      if (me.block == 0 && tails_collide(c, sm.n[me.request])) {
+        // every thread of the CTA has its values of the tail: the open rows may take their place
+        const AppendRows<T> rows = rows_of<T>(p, me.layer, value);
+        const int low = (c + sm.n[me.request]) / kPage * kPage, left = c + sm.n[me.request] - low;
+        for (int u = tid; u < left * 16; u += kAppendThreads) {
+          const int t = low + (u >> 4), at = head * kHeadDim + 8 * (u & 15);
+          Vec8<T> v;
+          v.load(rows.fresh + static_cast<size_t>(sm.q0[me.request] + t - c) * kRowElems + at);
+          v.store(const_cast<T*>(rows.tail) + tail_row(sm.slot[me.request], t) * kRowElems + at);
+        }
+      }
     }
-  }
-  if (b > 0) return;
-  const int low = max(r.ctx, end * kPage), rows = r.ctx + n - low;
-  constexpr int kVecs = kHeads * kHeadDim / 8;
-  for (int u = threadIdx.x; u < rows * kVecs; u += 256) {
-    const int token = low + u / kVecs, e = h0 * kHeadDim + (u % kVecs) * 8;
-    const size_t from = static_cast<size_t>(token - r.ctx) * kRowElems + e, to = tail_row(r.slot, token) * kRowElems + e;
-    Vec8<T> a, v;
-    a.load(nk + from);
-    v.load(nv + from);
-    a.store(tk + to);
-    v.store(tv + to);
+    // open rows: (layer, row), the row fastest
+    const long long rows = static_cast<long long>(opens) * p.layers;
+    constexpr int kWarps = kAppendThreads / 32, kVecs = kRowElems / 8 / 32;
+#pragma unroll 1
+    for (long long i = static_cast<long long>(blockIdx.x) * kWarps + warp; i < rows; i += static_cast<long long>(gridDim.x) * kWarps) {
+      const int layer = static_cast<int>(i / opens), o_at = static_cast<int>(i % opens);
+      const int r = find_above(sm.open, num, o_at), c = sm.ctx[r], end = c + sm.n[r];
+      const int t = max(c, end / kPage * kPage) + o_at - (r > 0 ? sm.open[r - 1] : 0);
+      const size_t from = static_cast<size_t>(sm.q0[r] + t - c) * kRowElems + 8 * lane;
+      const size_t to = tail_row(sm.slot[r], t) * kRowElems + 8 * lane;
+      const AppendRows<T> k = rows_of<T>(p, layer, false), v = rows_of<T>(p, layer, true);
+      Vec8<T> a[2][kVecs];
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) {
+        a[0][u].load(k.fresh + from + 256 * u);
+        a[1][u].load(v.fresh + from + 256 * u);
+      }
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) {
+        a[0][u].store(const_cast<T*>(k.tail) + to + 256 * u);
+        a[1][u].store(const_cast<T*>(v.tail) + to + 256 * u);
+      }
+    }
+    __syncthreads();                                          // the lists are made again
   }
 }
 
