@@ -13,6 +13,7 @@
 // wait unquantised in block (n / 64) & 1 of its slot's two tail blocks [2][64][8][128]. Blocks
 // alternate, so an append that fills one writes the rows behind it into the other.
 #pragma once
+#include <type_traits>
 #include "attention.cuh"
 
 namespace dspark {
@@ -301,14 +302,20 @@ struct Quantizer {
     }
     return __uint_as_float((__float_as_uint(x * inv) + 8u) & ~15u);
   }
+  // Whether codes are quotients of the values as they are. Not: a zero block, and a NaN one, whose
+  // scale says so (codes 0); a tiny one.
+  __device__ __forceinline__ bool plain() const { return a > 0.f && !(sizeof(T) == 2 && tiny); }
   // 4 codes in a word, x[0] lowest
+  template <bool kPlain>
   __device__ __forceinline__ uint32_t code4(float x0, float x1, float x2, float x3) const {
-    if (!(a > 0.f)) return 0u;                                // a zero block; a NaN one, whose scale says so
-    if (sizeof(T) == 2 && tiny) {
-      x0 *= 0x1p100f;
-      x1 *= 0x1p100f;
-      x2 *= 0x1p100f;
-      x3 *= 0x1p100f;
+    if (!kPlain) {
+      if (!(a > 0.f)) return 0u;
+      if (sizeof(T) == 2) {
+        x0 *= 0x1p100f;
+        x1 *= 0x1p100f;
+        x2 *= 0x1p100f;
+        x3 *= 0x1p100f;
+      }
     }
     const float q[4] = {quotient(x0), quotient(x1), quotient(x2), quotient(x3)};
     uint32_t w[4];
@@ -329,10 +336,9 @@ struct Quantizer {
 // Persistent CTAs (256 threads). Each looks at the batch itself, 256 requests at a time: how many
 // blocks get full and which rows stay open. Then all of them share two lists. First the full
 // blocks: an item is K or V of one (block, head, layer), 64 x 128 values; a CTA keeps its head and
-// kind, so that 16 neighbours read whole rows. Thread (g, c) takes rows 4 g .. 4 g + 3
-// (g = 2 warp + lane / 16) and dims 8 c .. 8 c + 7, so that a warp's loads are whole 256 bytes of a
-// head and a thread holds four tokens of a dim, one word of V; the next item's loads are issued
-// before this one is reduced. Then the open rows, K and V of one (row, layer) a
+// kind, so that 16 neighbours read whole rows. Thread (g, c) takes rows 4 g .. 4 g + 3 and dims
+// 8 c .. 8 c + 7: eight lanes of a warp read 128 bytes of a row, and a thread holds four tokens of a
+// dim, one word of V. The next item's loads are issued before this one is reduced. Then the open rows, K and V of one (row, layer) a
 // warp. Bound by the bytes where blocks get full; a round of a few rows by the look at the batch
 // and one pass over its rows.
 //
@@ -345,7 +351,7 @@ constexpr int kAppendCtas = sizeof(T) == 2 ? 4 : 2;            // of an SM
 struct AppendSmem {
   uint32_t top[8];
   int sum[2][8];
-  uint32_t v[kHeadDim * 16];                                  // [dim][token / 4], columns rotated by dim / 8
+  uint4 v[kHeadDim * 4];                                      // [dim][token / 16], columns permuted by dim / 8
   int full[kAppendThreads], open[kAppendThreads];             // inclusive sums over the requests
   int q0[kAppendThreads], ctx[kAppendThreads], slot[kAppendThreads], n[kAppendThreads];
 };
@@ -383,7 +389,7 @@ template <typename T, int kCode>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T>) append_kernel(const AppendParams p) {
   __shared__ AppendSmem sm;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = 2 * warp + (lane >> 4), d0 = 8 * (lane & 15);
+  const int g = 4 * (warp >> 1) + (lane >> 3), c8 = 8 * (warp & 1) + (lane & 7), d0 = 8 * c8;
 #pragma unroll 1
   for (int base = 0; base < p.batch.requests; base += kAppendThreads) {
     int full = 0, open = 0, q0 = 0, ctx = 0, slot = 0, n = 0;
@@ -458,11 +464,19 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T>) append_kernel(
     auto load = [&](const AppendItem& x, Vec8<T>(&v)[4]) {
       const AppendRows<T> rows = rows_of<T>(p, x.layer, value);
       const int c = sm.ctx[x.request], t0 = (c / kPage + x.block) * kPage + 4 * g;
+      const size_t at = head * kHeadDim + d0;
+      const long long fresh = sm.q0[x.request] + t0 - c;       // row of the batch (only the tail's come before it)
+      if (x.block > 0 || c % kPage == 0) {
+        const T* src = rows.fresh + fresh * kRowElems + at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i].load(src + i * kRowElems);
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int t = t0 + i;
-        const size_t row = t < c ? tail_row(sm.slot[x.request], t) : static_cast<size_t>(sm.q0[x.request] + t - c);
-        v[i].load((t < c ? rows.tail : rows.fresh) + row * kRowElems + head * kHeadDim + d0);
+        const bool old = t0 + i < c;
+        v[i].load((old ? rows.tail : rows.fresh) +
+                  (old ? static_cast<long long>(tail_row(sm.slot[x.request], t0 + i)) : fresh + i) * kRowElems + at);
       }
     };
     Vec8<T> next[4];
@@ -497,34 +511,33 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T>) append_kernel(
       const bool ok = id >= 0 && id < p.cache.pages;          // (uniform over the CTA)
       if (!ok && tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
       const size_t page = (static_cast<size_t>(me.layer) * p.cache.pages + (ok ? id : 0)) * kKVHeads + head;
-      if (!value) {
-        uint8_t* kd = p.cache.key + page * kHeadBytes + (d0 >> 6) * (kPage * 64) + (d0 & 63);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float e[8];
-          cur[i].get(e);
-          if (ok)
-            *reinterpret_cast<uint2*>(kd + (4 * g + i) * 64) =
-                make_uint2(q.code4(e[0], e[1], e[2], e[3]), q.code4(e[4], e[5], e[6], e[7]));
-        }
-        if (ok && tid == 0) p.cache.key_scale[page] = q.scale;
-        __syncthreads();
-      } else {
+      auto store = [&](auto plain) {
+        constexpr bool kPlain = decltype(plain)::value;
         float e[4][8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) cur[i].get(e[i]);
+        if (!value) {
+          uint8_t* kd = p.cache.key + page * kHeadBytes + (d0 >> 6) * (kPage * 64) + (d0 & 63) + 4 * g * 64;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sm.v[(d0 + k) * 16 + (g ^ (lane & 15))] = q.code4(e[0][k], e[1][k], e[2][k], e[3][k]);
-        __syncthreads();
+          for (int i = 0; i < 4; ++i) {
+            const uint2 w = make_uint2(q.template code4<kPlain>(e[i][0], e[i][1], e[i][2], e[i][3]),
+                                       q.template code4<kPlain>(e[i][4], e[i][5], e[i][6], e[i][7]));
+            if (ok) *reinterpret_cast<uint2*>(kd + i * 64) = w;
+          }
+        } else {
+          uint32_t* w = reinterpret_cast<uint32_t*>(sm.v) + d0 * 16 + 4 * ((g >> 2) ^ (c8 & 3)) + (g & 3);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[16 * k] = q.template code4<kPlain>(e[0][k], e[1][k], e[2][k], e[3][k]);
+        }
+      };
+      if (q.plain()) store(std::true_type{}); else store(std::false_type{});
+      __syncthreads();
+      if (value && ok) {
         uint4* vd = reinterpret_cast<uint4*>(p.cache.value + page * kHeadBytes);
 #pragma unroll
-        for (int u = tid; u < kHeadDim * 4; u += kAppendThreads) {
-          const uint32_t* w = sm.v + (u >> 2) * 16;
-          const int j = 4 * (u & 3), rot = (u >> 5) & 15;
-          if (ok) vd[u] = make_uint4(w[j ^ rot], w[(j + 1) ^ rot], w[(j + 2) ^ rot], w[(j + 3) ^ rot]);
-        }
-        if (ok && tid == 0) p.cache.value_scale[page] = q.scale;
+        for (int u = tid; u < kHeadDim * 4; u += kAppendThreads) vd[u] = sm.v[(u & ~3) + ((u & 3) ^ ((u >> 5) & 3))];
       }
+      if (ok && tid == 0) (value ? p.cache.value_scale : p.cache.key_scale)[page] = q.scale;
       if (me.block == 0 && tails_collide(c, sm.n[me.request])) {
         // every thread of the CTA has its values of the tail: the open rows may take their place
         const AppendRows<T> rows = rows_of<T>(p, me.layer, value);
