@@ -593,8 +593,8 @@ int dspark_varlen_attn_noalloc(const void* q, const void* k, const void* v, cons
  * dspark_quant_attn: bottom-right causal attention of one layer. Keys of request i are its
  * pages' tokens, its open rows and its new rows, of which query row r sees those up to its
  * own. q and out [total_q, 16, 128], new_k / new_v [total_q, 8, 128] in `dtype`; out may be q
- * and otherwise overlaps nothing that is read. bf16 needs the plan and a workspace of
- * dspark_quant_workspace_size bytes, used by this call alone until it is done. A NaN or
+ * and otherwise overlaps nothing that is read. The workspace, of dspark_quant_workspace_size
+ * bytes, is used by this call alone until it is done; bf16 needs the plan too. A NaN or
  * infinity in a new row reaches only the rows that see it.
  *
  * dspark_quant_append: the first counts[i] (null: all) new rows of request i follow its

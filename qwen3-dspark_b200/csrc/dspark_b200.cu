@@ -1546,20 +1546,29 @@ int dspark_quant_attn(const void* q, const void* new_k, const void* new_v, const
   int sms = 0;
   int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < quant::attn_workspace(sms) ||
+      overlap(workspace, workspace_bytes, out, out_bytes) || overlap(workspace, workspace_bytes, q, out_bytes))
+    return DSPARK_ERR_INVALID_ARGUMENT;
   if (cache->dtype == DSPARK_DTYPE_F32) {
+    const int blocks = (batch->max_q + kQBlock - 1) / kQBlock;
+    const long long items = static_cast<long long>(b.requests) * blocks * kKVHeads;
+    if (blocks > 65535) return DSPARK_ERR_UNSUPPORTED;
+    // two CTAs an SM; without as many, the keys are split (the partial rows fit the workspace: 2 x 8 an SM)
+    const int splits = static_cast<int>(std::min<long long>(std::max<long long>(2ll * sms / items, 1), quant::kF32Splits));
     const quant::F32Params fp{static_cast<const float*>(q), static_cast<const float*>(new_k),
-                              static_cast<const float*>(new_v), static_cast<float*>(out), c, b, scale};
-    const dim3 grid(b.requests, (batch->max_q + kQBlock - 1) / kQBlock, kKVHeads);
-    if (grid.y > 65535) return DSPARK_ERR_UNSUPPORTED;
+                              static_cast<const float*>(new_v), static_cast<float*>(out), c, b, scale, splits,
+                              static_cast<float*>(workspace)};
+    const dim3 grid(b.requests, blocks, kKVHeads * splits);
     if (cache->code == DSPARK_CODE_INT8)
       quant::f32_attn_kernel<quant::kInt8><<<grid, quant::kF32AttnThreads, quant::kF32AttnSmem, stream>>>(fp);
     else
       quant::f32_attn_kernel<quant::kE4M3><<<grid, quant::kF32AttnThreads, quant::kF32AttnSmem, stream>>>(fp);
+    st = launch_status();
+    if (st != DSPARK_OK || splits == 1) return st;
+    quant::f32_merge_kernel<<<dim3(b.requests, blocks, kKVHeads), quant::kF32AttnThreads, 0, stream>>>(fp);
     return launch_status();
   }
-  if (!plan || !aligned(plan, 16) || !workspace || !aligned(workspace, 16) || workspace_bytes < quant::attn_workspace(sms) ||
-      overlap(workspace, workspace_bytes, out, out_bytes) || overlap(workspace, workspace_bytes, q, out_bytes))
-    return DSPARK_ERR_INVALID_ARGUMENT;
+  if (!plan || !aligned(plan, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
   const quant::AttnParamsQ ap{static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(new_k),
                               static_cast<const __nv_bfloat16*>(new_v), static_cast<__nv_bfloat16*>(out), c, b, plan, sms,
                               scale * 1.4426950408889634f, static_cast<float*>(workspace)};

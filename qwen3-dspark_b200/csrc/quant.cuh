@@ -85,10 +85,12 @@ __device__ __forceinline__ float2 decode2(uint32_t two) {
 }
 
 // ---------------------------------------------------------------------------
-// Float32 attention on the CUDA cores: one CTA per (request, 8 query rows, KV head), a warp
-// per (row, query head). 64 keys at a time are decoded into shared memory; lane l scores keys
-// l and l + 32 and then holds dims 4 l .. 4 l + 3 of the output.
-constexpr int kF32AttnThreads = 16 * 32;
+// Float32 attention on the CUDA cores: one CTA per (request, 8 query rows, KV head, split), a warp
+// per (row, query head). Steps of 64 keys are decoded into shared memory, the next step's codes
+// on their way meanwhile; lane l scores keys l and l + 32 and then holds dims 4 l .. 4 l + 3 of the
+// output. Bound by the arithmetic of a step (2 us); where the batch has too few CTAs, a request's
+// steps are split among up to 16, whose partial rows a second launch adds up.
+constexpr int kF32AttnThreads = 16 * 32, kF32Splits = 16;
 constexpr int kF32KPitch = kHeadDim + 4;                    // float4 reads of 8 rows hit distinct banks
 constexpr size_t kF32AttnSmem = sizeof(float) * (kPage * kF32KPitch + kPage * kHeadDim + 16 * kHeadDim);
 
@@ -100,7 +102,15 @@ struct F32Params {
   Cache cache;
   Batch batch;
   float scale;
+  int splits;
+  float* part;               // [request][8 rows][8 heads][split][16 * 128 + 32]
 };
+// Partial rows of a CTA (also of the tensor-core kernel): 16 x 128, then (maximum, sum) per row.
+constexpr int kPartFloats = 16 * kHeadDim + 32;
+__device__ __forceinline__ float* f32_part(const F32Params& p, int head) {
+  const size_t item = (static_cast<size_t>(blockIdx.x) * gridDim.y + blockIdx.y) * kKVHeads + head;
+  return p.part + item * p.splits * kPartFloats;
+}
 
 template <int kCode>
 __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Params p) {
@@ -108,7 +118,8 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
   float* sk = reinterpret_cast<float*>(smem4);
   float* sv = sk + kPage * kF32KPitch;
   float* sq = sv + kPage * kHeadDim;
-  const int h = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.z % kKVHeads, split = blockIdx.z / kKVHeads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Request req = load_request(p.batch, p.cache, blockIdx.x);
   const int r0 = blockIdx.y * kQBlock;
   if (!req.ok) {
@@ -127,21 +138,37 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
   const float* nk = p.new_k + static_cast<size_t>(req.q0) * kRowElems + h * kHeadDim;
   const float* nv = p.new_v + static_cast<size_t>(req.q0) * kRowElems + h * kHeadDim;
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int step = 0; step < full + (visible + kPage - 1) / kPage; ++step) {
-    float ks = 1.f, vs = 1.f;
-    int keys = kPage, limit = kPage;                          // keys loaded; keys that this warp's row sees
+  const int steps = full + (visible + kPage - 1) / kPage;
+  const int first = static_cast<int>(static_cast<long long>(steps) * split / p.splits);
+  const int last = static_cast<int>(static_cast<long long>(steps) * (split + 1) / p.splits);
+  uint4 kc = make_uint4(0u, 0u, 0u, 0u), vc = kc;
+  float ks = 0.f, vs = 0.f;
+  int id = -1;
+  auto fetch = [&](int step) {                                // codes and scales of a page
+    id = -1;
+    if (step >= min(full, last)) return;
+    id = req.table[step];
+    if (id < 0 || id >= p.cache.pages) {                      // (uniform over the CTA)
+      if (tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
+      id = -1;
+      return;
+    }
+    const size_t at = static_cast<size_t>(id) * kKVHeads + h;
+    ks = p.cache.key_scale[at];
+    vs = p.cache.value_scale[at];
+    kc = reinterpret_cast<const uint4*>(p.cache.key + at * kHeadBytes)[tid];
+    vc = reinterpret_cast<const uint4*>(p.cache.value + at * kHeadBytes)[tid];
+  };
+  fetch(first);
+#pragma unroll 1
+  for (int step = first; step < last; ++step) {
+    float pks = 1.f, pvs = 1.f;
+    int limit = kPage;                                        // keys that this warp's row sees
     __syncthreads();
     if (step < full) {
-      const int id = req.table[step];
-      if (id < 0 || id >= p.cache.pages) {                    // (uniform over the CTA)
-        if (tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
-        continue;
-      }
-      const size_t at = static_cast<size_t>(id) * kKVHeads + h;
-      ks = p.cache.key_scale[at];
-      vs = p.cache.value_scale[at];
-      const uint4 kc = reinterpret_cast<const uint4*>(p.cache.key + at * kHeadBytes)[tid];
-      const uint4 vc = reinterpret_cast<const uint4*>(p.cache.value + at * kHeadBytes)[tid];
+      const bool there = id >= 0;
+      pks = ks;
+      pvs = vs;
       const uint32_t kw[4] = {kc.x, kc.y, kc.z, kc.w}, vw[4] = {vc.x, vc.y, vc.z, vc.w};
       float* kd = sk + ((tid & 255) >> 2) * kF32KPitch + (tid >> 8) * 64 + (tid & 3) * 16;
       float* vd = sv + (tid & 3) * 16 * kHeadDim + (tid >> 2);
@@ -155,9 +182,10 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
         vd[(4 * w + 2) * kHeadDim] = d.x;
         vd[(4 * w + 3) * kHeadDim] = d.y;
       }
+      fetch(step + 1);
+      if (!there) continue;
     } else {
-      const int t0 = (step - full) * kPage;
-      keys = min(kPage, visible - t0);
+      const int t0 = (step - full) * kPage, keys = min(kPage, visible - t0);
       limit = min(keys, tail + row + 1 - t0);
       for (int u = tid; u < keys * 32; u += kF32AttnThreads) {
         const int t = t0 + (u >> 5), d = 4 * (u & 31);
@@ -167,6 +195,7 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
       }
     }
     __syncthreads();
+    if (!live) continue;                                      // (a whole warp)
     float s[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -181,7 +210,7 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
           dot = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, dot))));
         }
       }
-      s[e] = j < limit ? dot * (ks * p.scale) : -INFINITY;
+      s[e] = j < limit ? dot * (pks * p.scale) : -INFINITY;
     }
     float mx = fmaxf(s[0], s[1]);
 #pragma unroll
@@ -194,6 +223,7 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
     l = l * alpha + sum;
     m = mn;
     float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int j = 0; j < limit; ++j) {                         // (keys that the row does not see are not touched)
       const float w = __shfl_sync(0xffffffffu, j < 32 ? e0 : e1, j & 31);
       const float4 v = *reinterpret_cast<const float4*>(sv + j * kHeadDim + 4 * lane);
@@ -203,10 +233,51 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
       a[3] = fmaf(w, v.w, a[3]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = fmaf(a[i], vs, o[i] * alpha);
+    for (int i = 0; i < 4; ++i) o[i] = fmaf(a[i], pvs, o[i] * alpha);
   }
-  if (live)
+  if (!live) return;
+  if (p.splits == 1) {
     *reinterpret_cast<float4*>(p.out + q_at + 4 * lane) = make_float4(o[0] / l, o[1] / l, o[2] / l, o[3] / l);
+    return;
+  }
+  float* part = f32_part(p, h) + static_cast<size_t>(split) * kPartFloats;
+  reinterpret_cast<float4*>(part + warp * kHeadDim)[lane] = make_float4(o[0], o[1], o[2], o[3]);
+  if (lane == 0) reinterpret_cast<float2*>(part + 16 * kHeadDim)[warp] = make_float2(m, l);
+}
+
+// Grid (requests, 8-row blocks, heads): adds up the splits of f32_attn_kernel, a warp a row.
+__global__ void __launch_bounds__(kF32AttnThreads) f32_merge_kernel(const F32Params p) {
+  const int h = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Request req = load_request(p.batch, p.cache, blockIdx.x);
+  const int row = blockIdx.y * kQBlock + (warp & 7);
+  if (!req.ok || row >= req.q_len) return;
+  const float* part = f32_part(p, h);
+  float m = -INFINITY, l = 0.f;
+  float4 v[kF32Splits];
+  float2 ml[kF32Splits];
+#pragma unroll
+  for (int s = 0; s < kF32Splits; ++s) {
+    ml[s] = make_float2(-INFINITY, 0.f);
+    v[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s < p.splits) {
+      ml[s] = reinterpret_cast<const float2*>(part + s * kPartFloats + 16 * kHeadDim)[warp];
+      v[s] = reinterpret_cast<const float4*>(part + s * kPartFloats + warp * kHeadDim)[lane];
+    }
+    m = fmaxf(m, ml[s].x);
+  }
+  const float mu = m == -INFINITY ? 0.f : m;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < kF32Splits; ++s) {
+    const float w = expf(ml[s].x - mu);
+    l = fmaf(ml[s].y, w, l);
+    o[0] = fmaf(v[s].x, w, o[0]);
+    o[1] = fmaf(v[s].y, w, o[1]);
+    o[2] = fmaf(v[s].z, w, o[2]);
+    o[3] = fmaf(v[s].w, w, o[3]);
+  }
+  const size_t at = (static_cast<size_t>(req.q0 + row) * kQHeads + 2 * h + (warp >> 3)) * kHeadDim + 4 * lane;
+  *reinterpret_cast<float4*>(p.out + at) = make_float4(o[0] / l, o[1] / l, o[2] / l, o[3] / l);
 }
 
 // ---------------------------------------------------------------------------

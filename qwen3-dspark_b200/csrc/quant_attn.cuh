@@ -229,8 +229,7 @@ struct AttnParamsQ {
   float scale_log2;
   float* part;               // [grid][2][8][16 * 128 + 32]
 };
-// Partial rows of one (CTA, slot, head): 16 x 128 float32, then (maximum, sum) per row.
-constexpr int kPartFloats = 16 * kHeadDim + 32;
+// Partial rows of one (CTA, slot, head).
 __host__ __device__ inline size_t part_index(int cta, int slot, int head) {
   return ((static_cast<size_t>(cta) * 2 + slot) * kKVHeads + head) * kPartFloats;
 }

@@ -15,7 +15,6 @@ bf16 rows run on the tensor cores, float32 rows (the exact configuration) on CUD
 """
 import ctypes
 import heapq
-import math
 from dataclasses import dataclass
 
 import torch
@@ -98,6 +97,8 @@ class QuantizedLayout:
             cu_query.data_ptr(), context.data_ptr(), table.data_ptr(), slots.data_ptr(), r, total, out.max_query,
             table.shape[1]))
         object.__setattr__(out, '_address', ctypes.addressof(out._struct))
+        object.__setattr__(out, '_plan_pointer', plan.data_ptr())
+        object.__setattr__(out, 'device', device)
         if replan:
             out.replan()
         return out
@@ -220,47 +221,49 @@ class QuantizedPages:
                 heapq.heappush(self._free, x)
 
     # -- device work --------------------------------------------------------------------
-    def _layout(self, layout):
-        if not isinstance(layout, QuantizedLayout) or layout.table.device != self.device:
-            raise ValueError('A QuantizedLayout on the cache\'s device is required')
-
-    @torch.no_grad()
     def append(self, key, value, layout, counts=None):
         """The first ``counts[i]`` (int32 [R] on the device; None: all) new rows of request i
         follow its tokens, in all layers in one launch: ``key`` / ``value`` [layers, rows, 8, 128]
         in the tails' dtype, of which the layout's rows are the first. A block of 64 that gets
         full is quantised into the page that the table holds for it; the rest waits in the
         tail. The layout's context lengths are the caller's to advance."""
-        self._layout(layout)
+        device, dtype = self.device, self.row_dtype
+        if not isinstance(layout, QuantizedLayout) or layout.device != device:
+            raise ValueError('append requires a QuantizedLayout on the cache\'s device')
         for t in (key, value):
-            if (not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != self.row_dtype or t.ndim != 4
-                    or tuple(t.shape[2:]) != (HKV, HEAD_DIM) or t.shape != key.shape or not t.is_contiguous()
-                    or t.requires_grad):
-                raise ValueError(f'append requires contiguous {self.row_dtype} rows [layers, rows, 8, 128] on '
-                                 f'{self.device} without autograd')
-        if key.shape[0] != self.layers or key.shape[1] < layout.query_tokens:
-            raise ValueError('append requires the rows of every layer and of every request')
-        if counts is not None and (not isinstance(counts, torch.Tensor) or counts.device != self.device
+            if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or t.ndim != 4
+                    or not t.is_contiguous() or t.requires_grad):
+                raise ValueError(f'append requires contiguous {dtype} rows [layers, rows, 8, 128] on {device} without '
+                                 'autograd')
+        layers, rows, heads, dim = key.shape
+        if (layers != self.layers or rows < layout.query_tokens or heads != HKV or dim != HEAD_DIM
+                or value.shape != key.shape):
+            raise ValueError('append requires the rows [layers, rows, 8, 128] of every layer and of every request')
+        if counts is not None and (not isinstance(counts, torch.Tensor) or counts.device != device
                                    or counts.dtype != torch.int32 or not counts.is_contiguous()
-                                   or counts.shape != (len(layout.query_lengths),)):
+                                   or counts.shape != layout.context.shape):
             raise ValueError('counts must be contiguous int32 [requests] on the device')
-        with _on_device(self.device):
+        with _on_device(device):
             _lib.check(_lib.load_library().dspark_quant_append(
-                key.data_ptr(), value.data_ptr(), key.shape[1], self._address, layout._address,
-                None if counts is None else counts.data_ptr(), _stream(self.device)), 'dspark_quant_append')
+                key.data_ptr(), value.data_ptr(), rows, self._address, layout._address,
+                None if counts is None else counts.data_ptr(), _stream(device)), 'dspark_quant_append')
 
     def _index(self, values, limit, what, distinct=False):
+        """(address, length, tensor to keep) of a list of indices: an int32 device tensor as it is, a
+        host list checked and uploaded."""
         if isinstance(values, torch.Tensor):
-            if values.device != self.device or values.dtype != torch.int32 or values.ndim != 1 or not values.is_contiguous():
+            if (values.dtype != torch.int32 or values.ndim != 1 or values.device != self.device
+                    or not values.is_contiguous()):
                 raise ValueError(f'{what} must be contiguous int32 [n] on the device')
-            return values
+            return values.data_ptr(), values.numel(), values
         values = _int_list(values, what, 0, limit)
         if distinct and len(set(values)) != len(values):
             raise ValueError(f'{what} must be distinct')
-        host = torch.tensor(values, dtype=torch.int32)
-        return host.pin_memory().to(self.device, non_blocking=True) if values else host.to(self.device)
+        if not values:
+            return None, 0, None
+        held = torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        return held.data_ptr(), len(values), held
 
-    @torch.no_grad()
     def copy(self, src=(), dst=(), *, tail_src=(), tail_dst=(), tail_lengths=()):
         """In all layers in one launch: pages ``src[k]`` -> ``dst[k]``, codes and scales, and the
         open rows of a request of ``tail_lengths[k]`` tokens from tail slot ``tail_src[k]`` to
@@ -268,19 +271,19 @@ class QuantizedPages:
         source a target: checked for lists; int32 device tensors are taken at their word,
         except that an id out of range is skipped and flagged. Users of pages do not change."""
         for a, b in ((src, dst), (tail_src, tail_dst)):
-            if len(a) != len(b):
-                raise ValueError('One target per source required')
             if not isinstance(a, torch.Tensor) and not isinstance(b, torch.Tensor) and set(a) & set(b):
                 raise ValueError('A source must not be a target')
-        if len(tail_lengths) != len(tail_src):
-            raise ValueError('One length per tail required')
-        s, d = self._index(src, self.pages, 'src'), self._index(dst, self.pages, 'dst', True)
-        ts, td = self._index(tail_src, self.slots, 'tail_src'), self._index(tail_dst, self.slots, 'tail_dst', True)
-        tn = self._index(tail_lengths, 2 ** 30, 'tail_lengths')
+        # (the uploads, if any, are on this stream: their memory is reused behind the launch)
         with _on_device(self.device):
-            _lib.check(_lib.load_library().dspark_quant_copy(
-                self._address, s.data_ptr(), d.data_ptr(), s.numel(), ts.data_ptr(), td.data_ptr(), tn.data_ptr(),
-                ts.numel(), _stream(self.device)), 'dspark_quant_copy')
+            s, n, _s = self._index(src, self.pages, 'src')
+            d, nd, _d = self._index(dst, self.pages, 'dst', True)
+            ts, m, _ts = self._index(tail_src, self.slots, 'tail_src')
+            td, md, _td = self._index(tail_dst, self.slots, 'tail_dst', True)
+            tn, mn, _tn = self._index(tail_lengths, 2 ** 30, 'tail_lengths')
+            if n != nd or m != md or m != mn:
+                raise ValueError('One target per source, and one length per tail, required')
+            _lib.check(_lib.load_library().dspark_quant_copy(self._address, s, d, n, ts, td, tn, m, _stream(self.device)),
+                       'dspark_quant_copy')
 
     @torch.no_grad()
     def values(self, ids):
@@ -314,7 +317,7 @@ class B200QuantizedKernel:
     everything up to itself. ``out`` (default: a new tensor) may be ``query`` itself and
     otherwise must not overlap what is read.
 
-    bf16 partial rows live in a workspace that each call allocates on its own stream, so
+    Partial rows live in a workspace that each call allocates on its own stream, so
     calls on different streams and in different captured graphs share nothing.
     """
     backend_name = QUANT_BACKEND
@@ -330,16 +333,16 @@ class B200QuantizedKernel:
         device = self.device
         if not isinstance(pages, QuantizedPages) or pages.device != device:
             raise ValueError('B200 quantized attention requires QuantizedPages on its GPU')
-        pages._layout(layout)
+        if not isinstance(layout, QuantizedLayout) or layout.device != device:
+            raise ValueError('B200 quantized attention requires a QuantizedLayout on its GPU')
         dtype, n = pages.row_dtype, layout.query_tokens
-        rows, kv = (n, HQ, HEAD_DIM), (n, HKV, HEAD_DIM)
-        for t, shape in ((query, rows), (key, kv), (value, kv)) + (((out, rows),) if out is not None else ()):
-            if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or t.requires_grad
-                    or not t.is_contiguous()):
+        for t, heads in ((query, HQ), (key, HKV), (value, HKV), (query if out is None else out, HQ)):
+            if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or not t.is_contiguous()
+                    or t.requires_grad):
                 raise ValueError(f'B200 quantized attention requires no-autograd contiguous {dtype} THD tensors on its GPU')
-            if t.shape != shape:
+            if t.shape != (n, heads, HEAD_DIM):
                 raise ValueError('Rows must match the layout, with Hq16/Hkv8/D128 heads')
-        if not isinstance(scale, (float, int)) or not math.isfinite(scale) or scale != SCALE:
+        if scale != SCALE:
             raise ValueError('B200 quantized attention requires the 1/sqrt(128) scale')
         if type(layer) is not int or not 0 <= layer < pages.layers:
             raise ValueError('No such layer in the cache')
@@ -348,12 +351,10 @@ class B200QuantizedKernel:
                 out = torch.empty_like(query)
             if n == 0:
                 return out
-            ws, nbytes = None, 0
-            if dtype == torch.bfloat16:
-                nbytes = _workspace_bytes.get(device.index) or workspace_bytes(device)
-                ws = query.new_empty(nbytes // 2)
+            nbytes = _workspace_bytes.get(device.index) or workspace_bytes(device)
+            ws = query.new_empty(nbytes // query.element_size())
             _lib.check(_lib.load_library().dspark_quant_attn(
                 query.data_ptr(), key.data_ptr(), value.data_ptr(), pages._address, layer, layout._address,
-                layout.plan.data_ptr(), scale, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                layout._plan_pointer, scale, out.data_ptr(), ws.data_ptr(), nbytes,
                 _stream(device)), 'dspark_quant_attn')
         return out
