@@ -583,7 +583,8 @@ int dspark_varlen_attn_noalloc(const void* q, const void* k, const void* v, cons
  * [cu_q[i], cu_q[i + 1]) of q / new_k / new_v, of total_q in all. Values of the device arrays
  * are checked by the kernels: a request or page that does not fit is skipped and sets
  * DSPARK_DEVICE_BAD_ARGUMENT. Tensors are 16-byte aligned. max_q: no fewer than the longest
- * request's new rows. The structures themselves are HOST memory, read during the call.
+ * request's new rows; min_q: no more than the fewest that a request with any has (they choose
+ * the kernels). The structures themselves are HOST memory, read during the call.
  *
  * dspark_quant_plan writes the work plan of a batch (dspark_quant_plan_words words, for
  * num_requests requests and total_q rows) from the device's cu_q and ctx_len: one small launch
@@ -625,7 +626,7 @@ typedef struct {
   const int32_t* ctx_len;   /* [num_requests] */
   const int32_t* table;     /* [num_requests][table_width] */
   const int32_t* slots;     /* [num_requests] */
-  int num_requests, total_q, max_q, table_width;
+  int num_requests, total_q, max_q, min_q, table_width;
 } dspark_quant_batch;
 int dspark_quant_plan_words(int device, int num_requests, long long total_q, long long* words);
 int dspark_quant_workspace_size(int device, size_t* bytes);

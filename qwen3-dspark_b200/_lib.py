@@ -32,7 +32,7 @@ class QuantCache(ctypes.Structure):
 class QuantBatch(ctypes.Structure):
     """dspark_quant_batch"""
     _fields_ = [(n, _vp) for n in ('cu_q', 'ctx_len', 'table', 'slots')] + \
-               [(n, _i) for n in ('num_requests', 'total_q', 'max_q', 'table_width')]
+               [(n, _i) for n in ('num_requests', 'total_q', 'max_q', 'min_q', 'table_width')]
 
 
 # name -> (restype, argtypes); mirrors include/dspark_b200.h

@@ -24,6 +24,7 @@
 #include "norm.cuh"
 #include "prefix.cuh"
 #include "quant_attn.cuh"
+#include "quant_wide.cuh"
 #include "sampling.cuh"
 #include "train.cuh"
 #include "verify.cuh"
@@ -84,22 +85,28 @@ int prefix_setup(int max_smem_optin) {
 
 // Sets the kernels of the paged 8-bit cache up; what it finds concerns them alone.
 int quant_setup(int max_smem_optin) {
-  if (static_cast<size_t>(max_smem_optin) < quant::kAttnSmemQ) return DSPARK_ERR_UNSUPPORTED;
+  if (static_cast<size_t>(max_smem_optin) < std::max<size_t>(quant::kAttnSmemQ, quant::kSmemBytesW)) return DSPARK_ERR_UNSUPPORTED;
   const int bytes = static_cast<int>(quant::kAttnSmemQ), f32_bytes = static_cast<int>(quant::kF32AttnSmem);
   const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
   if (cudaFuncSetAttribute(quant::quant_attn_kernel<quant::kInt8>, attr, bytes) != cudaSuccess ||
       cudaFuncSetAttribute(quant::quant_attn_kernel<quant::kE4M3>, attr, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(quant::quant_wide_kernel<quant::kInt8>, attr, quant::kSmemBytesW) != cudaSuccess ||
+      cudaFuncSetAttribute(quant::quant_wide_kernel<quant::kE4M3>, attr, quant::kSmemBytesW) != cudaSuccess ||
       cudaFuncSetAttribute(quant::f32_attn_kernel<quant::kInt8>, attr, f32_bytes) != cudaSuccess ||
       cudaFuncSetAttribute(quant::f32_attn_kernel<quant::kE4M3>, attr, f32_bytes) != cudaSuccess) {
     cudaGetLastError();
     return DSPARK_ERR_CUDA;
   }
-  // the register split must fit what the CTA is launched with (a setmaxnreg.inc beyond it would wait forever)
-  for (const void* k : {reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kInt8>),
-                        reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kE4M3>)}) {
+  // the register splits must fit what the CTAs are launched with (a setmaxnreg.inc beyond it would wait forever)
+  const struct { const void* kernel; int threads, need; } splits[] = {
+      {reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kInt8>), quant::kAttnThreadsQ, 256 * quant::kHeadRegs + 128 * quant::kFetchRegs},
+      {reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kE4M3>), quant::kAttnThreadsQ, 256 * quant::kHeadRegs + 128 * quant::kFetchRegs},
+      {reinterpret_cast<const void*>(quant::quant_wide_kernel<quant::kInt8>), quant::kWideThreads, 256 * (quant::kSoftmaxRegsW + quant::kOtherRegsW)},
+      {reinterpret_cast<const void*>(quant::quant_wide_kernel<quant::kE4M3>), quant::kWideThreads, 256 * (quant::kSoftmaxRegsW + quant::kOtherRegsW)}};
+  for (const auto& x : splits) {
     cudaFuncAttributes a;
-    if (cudaFuncGetAttributes(&a, k) != cudaSuccess) return DSPARK_ERR_CUDA;
-    if (a.numRegs * quant::kAttnThreadsQ < 256 * quant::kHeadRegs + 128 * quant::kFetchRegs) return DSPARK_ERR_UNSUPPORTED;
+    if (cudaFuncGetAttributes(&a, x.kernel) != cudaSuccess) return DSPARK_ERR_CUDA;
+    if (a.numRegs * x.threads < x.need) return DSPARK_ERR_UNSUPPORTED;
   }
   return DSPARK_OK;
 }
@@ -479,7 +486,8 @@ bool quant_batch(quant::Batch& b, const dspark_quant_batch* x) {
   b = quant::Batch{x->cu_q, x->ctx_len, x->table, x->slots, x->num_requests, x->total_q, x->table_width};
   for (const int32_t* t : {x->cu_q, x->ctx_len, x->table, x->slots})
     if (t == nullptr || !aligned(t, 4)) return false;
-  return x->num_requests >= 1 && x->total_q >= 0 && x->max_q >= 0 && x->max_q <= x->total_q && x->table_width >= 1;
+  return x->num_requests >= 1 && x->total_q >= 0 && x->max_q >= 0 && x->max_q <= x->total_q && x->min_q >= 0 &&
+         x->min_q <= x->max_q && x->table_width >= 1;
 }
 
 // The status of the current device, and its SM count.
@@ -1502,7 +1510,7 @@ int dspark_quant_workspace_size(int device, size_t* bytes) {
   DeviceInfo d;
   const int st = device_info(device, &d);
   if (st != DSPARK_OK) return st;
-  *bytes = quant::attn_workspace(d.sms);
+  *bytes = std::max(quant::attn_workspace(d.sms), quant::wide_workspace(d.sms));
   return DSPARK_OK;
 }
 
@@ -1513,8 +1521,9 @@ int dspark_quant_plan(const dspark_quant_batch* batch, int32_t* plan, long long 
   const int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;
   if (plan_words < quant::plan_words(sms, b.requests, b.rows)) return DSPARK_ERR_INVALID_ARGUMENT;
-  const quant::PlanParams pp{b.cu_q, b.ctx, b.slot, b.requests, b.rows, b.width, sms, plan};
-  quant::plan_kernel<<<1, quant::kPlanThreads, 0, stream>>>(pp);
+  const bool wide = batch->max_q >= quant::kWideRows;
+  const quant::PlanParams pp{b.cu_q, b.ctx, b.slot, b.requests, b.rows, b.width, sms, wide ? quant::kWideRows : 0, plan};
+  quant::plan_kernel<<<wide ? 2 : 1, quant::kPlanThreads, 0, stream>>>(pp);
   return launch_status();
 }
 
@@ -1546,7 +1555,7 @@ int dspark_quant_attn(const void* q, const void* new_k, const void* new_v, const
   int sms = 0;
   int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;
-  if (!workspace || !aligned(workspace, 16) || workspace_bytes < quant::attn_workspace(sms) ||
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < std::max(quant::attn_workspace(sms), quant::wide_workspace(sms)) ||
       overlap(workspace, workspace_bytes, out, out_bytes) || overlap(workspace, workspace_bytes, q, out_bytes))
     return DSPARK_ERR_INVALID_ARGUMENT;
   if (cache->dtype == DSPARK_DTYPE_F32) {
@@ -1572,11 +1581,27 @@ int dspark_quant_attn(const void* q, const void* new_k, const void* new_v, const
   const quant::AttnParamsQ ap{static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(new_k),
                               static_cast<const __nv_bfloat16*>(new_v), static_cast<__nv_bfloat16*>(out), c, b, plan, sms,
                               scale * 1.4426950408889634f, static_cast<float*>(workspace)};
-  st = launch_dependent(cache->code == DSPARK_CODE_INT8 ? quant::quant_attn_kernel<quant::kInt8>
-                                                        : quant::quant_attn_kernel<quant::kE4M3>,
-                        dim3(sms), quant::kAttnThreadsQ, quant::kAttnSmemQ, stream, ap);
+  const bool int8 = cache->code == DSPARK_CODE_INT8;
+  if (batch->min_q < quant::kWideRows) {
+    st = launch_dependent(int8 ? quant::quant_attn_kernel<quant::kInt8> : quant::quant_attn_kernel<quant::kE4M3>, dim3(sms),
+                          quant::kAttnThreadsQ, quant::kAttnSmemQ, stream, ap);
+    if (st != DSPARK_OK) return st;
+    st = launch_dependent(quant::quant_merge_kernel, dim3(sms, kKVHeads), 256, 0, stream, ap);
+    if (st != DSPARK_OK) return st;
+  }
+  if (batch->max_q < quant::kWideRows) return DSPARK_OK;
+  quant::MapsW maps;
+  const long long tail_rows = static_cast<long long>(c.slots) * 2 * quant::kPage;
+  if ((st = encode_rows_map(&maps.q, q, b.rows, kQHeads, 2, 32)) != DSPARK_OK ||
+      (st = encode_rows_map(&maps.tail_k, c.tail_key, tail_rows, kKVHeads, 1, 32)) != DSPARK_OK ||
+      (st = encode_rows_map(&maps.tail_v, c.tail_value, tail_rows, kKVHeads, 1, 32)) != DSPARK_OK ||
+      (st = encode_rows_map(&maps.new_k, new_k, b.rows, kKVHeads, 1, 32)) != DSPARK_OK ||
+      (st = encode_rows_map(&maps.new_v, new_v, b.rows, kKVHeads, 1, 32)) != DSPARK_OK)
+    return st;
+  st = launch_dependent(int8 ? quant::quant_wide_kernel<quant::kInt8> : quant::quant_wide_kernel<quant::kE4M3>, dim3(sms),
+                        quant::kWideThreads, quant::kSmemBytesW, stream, maps, ap);
   if (st != DSPARK_OK) return st;
-  return launch_dependent(quant::quant_merge_kernel, dim3(sms, kKVHeads), 256, 0, stream, ap);
+  return launch_dependent(quant::quant_wide_merge_kernel, dim3(sms, quant::kPartRowsW / 32), 256, 0, stream, ap);
 }
 
 int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows, const dspark_quant_cache* cache,

@@ -47,41 +47,56 @@ constexpr int kCtaWords = 12;       // first item, its first unit, last item, it
 constexpr int kMergeWords = 4;      // item (-1: none), last contributor, slot of the first
 constexpr int kItemWordsQ = 12;
 // item: first global row | rows | row in the request | request | row units | pages | tokens | tail slot |
-//       start and cost in the plan's numbering
-enum ItemWord { kIRow = 0, kIRows, kIR0, kIRequest, kIRowUnits, kIPages, kICtx, kISlot, kIStart, kICost };
+//       start and cost in the plan's numbering | head (wide: units are blocks of keys)
+enum ItemWord { kIRow = 0, kIRows, kIR0, kIRequest, kIRowUnits, kIPages, kICtx, kISlot, kIStart, kICost, kIHead };
 __host__ __device__ constexpr int plan_cta_at() { return kQHeadWords; }
 __host__ __device__ constexpr int plan_merge_at(int grid) { return kQHeadWords + grid * kCtaWords; }
 __host__ __device__ constexpr int plan_items_at(int grid) { return kQHeadWords + grid * (kCtaWords + kMergeWords); }
-__host__ __device__ inline long long plan_words(int grid, long long requests, long long rows) {
+// Two plans one behind the other: of the requests with few new rows (this file's kernel) and of
+// those with kWideRows or more (quant_wide.cuh), whose items are 128 query rows of one head.
+constexpr int kWideRows = 32, kWideItemRows = 128, kWideKeys = 128;
+__host__ __device__ inline long long narrow_plan_words(int grid, long long requests, long long rows) {
   return plan_items_at(grid) + kItemWordsQ * (rows / kQBlock + requests);
+}
+__host__ __device__ inline long long plan_words(int grid, long long requests, long long rows) {
+  return narrow_plan_words(grid, requests, rows) + plan_items_at(grid) +
+         kItemWordsQ * kKVHeads * (rows / kWideItemRows + requests);
 }
 
 // Units' worth of a new item (its queries, a partial row) and the least range of a CTA.
-constexpr int kItemCost = 0, kMinUnits = 1;
+constexpr int kItemCost = 0, kMinUnits = 1, kWideItemCost = 2, kWideMinUnits = 4;
 
 struct PlanParams {
   const int* cu_q;
   const int* ctx;
   const int* slot;
   int requests, rows, width, grid;
+  int wide_rows;             // requests with as many new rows are in the second plan (0: none)
   int* plan;
 };
 
 constexpr int kPlanThreads = 1024;
 __device__ __forceinline__ int units_of(int keys) { return (keys + kRowUnit - 1) / kRowUnit; }
-// of the open rows and of the new rows that an item sees
-__device__ __forceinline__ int row_units(int ctx, int q_len, int r0) {
+// Units of the open rows and of the new rows that an item sees, and of the pages.
+__device__ __forceinline__ int row_units(int ctx, int q_len, int r0, bool wide) {
+  if (wide) return (ctx % kPage ? 1 : 0) + (min(r0 + kWideItemRows, q_len) + kWideKeys - 1) / kWideKeys;
   return units_of(ctx % kPage) + units_of(min(r0 + kQBlock, q_len));
 }
+__device__ __forceinline__ int page_units(int ctx, bool wide) { return wide ? (ctx / kPage + 1) / 2 : ctx / kPage; }
 
-// One CTA. Requests whose lengths do not fit the batch have no items (the status is set).
+// CTA 0 makes the first plan, CTA 1 the second. Requests whose lengths do not fit the batch have no
+// items (the status is set).
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   __shared__ long long s_cost[32];
   __shared__ int s_items[32];
   __shared__ long long carry_cost;
   __shared__ int carry_items;
+  const bool wide = blockIdx.x == 1;
+  const int block_rows = wide ? kWideItemRows : kQBlock, heads = wide ? kKVHeads : 1;
+  const int item_cost = wide ? kWideItemCost : kItemCost, min_units = wide ? kWideMinUnits : kMinUnits;
+  int* plan = p.plan + (wide ? narrow_plan_words(p.grid, p.requests, p.rows) : 0);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int* items = p.plan + plan_items_at(p.grid);
+  int* items = plan + plan_items_at(p.grid);
   if (tid == 0) {
     carry_cost = 0;
     carry_items = 0;
@@ -97,9 +112,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       ctx = p.ctx[i];
       slot = p.slot[i];
       if (q0 >= 0 && q_len >= 0 && q0 <= p.rows - q_len && ctx >= 0 && ctx / kPage <= p.width) {
-        n = (q_len + kQBlock - 1) / kQBlock;
-        for (int x = 0; x < n; ++x) cost += kItemCost + ctx / kPage + row_units(ctx, q_len, x * kQBlock);
-      } else {
+        if ((p.wide_rows > 0 && q_len >= p.wide_rows) == wide) n = (q_len + block_rows - 1) / block_rows;
+        for (int x = 0; x < n; ++x) cost += heads * (item_cost + page_units(ctx, wide) + row_units(ctx, q_len, x * block_rows, wide));
+        n *= heads;
+      } else if (!wide) {
         atomicOr(&g_device_status, kStatusBadArgument);
       }
     }
@@ -139,12 +155,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     long long at = carry_cost + (warp > 0 ? s_cost[warp - 1] : 0) + c - cost;
     int idx = carry_items + (warp > 0 ? s_items[warp - 1] : 0) + m - n;
     for (int x = 0; x < n; ++x, ++idx) {
-      const int ru = row_units(ctx, q_len, x * kQBlock), full = ctx / kPage, total = kItemCost + full + ru;
+      const int r0 = x / heads * block_rows, ru = row_units(ctx, q_len, r0, wide), pu = page_units(ctx, wide);
       int4* w = reinterpret_cast<int4*>(items + static_cast<size_t>(idx) * kItemWordsQ);
-      w[0] = make_int4(q0 + x * kQBlock, min(kQBlock, q_len - x * kQBlock), x * kQBlock, i);
-      w[1] = make_int4(ru, full, ctx, slot);
-      w[2] = make_int4(static_cast<int>(at), total, 0, 0);
-      at += total;
+      w[0] = make_int4(q0 + r0, min(block_rows, q_len - r0), r0, i);
+      w[1] = make_int4(ru, pu, ctx, slot);
+      w[2] = make_int4(static_cast<int>(at), item_cost + pu + ru, x % heads, 0);
+      at += item_cost + pu + ru;
     }
     __syncthreads();
     if (tid == 0) {
@@ -159,7 +175,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     if (tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
     total = 0;
   }
-  const long long want = total / kMinUnits;
+  const long long want = total / min_units;
   const int ranges = total == 0 ? 0 : static_cast<int>(want < 1 ? 1 : (want < p.grid ? want : p.grid));
   // position in the costs -> (item, unit); the cost of an item comes before its first unit
   auto find = [&](long long pos, int& item, int& unit) {
@@ -168,12 +184,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       const int mid = (lo + hi + 1) >> 1;
       if (items[static_cast<size_t>(mid) * kItemWordsQ + kIStart] <= pos) lo = mid; else hi = mid - 1;
     }
-    const long long u = pos - items[static_cast<size_t>(lo) * kItemWordsQ + kIStart] - kItemCost;
+    const long long u = pos - items[static_cast<size_t>(lo) * kItemWordsQ + kIStart] - item_cost;
     item = lo;
     unit = u > 0 ? static_cast<int>(u) : 0;
   };
-  int4* ctas = reinterpret_cast<int4*>(p.plan + plan_cta_at());
-  int4* merges = reinterpret_cast<int4*>(p.plan + plan_merge_at(p.grid));
+  int4* ctas = reinterpret_cast<int4*>(plan + plan_cta_at());
+  int4* merges = reinterpret_cast<int4*>(plan + plan_merge_at(p.grid));
   for (int c = tid; c < p.grid; c += kPlanThreads) {
     int4 range = make_int4(0, 0, -1, 0), merge = make_int4(-1, 0, 0, 0);
     if (c < ranges) {
@@ -208,11 +224,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     merges[c] = merge;
   }
   if (tid == 0) {
-    p.plan[kQGrid] = p.grid;
-    p.plan[kQItems] = count;
-    p.plan[kQRequests] = p.requests;
-    p.plan[kQRows] = p.rows;
-    p.plan[kQMagic] = kPlanMagicQ;
+    plan[kQGrid] = p.grid;
+    plan[kQItems] = count;
+    plan[kQRequests] = p.requests;
+    plan[kQRows] = p.rows;
+    plan[kQMagic] = kPlanMagicQ;
   }
 }
 

@@ -1,0 +1,755 @@
+// Attention over the paged 8-bit cache for requests with many new rows (prompts and their
+// chunks), on the tcgen05 tensor cores. The same sums as quant_attn.cuh.
+//
+// An item is up to 128 query rows of a request x the two query heads of a KV head = two MMA tiles A
+// and B of 128 rows (row m of a tile = 2 * query row + head) that share every block of keys, so a
+// page is decoded once per 256 rows. Units are blocks of up to 128 keys: the open rows, the new
+// rows, pairs of pages. The plan cuts the units of all items into equal ranges, one per CTA, and
+// a second launch merges what was cut. Roles (512 threads):
+//   warps 0-3, 4-7  softmax of tile A / B: one thread per row, the block's scores in registers; P
+//                   (bf16) overwrites its S columns in TMEM; O is rescaled only when the running
+//                   maximum grows by more than 2^8;
+//   warps 8, 9      MMA issuers of tile A / B, which take turns: a turn is PV(b) and QK(b + 1), so
+//                   that one tile's softmax runs under the other's products;
+//   warp 10         fetches Q (TMA), the codes of pages (bulk copies into a ring of 2 x 16 KB) and
+//                   their scales;
+//   warps 12-15     turn codes into bf16 operands, 4 stages of 32 KB in the 128-byte swizzle, and
+//                   fetch unquantised rows into the same stages (TMA).
+// Codes are bf16 exactly; K's scale multiplies the scores of its page's columns, V's is added to
+// the exponent (p vs = 2^(s f - m + log2 vs)), so no rounding comes on top of P's own (bf16, 2^-8
+// of each weight). V of a page lies [dim][key], which is the K-major operand of the second
+// product; unquantised V is taken N-major. Every wait is bounded; a wait that runs out raises the
+// CTA's abort flag, copies and MMAs in flight are drained and TMEM is released.
+#pragma once
+#include "prefix.cuh"
+#include "quant_attn.cuh"
+
+namespace dspark {
+namespace quant {
+
+constexpr int kStagesW = 4, kRawW = 2;
+constexpr int kWideThreads = 512;
+constexpr int kTileQ = 64, kItemQ = kWideItemRows;          // query rows of a tile, of an item
+constexpr int kKeysW = kWideKeys;                           // keys of a block
+constexpr int kChunkW = 32;                                 // pages whose scales are held at a time
+constexpr uint32_t kSmemQW = 0, kSmemRingW = 2 * 32768, kSmemRawW = kSmemRingW + kStagesW * 32768;
+constexpr uint32_t kSmemScalesW = kSmemRawW + kRawW * 16384;          // [2][kChunkW] (ks, vs)
+constexpr uint32_t kSmemBarW = kSmemScalesW + 2 * kChunkW * 8;
+enum BarW {
+  kWQFull = 0, kWQEmpty, kWRawFull, kWRawEmpty = kWRawFull + kRawW, kWFull = kWRawEmpty + kRawW,
+  kWEmpty = kWFull + kStagesW, kWFixed = kWEmpty + kStagesW, kWSFull = kWFixed + kStagesW, kWPFull = kWSFull + 2,
+  kWODone = kWPFull + 2, kWOFree = kWODone + 2, kWTurn = kWOFree + 2, kWDrain = kWTurn + 2, kWChunk = kWDrain + 1,
+  kWChunkFree = kWChunk + 2, kWBars = kWChunkFree + 2
+};
+constexpr uint32_t kSmemSlotW = kSmemBarW + kWBars * 8;
+constexpr uint32_t kSmemAbortW = kSmemSlotW + 4, kSmemPoisonW = kSmemAbortW + 4;
+constexpr uint32_t kSmemBytesW = 1024 + kSmemPoisonW + 16;
+// Registers of a softmax thread and of the others after setmaxnreg: the launch's own, 512 x 128.
+constexpr int kSoftmaxRegsW = 192, kOtherRegsW = 64;
+constexpr uint32_t kTmemSW = 0, kTmemOW = 256;
+
+struct MapsW {
+  CUtensorMap q;                                            // boxes of 32 query rows x 2 heads x 64 d
+  CUtensorMap tail_k, tail_v, new_k, new_v;                 // boxes of 32 rows of a head x 64 d
+};
+
+// Partial rows of one (CTA, slot): 256 rows x 128 float32 as [d / 4][row][4], so that 32 rows of a
+// warp store 512 contiguous bytes, then (maximum, sum) per row.
+constexpr int kPartRowsW = 256, kPartFloatsW = kPartRowsW * (kHeadDim + 2);
+__host__ __device__ inline size_t part_index_w(int cta, int slot) { return (static_cast<size_t>(cta) * 2 + slot) * kPartFloatsW; }
+inline size_t wide_workspace(int grid) { return part_index_w(grid, 0) * sizeof(float); }
+
+struct ItemW {
+  int q0, rows, r0, request, row_blocks, page_blocks, ctx, slot, head;
+  __device__ __forceinline__ int tail() const { return ctx % kPage; }
+  __device__ __forceinline__ int tails() const { return ctx % kPage ? 1 : 0; }
+};
+__device__ __forceinline__ const int* wide_plan(const AttnParamsQ& p) {
+  return p.plan + narrow_plan_words(p.grid, p.batch.requests, p.batch.rows);
+}
+__device__ __forceinline__ ItemW load_item_w(const int* plan, int grid, int idx) {
+  const int4* w = reinterpret_cast<const int4*>(plan + plan_items_at(grid) + static_cast<size_t>(idx) * kItemWordsQ);
+  const int4 a = __ldg(w), b = __ldg(w + 1), c = __ldg(w + 2);
+  return ItemW{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.z};
+}
+
+// A block of an item: unit u.
+struct BlockW {
+  bool page, fresh;                                         // pages; new rows (else the open ones)
+  int keys, first;                                          // first: page, or row of its source's part
+  int see0;                                                 // keys that query row 0 of the item sees; row x sees x more
+};
+__device__ __forceinline__ BlockW block_of(const ItemW& it, int u, int slots) {
+  const int tails = it.tails();
+  if (u >= it.row_blocks) {
+    const int first = 2 * (u - it.row_blocks);
+    return BlockW{true, false, min(2, it.ctx / kPage - first) * kPage, first, kKeysW};
+  }
+  if (u < tails) return BlockW{false, false, it.tail(), 0, it.slot >= 0 && it.slot < slots ? kKeysW : -kItemQ};
+  const int j = (u - tails) * kKeysW;
+  return BlockW{false, true, min(kKeysW, it.r0 + it.rows - j), j, it.r0 + 1 - j};
+}
+// Whether V of a row block is looked at before its product: rows up to the next multiple of 16 are
+// zeroed, and what is not finite is taken out of rows that not every query row sees.
+__device__ __forceinline__ bool fixes(const BlockW& b) { return !b.page && ((b.keys & 15) != 0 || (b.fresh && b.see0 < b.keys)); }
+
+// The segment of an item in a CTA's range.
+struct RangeW {
+  int4 r;
+  __device__ __forceinline__ int begin(int idx) const { return idx == r.x ? r.y : 0; }
+  __device__ __forceinline__ int end(int idx, const ItemW& it) const { return idx == r.z ? r.w : it.row_blocks + it.page_blocks; }
+};
+
+template <int kStages>
+struct RingW {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// ---- warp 10 --------------------------------------------------------------------------------------
+__device__ __forceinline__ void wide_fetch(const AttnParamsQ& p, const MapsW& maps, const int* plan, RangeW range,
+                                           uint8_t* smem, uint32_t sbase, volatile int* abort_flag) {
+  const int lane = threadIdx.x & 31;
+  auto bar = [&](int i) { return sbase + kSmemBarW + 8u * i; };
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  RingW<kRawW> raw;
+  int it = 0, chunks = 0, uses = 0;
+  bool ok = true;
+#pragma unroll 1
+  for (int idx = range.r.x; idx <= range.r.z && ok; ++idx, ++it) {
+    const ItemW x = load_item_w(plan, p.grid, idx);
+    if (!(ok = wait(kWQEmpty, (it & 1) ^ 1))) break;
+    if (lane == 0) {
+      // 32 query rows (64 MMA rows, 8 KB per half) a box
+      const int boxes = (x.rows + 31) >> 5;
+      mbar_arrive_expect_tx(bar(kWQFull), 16384u * boxes);
+      for (int t = 0; t < boxes; ++t) {
+        const uint32_t dst = sbase + kSmemQW + (t >> 1) * 32768 + (t & 1) * 8192;
+        tma_load_3d(dst, &maps.q, 0, 2 * x.head, x.q0 + 32 * t, bar(kWQFull));
+        tma_load_3d(dst + 16384, &maps.q, 64, 2 * x.head, x.q0 + 32 * t, bar(kWQFull));
+      }
+      if (x.slot < 0 || x.slot >= p.cache.slots) atomicOr(&g_device_status, kStatusBadArgument);
+    }
+    __syncwarp();
+    const int ub = max(range.begin(idx) - x.row_blocks, 0), ue = max(range.end(idx, x) - x.row_blocks, 0);
+    const int pages = x.ctx / kPage;
+    int id = 0;
+#pragma unroll 1
+    for (int b = ub; b < ue && ok; ++b) {
+      const int at = (2 * (b - ub)) % kChunkW;              // page of the chunk
+      if (at == 0) {
+        const int page = 2 * b + lane, slot = chunks & 1;
+        float2 scales = make_float2(0.f, -1.f);             // (a negative V scale: the page is left out)
+        id = 0;
+        if (page < min(2 * ue, pages)) {
+          id = __ldg(p.batch.table + static_cast<size_t>(x.request) * p.batch.width + page);
+          if (id >= 0 && id < p.cache.pages) {
+            const size_t s = static_cast<size_t>(id) * kKVHeads + x.head;
+            scales = make_float2(__ldg(p.cache.key_scale + s), __ldg(p.cache.value_scale + s));
+          } else {
+            atomicOr(&g_device_status, kStatusBadArgument);
+            id = 0;
+          }
+        }
+        if (!(ok = wait(kWChunkFree + slot, ((chunks >> 1) & 1) ^ 1))) break;
+        reinterpret_cast<float2*>(smem + kSmemScalesW)[slot * kChunkW + lane] = scales;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kWChunk + slot));
+        ++chunks;
+      }
+      const int num = min(2, pages - 2 * b);
+      const int id0 = __shfl_sync(0xffffffffu, id, at), id1 = __shfl_sync(0xffffffffu, id, at + 1);
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {
+        if (!(ok = wait(kWRawEmpty + raw.stage, raw.phase ^ 1))) break;
+        if (lane == 0) {
+          const uint32_t full = bar(kWRawFull + raw.stage), dst = sbase + kSmemRawW + raw.stage * 16384;
+          const uint8_t* src = (v ? p.cache.value : p.cache.key) + static_cast<size_t>(x.head) * kHeadBytes;
+          mbar_arrive_expect_tx(full, num * kHeadBytes);
+          bulk_load(dst, src + static_cast<size_t>(id0) * kPageBytes, kHeadBytes, full);
+          if (num == 2) bulk_load(dst + kHeadBytes, src + static_cast<size_t>(id1) * kPageBytes, kHeadBytes, full);
+        }
+        __syncwarp();
+        ++uses;
+        raw.next();
+      }
+    }
+  }
+  if (!ok) *abort_flag = 1;
+  // copies in flight land before the CTA can exit (a no-op when all were consumed)
+  volatile int never = 0;
+  if (it > 0) train::wait_or_abort(bar(kWQFull), (it - 1) & 1, &never);
+  for (int s = 0; s < kRawW && s < uses; ++s) {
+    const int last_use = uses - 1 - (uses - 1 - s) % kRawW;
+    train::wait_or_abort(bar(kWRawFull + s), (last_use / kRawW) & 1, &never);
+  }
+}
+
+// ---- warps 12-15 ----------------------------------------------------------------------------------
+// 4 codes of a word as two pairs of bf16. int8: the byte's low 7 bits on top of 128, less 128 or 256
+// by its sign; e4m3: over halves and floats.
+template <int kCode>
+__device__ __forceinline__ void decode4_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (kCode == kInt8) {
+    const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
+    const uint32_t a0 = a & 0xff7fff7fu, a1 = a & 0xff80ff80u, b0 = b & 0xff7fff7fu, b1 = b & 0xff80ff80u;
+    const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a0), *reinterpret_cast<const __nv_bfloat162*>(&a1));
+    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b0), *reinterpret_cast<const __nv_bfloat162*>(&b1));
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    uint32_t a, b;
+    e4m3x4_to_f16x4(w, a, b);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    lo = pack_bf16x2(x.x, x.y);
+    hi = pack_bf16x2(y.x, y.y);
+  }
+}
+
+template <int kCode>
+__device__ __forceinline__ void wide_convert(const AttnParamsQ& p, const MapsW& maps, const int* plan, RangeW range,
+                                             uint8_t* smem, uint32_t sbase, volatile int* abort_flag) {
+  const int tid = threadIdx.x - 384, warp = tid >> 5, lane = tid & 31;
+  auto bar = [&](int i) { return sbase + kSmemBarW + 8u * i; };
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  volatile int* poison = reinterpret_cast<volatile int*>(smem + kSmemPoisonW);
+  RingW<kStagesW> ring;
+  RingW<kRawW> raw;
+  bool ok = true;
+  uint32_t rows_in = 0;                                     // stages whose last fill was a TMA copy (bits), of this phase
+#pragma unroll 1
+  for (int idx = range.r.x; idx <= range.r.z && ok; ++idx) {
+    const ItemW x = load_item_w(plan, p.grid, idx);
+    const int ue = range.end(idx, x);
+#pragma unroll 1
+    for (int u = range.begin(idx); u < ue && ok; ++u) {
+      const BlockW b = block_of(x, u, p.cache.slots);
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {
+        const uint32_t full = bar(kWFull + ring.stage);
+        uint8_t* stage = smem + kSmemRingW + ring.stage * 32768;
+        if (b.page) {
+          if (!(ok = wait(kWRawFull + raw.stage, raw.phase)) || !(ok = wait(kWEmpty + ring.stage, ring.phase ^ 1))) break;
+          // 64 codes of a raw row become 128 bytes of an operand row, 16-byte chunks permuted by its
+          // low bits. K: raw rows [page][half][key], operand rows [half][64 page + key]; V: [page][dim]
+          const uint4* src = reinterpret_cast<const uint4*>(smem + kSmemRawW + raw.stage * 16384) + tid;
+          const int count = b.keys * 2 * 4;                 // 16-byte chunks: 128 raw rows a page, 4 each
+#pragma unroll 2
+          for (int c0 = 0; c0 < count; c0 += 256) {
+            uint4 w[2];
+            w[0] = src[c0];
+            w[1] = src[c0 + 128];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int chunk = c0 + 128 * e + tid, line = chunk >> 2, quarter = chunk & 3;
+              const int page = line >> 7, rest = line & 127;
+              const int row = v ? rest : (rest & 63) + 64 * page, half = v ? page : rest >> 6;
+              uint4 o[2];
+              decode4_bf16<kCode>(w[e].x, o[0].x, o[0].y);
+              decode4_bf16<kCode>(w[e].y, o[0].z, o[0].w);
+              decode4_bf16<kCode>(w[e].z, o[1].x, o[1].y);
+              decode4_bf16<kCode>(w[e].w, o[1].z, o[1].w);
+              uint4* dst = reinterpret_cast<uint4*>(stage + half * 16384 + row * 128);
+              dst[(2 * quarter) ^ (row & 7)] = o[0];
+              dst[(2 * quarter + 1) ^ (row & 7)] = o[1];
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(full);
+            mbar_arrive(bar(kWRawEmpty + raw.stage));
+          }
+          raw.next();
+          rows_in &= ~(1u << ring.stage);
+        } else {
+          if (!(ok = wait(kWEmpty + ring.stage, ring.phase ^ 1))) break;
+          if (lane == 0) {
+            if (warp == 0) {
+              const CUtensorMap* map = b.fresh ? (v ? &maps.new_v : &maps.new_k) : (v ? &maps.tail_v : &maps.tail_k);
+              const bool there = x.slot >= 0 && x.slot < p.cache.slots;
+              const int row = b.fresh ? x.q0 - x.r0 + b.first : (there ? static_cast<int>(tail_row(x.slot, x.ctx - x.tail())) : 0);
+              const int boxes = (b.keys + 31) >> 5;
+              const uint32_t dst = sbase + kSmemRingW + ring.stage * 32768;
+              mbar_arrive_expect_tx(full, boxes * 8192u);
+              for (int i = 0; i < boxes; ++i) {
+                tma_load_3d(dst + i * 4096, map, 0, x.head, row + 32 * i, full);
+                tma_load_3d(dst + 16384 + i * 4096, map, 64, x.head, row + 32 * i, full);
+              }
+            } else {
+              mbar_arrive(full);
+            }
+          }
+          __syncwarp();
+          rows_in |= 1u << ring.stage;
+          if (v == 1 && fixes(b)) {
+            if (!(ok = wait(kWFull + ring.stage, ring.phase))) break;
+            const int top = (b.keys + 15) & ~15;
+            const int from = b.fresh ? min(max(b.see0, 0), b.keys) : b.keys;
+            bool bad = false;
+            for (int u2 = tid; u2 < (top - from) * 16; u2 += 128) {
+              const int row = from + (u2 >> 4);
+              uint4* at = reinterpret_cast<uint4*>(stage + ((u2 >> 3) & 1) * 16384 + row * 128) + (u2 & 7);
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);
+              if (row < b.keys) {
+                w = *at;
+                if (!not_finite(w.x) && !not_finite(w.y) && !not_finite(w.z) && !not_finite(w.w)) continue;
+                bad = true;
+                uint32_t* e = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if ((e[i] & 0x7f80u) == 0x7f80u) e[i] &= 0xffff0000u;
+                  if ((e[i] & 0x7f800000u) == 0x7f800000u) e[i] &= 0xffffu;
+                }
+              }
+              *at = w;
+            }
+            if (bad) poison[idx & 3] = idx + 1;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kWFixed + ring.stage));
+          }
+        }
+        ring.next();
+      }
+    }
+  }
+  if (!ok) *abort_flag = 1;
+  // TMA copies in flight land before the CTA can exit: the last fill of each stage that was one
+  // (a stage's phase is the ring's before it wrapped, the other one after)
+  if (!ok && warp == 0) {
+    volatile int never = 0;
+    for (int s = 0; s < kStagesW; ++s)
+      if (rows_in & (1u << s)) train::wait_or_abort(bar(kWFull + s), s < ring.stage ? ring.phase : ring.phase ^ 1, &never);
+  }
+}
+
+// ---- warps 8, 9 -----------------------------------------------------------------------------------
+__device__ __forceinline__ void wide_issue(const AttnParamsQ& p, const int* plan, RangeW range, int tile, uint32_t sbase,
+                                           uint32_t tmem, volatile int* abort_flag) {
+  auto bar = [&](int i) { return sbase + kSmemBarW + 8u * i; };
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  const uint32_t leader = prefix::elected();
+  RingW<kStagesW> ring;
+  int it = 0, mine = 0;                                     // items; of them, items with this tile
+  uint32_t p_phase = 0, fixed_phase = 0, turns = 0;         // fixed_phase: a parity bit per stage
+  const uint32_t s_col = tmem + kTmemSW + tile * 128, o_col = tmem + kTmemOW + tile * 128;
+  const uint64_t k_desc = train::smem_desc(sbase + kSmemRingW, 16, 1024);      // K-major: K, and V of pages
+  const uint64_t v_desc = train::smem_desc(sbase + kSmemRingW, 16384, 1024);   // N-major: V of rows
+  const uint64_t q_desc = train::smem_desc(sbase + kSmemQW + tile * 32768, 16, 1024);
+  bool ok = true;
+#pragma unroll 1
+  for (int idx = range.r.x; idx <= range.r.z && ok; ++idx, ++it) {
+    const ItemW x = load_item_w(plan, p.grid, idx);
+    const int ub = range.begin(idx), ue = range.end(idx, x);
+    if (!(ok = wait(kWQFull, it & 1))) break;
+    if (tile == 1 && x.rows <= kTileQ) {
+      // releases the stages as they fill (every phase is waited for)
+#pragma unroll 1
+      for (int u = ub; u < ue && ok; ++u) {
+        const BlockW b = block_of(x, u, p.cache.slots);
+        for (int v = 0; v < 2 && ok; ++v) {
+          if (!(ok = wait(kWFull + ring.stage, ring.phase))) break;
+          if (v == 1 && fixes(b)) {
+            ok = wait(kWFixed + ring.stage, (fixed_phase >> ring.stage) & 1);
+            fixed_phase ^= 1u << ring.stage;
+          }
+          if (leader) mbar_arrive(bar(kWEmpty + ring.stage));
+          ring.next();
+        }
+      }
+      if (ok && leader) mbar_arrive(bar(kWQEmpty));
+      continue;
+    }
+    const bool paired = x.rows > kTileQ;
+    auto take_turn = [&]() {
+      if (!paired) return true;
+      const bool got = wait(kWTurn + tile, (turns & 1) ^ (tile == 0 ? 1u : 0u));
+      ++turns;
+      return got;
+    };
+    auto pass_turn = [&]() {
+      if (paired && leader) mbar_arrive(bar(kWTurn + (tile ^ 1)));
+    };
+    auto issue_qk = [&](int stage, int keys) {
+      const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (32768 >> 4));
+      const uint32_t idesc = prefix::instr_desc_n(0, static_cast<uint32_t>((keys + 15) & ~15));
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+        train::umma_bf16(s_col, q_desc + off, kd + off, idesc, kk > 0);
+      }
+    };
+    BlockW b = block_of(x, ub, p.cache.slots);
+    if (!(ok = wait(kWFull + ring.stage, ring.phase)) || !(ok = take_turn())) break;
+    train::tc_fence_after();
+    if (leader) {
+      issue_qk(ring.stage, b.keys);
+      train::umma_commit(bar(kWSFull + tile));
+      train::umma_commit(bar(kWEmpty + ring.stage));
+      if (ub + 1 >= ue) train::umma_commit(bar(kWQEmpty));
+    }
+    __syncwarp();
+    pass_turn();
+    ring.next();
+#pragma unroll 1
+    for (int u = ub; u < ue && ok; ++u) {
+      const int vs = ring.stage, steps = (b.keys + 15) >> 4;
+      const bool more = u + 1 < ue, kmajor = b.page;
+      if (u == ub && !(ok = wait(kWOFree + tile, (mine & 1) ^ 1))) break;
+      if (!(ok = wait(kWFull + vs, ring.phase))) break;
+      if (fixes(b)) {
+        if (!(ok = wait(kWFixed + vs, (fixed_phase >> vs) & 1))) break;
+        fixed_phase ^= 1u << vs;
+      }
+      ring.next();
+      if (more) b = block_of(x, u + 1, p.cache.slots);
+      // every wait comes before the first MMA, every commit behind the last
+      if (more && !(ok = wait(kWFull + ring.stage, ring.phase))) break;
+      if (!(ok = take_turn())) break;
+      if (!(ok = wait(kWPFull + tile, p_phase))) break;
+      p_phase ^= 1;
+      train::tc_fence_after();
+      if (leader) {
+        const uint32_t at = static_cast<uint32_t>(vs * (32768 >> 4));
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          if (kk < steps) {
+            const uint64_t vd = kmajor ? k_desc + at + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4) : v_desc + at + kk * (2048 >> 4);
+            train::umma_bf16_ts(o_col, s_col + kk * 8, vd, prefix::instr_desc_n(kmajor ? 0 : 1, 128), (u > ub || kk > 0) ? 1u : 0u);
+          }
+        if (more) {
+          issue_qk(ring.stage, b.keys);
+          train::umma_commit(bar(kWSFull + tile));
+          train::umma_commit(bar(kWEmpty + ring.stage));
+          if (u + 2 >= ue) train::umma_commit(bar(kWQEmpty));
+        } else {
+          train::umma_commit(bar(kWODone + tile));
+        }
+        train::umma_commit(bar(kWEmpty + vs));
+      }
+      __syncwarp();
+      if (more) ring.next();
+      pass_turn();
+    }
+    ++mine;
+  }
+  if (!ok) *abort_flag = 1;
+  if (leader) train::umma_commit(bar(kWDrain));             // every MMA completes before TMEM is released
+  __syncwarp();
+  volatile int never = 0;
+  train::wait_or_abort(bar(kWDrain), 0, &never);
+}
+
+// ---- warps 0-7 ------------------------------------------------------------------------------------
+// One block of a row: kCols scores from TMEM, P back as packed bf16. `see` columns are visible, and
+// the halves' pages unless they are left out (a negative V scale).
+template <int kCols>
+__device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int see, const float2 (&scales)[2], bool page,
+                                           float scale_log2, bool first, prefix::RowState& st) {
+  constexpr int kHalf = kCols < 64 ? kCols : 64, kHalves = kCols / kHalf;
+  float s[kCols];
+  if constexpr (kCols == 128) {
+    train::tmem_ld128(s_addr, s);
+  } else {
+#pragma unroll
+    for (int c = 0; c < kCols / 32; ++c) train::tmem_ld32(s_addr + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
+  }
+  float f[kHalves], base[kHalves], iv[kHalves];
+  bool out[kHalves];
+#pragma unroll
+  for (int j = 0; j < kHalves; ++j) {
+    const float vs = page ? scales[j].y : 1.f;
+    f[j] = page ? scale_log2 * scales[j].x : scale_log2;
+    const bool plain = !page || vs == 0.f;                  // (a zero block: its codes are zero)
+    base[j] = plain ? 0.f : __log2f(vs);
+    iv[j] = plain ? 1.f : 1.f / vs;
+    out[j] = vs < 0.f;
+    if (out[j]) {                                           // p = 2^(0 s - infinity)
+      f[j] = iv[j] = 0.f;
+      base[j] = -INFINITY;
+    }
+  }
+  if (!__all_sync(0xffffffffu, see >= kCols)) {
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) s[i] = i < see ? s[i] : -INFINITY;
+  }
+  float m_new = st.m;
+#pragma unroll
+  for (int j = 0; j < kHalves; ++j) {
+    const float top = __fmul_rn(prefix::max_n<kHalf>(*reinterpret_cast<const float(*)[kHalf]>(&s[j * kHalf])), f[j]);
+    m_new = out[j] ? m_new : fmaxf(m_new, top);
+  }
+  const bool raise = m_new > st.m + 8.f;
+  float alpha = 1.f;
+  if (raise) {
+    alpha = ex2(st.m - m_new);
+    st.m = m_new;
+  }
+  // the block's S was committed behind the previous PV: O is complete
+  if (!first && __any_sync(0xffffffffu, raise)) prefix::rescale_o(o_addr, alpha);
+  // one fma a score, off by 2^-24 |m|; scores of thousands are scaled and shifted first, one by one
+  if (__any_sync(0xffffffffu, fabsf(st.m) > 1024.f && st.m > prefix::kNoMax)) {
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) s[i] = __fsub_rn(__fmul_rn(s[i], f[i / kHalf]), st.m);
+#pragma unroll
+    for (int j = 0; j < kHalves; ++j) f[j] = 1.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kHalves; ++j) base[j] -= st.m;
+  }
+  st.l *= alpha;
+#pragma unroll
+  for (int j = 0; j < kHalves; ++j) {
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < kHalf / 32; ++c) {
+      uint32_t pk[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float a = ex2(fmaf(s[j * kHalf + 32 * c + 2 * i], f[j], base[j]));
+        const float b = ex2(fmaf(s[j * kHalf + 32 * c + 2 * i + 1], f[j], base[j]));
+        sum[i & 1] += a + b;
+        pk[i] = pack_bf16x2(a, b);
+      }
+      prefix::tmem_st16(s_addr + (j * kHalf >> 1) + 16 * c, pk);
+    }
+    st.l = fmaf(sum[0] + sum[1], iv[j], st.l);
+  }
+  prefix::tmem_st_wait();
+}
+
+__device__ __forceinline__ void wide_softmax(const AttnParamsQ& p, const int* plan, RangeW range, uint8_t* smem, uint32_t sbase,
+                                             uint32_t tmem, volatile int* abort_flag) {
+  auto bar = [&](int i) { return sbase + kSmemBarW + 8u * i; };
+  auto wait = [&](int i, uint32_t parity) {
+    return __all_sync(0xffffffffu, train::wait_or_abort(bar(i), parity, abort_flag)) != 0;
+  };
+  const int tile = threadIdx.x >> 7, m = threadIdx.x & 127, lane = threadIdx.x & 31;      // m: row of the tile == TMEM lane
+  const uint32_t lanes = static_cast<uint32_t>(m & ~31) << 16;
+  const uint32_t s_addr = tmem + lanes + kTmemSW + tile * 128, o_addr = tmem + lanes + kTmemOW + tile * 128;
+  const int lt = tile * kTileQ + (m >> 1);                  // query row of the item
+  const volatile int* poison = reinterpret_cast<const volatile int*>(smem + kSmemPoisonW);
+  uint32_t s_phase = 0, o_phase = 0;
+  int chunks = 0;
+  bool ok = true;
+#pragma unroll 1
+  for (int idx = range.r.x; idx <= range.r.z && ok; ++idx) {
+    const ItemW x = load_item_w(plan, p.grid, idx);
+    const int ub = range.begin(idx), ue = range.end(idx, x);
+    const bool active = tile == 0 || x.rows > kTileQ, row_ok = lt < x.rows, warp_ok = lt - (lane >> 1) < x.rows;
+    prefix::RowState st{prefix::kNoMax, 0.f};
+    const int pages0 = max(ub, x.row_blocks);
+#pragma unroll 1
+    for (int u = ub; u < ue && ok; ++u) {
+      const BlockW b = block_of(x, u, p.cache.slots);
+      const int at = (2 * (u - pages0)) % kChunkW;
+      const bool last = b.page && (u + 1 == ue || at + 2 == kChunkW);
+      float2 scales[2] = {};
+      if (b.page) {
+        if (at == 0 && !(ok = wait(kWChunk + (chunks & 1), (chunks >> 1) & 1))) break;
+        const float2* held = reinterpret_cast<const float2*>(smem + kSmemScalesW) + (chunks & 1) * kChunkW + at;
+        scales[0] = held[0];
+        scales[1] = held[1];
+      }
+      if (active) {
+        if (!(ok = wait(kWSFull + tile, s_phase))) break;
+        s_phase ^= 1;
+        if (warp_ok) {
+          train::tc_fence_after();
+          const int see = row_ok ? min(b.keys, b.see0 + lt) : 0;
+          if (b.keys > 64)
+            wide_block<128>(s_addr, o_addr, see, scales, b.page, p.scale_log2, u == ub, st);
+          else if (b.keys > 32)
+            wide_block<64>(s_addr, o_addr, see, scales, b.page, p.scale_log2, u == ub, st);
+          else
+            wide_block<32>(s_addr, o_addr, see, scales, b.page, p.scale_log2, u == ub, st);
+          train::tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kWPFull + tile));
+      }
+      if (last) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kWChunkFree + (chunks & 1)));
+        ++chunks;
+      }
+    }
+    if (!ok) break;
+    if (!active) continue;
+    if (!(ok = wait(kWODone + tile, o_phase))) break;
+    o_phase ^= 1;
+    train::tc_fence_after();
+    const bool cut = ub > 0 || ue < x.row_blocks + x.page_blocks;
+    const float inv = cut ? 1.f : 1.f / st.l;
+    const bool poisoned = poison[idx & 3] == idx + 1;
+    const int row = tile * 128 + m;
+    float* part = p.part + part_index_w(blockIdx.x, idx == range.r.x ? 0 : 1);
+    __nv_bfloat16* orow = p.out + (static_cast<size_t>(x.q0 + (row_ok ? lt : 0)) * kQHeads + 2 * x.head + (m & 1)) * kHeadDim;
+    if (warp_ok) {
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        train::tmem_ld32(o_addr + 32 * c, o);
+        if (poisoned && row_ok) {
+          // a new row's V that is not finite was taken out of the product: rows that see it get it here
+#pragma unroll 1
+          for (int j = 0; j <= x.r0 + lt; ++j) {
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(p.new_v + static_cast<size_t>(x.q0 - x.r0 + j) * kRowElems +
+                                                                  x.head * kHeadDim + 32 * c);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t w = v[i];
+              if ((w & 0x7f80u) == 0x7f80u) o[2 * i] += __uint_as_float(w << 16);
+              if ((w & 0x7f800000u) == 0x7f800000u) o[2 * i + 1] += __uint_as_float(w & 0xffff0000u);
+            }
+          }
+        }
+        if (row_ok && !cut) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(orow + 32 * c + 8 * j) =
+                make_uint4(pack_bf16x2(o[8 * j] * inv, o[8 * j + 1] * inv), pack_bf16x2(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                           pack_bf16x2(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_bf16x2(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+        } else if (row_ok) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            __stcg(reinterpret_cast<float4*>(part) + (8 * c + j) * kPartRowsW + row,
+                   make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
+        }
+      }
+      if (row_ok && cut) __stcg(reinterpret_cast<float2*>(part + kPartRowsW * kHeadDim) + row, make_float2(st.m, st.l));
+    }
+    train::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kWOFree + tile));
+  }
+  if (!ok) *abort_flag = 1;
+}
+
+template <int kCode>
+__global__ void __launch_bounds__(kWideThreads, 1) quant_wide_kernel(const __grid_constant__ MapsW maps, const AttnParamsQ p) {
+  extern __shared__ uint8_t smem_w[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_w) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem), bars = sbase + kSmemBarW;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemAbortW);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWBars; ++i) {
+      uint32_t count = 1;
+      if (i == kWQEmpty || i == kWDrain || (i >= kWEmpty && i < kWFixed)) count = 2;             // both issuers
+      if ((i >= kWRawEmpty && i < kWEmpty) || (i >= kWFixed && i < kWSFull)) count = 4;          // converting warps
+      if ((i >= kWPFull && i < kWODone) || (i >= kWOFree && i < kWTurn)) count = 4;              // softmax warps
+      if (i >= kWChunkFree) count = 8;
+      mbar_init(bars + 8u * i, count);
+    }
+    *abort_flag = 0;
+    for (int i = 0; i < 4; ++i) reinterpret_cast<volatile int*>(smem + kSmemPoisonW)[i] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) train::tmem_alloc(sbase + kSmemSlotW, 512);
+  train::tc_fence_before();
+  __syncthreads();
+  train::tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kSmemSlotW);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int* plan = wide_plan(p);
+  const int4 head = __ldg(reinterpret_cast<const int4*>(plan));
+  RangeW range{__ldg(reinterpret_cast<const int4*>(plan + plan_cta_at()) + 3 * blockIdx.x)};
+  if (head.x != kPlanMagicQ || head.y != p.grid || head.w != p.batch.requests || __ldg(plan + kQRows) != p.batch.rows) {
+    if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
+    range.r = make_int4(0, 0, -1, 0);
+  }
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegsW));
+    wide_softmax(p, plan, range, smem, sbase, tmem, abort_flag);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegsW));
+    if (warp < 10)
+      wide_issue(p, plan, range, warp - 8, sbase, tmem, abort_flag);
+    else if (warp == 10)
+      wide_fetch(p, maps, plan, range, smem, sbase, abort_flag);
+    else if (warp >= 12)
+      wide_convert<kCode>(p, maps, plan, range, smem, sbase, abort_flag);
+  }
+  train::tc_fence_before();
+  __syncthreads();
+  train::tc_fence_after();
+  if (warp == 8) train::tmem_dealloc(tmem, 512);
+}
+
+// Grid (CTAs, 8), 256 threads: CTA (c, g) merges rows 32 g .. 32 g + 31 of the cut item whose first
+// contributor is c: a lane a row, a warp 16 dims.
+__global__ void __launch_bounds__(256) quant_wide_merge_kernel(const AttnParamsQ p) {
+  const int c0 = blockIdx.x, warp = threadIdx.x >> 5, row = blockIdx.y * 32 + (threadIdx.x & 31);
+  const int* plan = wide_plan(p);
+  const int4 head = __ldg(reinterpret_cast<const int4*>(plan));
+  const int4 merge = __ldg(reinterpret_cast<const int4*>(plan + plan_merge_at(p.grid)) + c0);
+  if (head.x != kPlanMagicQ || head.y != p.grid || merge.x < 0 || merge.x >= head.z || merge.y <= c0 || merge.y >= p.grid)
+    return;
+  const ItemW it = load_item_w(plan, p.grid, merge.x);
+  const int lt = row >> 1;                                  // (tile B's row 0 is query row 64)
+  if (lt >= it.rows || it.rows > kItemQ || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return;
+  const float* first = p.part + part_index_w(c0, merge.z & 1);
+  const float* rest = p.part + part_index_w(c0, 0);
+  const size_t pitch = part_index_w(1, 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int parts = merge.y - c0 + 1;
+  float m = prefix::kNoMax, l = 0.f, o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+#pragma unroll 1
+  for (int k0 = 0; k0 < parts; k0 += 2) {
+    float2 ml[2];
+    float4 v[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float* at = k0 + i == 0 ? first : rest + min(k0 + i, parts - 1) * pitch;
+      ml[i] = __ldcg(reinterpret_cast<const float2*>(at + kPartRowsW * kHeadDim) + row);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[i][d] = __ldcg(reinterpret_cast<const float4*>(at) + (4 * warp + d) * kPartRowsW + row);
+      if (k0 + i >= parts) ml[i] = make_float2(prefix::kNoMax, 0.f);
+    }
+    const float top = fmaxf(m, fmaxf(ml[0].x, ml[1].x)), a = ex2(m - top);
+    m = top;
+    l *= a;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] *= a;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (k0 + i >= parts) break;
+      const float w = ex2(ml[i].x - top);
+      l = fmaf(ml[i].y, w, l);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        o[4 * d] = fmaf(v[i][d].x, w, o[4 * d]);
+        o[4 * d + 1] = fmaf(v[i][d].y, w, o[4 * d + 1]);
+        o[4 * d + 2] = fmaf(v[i][d].z, w, o[4 * d + 2]);
+        o[4 * d + 3] = fmaf(v[i][d].w, w, o[4 * d + 3]);
+      }
+    }
+  }
+  const float inv = 1.f / l;
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
+  uint4* out = reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(it.q0 + lt) * kQHeads + 2 * it.head + (row & 1)) * kHeadDim + 16 * warp);
+  out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  out[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+}  // namespace quant
+}  // namespace dspark

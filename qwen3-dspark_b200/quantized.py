@@ -95,7 +95,7 @@ class QuantizedLayout:
         out = cls(q, context_lengths, cu_query, context, table, slots, plan, total, max(q))
         object.__setattr__(out, '_struct', _lib.QuantBatch(
             cu_query.data_ptr(), context.data_ptr(), table.data_ptr(), slots.data_ptr(), r, total, out.max_query,
-            table.shape[1]))
+            min((n for n in q if n), default=0), table.shape[1]))
         object.__setattr__(out, '_address', ctypes.addressof(out._struct))
         object.__setattr__(out, '_plan_pointer', plan.data_ptr())
         object.__setattr__(out, 'device', device)
