@@ -97,16 +97,12 @@ int quant_setup(int max_smem_optin) {
     cudaGetLastError();
     return DSPARK_ERR_CUDA;
   }
-  // the register splits must fit what the CTAs are launched with (a setmaxnreg.inc beyond it would wait forever)
-  const struct { const void* kernel; int threads, need; } splits[] = {
-      {reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kInt8>), quant::kAttnThreadsQ, 256 * quant::kHeadRegs + 128 * quant::kFetchRegs},
-      {reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kE4M3>), quant::kAttnThreadsQ, 256 * quant::kHeadRegs + 128 * quant::kFetchRegs},
-      {reinterpret_cast<const void*>(quant::quant_wide_kernel<quant::kInt8>), quant::kWideThreads, 256 * (quant::kSoftmaxRegsW + quant::kOtherRegsW)},
-      {reinterpret_cast<const void*>(quant::quant_wide_kernel<quant::kE4M3>), quant::kWideThreads, 256 * (quant::kSoftmaxRegsW + quant::kOtherRegsW)}};
-  for (const auto& x : splits) {
+  // the register split must fit what the CTA is launched with (a setmaxnreg.inc beyond it would wait forever)
+  for (const void* k : {reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kInt8>),
+                        reinterpret_cast<const void*>(quant::quant_attn_kernel<quant::kE4M3>)}) {
     cudaFuncAttributes a;
-    if (cudaFuncGetAttributes(&a, x.kernel) != cudaSuccess) return DSPARK_ERR_CUDA;
-    if (a.numRegs * x.threads < x.need) return DSPARK_ERR_UNSUPPORTED;
+    if (cudaFuncGetAttributes(&a, k) != cudaSuccess) return DSPARK_ERR_CUDA;
+    if (a.numRegs * quant::kAttnThreadsQ < 256 * quant::kHeadRegs + 128 * quant::kFetchRegs) return DSPARK_ERR_UNSUPPORTED;
   }
   return DSPARK_OK;
 }

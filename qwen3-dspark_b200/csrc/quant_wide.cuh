@@ -44,8 +44,6 @@ enum BarW {
 constexpr uint32_t kSmemSlotW = kSmemBarW + kWBars * 8;
 constexpr uint32_t kSmemAbortW = kSmemSlotW + 4, kSmemPoisonW = kSmemAbortW + 4;
 constexpr uint32_t kSmemBytesW = 1024 + kSmemPoisonW + 16;
-// Registers of a softmax thread and of the others after setmaxnreg: the launch's own, 512 x 128.
-constexpr int kSoftmaxRegsW = 192, kOtherRegsW = 64;
 constexpr uint32_t kTmemSW = 0, kTmemOW = 256;
 
 struct MapsW {
@@ -214,6 +212,36 @@ __device__ __forceinline__ void decode4_bf16(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
+// The codes of one or two pages' K or V of a head as an operand: 64 codes of a raw row become 128
+// bytes of an operand row, 16-byte chunks permuted by its low bits. Raw rows are [page][half][key]
+// (K) or [page][dim] (V), operand rows [half][64 page + key] or [page][dim]. Thread t of the 128
+// takes 16 codes, quarter t % 4, of every 32nd raw row.
+template <int kCode>
+__device__ __forceinline__ void wide_operand(uint8_t* stage, const uint8_t* src, int tid, bool value, int pages) {
+  const int line = tid >> 2, quarter = tid & 3;
+  uint8_t* d0 = stage + line * 128 + (((2 * quarter) ^ (line & 7)) << 4);
+  uint8_t* d1 = stage + line * 128 + (((2 * quarter + 1) ^ (line & 7)) << 4);
+  const int third = value ? 8192 : 16384;                   // operand rows of raw rows 64 .. 127 of a page
+#pragma unroll 1
+  for (int page = 0; page < pages; ++page) {
+    const int at = page * (value ? 16384 : 8192);
+    uint4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(src + (4 * page + i) * 2048);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int to = at + (i >> 1) * third + (i & 1) * 4096;
+      uint4 o[2];
+      decode4_bf16<kCode>(w[i].x, o[0].x, o[0].y);
+      decode4_bf16<kCode>(w[i].y, o[0].z, o[0].w);
+      decode4_bf16<kCode>(w[i].z, o[1].x, o[1].y);
+      decode4_bf16<kCode>(w[i].w, o[1].z, o[1].w);
+      *reinterpret_cast<uint4*>(d0 + to) = o[0];
+      *reinterpret_cast<uint4*>(d1 + to) = o[1];
+    }
+  }
+}
+
 template <int kCode>
 __device__ __forceinline__ void wide_convert(const AttnParamsQ& p, const MapsW& maps, const int* plan, RangeW range,
                                              uint8_t* smem, uint32_t sbase, volatile int* abort_flag) {
@@ -240,30 +268,8 @@ __device__ __forceinline__ void wide_convert(const AttnParamsQ& p, const MapsW& 
         uint8_t* stage = smem + kSmemRingW + ring.stage * 32768;
         if (b.page) {
           if (!(ok = wait(kWRawFull + raw.stage, raw.phase)) || !(ok = wait(kWEmpty + ring.stage, ring.phase ^ 1))) break;
-          // 64 codes of a raw row become 128 bytes of an operand row, 16-byte chunks permuted by its
-          // low bits. K: raw rows [page][half][key], operand rows [half][64 page + key]; V: [page][dim]
-          const uint4* src = reinterpret_cast<const uint4*>(smem + kSmemRawW + raw.stage * 16384) + tid;
-          const int count = b.keys * 2 * 4;                 // 16-byte chunks: 128 raw rows a page, 4 each
-#pragma unroll 2
-          for (int c0 = 0; c0 < count; c0 += 256) {
-            uint4 w[2];
-            w[0] = src[c0];
-            w[1] = src[c0 + 128];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int chunk = c0 + 128 * e + tid, line = chunk >> 2, quarter = chunk & 3;
-              const int page = line >> 7, rest = line & 127;
-              const int row = v ? rest : (rest & 63) + 64 * page, half = v ? page : rest >> 6;
-              uint4 o[2];
-              decode4_bf16<kCode>(w[e].x, o[0].x, o[0].y);
-              decode4_bf16<kCode>(w[e].y, o[0].z, o[0].w);
-              decode4_bf16<kCode>(w[e].z, o[1].x, o[1].y);
-              decode4_bf16<kCode>(w[e].w, o[1].z, o[1].w);
-              uint4* dst = reinterpret_cast<uint4*>(stage + half * 16384 + row * 128);
-              dst[(2 * quarter) ^ (row & 7)] = o[0];
-              dst[(2 * quarter + 1) ^ (row & 7)] = o[1];
-            }
-          }
+          const uint8_t* src = smem + kSmemRawW + raw.stage * 16384 + tid * 16;
+          wide_operand<kCode>(stage, src, tid, v == 1, b.keys >> 6);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -422,14 +428,23 @@ __device__ __forceinline__ void wide_issue(const AttnParamsQ& p, const int* plan
       if (!(ok = wait(kWPFull + tile, p_phase))) break;
       p_phase ^= 1;
       train::tc_fence_after();
+      // (a loop for each kind of V: with the descriptors selected inside, an MMA took 135 cycles to issue)
       if (leader) {
-        const uint32_t at = static_cast<uint32_t>(vs * (32768 >> 4));
+        const uint32_t acc = u > ub ? 1u : 0u;
+        if (kmajor) {
+          const uint64_t vd = k_desc + static_cast<uint32_t>(vs * (32768 >> 4));
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          if (kk < steps) {
-            const uint64_t vd = kmajor ? k_desc + at + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4) : v_desc + at + kk * (2048 >> 4);
-            train::umma_bf16_ts(o_col, s_col + kk * 8, vd, prefix::instr_desc_n(kmajor ? 0 : 1, 128), (u > ub || kk > 0) ? 1u : 0u);
-          }
+          for (int kk = 0; kk < 8; ++kk)
+            if (kk < steps)
+              train::umma_bf16_ts(o_col, s_col + kk * 8, vd + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                                  prefix::instr_desc_n(0, 128), kk > 0 ? 1u : acc);
+        } else {
+          const uint64_t vd = v_desc + static_cast<uint32_t>(vs * (32768 >> 4));
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            if (kk < steps)
+              train::umma_bf16_ts(o_col, s_col + kk * 8, vd + kk * (2048 >> 4), prefix::instr_desc_n(1, 128), kk > 0 ? 1u : acc);
+        }
         if (more) {
           issue_qk(ring.stage, b.keys);
           train::umma_commit(bar(kWSFull + tile));
@@ -454,43 +469,35 @@ __device__ __forceinline__ void wide_issue(const AttnParamsQ& p, const int* plan
 }
 
 // ---- warps 0-7 ------------------------------------------------------------------------------------
-// One block of a row: kCols scores from TMEM, P back as packed bf16. `see` columns are visible, and
-// the halves' pages unless they are left out (a negative V scale).
-template <int kCols>
-__device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int see, const float2 (&scales)[2], bool page,
-                                           float scale_log2, bool first, prefix::RowState& st) {
-  constexpr int kHalf = kCols < 64 ? kCols : 64, kHalves = kCols / kHalf;
-  float s[kCols];
-  if constexpr (kCols == 128) {
-    train::tmem_ld128(s_addr, s);
-  } else {
+// 64 of a row's scores; those from `see` on are hidden.
+__device__ __forceinline__ void wide_scores(uint32_t addr, int see, bool full, float (&s)[64]) {
 #pragma unroll
-    for (int c = 0; c < kCols / 32; ++c) train::tmem_ld32(s_addr + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
-  }
-  float f[kHalves], base[kHalves], iv[kHalves];
-  bool out[kHalves];
+  for (int c = 0; c < 2; ++c) train::tmem_ld32_async(addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+  train::tmem_ld_wait();
 #pragma unroll
-  for (int j = 0; j < kHalves; ++j) {
-    const float vs = page ? scales[j].y : 1.f;
-    f[j] = page ? scale_log2 * scales[j].x : scale_log2;
-    const bool plain = !page || vs == 0.f;                  // (a zero block: its codes are zero)
-    base[j] = plain ? 0.f : __log2f(vs);
-    iv[j] = plain ? 1.f : 1.f / vs;
-    out[j] = vs < 0.f;
-    if (out[j]) {                                           // p = 2^(0 s - infinity)
-      f[j] = iv[j] = 0.f;
-      base[j] = -INFINITY;
-    }
-  }
-  if (!__all_sync(0xffffffffu, see >= kCols)) {
+  for (int c = 0; c < 2; ++c) train::tmem_ld_landed(*reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+  if (!full) {
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) s[i] = i < see ? s[i] : -INFINITY;
+    for (int i = 0; i < 64; ++i) s[i] = i < see ? s[i] : -INFINITY;
   }
+}
+
+// One block of a row, one or two halves of 64 columns: scores from TMEM, P back as packed bf16. `see`
+// columns are visible, and the halves' pages unless they are left out (a negative V scale). The
+// second half's scores are read twice, for the maximum and for P, and the halves are a loop: the roles' code
+// takes turns in the instruction cache of an SM quarter (unrolled over 128 columns, with the
+// converters unrolled too, a warp waited for instructions 2.7 cycles in 9).
+__device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int halves, int see, const float2* scales,
+                                           bool page, float scale_log2, bool first, prefix::RowState& st) {
+  const bool full = __all_sync(0xffffffffu, see >= 64 * halves) != 0;
+  float s[64];
   float m_new = st.m;
-#pragma unroll
-  for (int j = 0; j < kHalves; ++j) {
-    const float top = __fmul_rn(prefix::max_n<kHalf>(*reinterpret_cast<const float(*)[kHalf]>(&s[j * kHalf])), f[j]);
-    m_new = out[j] ? m_new : fmaxf(m_new, top);
+#pragma unroll 1
+  for (int j = halves - 1; j >= 0; --j) {
+    const float2 sc = page ? scales[j] : make_float2(1.f, 1.f);
+    wide_scores(s_addr + 64 * j, see - 64 * j, full, s);
+    const float top = __fmul_rn(prefix::max_n<64>(s), scale_log2 * sc.x);
+    m_new = sc.y < 0.f ? m_new : fmaxf(m_new, top);
   }
   const bool raise = m_new > st.m + 8.f;
   float alpha = 1.f;
@@ -501,32 +508,39 @@ __device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int
   // the block's S was committed behind the previous PV: O is complete
   if (!first && __any_sync(0xffffffffu, raise)) prefix::rescale_o(o_addr, alpha);
   // one fma a score, off by 2^-24 |m|; scores of thousands are scaled and shifted first, one by one
-  if (__any_sync(0xffffffffu, fabsf(st.m) > 1024.f && st.m > prefix::kNoMax)) {
-#pragma unroll
-    for (int i = 0; i < kCols; ++i) s[i] = __fsub_rn(__fmul_rn(s[i], f[i / kHalf]), st.m);
-#pragma unroll
-    for (int j = 0; j < kHalves; ++j) f[j] = 1.f;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kHalves; ++j) base[j] -= st.m;
-  }
+  const bool far = __any_sync(0xffffffffu, fabsf(st.m) > 1024.f && st.m > prefix::kNoMax) != 0;
   st.l *= alpha;
+#pragma unroll 1
+  for (int j = 0; j < halves; ++j) {
+    const float2 sc = page ? scales[j] : make_float2(1.f, 1.f);
+    if (j > 0) wide_scores(s_addr + 64 * j, see - 64 * j, full, s);      // (the first half's are still here)
+    const bool plain = !page || sc.y == 0.f;                // (a zero block: its codes are zero)
+    float base = plain ? 0.f : __log2f(sc.y), iv = plain ? 1.f : __frcp_rn(sc.y), f = scale_log2 * sc.x;
+    if (far) {
 #pragma unroll
-  for (int j = 0; j < kHalves; ++j) {
-    float sum[2] = {0.f, 0.f};
+      for (int i = 0; i < 64; ++i) s[i] = __fsub_rn(__fmul_rn(s[i], f), st.m);
+      f = 1.f;
+    } else {
+      base -= st.m;
+    }
+    if (sc.y < 0.f) {                                       // left out: p = 2^(0 s - infinity)
+      f = iv = 0.f;
+      base = -INFINITY;
+    }
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < kHalf / 32; ++c) {
+    for (int c = 0; c < 2; ++c) {
       uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float a = ex2(fmaf(s[j * kHalf + 32 * c + 2 * i], f[j], base[j]));
-        const float b = ex2(fmaf(s[j * kHalf + 32 * c + 2 * i + 1], f[j], base[j]));
-        sum[i & 1] += a + b;
+        const float a = ex2(fmaf(s[32 * c + 2 * i], f, base));
+        const float b = ex2(fmaf(s[32 * c + 2 * i + 1], f, base));
+        sum[i & 3] += a + b;
         pk[i] = pack_bf16x2(a, b);
       }
-      prefix::tmem_st16(s_addr + (j * kHalf >> 1) + 16 * c, pk);
+      prefix::tmem_st16(s_addr + 32 * j + 16 * c, pk);
     }
-    st.l = fmaf(sum[0] + sum[1], iv[j], st.l);
+    st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), iv, st.l);
   }
   prefix::tmem_st_wait();
 }
@@ -557,25 +571,15 @@ __device__ __forceinline__ void wide_softmax(const AttnParamsQ& p, const int* pl
       const BlockW b = block_of(x, u, p.cache.slots);
       const int at = (2 * (u - pages0)) % kChunkW;
       const bool last = b.page && (u + 1 == ue || at + 2 == kChunkW);
-      float2 scales[2] = {};
-      if (b.page) {
-        if (at == 0 && !(ok = wait(kWChunk + (chunks & 1), (chunks >> 1) & 1))) break;
-        const float2* held = reinterpret_cast<const float2*>(smem + kSmemScalesW) + (chunks & 1) * kChunkW + at;
-        scales[0] = held[0];
-        scales[1] = held[1];
-      }
+      const float2* scales = reinterpret_cast<const float2*>(smem + kSmemScalesW) + (chunks & 1) * kChunkW + at;
+      if (b.page && at == 0 && !(ok = wait(kWChunk + (chunks & 1), (chunks >> 1) & 1))) break;
       if (active) {
         if (!(ok = wait(kWSFull + tile, s_phase))) break;
         s_phase ^= 1;
         if (warp_ok) {
           train::tc_fence_after();
           const int see = row_ok ? min(b.keys, b.see0 + lt) : 0;
-          if (b.keys > 64)
-            wide_block<128>(s_addr, o_addr, see, scales, b.page, p.scale_log2, u == ub, st);
-          else if (b.keys > 32)
-            wide_block<64>(s_addr, o_addr, see, scales, b.page, p.scale_log2, u == ub, st);
-          else
-            wide_block<32>(s_addr, o_addr, see, scales, b.page, p.scale_log2, u == ub, st);
+          wide_block(s_addr, o_addr, b.keys > 64 ? 2 : 1, see, scales, b.page, p.scale_log2, u == ub, st);
           train::tc_fence_before();
         }
         __syncwarp();
@@ -673,18 +677,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) quant_wide_kernel(const __gri
     if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
     range.r = make_int4(0, 0, -1, 0);
   }
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegsW));
+  if (warp < 8)
     wide_softmax(p, plan, range, smem, sbase, tmem, abort_flag);
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegsW));
-    if (warp < 10)
-      wide_issue(p, plan, range, warp - 8, sbase, tmem, abort_flag);
-    else if (warp == 10)
-      wide_fetch(p, maps, plan, range, smem, sbase, abort_flag);
-    else if (warp >= 12)
-      wide_convert<kCode>(p, maps, plan, range, smem, sbase, abort_flag);
-  }
+  else if (warp < 10)
+    wide_issue(p, plan, range, warp - 8, sbase, tmem, abort_flag);
+  else if (warp == 10)
+    wide_fetch(p, maps, plan, range, smem, sbase, abort_flag);
+  else if (warp >= 12)
+    wide_convert<kCode>(p, maps, plan, range, smem, sbase, abort_flag);
   train::tc_fence_before();
   __syncthreads();
   train::tc_fence_after();
