@@ -54,7 +54,7 @@ __host__ __device__ constexpr int plan_merge_at(int grid) { return kQHeadWords +
 __host__ __device__ constexpr int plan_items_at(int grid) { return kQHeadWords + grid * (kCtaWords + kMergeWords); }
 // Two plans one behind the other: of the requests with few new rows (this file's kernel) and of
 // those with kWideRows or more (quant_wide.cuh), whose items are 128 query rows of one head.
-constexpr int kWideRows = 32, kWideItemRows = 128, kWideKeys = 128;
+constexpr int kWideRows = 41, kWideItemRows = 128, kWideKeys = 128;
 __host__ __device__ inline long long narrow_plan_words(int grid, long long requests, long long rows) {
   return plan_items_at(grid) + kItemWordsQ * (rows / kQBlock + requests);
 }
@@ -64,7 +64,7 @@ __host__ __device__ inline long long plan_words(int grid, long long requests, lo
 }
 
 // Units' worth of a new item (its queries, a partial row) and the least range of a CTA.
-constexpr int kItemCost = 0, kMinUnits = 1, kWideItemCost = 2, kWideMinUnits = 4;
+constexpr int kItemCost = 0, kMinUnits = 1, kWideItemCost = 0, kWideMinUnits = 4;
 
 struct PlanParams {
   const int* cu_q;
