@@ -479,7 +479,7 @@ bool quant_cache(quant::Cache& c, const dspark_quant_cache* x) {
 
 bool quant_batch(quant::Batch& b, const dspark_quant_batch* x) {
   if (x == nullptr) return false;
-  b = quant::Batch{x->cu_q, x->ctx_len, x->table, x->slots, x->num_requests, x->total_q, x->table_width};
+  b = quant::Batch{x->cu_q, x->ctx_len, x->table, x->slots, x->num_requests, x->total_q, x->table_width, x->min_q, x->max_q};
   for (const int32_t* t : {x->cu_q, x->ctx_len, x->table, x->slots})
     if (t == nullptr || !aligned(t, 4)) return false;
   return x->num_requests >= 1 && x->total_q >= 0 && x->max_q >= 0 && x->max_q <= x->total_q && x->min_q >= 0 &&
@@ -744,6 +744,15 @@ int dspark_verify_prep(const void* q_raw, long long ld_q, const void* k_raw, lon
   for (const void* x : {q_raw, k_raw, v_raw, q_norm_weight, k_norm_weight, rope_table, static_cast<const void*>(q_out),
                         static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
     if (x == nullptr || !aligned(x, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
+  // outputs share no byte with the projections or with each other
+  const struct { const void* p; size_t bytes; } in[] = {
+      {q_raw, 2 * (static_cast<size_t>(total_q - 1) * ld_q + q_row)}, {k_raw, 2 * (static_cast<size_t>(total_q - 1) * ld_k + kv_row)},
+      {v_raw, 2 * (static_cast<size_t>(total_q - 1) * ld_v + kv_row)}},
+      out[] = {{q_out, 2ull * total_q * q_row}, {k_out, 2ull * total_q * kv_row}, {v_out, 2ull * total_q * kv_row}};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j)
+      if (overlap(out[i].p, out[i].bytes, in[j].p, in[j].bytes) || (i < j && overlap(out[i].p, out[i].bytes, out[j].p, out[j].bytes)))
+        return DSPARK_ERR_INVALID_ARGUMENT;
   const VerifyPrepParams vp{static_cast<const __nv_bfloat16*>(q_raw), static_cast<const __nv_bfloat16*>(k_raw),
                             static_cast<const __nv_bfloat16*>(v_raw), static_cast<const __nv_bfloat16*>(q_norm_weight),
                             static_cast<const __nv_bfloat16*>(k_norm_weight), static_cast<const uint32_t*>(rope_table),
@@ -1518,7 +1527,7 @@ int dspark_quant_plan(const dspark_quant_batch* batch, int32_t* plan, long long 
   if (st != DSPARK_OK) return st;
   if (plan_words < quant::plan_words(sms, b.requests, b.rows)) return DSPARK_ERR_INVALID_ARGUMENT;
   const bool wide = batch->max_q >= quant::kWideRows;
-  const quant::PlanParams pp{b.cu_q, b.ctx, b.slot, b.requests, b.rows, b.width, sms, wide ? quant::kWideRows : 0, plan};
+  const quant::PlanParams pp{b.cu_q, b.ctx, b.slot, b.requests, b.rows, b.width, b.min_q, b.max_q, sms, wide ? quant::kWideRows : 0, plan};
   quant::plan_kernel<<<wide ? 2 : 1, quant::kPlanThreads, 0, stream>>>(pp);
   return launch_status();
 }
@@ -1546,13 +1555,17 @@ int dspark_quant_attn(const void* q, const void* new_k, const void* new_v, const
   if ((out != q && overlap(out, out_bytes, q, out_bytes)) || overlap(out, out_bytes, new_k, new_bytes) ||
       overlap(out, out_bytes, new_v, new_bytes) || overlap(out, out_bytes, c.tail_key, tail_bytes) ||
       overlap(out, out_bytes, c.tail_value, tail_bytes) || overlap(out, out_bytes, c.key, code_bytes) ||
-      overlap(out, out_bytes, c.value, code_bytes))
+      overlap(out, out_bytes, c.value, code_bytes) || overlap(out, out_bytes, c.key_scale, 4 * scales) ||
+      overlap(out, out_bytes, c.value_scale, 4 * scales))
     return DSPARK_ERR_INVALID_ARGUMENT;
   int sms = 0;
   int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < std::max(quant::attn_workspace(sms), quant::wide_workspace(sms)) ||
-      overlap(workspace, workspace_bytes, out, out_bytes) || overlap(workspace, workspace_bytes, q, out_bytes))
+      overlap(workspace, workspace_bytes, out, out_bytes) || overlap(workspace, workspace_bytes, q, out_bytes) ||
+      overlap(workspace, workspace_bytes, new_k, new_bytes) || overlap(workspace, workspace_bytes, new_v, new_bytes) ||
+      overlap(workspace, workspace_bytes, c.tail_key, tail_bytes) || overlap(workspace, workspace_bytes, c.tail_value, tail_bytes) ||
+      overlap(workspace, workspace_bytes, c.key, code_bytes) || overlap(workspace, workspace_bytes, c.value, code_bytes))
     return DSPARK_ERR_INVALID_ARGUMENT;
   if (cache->dtype == DSPARK_DTYPE_F32) {
     const int blocks = (batch->max_q + kQBlock - 1) / kQBlock;
@@ -1608,6 +1621,15 @@ int dspark_quant_append(const void* new_k, const void* new_v, long long new_rows
     return DSPARK_ERR_INVALID_ARGUMENT;
   if (batch->max_q == 0) return DSPARK_OK;
   if (!new_k || !new_v || !aligned(new_k, 16) || !aligned(new_v, 16)) return DSPARK_ERR_INVALID_ARGUMENT;
+  // the new rows are read while pages, scales and tails are written
+  const size_t layers = cache->num_layers, row = row_bytes(cache->dtype), scale_bytes = layers * ap.cache.pages * kKVHeads * 4;
+  const size_t new_bytes = layers * new_rows * row, tail_bytes = layers * ap.cache.slots * 2 * quant::kPage * row;
+  for (const void* rows : {new_k, new_v})
+    if (overlap(rows, new_bytes, cache->key, layers * ap.cache.pages * quant::kPageBytes) ||
+        overlap(rows, new_bytes, cache->value, layers * ap.cache.pages * quant::kPageBytes) ||
+        overlap(rows, new_bytes, cache->key_scale, scale_bytes) || overlap(rows, new_bytes, cache->value_scale, scale_bytes) ||
+        overlap(rows, new_bytes, cache->tail_key, tail_bytes) || overlap(rows, new_bytes, cache->tail_value, tail_bytes))
+      return DSPARK_ERR_INVALID_ARGUMENT;
   int sms = 0;
   const int st = quant_device(&sms);
   if (st != DSPARK_OK) return st;

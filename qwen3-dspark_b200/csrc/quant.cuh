@@ -44,6 +44,7 @@ struct Batch {
   const int* table;          // [R][width] page ids
   const int* slot;           // [R] tail slots
   int requests, rows, width;
+  int min_q, max_q;          // rows of the requests that have any
 };
 
 // One request of a batch; ok is false (and nothing else is used) where its metadata does not
@@ -53,6 +54,10 @@ struct Request {
   const int* table;
   bool ok;
 };
+// The launches are made for requests of so many rows.
+__device__ __forceinline__ bool rows_fit(int min_q, int max_q, int q_len) {
+  return q_len == 0 || (q_len >= min_q && q_len <= max_q);
+}
 __device__ __forceinline__ Request load_request(const Batch& b, const Cache& c, int i) {
   Request r;
   r.q0 = b.cu_q[i];
@@ -60,8 +65,8 @@ __device__ __forceinline__ Request load_request(const Batch& b, const Cache& c, 
   r.ctx = b.ctx[i];
   r.slot = b.slot[i];
   r.table = b.table + static_cast<size_t>(i) * b.width;
-  r.ok = r.q0 >= 0 && r.q_len >= 0 && r.q0 <= b.rows - r.q_len && r.ctx >= 0 && r.ctx / kPage <= b.width &&
-         r.slot >= 0 && r.slot < c.slots;
+  r.ok = r.q0 >= 0 && r.q_len >= 0 && r.q0 <= b.rows - r.q_len && rows_fit(b.min_q, b.max_q, r.q_len) && r.ctx >= 0 &&
+         r.ctx / kPage <= b.width && r.slot >= 0 && r.slot < c.slots;
   return r;
 }
 __device__ __forceinline__ size_t tail_row(int slot, int token) {

@@ -42,7 +42,7 @@ constexpr int kChunk = 32;                                  // units whose ids a
 // ---------------------------------------------------------------------------
 // Plan: int32 words [head | CTA ranges | merges | items].
 constexpr int kPlanMagicQ = 0x51a77e11;
-enum PlanWord { kQMagic = 0, kQGrid, kQItems, kQRequests, kQRows, kQHeadWords = 8 };
+enum PlanWord { kQMagic = 0, kQGrid, kQItems, kQRequests, kQRows, kQWidth, kQHeadWords = 8 };
 constexpr int kCtaWords = 12;       // first item, its first unit, last item, its end unit, the first item's 8 words
 constexpr int kMergeWords = 4;      // item (-1: none), last contributor, slot of the first
 constexpr int kItemWordsQ = 12;
@@ -70,7 +70,7 @@ struct PlanParams {
   const int* cu_q;
   const int* ctx;
   const int* slot;
-  int requests, rows, width, grid;
+  int requests, rows, width, min_q, max_q, grid;
   int wide_rows;             // requests with as many new rows are in the second plan (0: none)
   int* plan;
 };
@@ -84,13 +84,14 @@ __device__ __forceinline__ int row_units(int ctx, int q_len, int r0, bool wide) 
 }
 __device__ __forceinline__ int page_units(int ctx, bool wide) { return wide ? (ctx / kPage + 1) / 2 : ctx / kPage; }
 
-// CTA 0 makes the first plan, CTA 1 the second. Requests whose lengths do not fit the batch have no
-// items (the status is set).
+// CTA 0 makes the first plan, CTA 1 the second. A request whose lengths do not fit the batch has no
+// items, and where rows of requests are out of order or range no request has (the status is set).
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   __shared__ long long s_cost[32];
   __shared__ int s_items[32];
   __shared__ long long carry_cost;
   __shared__ int carry_items;
+  __shared__ int disorder;
   const bool wide = blockIdx.x == 1;
   const int block_rows = wide ? kWideItemRows : kQBlock, heads = wide ? kKVHeads : 1;
   const int item_cost = wide ? kWideItemCost : kItemCost, min_units = wide ? kWideMinUnits : kMinUnits;
@@ -100,7 +101,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   if (tid == 0) {
     carry_cost = 0;
     carry_items = 0;
+    disorder = 0;
   }
+  // (what an ordered batch needs at most)
+  const unsigned room = static_cast<unsigned>(p.rows / block_rows + p.requests) * heads;
   __syncthreads();
   for (int base = 0; base < p.requests; base += kPlanThreads) {
     const int i = base + tid;
@@ -111,7 +115,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       q_len = p.cu_q[i + 1] - q0;
       ctx = p.ctx[i];
       slot = p.slot[i];
-      if (q0 >= 0 && q_len >= 0 && q0 <= p.rows - q_len && ctx >= 0 && ctx / kPage <= p.width) {
+      const bool ordered = q0 >= 0 && q_len >= 0 && q0 <= p.rows - q_len;
+      if (!ordered) disorder = 1;
+      if (ordered && rows_fit(p.min_q, p.max_q, q_len) && ctx >= 0 && ctx / kPage <= p.width) {
         if ((p.wide_rows > 0 && q_len >= p.wide_rows) == wide) n = (q_len + block_rows - 1) / block_rows;
         for (int x = 0; x < n; ++x) cost += heads * (item_cost + page_units(ctx, wide) + row_units(ctx, q_len, x * block_rows, wide));
         n *= heads;
@@ -154,7 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     __syncthreads();
     long long at = carry_cost + (warp > 0 ? s_cost[warp - 1] : 0) + c - cost;
     int idx = carry_items + (warp > 0 ? s_items[warp - 1] : 0) + m - n;
-    for (int x = 0; x < n; ++x, ++idx) {
+    for (int x = 0; x < n && static_cast<unsigned>(idx) < room; ++x, ++idx) {
       const int r0 = x / heads * block_rows, ru = row_units(ctx, q_len, r0, wide), pu = page_units(ctx, wide);
       int4* w = reinterpret_cast<int4*>(items + static_cast<size_t>(idx) * kItemWordsQ);
       w[0] = make_int4(q0 + r0, min(block_rows, q_len - r0), r0, i);
@@ -169,8 +175,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     }
     __syncthreads();
   }
-  const int count = carry_items;
-  long long total = carry_cost;
+  const int count = disorder ? 0 : carry_items;
+  long long total = disorder ? 0 : carry_cost;
   if (total >= (1ll << 31)) {                                // (the starts are 32-bit words)
     if (tid == 0) atomicOr(&g_device_status, kStatusBadArgument);
     total = 0;
@@ -228,6 +234,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     plan[kQItems] = count;
     plan[kQRequests] = p.requests;
     plan[kQRows] = p.rows;
+    plan[kQWidth] = p.width;
     plan[kQMagic] = kPlanMagicQ;
   }
 }
@@ -250,6 +257,19 @@ __host__ __device__ inline size_t part_index(int cta, int slot, int head) {
   return ((static_cast<size_t>(cta) * 2 + slot) * kKVHeads + head) * kPartFloats;
 }
 inline size_t attn_workspace(int grid) { return part_index(grid, 0, 0) * sizeof(float); }
+
+// Whether the plan was made for this batch's numbers (memory that never held one says no).
+__device__ __forceinline__ bool plan_fits(const AttnParamsQ& p, const int* plan) {
+  const int4 head = __ldg(reinterpret_cast<const int4*>(plan));
+  const int2 more = __ldg(reinterpret_cast<const int2*>(plan + kQRows));
+  return head.x == kPlanMagicQ && head.y == p.grid && head.w == p.batch.requests && more.x == p.batch.rows &&
+         more.y == p.batch.width;
+}
+// A merge's CTAs without work leave at once; one always waits, so that the launch does not end before
+// the attention does (the next launch may be a dependent of this one alone).
+__device__ __forceinline__ void merge_idle() {
+  if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 struct ItemQ {
   int q0, rows, r0, request, row_units, pages, ctx, slot;
@@ -623,10 +643,8 @@ __global__ void __launch_bounds__(kAttnThreadsQ, 1) quant_attn_kernel(const Attn
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int4* cta = reinterpret_cast<const int4*>(p.plan + plan_cta_at()) + 3 * blockIdx.x;
-  const int4 head = __ldg(reinterpret_cast<const int4*>(p.plan));
-  const int head_rows = __ldg(p.plan + kQRows);
   const int4 range = __ldg(cta);
-  if (head.x != kPlanMagicQ || head.y != p.grid || head.w != p.batch.requests || head_rows != p.batch.rows) {
+  if (!plan_fits(p, p.plan)) {
     if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
     return;
   }
@@ -876,12 +894,11 @@ __global__ void __launch_bounds__(256) quant_merge_kernel(const AttnParamsQ p) {
   __shared__ float4 s_o[8][2][32];
   __shared__ float2 s_ml[8][2];
   const int c0 = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int4 head = __ldg(reinterpret_cast<const int4*>(p.plan));
   const int4 merge = __ldg(reinterpret_cast<const int4*>(p.plan + plan_merge_at(p.grid)) + c0);
-  if (head.x != kPlanMagicQ || head.y != p.grid || merge.x < 0 || merge.x >= head.z || merge.y <= c0 || merge.y >= p.grid)
-    return;
+  const int count = __ldg(p.plan + kQItems);
+  if (!plan_fits(p, p.plan) || merge.x < 0 || merge.x >= count || merge.y <= c0 || merge.y >= p.grid) return merge_idle();
   const ItemQ it = load_item_q(p, merge.x);
-  if (it.rows < 1 || it.rows > kQBlock || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return;
+  if (it.rows < 1 || it.rows > kQBlock || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return merge_idle();
   const int shift = it.rows > 4 ? 3 : (it.rows > 2 ? 2 : it.rows - 1);     // 2^shift rows, 8 >> shift warps each
   const int r = warp & ((1 << shift) - 1), group = warp >> shift, step = 8 >> shift;
   const bool live = r < it.rows;

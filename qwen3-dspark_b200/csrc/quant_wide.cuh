@@ -482,6 +482,8 @@ __device__ __forceinline__ void wide_scores(uint32_t addr, int see, bool full, f
   }
 }
 
+constexpr float kTinyScale = 1.f / 18446744073709551616.f;  // 2^-64
+
 // One block of a row, one or two halves of 64 columns: scores from TMEM, P back as packed bf16. `see`
 // columns are visible, and the halves' pages unless they are left out (a negative V scale). The
 // second half's scores are read twice, for the maximum and for P, and the halves are a loop: the roles' code
@@ -526,6 +528,14 @@ __device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int
     if (sc.y < 0.f) {                                       // left out: p = 2^(0 s - infinity)
       f = iv = 0.f;
       base = -INFINITY;
+    }
+    if (!plain && sc.y > 0.f && sc.y < kTinyScale) {        // p vs may be below the least float: the sum apart
+      const float shift = far ? 0.f : -st.m;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) sum += ex2(fmaf(s[i], f, shift));
+      st.l += sum;
+      iv = 0.f;
     }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -671,9 +681,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) quant_wide_kernel(const __gri
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int* plan = wide_plan(p);
-  const int4 head = __ldg(reinterpret_cast<const int4*>(plan));
   RangeW range{__ldg(reinterpret_cast<const int4*>(plan + plan_cta_at()) + 3 * blockIdx.x)};
-  if (head.x != kPlanMagicQ || head.y != p.grid || head.w != p.batch.requests || __ldg(plan + kQRows) != p.batch.rows) {
+  if (!plan_fits(p, plan)) {
     if (threadIdx.x == 0) atomicOr(&g_device_status, kStatusBadArgument);
     range.r = make_int4(0, 0, -1, 0);
   }
@@ -696,13 +705,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) quant_wide_kernel(const __gri
 __global__ void __launch_bounds__(256) quant_wide_merge_kernel(const AttnParamsQ p) {
   const int c0 = blockIdx.x, warp = threadIdx.x >> 5, row = blockIdx.y * 32 + (threadIdx.x & 31);
   const int* plan = wide_plan(p);
-  const int4 head = __ldg(reinterpret_cast<const int4*>(plan));
   const int4 merge = __ldg(reinterpret_cast<const int4*>(plan + plan_merge_at(p.grid)) + c0);
-  if (head.x != kPlanMagicQ || head.y != p.grid || merge.x < 0 || merge.x >= head.z || merge.y <= c0 || merge.y >= p.grid)
-    return;
+  const int count = __ldg(plan + kQItems);
+  if (!plan_fits(p, plan) || merge.x < 0 || merge.x >= count || merge.y <= c0 || merge.y >= p.grid) return merge_idle();
   const ItemW it = load_item_w(plan, p.grid, merge.x);
   const int lt = row >> 1;                                  // (tile B's row 0 is query row 64)
-  if (lt >= it.rows || it.rows > kItemQ || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return;
+  if (lt >= it.rows || it.rows > kItemQ || it.q0 < 0 || it.q0 + it.rows > p.batch.rows) return merge_idle();
   const float* first = p.part + part_index_w(c0, merge.z & 1);
   const float* rest = p.part + part_index_w(c0, 0);
   const size_t pitch = part_index_w(1, 0);

@@ -1,0 +1,152 @@
+"""Refusals and host bookkeeping of the paged 8-bit cache that need no GPU."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def lib_and_types(pkg):
+    import importlib
+    return pkg.load_library(), importlib.import_module('qwen3-dspark_b200._lib')
+
+
+def cache(L, base=1 << 32, **change):
+    """A dspark_quant_cache of distinct aligned addresses (never read: every call below is refused)."""
+    v = dict(key=base, value=base + (1 << 30), key_scale=base + (2 << 30), value_scale=base + (2 << 30) + (1 << 20),
+             tail_key=base + (3 << 30), tail_value=base + (4 << 30), num_layers=2, num_pages=10, num_slots=3, code=0, dtype=0)
+    v.update(change)
+    return L.QuantCache(**v)
+
+
+def batch(L, base=1 << 20, **change):
+    v = dict(cu_q=base, ctx_len=base + 4096, table=base + 8192, slots=base + 12288, num_requests=2, total_q=5, max_q=3,
+             min_q=2, table_width=4)
+    v.update(change)
+    return L.QuantBatch(**v)
+
+
+def test_structures_match_the_header(pkg):
+    _, L = lib_and_types(pkg)
+    text = open(os.path.join(ROOT, 'include', 'dspark_b200.h')).read()
+    text = re.sub(r'/\*.*?\*/', '', text, flags=re.S)
+    for name, cls in (('dspark_quant_cache', L.QuantCache), ('dspark_quant_batch', L.QuantBatch)):
+        body = re.search(r'typedef struct \{([^}]*)\} ' + name, text).group(1)
+        fields = []
+        for line in body.split(';'):
+            m = re.match(r'\s*(const )?(void|float|int32_t|int)\s*(\*?)\s*(.*)', line, re.S)
+            if m:
+                fields += [(x.strip(), ctypes.c_void_p if m.group(3) else ctypes.c_int) for x in m.group(4).split(',')]
+        assert fields == [(n, t) for n, t in cls._fields_]
+
+
+def test_entries_refuse_before_any_device_work(pkg):
+    lib, L = lib_and_types(pkg)
+    at = lambda s: ctypes.addressof(s)  # noqa: E731
+    rows, out, plan, ws = 5 << 32, 6 << 32, 7 << 32, 8 << 32
+    good_c, good_b = cache(L), batch(L)
+    attn = lambda c, b, q=rows, k=rows + (1 << 20), v=rows + (2 << 20), layer=0, o=out, scale=128 ** -0.5: (  # noqa: E731
+        lib.dspark_quant_attn(q, k, v, None if c is None else at(c), layer, None if b is None else at(b), plan, scale, o, ws,
+                              0, None))
+    append = lambda c, b, k=rows, v=rows + (1 << 20), n=5: lib.dspark_quant_append(k, v, n, at(c), at(b), None, None)  # noqa: E731
+    bad_caches = [dict(key=None), dict(value=8), dict(key_scale=None), dict(tail_value=4), dict(num_layers=0),
+                  dict(num_pages=0), dict(num_slots=0), dict(code=2), dict(dtype=2), dict(num_layers=70000)]
+    bad_batches = [dict(cu_q=None), dict(table=None), dict(slots=2), dict(num_requests=0), dict(total_q=-1), dict(max_q=6),
+                   dict(min_q=4), dict(min_q=-1), dict(table_width=0)]
+    for change in bad_caches:
+        assert attn(cache(L, **change), good_b) == 1, change
+        assert append(cache(L, **change), good_b) == 1, change
+        assert lib.dspark_quant_copy(at(cache(L, **change)), 16, 32, 1, None, None, None, 0, None) == 1, change
+    for change in bad_batches:
+        assert attn(good_c, batch(L, **change)) == 1, change
+        assert append(good_c, batch(L, **change)) == 1, change
+        assert lib.dspark_quant_plan(at(batch(L, **change)), plan, 1 << 20, None) == 1, change
+    assert attn(None, good_b) == 1 and attn(good_c, None) == 1
+    assert attn(good_c, good_b, layer=2) == 1 and attn(good_c, good_b, layer=-1) == 1
+    assert attn(good_c, good_b, scale=0.0) == 1 and attn(good_c, good_b, q=None) == 1 and attn(good_c, good_b, o=rows + 8) == 1
+    # the output may be the query, and shares no byte with anything else that is read
+    assert attn(good_c, good_b, o=rows + 4096) == 1
+    assert attn(good_c, good_b, o=rows + (1 << 20)) == 1
+    assert attn(good_c, good_b, o=good_c.tail_key) == 1
+    assert attn(good_c, good_b, o=good_c.key + 65536 * 9) == 1
+    assert append(good_c, good_b, n=4) == 1                                    # fewer rows than the batch has
+    assert append(good_c, good_b, k=None) == 1 and append(good_c, good_b, v=rows + 4) == 1
+    assert append(good_c, good_b, k=good_c.tail_key + 4096) == 1               # rows read and written
+    assert append(good_c, good_b, v=good_c.value_scale) == 1
+    assert lib.dspark_quant_plan(at(good_b), None, 1 << 20, None) == 1
+    assert lib.dspark_quant_plan(at(good_b), plan + 4, 1 << 20, None) == 1
+    assert lib.dspark_quant_copy(at(good_c), None, 32, 1, None, None, None, 0, None) == 1
+    assert lib.dspark_quant_copy(at(good_c), 16, 32, -1, None, None, None, 0, None) == 1
+    assert lib.dspark_quant_copy(at(good_c), None, None, 0, 16, 32, None, 1, None) == 1
+    words, size = ctypes.c_longlong(0), None
+    assert lib.dspark_quant_plan_words(0, 0, 5, ctypes.byref(words)) == 1
+    assert lib.dspark_quant_plan_words(0, 1, -1, ctypes.byref(words)) == 1
+    assert lib.dspark_quant_plan_words(0, 1, 5, None) == 1 and lib.dspark_quant_workspace_size(0, size) == 1
+    # nothing to do: no launch, no device needed
+    empty = batch(L, total_q=0, max_q=0, min_q=0)
+    assert attn(good_c, empty) == 0 and append(good_c, empty) == 0
+    assert lib.dspark_quant_copy(at(good_c), None, None, 0, None, None, None, 0, None) == 0
+
+
+def test_verify_prep_refuses(pkg):
+    lib, _ = lib_and_types(pkg)
+    a = [(i + 1) << 24 for i in range(9)]
+    call = lambda p=a, ld=(2048, 1024, 1024), n=4, eps=1e-6: lib.dspark_verify_prep(  # noqa: E731
+        p[0], ld[0], p[1], ld[1], p[2], ld[2], p[3], p[4], p[5], eps, n, p[6], p[7], p[8], None)
+    for i in range(9):
+        assert call(a[:i] + [None] + a[i + 1:]) == 1 and call(a[:i] + [a[i] + 8] + a[i + 1:]) == 1
+    assert call(ld=(2040, 1024, 1024)) == 1 and call(ld=(2048, 1028, 1024)) == 1
+    assert call(n=0) == 1 and call(eps=0.0) == 1
+    assert call(a[:6] + [a[0]] + a[7:]) == 1 and call(a[:7] + [a[2] + 2048] + a[8:]) == 1 and call(a[:8] + [a[7] + 64]) == 1
+
+
+def pool_without_gpu(pkg, pages):
+    p = object.__new__(pkg.QuantizedPages)
+    p.pages, p.users, p._free = pages, [0] * pages, list(range(pages))
+    return p
+
+
+def test_page_owners(pkg):
+    p = pool_without_gpu(pkg, 6)
+    a = p.allocate(3)
+    assert a == [0, 1, 2] and p.free_pages == 3
+    p.share(a[:2])
+    b = p.allocate(2)
+    p.free(a)
+    assert p.free_pages == 2 and p.users == [1, 1, 0, 1, 1, 0]
+    assert p.allocate(1) == [2]                         # the lowest free id
+    p.free([0, 1])
+    p.free(b)
+    assert p.free_pages == 5
+    for call in (lambda: p.allocate(6), lambda: p.allocate(-1), lambda: p.allocate(1.0), lambda: p.free([0]),
+                 lambda: p.share([5]), lambda: p.free([6]), lambda: p.free([-1]), lambda: p.free([2, 2])):
+        before = (list(p.users), sorted(p._free))
+        with pytest.raises(ValueError):
+            call()
+        assert (p.users, sorted(p._free)) == before
+    assert p.allocate(0) == []
+
+
+def test_python_refuses_what_is_not_on_a_gpu(pkg):
+    with pytest.raises(ValueError):
+        pkg.QuantizedLayout.from_lengths([1], [5], torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        pkg.QuantizedLayout.from_lengths([], [], torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        pkg.QuantizedLayout.from_lengths([-1], [5], torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    t = torch.zeros((1, 1, 8, 2, 64, 64), dtype=torch.int8)
+    with pytest.raises(ValueError):
+        pkg.QuantizedPages(t, t, t, t, t, t)
+    with pytest.raises(ValueError):
+        pkg.QuantizedPages.empty(layers=0, pages=1, slots=1, device='cpu')
+    with pytest.raises(ValueError):
+        pkg.QuantizedPages.empty(layers=1, pages=1, slots=1, dtype=torch.int16, device='cpu')
+    with pytest.raises(RuntimeError):
+        pkg.B200QuantizedKernel('cpu')
+    with pytest.raises(ValueError):
+        pkg.B200QuantizedTargetKV(layers=1, slots=1, context_capacity=64, max_query_tokens=1, cache='int4')
+    with pytest.raises(ValueError):
+        pkg.B200QuantizedTargetKV(layers=1, slots=1, context_capacity=64, max_query_tokens=1, pages=0)
