@@ -90,14 +90,28 @@ __device__ __forceinline__ float2 decode2(uint32_t two) {
 }
 
 // ---------------------------------------------------------------------------
-// Float32 attention on the CUDA cores: one CTA per (request, 8 query rows, KV head, split), a warp
-// per (row, query head). Steps of 64 keys are decoded into shared memory, the next step's codes
-// on their way meanwhile; lane l scores keys l and l + 32 and then holds dims 4 l .. 4 l + 3 of the
-// output. Bound by the arithmetic of a step (2 us); where the batch has too few CTAs, a request's
-// steps are split among up to 16, whose partial rows a second launch adds up.
+// Float32 attention on the CUDA cores: one CTA per (request, 8 query rows, KV head, split), which are
+// 16 rows (2 * query row + query head). Steps of 64 keys are decoded into shared memory, the next
+// step's codes on their way meanwhile. A thread scores 4 rows x 4 keys over 16 dims (8 lanes share a
+// tile and add up) and holds 4 rows x 4 dims of the output over 16 keys of each step, so that a
+// float4 read from shared memory feeds 8 products; with a row a warp it fed 4 and those reads bound
+// the kernel. Warps whose rows do not exist skip both products. Where the batch has too few CTAs, a
+// request's steps are split among up to 16, whose partial rows a dependent launch adds up. 6 requests
+// of 7 rows behind up to 900 tokens: 17.8 us (a row a warp: 30), most of it the chain of loads, a
+// step or two and the merge.
 constexpr int kF32AttnThreads = 16 * 32, kF32Splits = 16;
-constexpr int kF32KPitch = kHeadDim + 4;                    // float4 reads of 8 rows hit distinct banks
-constexpr size_t kF32AttnSmem = sizeof(float) * (kPage * kF32KPitch + kPage * kHeadDim + 16 * kHeadDim);
+constexpr int kF32KPitch = kHeadDim + 4;                    // float4 reads of 8 lanes hit distinct banks
+constexpr int kF32SPitch = kPage + 8, kF32PPitch = 16 + 4;
+struct F32Smem {
+  float k[kPage * kF32KPitch];                              // [key][dim]; at the end the output's 4 parts
+  float v[kPage * kHeadDim];                                // [key][dim ^ 8 (key / 16)]
+  float q[16 * kHeadDim];
+  float s[16 * kF32SPitch];                                 // scores [row][key]
+  float p[kPage * kF32PPitch];                              // probabilities [key][row]
+  float alpha[16];
+};
+static_assert(sizeof(float) * 4 * 16 * kHeadDim <= sizeof(F32Smem::k), "the output's parts take the place of K");
+constexpr size_t kF32AttnSmem = sizeof(F32Smem);
 
 struct F32Params {
   const float* q;            // [rows, 16, 128]
@@ -116,13 +130,13 @@ __device__ __forceinline__ float* f32_part(const F32Params& p, int head) {
   const size_t item = (static_cast<size_t>(blockIdx.x) * gridDim.y + blockIdx.y) * kKVHeads + head;
   return p.part + item * p.splits * kPartFloats;
 }
+__device__ __forceinline__ int f32_v_at(int key, int dim) { return key * kHeadDim + (dim ^ (8 * ((key >> 4) & 3))); }
 
 template <int kCode>
-__global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Params p) {
+__global__ void __launch_bounds__(kF32AttnThreads, 2) f32_attn_kernel(const F32Params p) {
   extern __shared__ float4 smem4[];
-  float* sk = reinterpret_cast<float*>(smem4);
-  float* sv = sk + kPage * kF32KPitch;
-  float* sq = sv + kPage * kHeadDim;
+  F32Smem& sm = *reinterpret_cast<F32Smem*>(smem4);
+  asm volatile("griddepcontrol.launch_dependents;");        // (the merge waits for this grid's end)
   const int h = blockIdx.z % kKVHeads, split = blockIdx.z / kKVHeads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Request req = load_request(p.batch, p.cache, blockIdx.x);
@@ -132,17 +146,21 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
     return;
   }
   if (r0 >= req.q_len) return;
-  const int row = r0 + (warp & 7), head = 2 * h + (warp >> 3);
+  // row `warp` of the CTA: its softmax is this warp's
+  const int row = r0 + (warp >> 1), head = 2 * h + (warp & 1);
   const bool live = row < req.q_len;
   const size_t q_at = (static_cast<size_t>(req.q0 + (live ? row : r0)) * kQHeads + head) * kHeadDim;
-  *reinterpret_cast<float4*>(sq + warp * kHeadDim + 4 * lane) = *reinterpret_cast<const float4*>(p.q + q_at + 4 * lane);
+  *reinterpret_cast<float4*>(sm.q + warp * kHeadDim + 4 * lane) = *reinterpret_cast<const float4*>(p.q + q_at + 4 * lane);
+  // rows 4 tile .. 4 tile + 3, keys 16 part .. 16 part + 15: this warp's part of the products
+  const int tile = warp & 3, part = warp >> 2;
+  const bool tile_live = r0 + 2 * tile < req.q_len;
   const int full = req.ctx / kPage, tail = req.ctx % kPage;
   const int visible = tail + min(r0 + kQBlock, req.q_len);   // unquantised keys that a row of this CTA sees
   const float* tk = static_cast<const float*>(p.cache.tail_key) + tail_row(req.slot, req.ctx - tail) * kRowElems + h * kHeadDim;
   const float* tv = static_cast<const float*>(p.cache.tail_value) + tail_row(req.slot, req.ctx - tail) * kRowElems + h * kHeadDim;
   const float* nk = p.new_k + static_cast<size_t>(req.q0) * kRowElems + h * kHeadDim;
   const float* nv = p.new_v + static_cast<size_t>(req.q0) * kRowElems + h * kHeadDim;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f, o[4][4] = {};
   const int steps = full + (visible + kPage - 1) / kPage;
   const int first = static_cast<int>(static_cast<long long>(steps) * split / p.splits);
   const int last = static_cast<int>(static_cast<long long>(steps) * (split + 1) / p.splits);
@@ -168,15 +186,16 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
 #pragma unroll 1
   for (int step = first; step < last; ++step) {
     float pks = 1.f, pvs = 1.f;
-    int limit = kPage;                                        // keys that this warp's row sees
+    const int t0 = (step - full) * kPage;                     // (row steps) the first key
+    int keys = kPage;
     __syncthreads();
     if (step < full) {
       const bool there = id >= 0;
       pks = ks;
       pvs = vs;
       const uint32_t kw[4] = {kc.x, kc.y, kc.z, kc.w}, vw[4] = {vc.x, vc.y, vc.z, vc.w};
-      float* kd = sk + ((tid & 255) >> 2) * kF32KPitch + (tid >> 8) * 64 + (tid & 3) * 16;
-      float* vd = sv + (tid & 3) * 16 * kHeadDim + (tid >> 2);
+      float* kd = sm.k + ((tid & 255) >> 2) * kF32KPitch + (tid >> 8) * 64 + (tid & 3) * 16;
+      float* vd = sm.v + f32_v_at((tid & 3) * 16, tid >> 2);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float2 a = decode2<kCode>(kw[w]), b = decode2<kCode>(kw[w] >> 16);
@@ -190,71 +209,148 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_attn_kernel(const F32Para
       fetch(step + 1);
       if (!there) continue;
     } else {
-      const int t0 = (step - full) * kPage, keys = min(kPage, visible - t0);
-      limit = min(keys, tail + row + 1 - t0);
+      keys = min(kPage, visible - t0);
       for (int u = tid; u < keys * 32; u += kF32AttnThreads) {
-        const int t = t0 + (u >> 5), d = 4 * (u & 31);
+        const int j = u >> 5, t = t0 + j, d = 4 * (u & 31);
         const size_t at = static_cast<size_t>(t < tail ? t : t - tail) * kRowElems + d;
-        *reinterpret_cast<float4*>(sk + (u >> 5) * kF32KPitch + d) = *reinterpret_cast<const float4*>((t < tail ? tk : nk) + at);
-        *reinterpret_cast<float4*>(sv + (u >> 5) * kHeadDim + d) = *reinterpret_cast<const float4*>((t < tail ? tv : nv) + at);
+        *reinterpret_cast<float4*>(sm.k + j * kF32KPitch + d) = *reinterpret_cast<const float4*>((t < tail ? tk : nk) + at);
+        *reinterpret_cast<float4*>(sm.v + f32_v_at(j, d)) = *reinterpret_cast<const float4*>((t < tail ? tv : nv) + at);
       }
     }
     __syncthreads();
-    if (!live) continue;                                      // (a whole warp)
-    float s[2];
+    if (tile_live && 16 * part < keys) {                      // (scores behind the last key are not used)
+      float acc[4][4] = {};
+      const float* kr = sm.k + (16 * part + 4 * (lane >> 3)) * kF32KPitch + 4 * (lane & 7);
+      const float* qr = sm.q + 4 * tile * kHeadDim + 4 * (lane & 7);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int j = lane + 32 * e;
-      float dot = 0.f;
-      if (j < limit) {
-        const float4* kr = reinterpret_cast<const float4*>(sk + j * kF32KPitch);
-        const float4* qr = reinterpret_cast<const float4*>(sq + warp * kHeadDim);
-#pragma unroll 8
-        for (int d = 0; d < 32; ++d) {
-          const float4 a = qr[d], b = kr[d];
-          dot = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, dot))));
+      for (int i = 0; i < 4; ++i) {
+        float4 kf[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) kf[c] = *reinterpret_cast<const float4*>(kr + c * kF32KPitch + 32 * i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float4 a = *reinterpret_cast<const float4*>(qr + r * kHeadDim + 32 * i);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            acc[r][c] = fmaf(a.x, kf[c].x, fmaf(a.y, kf[c].y, fmaf(a.z, kf[c].z, fmaf(a.w, kf[c].w, acc[r][c]))));
         }
       }
-      s[e] = j < limit ? dot * (pks * p.scale) : -INFINITY;
+      // over the 8 lanes of a tile: each halving keeps the rows, then the keys, of the lane's bit
+      float two[2][4], one[4], s[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float keep = lane & 4 ? acc[r + 2][c] : acc[r][c], give = lane & 4 ? acc[r][c] : acc[r + 2][c];
+          two[r][c] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+        }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float keep = lane & 2 ? two[1][c] : two[0][c], give = lane & 2 ? two[0][c] : two[1][c];
+        one[c] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float keep = lane & 1 ? one[c + 2] : one[c], give = lane & 1 ? one[c] : one[c + 2];
+        s[c] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+      }
+      *reinterpret_cast<float2*>(sm.s + (4 * tile + ((lane >> 1) & 3)) * kF32SPitch + 16 * part +
+                                 4 * (lane >> 3) + 2 * (lane & 1)) = make_float2(s[0], s[1]);
     }
-    float mx = fmaxf(s[0], s[1]);
+    __syncthreads();
+    if (live) {
+      const int limit = step < full ? kPage : min(keys, tail + row + 1 - t0);     // keys that the row sees
+      float s[2];
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = expf(m - mu);
-    const float e0 = expf(s[0] - mu), e1 = expf(s[1] - mu);
-    float sum = e0 + e1;
+      for (int e = 0; e < 2; ++e)
+        s[e] = lane + 32 * e < limit ? sm.s[warp * kF32SPitch + lane + 32 * e] * (pks * p.scale) : -INFINITY;
+      float mx = fmaxf(s[0], s[1]);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    l = l * alpha + sum;
-    m = mn;
-    float a[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = expf(m - mu);
+      const float e0 = expf(s[0] - mu), e1 = expf(s[1] - mu);
+      float sum = e0 + e1;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      l = l * alpha + sum;
+      m = mn;
+      sm.p[lane * kF32PPitch + warp] = e0 * pvs;
+      sm.p[(lane + 32) * kF32PPitch + warp] = e1 * pvs;
+      if (lane == 0) sm.alpha[warp] = alpha;
+    }
+    __syncthreads();
+    if (!tile_live) continue;
+    const float4 al = *reinterpret_cast<const float4*>(sm.alpha + 4 * tile);
+    const float a4[4] = {al.x, al.y, al.z, al.w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[r][d] *= a4[r];
+    const float* vr = sm.v + 16 * part * kHeadDim + ((4 * lane) ^ (8 * part));
+    const float* pr = sm.p + 16 * part * kF32PPitch + 4 * tile;
+    // the keys of this part that the tile's two query rows see
+    const int see0 = step < full ? 16 : min(keys, tail + r0 + 2 * tile + 1 - t0) - 16 * part;
+    const int see1 = step < full ? 16 : min(keys, tail + r0 + 2 * tile + 2 - t0) - 16 * part;
+    if (see0 >= 16) {
 #pragma unroll 4
-    for (int j = 0; j < limit; ++j) {                         // (keys that the row does not see are not touched)
-      const float w = __shfl_sync(0xffffffffu, j < 32 ? e0 : e1, j & 31);
-      const float4 v = *reinterpret_cast<const float4*>(sv + j * kHeadDim + 4 * lane);
-      a[0] = fmaf(w, v.x, a[0]);
-      a[1] = fmaf(w, v.y, a[1]);
-      a[2] = fmaf(w, v.z, a[2]);
-      a[3] = fmaf(w, v.w, a[3]);
-    }
+      for (int j = 0; j < 16; ++j) {
+        const float4 w = *reinterpret_cast<const float4*>(pr + j * kF32PPitch), v = *reinterpret_cast<const float4*>(vr + j * kHeadDim);
+        const float w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = fmaf(a[i], pvs, o[i] * alpha);
+        for (int r = 0; r < 4; ++r) {
+          o[r][0] = fmaf(w4[r], v.x, o[r][0]);
+          o[r][1] = fmaf(w4[r], v.y, o[r][1]);
+          o[r][2] = fmaf(w4[r], v.z, o[r][2]);
+          o[r][3] = fmaf(w4[r], v.w, o[r][3]);
+        }
+      }
+    } else {                                                  // what a row does not see stays out, whatever it holds
+#pragma unroll 1
+      for (int j = 0; j < min(see1, 16); ++j) {
+        const float4 w = *reinterpret_cast<const float4*>(pr + j * kF32PPitch), v = *reinterpret_cast<const float4*>(vr + j * kHeadDim);
+        const float w4[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r < 2 && j >= see0) continue;
+          o[r][0] = fmaf(w4[r], v.x, o[r][0]);
+          o[r][1] = fmaf(w4[r], v.y, o[r][1]);
+          o[r][2] = fmaf(w4[r], v.z, o[r][2]);
+          o[r][3] = fmaf(w4[r], v.w, o[r][3]);
+        }
+      }
+    }
   }
+  __syncthreads();
+  if (tile_live)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<float4*>(sm.k + (part * 16 + 4 * tile + r) * kHeadDim + 4 * lane) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+  __syncthreads();
   if (!live) return;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 y = *reinterpret_cast<const float4*>(sm.k + (i * 16 + warp) * kHeadDim + 4 * lane);
+    x.x += y.x;
+    x.y += y.y;
+    x.z += y.z;
+    x.w += y.w;
+  }
   if (p.splits == 1) {
-    *reinterpret_cast<float4*>(p.out + q_at + 4 * lane) = make_float4(o[0] / l, o[1] / l, o[2] / l, o[3] / l);
+    *reinterpret_cast<float4*>(p.out + q_at + 4 * lane) = make_float4(x.x / l, x.y / l, x.z / l, x.w / l);
     return;
   }
-  float* part = f32_part(p, h) + static_cast<size_t>(split) * kPartFloats;
-  reinterpret_cast<float4*>(part + warp * kHeadDim)[lane] = make_float4(o[0], o[1], o[2], o[3]);
-  if (lane == 0) reinterpret_cast<float2*>(part + 16 * kHeadDim)[warp] = make_float2(m, l);
+  float* to = f32_part(p, h) + static_cast<size_t>(split) * kPartFloats;
+  reinterpret_cast<float4*>(to + warp * kHeadDim)[lane] = x;
+  if (lane == 0) reinterpret_cast<float2*>(to + 16 * kHeadDim)[warp] = make_float2(m, l);
 }
 
 // Grid (requests, 8-row blocks, heads): adds up the splits of f32_attn_kernel, a warp a row.
 __global__ void __launch_bounds__(kF32AttnThreads) f32_merge_kernel(const F32Params p) {
   const int h = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Request req = load_request(p.batch, p.cache, blockIdx.x);
-  const int row = blockIdx.y * kQBlock + (warp & 7);
+  const int row = blockIdx.y * kQBlock + (warp >> 1);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!req.ok || row >= req.q_len) return;
   const float* part = f32_part(p, h);
   float m = -INFINITY, l = 0.f;
@@ -281,7 +377,7 @@ __global__ void __launch_bounds__(kF32AttnThreads) f32_merge_kernel(const F32Par
     o[2] = fmaf(v[s].z, w, o[2]);
     o[3] = fmaf(v[s].w, w, o[3]);
   }
-  const size_t at = (static_cast<size_t>(req.q0 + row) * kQHeads + 2 * h + (warp >> 3)) * kHeadDim + 4 * lane;
+  const size_t at = (static_cast<size_t>(req.q0 + row) * kQHeads + 2 * h + (warp & 1)) * kHeadDim + 4 * lane;
   *reinterpret_cast<float4*>(p.out + at) = make_float4(o[0] / l, o[1] / l, o[2] / l, o[3] / l);
 }
 

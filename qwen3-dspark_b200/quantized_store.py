@@ -12,7 +12,7 @@ pages in use to the lowest ids.
 import torch
 
 from . import _lib
-from .kernels import HEAD_DIM, HKV, HQ, SCALE, runtime_identity
+from .kernels import HEAD_DIM, HKV, HQ, SCALE, _on_device, _stream, runtime_identity
 from .kv_store import B200PersistentTargetKV, Transaction, _BucketBuffers, _SlotTable, _upload
 from .quantized import CACHE_TYPES, PAGE, B200QuantizedKernel, QuantizedLayout, QuantizedPages, plan_words
 
@@ -260,10 +260,11 @@ class B200QuantizedTargetKV(B200PersistentTargetKV):
         table = self._rope_rows(tx, inv_freq, layout.cu_query, layout.context)
         tx.rope['planned'] = True                    # (a new table starts the dict over)
         keys, values = self._scratch(layer, n)
-        _lib.check(_lib.load_library().dspark_verify_prep(
-            q_raw.data_ptr(), lds[0], k_raw.data_ptr(), lds[1], v_raw.data_ptr(), lds[2], q_norm_weight.data_ptr(),
-            k_norm_weight.data_ptr(), table.data_ptr(), float(eps), n, out.data_ptr(), keys.data_ptr(),
-            values.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream), 'dspark_verify_prep')
+        with _on_device(self.device):
+            _lib.check(_lib.load_library().dspark_verify_prep(
+                q_raw.data_ptr(), lds[0], k_raw.data_ptr(), lds[1], v_raw.data_ptr(), lds[2], q_norm_weight.data_ptr(),
+                k_norm_weight.data_ptr(), table.data_ptr(), float(eps), n, out.data_ptr(), keys.data_ptr(),
+                values.data_ptr(), _stream(self.device)), 'dspark_verify_prep')
         self._kernel(out, keys, values, layout, scale=scale, pages=self.pages, layer=layer, out=out)
         self._staged.add(layer)
         return out
