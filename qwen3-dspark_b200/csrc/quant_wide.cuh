@@ -33,8 +33,8 @@ constexpr int kTileQ = 64, kItemQ = kWideItemRows;          // query rows of a t
 constexpr int kKeysW = kWideKeys;                           // keys of a block
 constexpr int kChunkW = 32;                                 // pages whose scales are held at a time
 constexpr uint32_t kSmemQW = 0, kSmemRingW = 2 * 32768, kSmemRawW = kSmemRingW + kStagesW * 32768;
-constexpr uint32_t kSmemScalesW = kSmemRawW + kRawW * 16384;          // [2][kChunkW] (ks, vs)
-constexpr uint32_t kSmemBarW = kSmemScalesW + 2 * kChunkW * 8;
+constexpr uint32_t kSmemScalesW = kSmemRawW + kRawW * 16384;          // [2][kChunkW] of page_scales
+constexpr uint32_t kSmemBarW = kSmemScalesW + 2 * kChunkW * 16;
 enum BarW {
   kWQFull = 0, kWQEmpty, kWRawFull, kWRawEmpty = kWRawFull + kRawW, kWFull = kWRawEmpty + kRawW,
   kWEmpty = kWFull + kStagesW, kWFixed = kWEmpty + kStagesW, kWSFull = kWFixed + kStagesW, kWPFull = kWSFull + 2,
@@ -110,6 +110,16 @@ struct RingW {
   }
 };
 
+// What the softmax needs of a page: the scores' factor f, log2 vs, 1 / vs, and whether the page is left out
+// or its values are so small that p vs may be below the least float, and the sum of p is taken apart.
+// p vs = 2^(f s + log2 vs - m), and the row's sum grows by p vs / vs. Zero blocks have codes 0 and keep p.
+constexpr float kPageIn = 0.f, kPageOut = 1.f, kPageTiny = 2.f;
+__device__ __forceinline__ float4 page_scales(float f, float vs) {
+  if (vs == 0.f) return make_float4(f, 0.f, 1.f, kPageIn);
+  if (vs < 1.f / 18446744073709551616.f) return make_float4(f, __log2f(vs), 0.f, kPageTiny);      // 2^-64
+  return make_float4(f, __log2f(vs), 1.f / vs, kPageIn);
+}
+
 // ---- warp 10 --------------------------------------------------------------------------------------
 __device__ __forceinline__ void wide_fetch(const AttnParamsQ& p, const MapsW& maps, const int* plan, RangeW range,
                                            uint8_t* smem, uint32_t sbase, volatile int* abort_flag) {
@@ -145,20 +155,20 @@ __device__ __forceinline__ void wide_fetch(const AttnParamsQ& p, const MapsW& ma
       const int at = (2 * (b - ub)) % kChunkW;              // page of the chunk
       if (at == 0) {
         const int page = 2 * b + lane, slot = chunks & 1;
-        float2 scales = make_float2(0.f, -1.f);             // (a negative V scale: the page is left out)
+        float4 scales = make_float4(0.f, -INFINITY, 0.f, kPageOut);
         id = 0;
         if (page < min(2 * ue, pages)) {
           id = __ldg(p.batch.table + static_cast<size_t>(x.request) * p.batch.width + page);
           if (id >= 0 && id < p.cache.pages) {
             const size_t s = static_cast<size_t>(id) * kKVHeads + x.head;
-            scales = make_float2(__ldg(p.cache.key_scale + s), __ldg(p.cache.value_scale + s));
+            scales = page_scales(__ldg(p.cache.key_scale + s) * p.scale_log2, __ldg(p.cache.value_scale + s));
           } else {
             atomicOr(&g_device_status, kStatusBadArgument);
             id = 0;
           }
         }
         if (!(ok = wait(kWChunkFree + slot, ((chunks >> 1) & 1) ^ 1))) break;
-        reinterpret_cast<float2*>(smem + kSmemScalesW)[slot * kChunkW + lane] = scales;
+        reinterpret_cast<float4*>(smem + kSmemScalesW)[slot * kChunkW + lane] = scales;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kWChunk + slot));
         ++chunks;
@@ -469,37 +479,82 @@ __device__ __forceinline__ void wide_issue(const AttnParamsQ& p, const int* plan
 }
 
 // ---- warps 0-7 ------------------------------------------------------------------------------------
-// 64 of a row's scores; those from `see` on are hidden.
-__device__ __forceinline__ void wide_scores(uint32_t addr, int see, bool full, float (&s)[64]) {
-#pragma unroll
-  for (int c = 0; c < 2; ++c) train::tmem_ld32_async(addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+// 64 of a row's scores, once they have landed.
+__device__ __forceinline__ void wide_landed(float (&s)[64]) {
   train::tmem_ld_wait();
 #pragma unroll
   for (int c = 0; c < 2; ++c) train::tmem_ld_landed(*reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-  if (!full) {
+}
+__device__ __forceinline__ void wide_scores(uint32_t addr, float (&s)[64]) {
 #pragma unroll
-    for (int i = 0; i < 64; ++i) s[i] = i < see ? s[i] : -INFINITY;
-  }
+  for (int c = 0; c < 2; ++c) train::tmem_ld32_async(addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+  wide_landed(s);
+}
+__device__ __forceinline__ float4 half_scales(const float4* scales, bool page, float scale_log2, int j) {
+  return page ? scales[j] : make_float4(scale_log2, 0.f, 1.f, kPageIn);
 }
 
-constexpr float kTinyScale = 1.f / 18446744073709551616.f;  // 2^-64
+// What few blocks need, 16 columns at a time and out of the usual path's way: keys that not every row
+// sees (those from `see` on are hidden), pages that are left out or nearly zero, and maxima of
+// thousands, where 2^(f s - m) as one fma would be off by 2^-24 |m|: there product, difference
+// and log2 vs are taken one by one.
+__device__ __noinline__ float wide_rare_max(uint32_t s_addr, int cols, int see, const float4* scales, bool page,
+                                            float scale_log2, float m) {
+#pragma unroll 1
+  for (int c = 0; c < cols; c += 16) {
+    uint32_t v[16];
+    prefix::tmem_ld16(s_addr + c, v);
+    const float4 sc = half_scales(scales, page, scale_log2, c >> 6);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = c + i < see ? fmaxf(top, __uint_as_float(v[i])) : top;
+    if (sc.w != kPageOut && c < see) m = fmaxf(m, __fmul_rn(top, sc.x));
+  }
+  return m;
+}
+__device__ __noinline__ float wide_rare_block(uint32_t s_addr, int cols, int see, const float4* scales, bool page,
+                                              float scale_log2, float m) {
+  float l = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < cols; c += 16) {
+    uint32_t v[16], pk[8];
+    prefix::tmem_ld16(s_addr + c, v);
+    const float4 sc = half_scales(scales, page, scale_log2, c >> 6);
+    const int limit = sc.w == kPageOut ? 0 : see - c;
+    float scaled = 0.f, plain = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float x = __fsub_rn(__fmul_rn(__uint_as_float(v[i]), sc.x), m), y = __fsub_rn(__fmul_rn(__uint_as_float(v[i + 1]), sc.x), m);
+      const float a = i < limit ? ex2(x + sc.y) : 0.f, b = i + 1 < limit ? ex2(y + sc.y) : 0.f;
+      scaled += a + b;
+      if (sc.w == kPageTiny) plain += (i < limit ? ex2(x) : 0.f) + (i + 1 < limit ? ex2(y) : 0.f);
+      pk[i >> 1] = pack_bf16x2(a, b);
+    }
+    prefix::tmem_st8(s_addr + (c >> 1), pk);
+    l += sc.w == kPageTiny ? plain : (sc.w == kPageOut ? 0.f : scaled * sc.z);
+  }
+  return l;
+}
 
 // One block of a row, one or two halves of 64 columns: scores from TMEM, P back as packed bf16. `see`
-// columns are visible, and the halves' pages unless they are left out (a negative V scale). The
-// second half's scores are read twice, for the maximum and for P, and the halves are a loop: the roles' code
-// takes turns in the instruction cache of an SM quarter (unrolled over 128 columns, with the
-// converters unrolled too, a warp waited for instructions 2.7 cycles in 9).
-__device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int halves, int see, const float2* scales,
-                                           bool page, float scale_log2, bool first, prefix::RowState& st) {
-  const bool full = __all_sync(0xffffffffu, see >= 64 * halves) != 0;
+// columns are visible. The second half's scores are read twice, for the maximum and for P (on the way
+// while the first half's exponentials are taken). The halves are loops, and what few blocks need is
+// elsewhere, because the roles' code takes turns in the instruction cache of an SM quarter: with
+// everything in line and unrolled a warp waited for instructions 2.7 cycles in 9.
+__device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int halves, int see, const float4* scales,
+                                           bool page, float scale_log2, bool first, const float4& sc0, const float4& sc1,
+                                           prefix::RowState& st) {
+  const bool full = __all_sync(0xffffffffu, see >= 64 * halves) && sc0.w == kPageIn && sc1.w == kPageIn;
   float s[64];
   float m_new = st.m;
+  if (full) {
 #pragma unroll 1
-  for (int j = halves - 1; j >= 0; --j) {
-    const float2 sc = page ? scales[j] : make_float2(1.f, 1.f);
-    wide_scores(s_addr + 64 * j, see - 64 * j, full, s);
-    const float top = __fmul_rn(prefix::max_n<64>(s), scale_log2 * sc.x);
-    m_new = sc.y < 0.f ? m_new : fmaxf(m_new, top);
+    for (int j = halves - 1; j >= 0; --j) {
+      wide_scores(s_addr + 64 * j, s);
+      m_new = fmaxf(m_new, __fmul_rn(prefix::max_n<64>(s), j ? sc1.x : sc0.x));
+    }
+  } else {
+    m_new = wide_rare_max(s_addr, 64 * halves, see, scales, page, scale_log2, m_new);
   }
   const bool raise = m_new > st.m + 8.f;
   float alpha = 1.f;
@@ -509,48 +564,30 @@ __device__ __forceinline__ void wide_block(uint32_t s_addr, uint32_t o_addr, int
   }
   // the block's S was committed behind the previous PV: O is complete
   if (!first && __any_sync(0xffffffffu, raise)) prefix::rescale_o(o_addr, alpha);
-  // one fma a score, off by 2^-24 |m|; scores of thousands are scaled and shifted first, one by one
-  const bool far = __any_sync(0xffffffffu, fabsf(st.m) > 1024.f && st.m > prefix::kNoMax) != 0;
   st.l *= alpha;
+  if (!full || __any_sync(0xffffffffu, fabsf(st.m) > 1024.f && st.m > prefix::kNoMax)) {
+    st.l += wide_rare_block(s_addr, 64 * halves, see, scales, page, scale_log2, st.m);
+  } else {
 #pragma unroll 1
-  for (int j = 0; j < halves; ++j) {
-    const float2 sc = page ? scales[j] : make_float2(1.f, 1.f);
-    if (j > 0) wide_scores(s_addr + 64 * j, see - 64 * j, full, s);      // (the first half's are still here)
-    const bool plain = !page || sc.y == 0.f;                // (a zero block: its codes are zero)
-    float base = plain ? 0.f : __log2f(sc.y), iv = plain ? 1.f : __frcp_rn(sc.y), f = scale_log2 * sc.x;
-    if (far) {
+    for (int j = 0; j < halves; ++j) {
+      if (j > 0) wide_landed(s);                            // (the first half's are still here)
+      const float f = j ? sc1.x : sc0.x, base = (j ? sc1.y : sc0.y) - st.m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 64; ++i) s[i] = __fsub_rn(__fmul_rn(s[i], f), st.m);
-      f = 1.f;
-    } else {
-      base -= st.m;
-    }
-    if (sc.y < 0.f) {                                       // left out: p = 2^(0 s - infinity)
-      f = iv = 0.f;
-      base = -INFINITY;
-    }
-    if (!plain && sc.y > 0.f && sc.y < kTinyScale) {        // p vs may be below the least float: the sum apart
-      const float shift = far ? 0.f : -st.m;
-      float sum = 0.f;
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) sum += ex2(fmaf(s[i], f, shift));
-      st.l += sum;
-      iv = 0.f;
-    }
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      uint32_t pk[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float a = ex2(fmaf(s[32 * c + 2 * i], f, base));
-        const float b = ex2(fmaf(s[32 * c + 2 * i + 1], f, base));
-        sum[i & 3] += a + b;
-        pk[i] = pack_bf16x2(a, b);
+        for (int i = 0; i < 16; ++i) {
+          const float a = ex2(fmaf(s[32 * c + 2 * i], f, base));
+          const float b = ex2(fmaf(s[32 * c + 2 * i + 1], f, base));
+          sum[i & 3] += a + b;
+          pk[i] = pack_bf16x2(a, b);
+        }
+        prefix::tmem_st16(s_addr + 32 * j + 16 * c, pk);
+        if (j + 1 < halves) train::tmem_ld32_async(s_addr + 64 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
       }
-      prefix::tmem_st16(s_addr + 32 * j + 16 * c, pk);
+      st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), j ? sc1.z : sc0.z, st.l);
     }
-    st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), iv, st.l);
   }
   prefix::tmem_st_wait();
 }
@@ -581,15 +618,18 @@ __device__ __forceinline__ void wide_softmax(const AttnParamsQ& p, const int* pl
       const BlockW b = block_of(x, u, p.cache.slots);
       const int at = (2 * (u - pages0)) % kChunkW;
       const bool last = b.page && (u + 1 == ue || at + 2 == kChunkW);
-      const float2* scales = reinterpret_cast<const float2*>(smem + kSmemScalesW) + (chunks & 1) * kChunkW + at;
+      const float4* scales = reinterpret_cast<const float4*>(smem + kSmemScalesW) + (chunks & 1) * kChunkW + at;
       if (b.page && at == 0 && !(ok = wait(kWChunk + (chunks & 1), (chunks >> 1) & 1))) break;
       if (active) {
+        const float4 sc0 = half_scales(scales, b.page, p.scale_log2, 0);
+        const float4 sc1 = b.keys > 64 ? half_scales(scales, b.page, p.scale_log2, 1) : sc0;
         if (!(ok = wait(kWSFull + tile, s_phase))) break;
         s_phase ^= 1;
         if (warp_ok) {
           train::tc_fence_after();
-          const int see = row_ok ? min(b.keys, b.see0 + lt) : 0;
-          wide_block(s_addr, o_addr, b.keys > 64 ? 2 : 1, see, scales, b.page, p.scale_log2, u == ub, st);
+          // (rows behind the item's last one hold anything and go nowhere)
+          wide_block(s_addr, o_addr, b.keys > 64 ? 2 : 1, min(b.keys, b.see0 + lt), scales, b.page, p.scale_log2, u == ub, sc0,
+                     sc1, st);
           train::tc_fence_before();
         }
         __syncwarp();
