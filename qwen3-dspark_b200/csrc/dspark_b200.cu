@@ -104,6 +104,12 @@ int quant_setup(int max_smem_optin) {
     if (cudaFuncGetAttributes(&a, k) != cudaSuccess) return DSPARK_ERR_CUDA;
     if (a.numRegs * quant::kAttnThreadsQ < 256 * quant::kHeadRegs + 128 * quant::kFetchRegs) return DSPARK_ERR_UNSUPPORTED;
   }
+  for (const void* k : {reinterpret_cast<const void*>(quant::quant_wide_kernel<quant::kInt8>),
+                        reinterpret_cast<const void*>(quant::quant_wide_kernel<quant::kE4M3>)}) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, k) != cudaSuccess) return DSPARK_ERR_CUDA;
+    if (a.numRegs * quant::kWideThreads < 256 * (quant::kSoftmaxRegsW + quant::kOtherRegsW)) return DSPARK_ERR_UNSUPPORTED;
+  }
   return DSPARK_OK;
 }
 
