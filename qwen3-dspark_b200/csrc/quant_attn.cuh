@@ -53,8 +53,12 @@ __host__ __device__ constexpr int plan_cta_at() { return kQHeadWords; }
 __host__ __device__ constexpr int plan_merge_at(int grid) { return kQHeadWords + grid * kCtaWords; }
 __host__ __device__ constexpr int plan_items_at(int grid) { return kQHeadWords + grid * (kCtaWords + kMergeWords); }
 // Two plans one behind the other: of the requests with few new rows (this file's kernel) and of
-// those with kWideRows or more (quant_wide.cuh), whose items are 128 query rows of one head.
-constexpr int kWideRows = 41, kWideItemRows = 128, kWideKeys = 128;
+// those with kWideRows or more (quant_wide.cuh), whose items are 128 query rows of one head. A page is
+// decoded once per 8 rows here and once per 128 there, where a block of keys costs the same whatever the
+// rows; int8, narrow against wide: 32 x 2048 tokens 24 rows 77 / 86 us, 32 rows 97 / 87, 40 rows 112 / 89;
+// 8 x 4096 24 rows 40 / 46, 32 rows 50 / 47, 40 rows 60 / 48; 1 x 8192 32 rows 30 / 29; 2 x 700, which
+// has few pages to decode, 15 / 21 at 32 and 19 / 23 at 64. From 33 on the gain outweighs that.
+constexpr int kWideRows = 33, kWideItemRows = 128, kWideKeys = 128;
 __host__ __device__ inline long long narrow_plan_words(int grid, long long requests, long long rows) {
   return plan_items_at(grid) + kItemWordsQ * (rows / kQBlock + requests);
 }

@@ -391,3 +391,12 @@ def test_calls_that_feed_one_another(pkg, rows):
     for _ in range(5):
         assert torch.equal(chain(False), want)
     status_clean(pkg)
+
+
+@pytest.mark.parametrize('dtype', U.CODES, ids=['int8', 'e4m3'])
+def test_lengths_around_the_change_of_kernels(pkg, dtype):
+    """Requests on both sides of where the wide kernel takes over, in one batch and each alone."""
+    for rows, contexts in (([32, 33, 31, 34], [130, 64, 200, 7]), ([32, 32], [63, 700]), ([33, 33], [63, 700]), ([33], [0])):
+        x, b = U.make(54, rows, contexts, dtype, BF16)
+        compare(run(pkg, x, b), x, b, BF16)
+    status_clean(pkg)
