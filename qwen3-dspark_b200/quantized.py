@@ -136,7 +136,7 @@ class QuantizedPages:
     the order in which the attention reads them; ``key_scale`` / ``value_scale`` float32
     [layers, pages, 8]; ``tail_key`` / ``tail_value`` [layers, slots, 2, 64, 8, 128] bf16 or
     float32: block b of a request that is still open lies in tail block b % 2 of its slot.
-    A full block is immutable, so requests may share its page.
+    A full block is immutable, so requests may share its page. Scales are not negative.
     """
 
     def __init__(self, key, value, key_scale, value_scale, tail_key, tail_value):
@@ -226,7 +226,8 @@ class QuantizedPages:
         follow its tokens, in all layers in one launch: ``key`` / ``value`` [layers, rows, 8, 128]
         in the tails' dtype, of which the layout's rows are the first. A block of 64 that gets
         full is quantised into the page that the table holds for it; the rest waits in the
-        tail. The layout's context lengths are the caller's to advance."""
+        tail. The layout's context lengths are the caller's to advance. No two requests of the
+        layout may fill the same page or have the same slot."""
         device, dtype = self.device, self.row_dtype
         if not isinstance(layout, QuantizedLayout) or layout.device != device:
             raise ValueError('append requires a QuantizedLayout on the cache\'s device')
